@@ -1,0 +1,322 @@
+// The paged K/V cache: rows quantised as they are written, read back, and moved when drafted tokens are dropped.
+//
+// A row (one token of one kv head) is stored on its own, so the cache grows by single tokens:
+//   K: int8 codes round(127 x / a), scale a / 127;   V: e4m3 codes of 448 x / a, scale a / 448;   a = max |x|.
+// Both roundings are to nearest, ties away from zero.  For 16-bit x the quotient is a ratio of small integers: it is a
+// tie exactly, or at least 2^-16 (relative, e4m3) resp. 2^-12 (absolute, int8) away from one.  So the product with the
+// reciprocal, pushed outwards by 2^-21, falls on the right side of every border and no division per element is needed.
+// Rows with an infinity or NaN store scale NaN and codes 0; rows with a < 2^-100 store zeros.
+#include "../../include/sage_b200.h"
+#include "sage_internal.h"
+#include "sage_paged.cuh"
+#include "sage_ptx.cuh"
+
+namespace sage {
+
+int paged_args(PagedArgs* out, void* k8, float* ks, void* v8, float* vs, int num_pages, int page_size, int Hkv, int D,
+               const int32_t* page_table, int64_t table_stride, int max_pages, const int32_t* lens, int* status) {
+  int shift = 4;
+  while (shift < 8 && (1 << shift) < page_size) ++shift;
+  if ((1 << shift) != page_size) {
+    set_error("page_size %d (a power of two from 16 to 256 required)", page_size);
+    return SAGE_ERR_UNSUPPORTED;
+  }
+  if (num_pages <= 0 || Hkv <= 0 || max_pages <= 0) {
+    set_error("empty cache (num_pages=%d Hkv=%d max_pages=%d)", num_pages, Hkv, max_pages);
+    return SAGE_ERR_UNSUPPORTED;
+  }
+  if ((reinterpret_cast<uintptr_t>(k8) & 15u) || (reinterpret_cast<uintptr_t>(v8) & 15u) || k8 == nullptr ||
+      v8 == nullptr || ks == nullptr || vs == nullptr) {
+    set_error("cache buffers: k8 / v8 must be 16-byte aligned, ks and vs non-null");
+    return SAGE_ERR_INVALID;
+  }
+  if (page_table == nullptr || lens == nullptr) {
+    set_error("page_table and lens must be device arrays");
+    return SAGE_ERR_INVALID;
+  }
+  int* word = status != nullptr ? status : default_status_word();
+  if (word == nullptr) {
+    set_error("no status word on this device");
+    return SAGE_ERR_LAUNCH;
+  }
+  *out = PagedArgs{static_cast<int8_t*>(k8), ks, static_cast<uint8_t*>(v8), vs, num_pages, shift, Hkv, D, page_table,
+                   table_stride, max_pages, lens, word};
+  return SAGE_OK;
+}
+
+constexpr float kTiny = 0x1p-100f;
+constexpr float kOutwards = 1.0f + 0x1p-21f;
+
+struct AppendArgs {
+  PagedArgs p;
+  const void* x[2];   // K, V
+  Strides3 st[2];
+  const int* counts;
+  int B, S;
+};
+
+// A group of LPR lanes (a power of two, D / 8 of them with data) holds one row of K and the same row of V, 8 channels a
+// lane; tokens of one head follow one another, as their rows do in a page.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
+  constexpr int LPR = D == 64 ? 8 : D == 256 ? 32 : 16;
+  const int lane = threadIdx.x % LPR;
+  const int64_t row = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
+  const int64_t bh = row / a.S;
+  const int s = (int)(row - bh * a.S);
+  const int b = (int)(bh / a.p.Hkv), h = (int)(bh - (int64_t)b * a.p.Hkv);
+  bool live = b < a.B;
+  int64_t dst = -1;
+  if (live) {
+    const int n = a.counts != nullptr ? a.counts[b] : a.S;
+    if (n < 0 || n > a.S) raise_invalid(a.p);
+    live = s < min(n, a.S);
+    if (live) dst = paged_row(a.p, b, h, (int64_t)a.p.lens[b] + s);
+    live = dst >= 0;
+  }
+  const bool data = live && lane * 8 < D;
+  float x[2][8];
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[w][i] = 0.0f;
+    if (data)
+      load8(static_cast<const T*>(a.x[w]) + b * a.st[w].b + s * a.st[w].s + h * a.st[w].h + lane * 8, x[w]);
+  }
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    // the largest magnitude as bits: NaN and infinity compare above every finite value
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[w][i]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o /= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const bool finite = top < 0x7f800000u;
+    const float amax = __uint_as_float(top);
+    const bool kept = finite && amax >= kTiny;
+    const float most = w == 0 ? 127.0f : 448.0f;
+    const float mul = __fdiv_rn(most, kept ? amax : most) * kOutwards;
+    const float scale = kept ? __fdiv_rn(amax, most) : finite ? 0.0f : __uint_as_float(0x7fc00000u);
+    uint32_t code[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (w == 0) {
+        uint32_t c = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          c |= (uint32_t)(uint8_t)(int8_t)__float2int_rn(kept ? x[w][4 * i + e] * mul : 0.0f) << (8 * e);
+        code[i] = c;
+      } else {
+        const float* y = x[w] + 4 * i;
+        code[i] = kept ? (uint32_t)pack_e4m3x2(y[0] * mul, y[1] * mul) |
+                               (uint32_t)pack_e4m3x2(y[2] * mul, y[3] * mul) << 16
+                         : 0u;
+      }
+    }
+    if (data) {
+      uint8_t* to = w == 0 ? reinterpret_cast<uint8_t*>(a.p.k8) : a.p.v8;
+      *reinterpret_cast<uint2*>(to + dst * D + lane * 8) = make_uint2(code[0], code[1]);
+      if (lane == 0) (w == 0 ? a.p.ks : a.p.vs)[dst] = scale;
+    }
+  }
+}
+
+struct ReadArgs {
+  PagedArgs p;
+  void* out[2];
+  Strides3 st[2];
+  int B, S;
+};
+
+// A thread reads 16 codes of K and of V and writes 16 channels of each.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) read_kernel(const ReadArgs a) {
+  constexpr int LPR = D / 16;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int c = (int)(id % LPR) * 16;
+  int64_t row = id / LPR;
+  const int h = (int)(row % a.p.Hkv);
+  row /= a.p.Hkv;
+  const int s = (int)(row % a.S);
+  const int64_t b64 = row / a.S;
+  if (b64 >= a.B) return;
+  const int b = (int)b64;
+  const int n = a.p.lens[b];
+  if (n < 0 || n > (int64_t)a.p.max_pages << a.p.page_shift) raise_invalid(a.p);
+  const int64_t src = s < n ? paged_row(a.p, b, h, s) : -1;
+  float x[2][16];
+#pragma unroll
+  for (int w = 0; w < 2; ++w)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[w][i] = 0.0f;
+  if (src >= 0) {
+    const uint4 k = *reinterpret_cast<const uint4*>(a.p.k8 + src * D + c);
+    const uint4 v = *reinterpret_cast<const uint4*>(a.p.v8 + src * D + c);
+    const float ks = a.p.ks[src], vs = a.p.vs[src];
+    const uint32_t kw[4] = {k.x, k.y, k.z, k.w}, vw[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      x[0][i] = (float)(int8_t)(kw[i / 4] >> (8 * (i % 4))) * ks;
+      const __nv_fp8_storage_t code = (__nv_fp8_storage_t)(vw[i / 4] >> (8 * (i % 4)));
+      x[1][i] = __half2float(__half(__nv_cvt_fp8_to_halfraw(code, __NV_E4M3))) * vs;
+    }
+  }
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    T* dst = static_cast<T*>(a.out[w]) + b * a.st[w].b + s * a.st[w].s + h * a.st[w].h + c;
+    store8(dst, x[w]);
+    store8(dst + 8, x[w] + 8);
+  }
+}
+
+struct KeepArgs {
+  PagedArgs p;
+  const int* keep;
+  int64_t keep_stride;
+  const int* counts;
+  int N;
+};
+
+// One CTA per (sequence, head).  Kept rows move to the front in chunks, in order: a chunk is read before any of it is
+// written, and since keep is strictly increasing (keep[i] >= i) no later chunk reads a row that an earlier one wrote.
+template <int D>
+__global__ void __launch_bounds__(256) keep_kernel(const KeepArgs a) {
+  constexpr int LPR = D / 16, ROWS = 256 / (2 * LPR);   // lanes per row of one tensor; rows of a chunk
+  const int b = blockIdx.x / a.p.Hkv, h = blockIdx.x % a.p.Hkv;
+  const int n = a.counts != nullptr ? a.counts[b] : a.N;
+  const int* keep = a.keep + b * a.keep_stride;
+  bool bad = n < 0 || n > a.N;
+  if (!bad)
+    for (int i = threadIdx.x; i < n; i += 256) bad |= keep[i] < 0 || (i > 0 && keep[i] <= keep[i - 1]);
+  if (__syncthreads_or(bad)) {
+    if (threadIdx.x == 0) raise_invalid(a.p);
+    return;
+  }
+  const int r = threadIdx.x / (2 * LPR), w = threadIdx.x / LPR % 2, lane = threadIdx.x % LPR;
+  uint8_t* codes = w == 0 ? reinterpret_cast<uint8_t*>(a.p.k8) : a.p.v8;
+  float* scales = w == 0 ? a.p.ks : a.p.vs;
+  const int64_t base = a.p.lens[b];
+  for (int i0 = 0; i0 < n; i0 += ROWS) {
+    const int i = i0 + r;
+    int64_t src = -1, dst = -1;
+    if (r < ROWS && i < n) {
+      src = paged_row(a.p, b, h, base + keep[i]);
+      dst = paged_row(a.p, b, h, base + i);
+    }
+    const bool move = src >= 0 && dst >= 0 && src != dst;
+    uint4 c = make_uint4(0, 0, 0, 0);
+    float scale = 0.0f;
+    if (move) {
+      c = *reinterpret_cast<const uint4*>(codes + src * D + lane * 16);
+      scale = scales[src];
+    }
+    __syncthreads();
+    if (move) {
+      *reinterpret_cast<uint4*>(codes + dst * D + lane * 16) = c;
+      if (lane == 0) scales[dst] = scale;
+    }
+  }
+}
+
+}  // namespace sage
+
+using namespace sage;
+
+extern "C" {
+
+int sage_paged_append(const void* k, const void* v, int dtype, int B, int S, int Hkv, int D, int64_t ksb, int64_t kss,
+                      int64_t ksh, int64_t vsb, int64_t vss, int64_t vsh, int8_t* k8, float* ks, uint8_t* v8, float* vs,
+                      int num_pages, int page_size, const int32_t* page_table, int64_t table_stride, int max_pages,
+                      const int32_t* lens, const int32_t* counts, int* status, void* stream) {
+  NvtxRange nvtx("sage_paged_append");
+  set_error("%s", "");
+  int rc = check_rows(dtype, B, S, Hkv, D);
+  if (rc == SAGE_OK) rc = check_rows_pointer(k, ksb, kss, ksh, "k");
+  if (rc == SAGE_OK) rc = check_rows_pointer(v, vsb, vss, vsh, "v");
+  AppendArgs a{};
+  if (rc == SAGE_OK)
+    rc = paged_args(&a.p, k8, ks, v8, vs, num_pages, page_size, Hkv, D, page_table, table_stride, max_pages, lens,
+                    status);
+  if (rc != SAGE_OK) return rc;
+  a.x[0] = k, a.x[1] = v;
+  a.st[0] = {ksb, kss, ksh}, a.st[1] = {vsb, vss, vsh};
+  a.counts = counts;
+  a.B = B, a.S = S;
+  const int per_block = 256 / (D == 64 ? 8 : D == 256 ? 32 : 16);
+  const int64_t blocks = ((int64_t)B * S * Hkv + per_block - 1) / per_block;
+  if (blocks > INT_MAX) {
+    set_error("append: %lld rows are too many for one call", (long long)B * S * Hkv);
+    return SAGE_ERR_UNSUPPORTED;
+  }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return by_head_dim(D, [&](auto d) {
+    if (dtype == SAGE_BF16)
+      append_kernel<__nv_bfloat16, decltype(d)::value><<<(int)blocks, 256, 0, st>>>(a);
+    else
+      append_kernel<__half, decltype(d)::value><<<(int)blocks, 256, 0, st>>>(a);
+    return launch_result("append");
+  });
+}
+
+int sage_paged_read(const int8_t* k8, const float* ks, const uint8_t* v8, const float* vs, int num_pages, int page_size,
+                    int Hkv, int D, const int32_t* page_table, int64_t table_stride, int max_pages, const int32_t* lens,
+                    int B, int S, void* k, void* v, int dtype, int64_t ksb, int64_t kss, int64_t ksh, int64_t vsb,
+                    int64_t vss, int64_t vsh, int* status, void* stream) {
+  NvtxRange nvtx("sage_paged_read");
+  set_error("%s", "");
+  int rc = check_rows(dtype, B, S, Hkv, D);
+  if (rc == SAGE_OK) rc = check_rows_pointer(k, ksb, kss, ksh, "k");
+  if (rc == SAGE_OK) rc = check_rows_pointer(v, vsb, vss, vsh, "v");
+  ReadArgs a{};
+  if (rc == SAGE_OK)
+    rc = paged_args(&a.p, const_cast<int8_t*>(k8), const_cast<float*>(ks), const_cast<uint8_t*>(v8),
+                    const_cast<float*>(vs), num_pages, page_size, Hkv, D, page_table, table_stride, max_pages, lens,
+                    status);
+  if (rc != SAGE_OK) return rc;
+  a.out[0] = k, a.out[1] = v;
+  a.st[0] = {ksb, kss, ksh}, a.st[1] = {vsb, vss, vsh};
+  a.B = B, a.S = S;
+  const int64_t blocks = ((int64_t)B * S * Hkv * (D / 16) + 255) / 256;
+  if (blocks > INT_MAX) {
+    set_error("read: %lld rows are too many for one call", (long long)B * S * Hkv);
+    return SAGE_ERR_UNSUPPORTED;
+  }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return by_head_dim(D, [&](auto d) {
+    if (dtype == SAGE_BF16)
+      read_kernel<__nv_bfloat16, decltype(d)::value><<<(int)blocks, 256, 0, st>>>(a);
+    else
+      read_kernel<__half, decltype(d)::value><<<(int)blocks, 256, 0, st>>>(a);
+    return launch_result("read");
+  });
+}
+
+int sage_paged_keep(int8_t* k8, float* ks, uint8_t* v8, float* vs, int num_pages, int page_size, int Hkv, int D,
+                    const int32_t* page_table, int64_t table_stride, int max_pages, const int32_t* lens,
+                    const int32_t* keep, int64_t keep_stride, int N, const int32_t* counts, int B, int* status,
+                    void* stream) {
+  NvtxRange nvtx("sage_paged_keep");
+  set_error("%s", "");
+  int rc = check_rows(SAGE_BF16, B, N, Hkv, D);
+  KeepArgs a{};
+  if (rc == SAGE_OK)
+    rc = paged_args(&a.p, k8, ks, v8, vs, num_pages, page_size, Hkv, D, page_table, table_stride, max_pages, lens,
+                    status);
+  if (rc == SAGE_OK && keep == nullptr) {
+    set_error("keep must be a device array");
+    rc = SAGE_ERR_INVALID;
+  }
+  if (rc == SAGE_OK && (int64_t)B * Hkv > INT_MAX) {
+    set_error("keep: %d sequences of %d heads are too many for one call", B, Hkv);
+    rc = SAGE_ERR_UNSUPPORTED;
+  }
+  if (rc != SAGE_OK) return rc;
+  a.keep = keep, a.keep_stride = keep_stride, a.counts = counts, a.N = N;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return by_head_dim(D, [&](auto d) {
+    keep_kernel<decltype(d)::value><<<B * Hkv, 256, 0, st>>>(a);
+    return launch_result("keep");
+  });
+}
+
+}  // extern "C"

@@ -1,0 +1,138 @@
+// Rotary positions for q and k, forward and gradient.
+//
+// Pair (x1, x2) of channels with frequency w_i at position p, a = p * w_i:
+//   y1 = m * (x1 cos a - x2 sin a),   y2 = m * (x2 cos a + x1 sin a);   the gradient is the same with -a.
+// Half layout pairs channel i with i + R/2, interleaved layout 2i with 2i + 1 (i < R/2); channels past R are copied.
+//
+// The angle is reduced in integers: a frequency is held in turns (w / 2 pi) as a 64-bit fixed-point fraction, so the
+// fraction of a turn at position p is the low 64 bits of p * turns, exact for any position (a product in 32-bit
+// floats is off by 0.06 radians at p = 10^6).  Its upper 32 bits go to sincospi.
+#include "../../include/sage_b200.h"
+#include "sage_internal.h"
+#include "sage_ptx.cuh"
+#include "sage_rows.cuh"
+
+namespace sage {
+
+struct RotaryArgs {
+  const void* in[2];   // q, k
+  void* out[2];
+  Strides3 in_st[2], out_st[2];
+  int heads[2];
+  int S, D, R, interleaved;
+  int64_t tokens;      // B * S
+  const void* positions;
+  int pos64;
+  int64_t pos_b, pos_s;
+  const uint64_t* turns;
+  float magnitude;     // factor of both cosine and sine
+  float sine_sign;     // -1 in the gradient
+  int slices;          // threads that share the heads of one token
+};
+
+// One thread holds 16 channels (8 pairs) of one token and walks over the heads, so each sine is computed once
+// for all of its heads.
+template <typename T>
+__global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
+  const int units = a.D / 16;
+  const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  const int u = (int)(id % units);
+  const int64_t rest = id / units;
+  const int64_t token = rest % a.tokens;
+  const int slice = (int)(rest / a.tokens);
+  if (slice >= a.slices) return;
+  const int64_t b = token / a.S, s = token - b * a.S;
+  const bool turned = u * 16 < a.R;
+  const int c0 = turned && !a.interleaved ? u * 8 : u * 16;          // first channel of each 8-channel part
+  const int c1 = turned && !a.interleaved ? a.R / 2 + u * 8 : u * 16 + 8;
+  float cs[8], sn[8];
+  if (turned) {
+    const int64_t at = b * a.pos_b + s * a.pos_s;
+    const uint64_t p = a.pos64 ? (uint64_t) static_cast<const int64_t*>(a.positions)[at]
+                               : (uint64_t)(int64_t) static_cast<const int*>(a.positions)[at];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint64_t turn = p * a.turns[u * 8 + e];
+      const int half_turns = (int)(uint32_t)((turn + 0x80000000ull) >> 32);   // units of 2^-31 half turns
+      sincospif((float)half_turns * 0x1p-31f, &sn[e], &cs[e]);
+      cs[e] *= a.magnitude;
+      sn[e] *= a.magnitude * a.sine_sign;
+    }
+  }
+  const int total = a.heads[0] + a.heads[1];
+  for (int h = slice; h < total; h += a.slices) {
+    const int w = h >= a.heads[0];
+    const int hh = h - (w ? a.heads[0] : 0);
+    const T* src = static_cast<const T*>(a.in[w]) + b * a.in_st[w].b + s * a.in_st[w].s + hh * a.in_st[w].h;
+    T* dst = static_cast<T*>(a.out[w]) + b * a.out_st[w].b + s * a.out_st[w].s + hh * a.out_st[w].h;
+    float x[16];
+    load8(src + c0, x);
+    load8(src + c1, x + 8);
+    if (turned) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        float& p1 = a.interleaved ? x[2 * e] : x[e];
+        float& p2 = a.interleaved ? x[2 * e + 1] : x[8 + e];
+        const float x1 = p1, x2 = p2;
+        p1 = x1 * cs[e] - x2 * sn[e];
+        p2 = x2 * cs[e] + x1 * sn[e];
+      }
+    }
+    store8(dst + c0, x);
+    store8(dst + c1, x + 8);
+  }
+}
+
+}  // namespace sage
+
+using namespace sage;
+
+extern "C" int sage_rotary(const void* q, const void* k, int dtype, int B, int S, int H, int Hkv, int D, int R,
+                           int interleaved, int64_t qsb, int64_t qss, int64_t qsh, int64_t ksb, int64_t kss,
+                           int64_t ksh, void* q_out, void* k_out, int64_t qosb, int64_t qoss, int64_t qosh,
+                           int64_t kosb, int64_t koss, int64_t kosh, const void* positions, int position_bits,
+                           int64_t psb, int64_t pss, const uint64_t* turns, float magnitude, int backward,
+                           void* stream) {
+  NvtxRange nvtx("sage_rotary");
+  set_error("%s", "");
+  int rc = check_rows(dtype, B, S, H, D);
+  if (rc != SAGE_OK) return rc;
+  if (R < 16 || R > D || R % 16 != 0 || Hkv < 0 || (position_bits != 32 && position_bits != 64)) {
+    set_error("rotary: rotary_dim %d (a multiple of 16 up to head_dim %d), kv heads %d, %d-bit positions", R, D, Hkv,
+              position_bits);
+    return SAGE_ERR_UNSUPPORTED;
+  }
+  if (positions == nullptr || turns == nullptr) {
+    set_error("rotary: positions and turns must be device arrays");
+    return SAGE_ERR_INVALID;
+  }
+  rc = check_rows_pointer(q, qsb, qss, qsh, "q");
+  if (rc == SAGE_OK) rc = check_rows_pointer(q_out, qosb, qoss, qosh, "q_out");
+  if (rc == SAGE_OK && Hkv > 0) rc = check_rows_pointer(k, ksb, kss, ksh, "k");
+  if (rc == SAGE_OK && Hkv > 0) rc = check_rows_pointer(k_out, kosb, koss, kosh, "k_out");
+  if (rc != SAGE_OK) return rc;
+  RotaryArgs a{};
+  a.in[0] = q, a.in[1] = k, a.out[0] = q_out, a.out[1] = k_out;
+  a.in_st[0] = {qsb, qss, qsh}, a.in_st[1] = {ksb, kss, ksh};
+  a.out_st[0] = {qosb, qoss, qosh}, a.out_st[1] = {kosb, koss, kosh};
+  a.heads[0] = H, a.heads[1] = Hkv;
+  a.S = S, a.D = D, a.R = R, a.interleaved = interleaved != 0;
+  a.tokens = (int64_t)B * S;
+  a.positions = positions, a.pos64 = position_bits == 64, a.pos_b = psb, a.pos_s = pss;
+  a.turns = turns;
+  a.magnitude = magnitude;
+  a.sine_sign = backward ? -1.0f : 1.0f;
+  a.slices = 1;
+  const int64_t threads = a.tokens * (D / 16) * a.slices;
+  const int64_t blocks = (threads + 255) / 256;
+  if (blocks > INT_MAX) {
+    set_error("rotary: %lld tokens are too many for one call", (long long)a.tokens);
+    return SAGE_ERR_UNSUPPORTED;
+  }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == SAGE_BF16)
+    rotary_kernel<__nv_bfloat16><<<(int)blocks, 256, 0, st>>>(a);
+  else
+    rotary_kernel<__half><<<(int)blocks, 256, 0, st>>>(a);
+  return launch_result("rotary");
+}

@@ -2,7 +2,8 @@
 
 Public names as in the reference package (src/rdna4_sage/__init__.py:17): ``sageattn``, ``attention``,
 ``is_available``, ``Unsupported``, ``ARCHS``, ``HEAD_DIMS``; plus the B200 additions (varlen, host-memory and
-multi-GPU entries, the quantised K/V cache).  Example::
+multi-GPU entries, the quantised K/V cache, the paged cache of a growing context with attention over it, rotary
+positions).  Example::
 
     import rdna4_sage
     o = rdna4_sage.sageattn(q, k, v, tensor_layout="HND")
@@ -16,9 +17,12 @@ from . import ops
 from ._attention import (ARCHS, HEAD_DIMS, QuantizedKV, Unsupported, attention_host, attention_quantized_kv,
                          attention_shard, check_supported, check_supported_varlen, device_arch, quantize_kv,
                          shard_heads)
+from ._paged import PagedKV, attention_paged_kv, paged_kv_append, paged_kv_keep, paged_kv_read
+from ._rotary import Rotary, rotary
 
 __all__ = ["sageattn", "attention", "attention_varlen", "attention_host", "attention_shard", "shard_heads",
-           "quantize_kv", "attention_quantized_kv", "QuantizedKV", "is_available", "Unsupported", "ARCHS",
+           "quantize_kv", "attention_quantized_kv", "QuantizedKV", "PagedKV", "paged_kv_append", "paged_kv_read",
+           "paged_kv_keep", "attention_paged_kv", "Rotary", "rotary", "is_available", "Unsupported", "ARCHS",
            "HEAD_DIMS"]
 __version__ = "0.2.1+b200"
 

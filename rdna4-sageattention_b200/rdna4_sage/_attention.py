@@ -39,14 +39,19 @@ def device_arch(device: torch.device) -> str:
     return _arch_cache[idx]
 
 
+def _copied(t: torch.Tensor):
+    """A contiguous copy in memory of its own (contiguous() keeps a tensor that is contiguous but not aligned)."""
+    return t.clone(memory_format=torch.contiguous_format)
+
+
 def _bsh(t: torch.Tensor, layout: str):
     """(batch, seq, head) element strides; the kernels need a 16-byte aligned base and strides
     (8 elements of a 16-bit type), otherwise the tensor is made contiguous.  Reference :59-67."""
     if t.stride(-1) != 1 or t.data_ptr() % 16:
-        t = t.contiguous()
+        t = _copied(t)
     st = (t.stride(0), t.stride(2), t.stride(1)) if layout == "HND" else (t.stride(0), t.stride(1), t.stride(2))
     if any(s % 8 for s in st):
-        t = t.contiguous()
+        t = _copied(t)
         st = (t.stride(0), t.stride(2), t.stride(1)) if layout == "HND" else (t.stride(0), t.stride(1), t.stride(2))
     return t, st
 
@@ -105,8 +110,9 @@ _watch: dict[int, tuple[torch.cuda.Event, torch.Tensor]] = {}
 
 def _raise_pending(device: torch.device) -> None:
     """Raise RuntimeError if work that completed on `device` since the last check reported an error."""
+    _raise_host_word(device)
     w = _watch.get(device.index)
-    if w is None or not w[0].query():
+    if w is None or torch.cuda.is_current_stream_capturing() or not w[0].query():   # no event query under capture
         return
     code = int(w[1][0])
     if code != 0:
@@ -114,6 +120,34 @@ def _raise_pending(device: torch.device) -> None:
         status_word(device).zero_()
         raise RuntimeError(f"rdna4_sage: an earlier kernel on cuda:{device.index} failed: "
                            f"{_lib.STATUS_NAMES.get(code, code)} (see check_status)")
+
+
+# The step calls of the paged cache report through a word in pinned host memory instead, which their kernels write only
+# on an error: nothing has to be copied behind each call, and reading it costs the host one load.
+_host_words: dict[int, tuple[torch.Tensor, ctypes.c_int32]] = {}
+
+
+def host_word(device: torch.device) -> int:
+    """Address of the device's error word in pinned host memory (made once, kept for the life of the process)."""
+    w = _host_words.get(device.index)
+    if w is None:
+        t = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+        w = _host_words.setdefault(device.index, (t, ctypes.c_int32.from_address(t.data_ptr())))
+    return w[0].data_ptr()
+
+
+def _raise_host_word(device: torch.device) -> None:
+    w = _host_words.get(device.index)
+    if w is not None and w[1].value != 0:
+        code, w[1].value = w[1].value, 0
+        raise RuntimeError(f"rdna4_sage: an earlier kernel on cuda:{device.index} failed: "
+                           f"{_lib.STATUS_NAMES.get(code, code)} (lengths, counts or page table of a paged K/V call)")
+
+
+def _checked(device: torch.device) -> None:
+    """RDNA4_SAGE_CHECK=1: raise at once what the call just enqueued reports."""
+    if _CHECK and not torch.cuda.is_current_stream_capturing():
+        check_status(device)
 
 
 def _watch_status(device: torch.device) -> None:
@@ -151,6 +185,7 @@ def check_status(device: torch.device | None = None) -> None:
     with torch.cuda.device(dev):
         rc = _lib.lib().sage_status_sync(w.data_ptr(), torch.cuda.current_stream(dev).cuda_stream)
     _lib.check(rc, "kernel status")
+    _raise_host_word(dev)
 
 
 def attention(q, k, v, layout="HND", sm_scale=None, is_causal=False, return_lse=False):

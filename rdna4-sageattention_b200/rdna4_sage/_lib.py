@@ -73,6 +73,18 @@ SIGNATURES = {
     "sage_attention_host_multi": (_c_i, [_c_p, _c_p, _c_p, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i, _c_i64, _c_i64,
                                          _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_d, _c_i, _c_p,
                                          _c_i64, _c_i64, _c_i64, _c_p, _c_i, _c_i, _c_p, _c_p, _c_sz, _c_p, _c_p]),
+    "sage_rotary": (_c_i, [_c_p, _c_p] + [_c_i] * 8 + [_c_i64] * 6 + [_c_p, _c_p] + [_c_i64] * 6 +
+                    [_c_p, _c_i, _c_i64, _c_i64, _c_p, _c_f, _c_i, _c_p]),
+    "sage_paged_append": (_c_i, [_c_p, _c_p] + [_c_i] * 5 + [_c_i64] * 6 + [_c_p] * 4 +
+                          [_c_i, _c_i, _c_p, _c_i64, _c_i, _c_p, _c_p, _c_p, _c_p]),
+    "sage_paged_read": (_c_i, [_c_p] * 4 + [_c_i] * 4 + [_c_p, _c_i64, _c_i, _c_p, _c_i, _c_i, _c_p, _c_p, _c_i] +
+                        [_c_i64] * 6 + [_c_p, _c_p]),
+    "sage_paged_keep": (_c_i, [_c_p] * 4 + [_c_i] * 4 + [_c_p, _c_i64, _c_i, _c_p, _c_p, _c_i64, _c_i, _c_p, _c_i,
+                                                         _c_p, _c_p]),
+    "sage_paged_attention_workspace_bytes": (_c_sz, [_c_i] * 5),
+    "sage_paged_attention": (_c_i, [_c_p] + [_c_i] * 6 + [_c_i64] * 3 + [_c_p] * 4 +
+                             [_c_i, _c_i, _c_p, _c_i64, _c_i, _c_p, _c_p, _c_p, _c_i64, _c_i64, _c_d, _c_p] +
+                             [_c_i64] * 3 + [_c_p, _c_p, _c_sz, _c_p, _c_p]),
     "sage_selftest_wait_timeout": (_c_i, [_c_p, _c_i, _c_p]),
     "sage_selftest_counter_timeout": (_c_i, [_c_p, _c_p, _c_i, _c_p]),
     "sage_status_sync": (_c_i, [_c_p, _c_p]),

@@ -1,0 +1,170 @@
+"""Rotary positions for q and k: the frequencies a model keeps (Rotary) and the op (rotary), with its gradient.
+
+The reference leaves positions to its callers; here they sit in front of attention() and of the paged K/V cache, which
+stores keys already turned.
+"""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _attention, _lib
+from ._attention import DTYPES, HEAD_DIMS, Unsupported, _bsh
+
+SCALINGS = (None, "linear", "ntk", "ramp")
+
+
+class Rotary:
+    """The frequencies of rotary positions on one GPU.
+
+    Channels 0 .. rotary_dim - 1 of each head (default: all of them; a multiple of 16) are turned in pairs: channel i
+    with i + rotary_dim / 2, or 2 i with 2 i + 1 when `interleaved`.  Pair i has frequency w_i = base^(-2 i / rotary_dim)
+    radians per position, scaled for contexts longer than the trained one by
+      scaling="linear"  w_i / factor
+      scaling="ntk"     base * factor^(rotary_dim / (rotary_dim - 2)) in place of base
+      scaling="ramp"    w_i (g / 1 + (1 - g) / factor), where g rises from 0 to 1 as the number of turns within
+                        original_len positions, r_i = original_len w_i / (2 pi), rises from ramp[0] to ramp[1]
+    `magnitude` multiplies the turned channels (default 1; for "ramp" 0.1 ln(factor) + 1).  `frequencies`: a tensor or
+    list of rotary_dim / 2 radians per position in place of all this.
+    """
+
+    def __init__(self, head_dim, rotary_dim=None, base=10000.0, interleaved=False, scaling=None, factor=1.0,
+                 original_len=None, ramp=(1.0, 32.0), magnitude=None, frequencies=None, device=None):
+        R = head_dim if rotary_dim is None else rotary_dim
+        if head_dim not in HEAD_DIMS:
+            raise Unsupported(f"head_dim {head_dim} (supported {HEAD_DIMS})")
+        if R < 16 or R > head_dim or R % 16:
+            raise Unsupported(f"rotary_dim {R} (a multiple of 16 up to head_dim {head_dim} required)")
+        if frequencies is not None:
+            if scaling is not None:
+                raise ValueError("give frequencies or a scaling, not both")
+            w = torch.as_tensor(frequencies, dtype=torch.float64, device="cpu").detach()
+            if w.shape != (R // 2,) or not bool(torch.isfinite(w).all()):
+                raise ValueError(f"frequencies: {R // 2} finite numbers required")
+        else:
+            w = _frequencies(R, base, scaling, factor, original_len, ramp)
+        if magnitude is None:
+            magnitude = 0.1 * math.log(factor) + 1.0 if scaling == "ramp" else 1.0
+        self.head_dim, self.rotary_dim, self.interleaved, self.magnitude = head_dim, R, bool(interleaved), float(magnitude)
+        self.frequencies = w
+        # turns per position as 64-bit fixed-point fractions, in (-1/2, 1/2] of a turn
+        turns = w / (2 * math.pi)
+        turns = [int(round((t - round(t)) * 2.0 ** 64)) for t in turns.tolist()]
+        self.turns = torch.tensor([min(max(t, -2 ** 63), 2 ** 63 - 1) for t in turns], dtype=torch.int64,
+                                  device="cuda" if device is None else device)
+
+
+def _frequencies(R, base, scaling, factor, original_len, ramp):
+    if scaling not in SCALINGS:
+        raise ValueError(f"scaling {scaling!r} (one of {SCALINGS})")
+    if not (base > 1.0 and math.isfinite(base) and factor > 0.0 and math.isfinite(factor)):
+        raise ValueError(f"base {base} (above 1) and factor {factor} (above 0) must be finite")
+    i = torch.arange(0, R, 2, dtype=torch.float64)
+    if scaling == "ntk":
+        base = base * factor ** (R / (R - 2))
+    w = base ** (-i / R)
+    if scaling == "linear":
+        return w / factor
+    if scaling == "ramp":
+        lo, hi = ramp
+        if original_len is None or original_len <= 0 or not lo < hi:
+            raise ValueError('scaling="ramp" needs original_len > 0 and ramp[0] < ramp[1]')
+        g = ((original_len * w / (2 * math.pi) - lo) / (hi - lo)).clamp(0.0, 1.0)
+        return w * (g + (1.0 - g) / factor)
+    return w
+
+
+def _check(q, k, positions, rope, layout):
+    """Raise Unsupported with the reason if the kernel cannot run these inputs (devices aside)."""
+    if layout not in ("HND", "NHD"):
+        raise Unsupported(f"layout {layout!r}")
+    h_ax, s_ax = (1, 2) if layout == "HND" else (2, 1)
+    for x in (q,) if k is None else (q, k):
+        if x.dtype not in DTYPES or x.dtype != q.dtype:
+            raise Unsupported(f"dtype {x.dtype} (fp16 or bf16, one for q and k, required)")
+        if x.dim() != 4 or x.shape[-1] != rope.head_dim:
+            raise Unsupported(f"4D tensors with head_dim {rope.head_dim} required")
+        if x.shape[0] != q.shape[0] or x.shape[s_ax] != q.shape[s_ax]:
+            raise Unsupported("q and k must hold the same tokens")
+    if positions.dtype not in (torch.int32, torch.int64):
+        raise Unsupported(f"positions {positions.dtype} (int32 or int64 required)")
+    B, S = q.shape[0], q.shape[s_ax]
+    if positions.shape not in ((S,), (1, S), (B, S)):
+        raise Unsupported(f"positions {tuple(positions.shape)}: (S,) or (B, S) of ({B}, {S}) tokens required")
+
+
+def _check_devices(tensors):
+    dev = tensors[0].device
+    if dev.type != "cuda" or any(t.device != dev for t in tensors):
+        raise Unsupported("tensors must be on one CUDA GPU")
+    _attention._check_arch(dev)
+    return dev
+
+
+def _launch(q, k, positions, rope, layout, backward):
+    """(q, k) turned, new tensors in the inputs' layout (k may be None)."""
+    dev = q.device
+    if q.numel() == 0 or k is not None and k.numel() == 0:
+        if q.numel() != 0 or k is not None and k.numel() != 0:
+            raise Unsupported("q and k must both hold heads")
+        return torch.empty_like(q), None if k is None else torch.empty_like(k)
+    B, S, H = (q.shape[0], q.shape[2], q.shape[1]) if layout == "HND" else q.shape[:3]
+    bsh = (0, 2, 1) if layout == "HND" else (0, 1, 2)
+    q, qs = _bsh(q, layout)
+    q_out = torch.empty_like(q)   # of a tensor that the kernels take, so it is one too
+    qos = [q_out.stride(i) for i in bsh]
+    if k is None:
+        k_out, Hkv, kp, kop, ks, kos = None, 0, None, None, (0, 0, 0), (0, 0, 0)
+    else:
+        k, ks = _bsh(k, layout)
+        k_out = torch.empty_like(k)
+        kos = [k_out.stride(i) for i in bsh]
+        Hkv, kp, kop = k.shape[1 if layout == "HND" else 2], k.data_ptr(), k_out.data_ptr()
+    at = positions.expand(B, S)
+    with torch.cuda.device(dev):
+        rc = _lib.lib().sage_rotary(q.data_ptr(), kp, DTYPES[q.dtype], B, S, H, Hkv, rope.head_dim, rope.rotary_dim,
+                                    rope.interleaved, *qs, *ks, q_out.data_ptr(), kop, *qos, *kos, at.data_ptr(),
+                                    32 if at.dtype == torch.int32 else 64, *at.stride(), rope.turns.data_ptr(),
+                                    rope.magnitude, backward, torch.cuda.current_stream(dev).cuda_stream)
+    _lib.check(rc, "sage_rotary")
+    return q_out, k_out
+
+
+class _RotaryFunction(torch.autograd.Function):
+    """The gradient of a turn is the turn by the negative angle, so the backward pass is the op itself again."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, rope, layout, backward):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(positions)
+        ctx.rope, ctx.layout, ctx.turn_back = rope, layout, not backward
+        q_out, k_out = _launch(q, k, positions, rope, layout, backward)
+        return q_out if k is None else (q_out, k_out)
+
+    @staticmethod
+    def backward(ctx, dq, dk=None):
+        positions, = ctx.saved_tensors
+        dq = dq if ctx.needs_input_grad[0] else None
+        dk = dk if ctx.needs_input_grad[1] else None
+        args = (positions, ctx.rope, ctx.layout, ctx.turn_back)
+        if dq is not None and dk is not None:
+            dq, dk = _RotaryFunction.apply(dq, dk, *args)
+        elif dq is not None:
+            dq = _RotaryFunction.apply(dq, None, *args)
+        elif dk is not None:
+            dk = _RotaryFunction.apply(dk, None, *args)
+        return dq, dk, None, None, None, None
+
+
+def rotary(q, k, positions, rope, tensor_layout="HND"):
+    """q and k turned to their positions: (B, H, S, D) and (B, Hkv, S, D) for "HND", (B, S, H, D) and (B, S, Hkv, D) for
+    "NHD", fp16 or bf16; new tensors of the same shapes and types (rounded once).  k may be None: the result is q
+    alone.  positions: int32 or int64 of any value, (S,) for all sequences or (B, S), on the GPU.  rope: a Rotary.
+    Differentiable in q and k.  Raises Unsupported for inputs the kernel does not take."""
+    _check(q, k, positions, rope, tensor_layout)
+    _check_devices((q, positions, rope.turns) if k is None else (q, k, positions, rope.turns))
+    if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad):
+        return _RotaryFunction.apply(q, k, positions, rope, tensor_layout, False)
+    q_out, k_out = _launch(q, k, positions, rope, tensor_layout, False)
+    return q_out if k is None else (q_out, k_out)
