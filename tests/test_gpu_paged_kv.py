@@ -185,7 +185,10 @@ def check_attention(q, cache, table, lens, mask=None, counts=None, layout="NHD",
     tol = torch.finfo(q.dtype).eps / 2 * want.abs() + mean * (2.0 ** -11 + weight[..., None]) + \
         (n * 2.0 ** -25 * 448 * top)[..., None] + 2.0 ** -25
     off = (got - want).abs()
-    over = want.abs() > torch.finfo(q.dtype).max                    # beyond the type: rounds to infinity
+    # the computed value lies within tol of want, and what reaches the type's largest value and half a step more
+    # (its step there is max eps / (2 - eps)) rounds to infinity
+    info = torch.finfo(q.dtype)
+    over = want.abs() + tol >= info.max * (1 + info.eps / 2 / (2 - info.eps))
     off = torch.where(over & (got == torch.copysign(torch.full_like(want, math.inf), want)), 0.0, off)
     assert bool((off <= tol).all()), (float((off / tol).max()), float(off.max()))
     empty = want_lse == -math.inf
