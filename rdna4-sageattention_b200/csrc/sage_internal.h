@@ -4,6 +4,7 @@
 #include <cstddef>
 #include <climits>
 #include <cstdint>
+#include <cuda.h>
 #include <cuda_runtime.h>
 #include <nvtx3/nvToolsExt.h>
 
@@ -120,6 +121,12 @@ int attention_rows_per_cta(int D);
 int attention_tail_split(int D, int causal, int varlen, int64_t planes, int Sq, int nsm, int64_t* main_ctas);
 
 int* default_status_word();
+
+// cuTensorMapEncodeTiled of the loaded driver (null if it has none).
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn();
 
 #ifdef SAGE_DEBUG
 // Debug builds: read and clear the first recorded violation of the attention kernels / the quantisers

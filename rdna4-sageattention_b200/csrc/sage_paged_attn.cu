@@ -16,8 +16,12 @@
 //
 // The query rows of a kv head (T tokens of H / Hkv heads) are cut into row tiles, the keys into tiles of 64.  All
 // (sequence, kv head, row tile, key tile) of a call form one list that the CTAs share evenly, whatever the lengths are: a
-// CTA walks a contiguous stretch of it with one load pipeline.  A row tile that falls to several CTAs is joined from
-// their partial (O, l, m') by a second small kernel, in the order of the keys.
+// CTA walks a contiguous stretch of it with one load pipeline (a producer warp that issues TMA boxes and prefetches page
+// numbers, and consumer warps that wait for nothing but their stage).  A row tile that falls to several CTAs is joined
+// from their partial (O, l, m') by a second small kernel, in the order of the keys.
+//
+// Both products are taken transposed, S^T = K Q^T and O^T = V^T P^T: keys and channels fill the 16 rows of an mma tile
+// and the query rows its 8 columns, so that the 1 to 8 rows of a single token's group cost one column tile.
 #include <algorithm>
 #include <atomic>
 #include <cmath>
@@ -30,8 +34,9 @@
 namespace sage {
 
 constexpr int kTileKeys = 64;
-constexpr int kStages = 3;
-constexpr int kThreads = 128;
+constexpr int kWarps = 4;                              // consumer warps
+constexpr int kThreads = 32 * (kWarps + 1);
+constexpr int kJoinThreads = 128;
 constexpr int kMinTiles = 2;               // tiles a CTA takes at the least
 constexpr float kZeroLog = -100.0f;        // log2 of a zero V scale in the running maximum
 
@@ -65,6 +70,7 @@ __device__ __forceinline__ int sequence(const PagedAttnArgs& a, int b, int& len,
 }
 
 // Sum over the CTA's threads before this one; `total` receives the sum over all.
+template <int THREADS>
 __device__ __forceinline__ int64_t scan_before(int64_t v, int64_t* warp_sums, int64_t& total) {
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   int64_t x = v;
@@ -79,7 +85,7 @@ __device__ __forceinline__ int64_t scan_before(int64_t v, int64_t* warp_sums, in
   total = 0;
   int64_t before = 0;
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
+  for (int w = 0; w < THREADS / 32; ++w) {
     if (w < warp) before += warp_sums[w];
     total += warp_sums[w];
   }
@@ -92,7 +98,7 @@ __device__ __forceinline__ int64_t list_length(const PagedAttnArgs& a, int64_t* 
   int len, fresh;
   for (int b = threadIdx.x; b < a.B; b += kThreads) mine += sequence(a, b, len, fresh);
   int64_t total;
-  scan_before(mine, warp_sums, total);
+  scan_before<kThreads>(mine, warp_sums, total);
   return total * (a.p.Hkv * a.row_tiles);
 }
 
@@ -110,7 +116,7 @@ __device__ __forceinline__ void find(const PagedAttnArgs& a, int64_t x, int64_t*
     const int mine = base + threadIdx.x;
     const int64_t v = mine < a.B ? (int64_t)sequence(a, mine, len, fresh) * per : 0;
     int64_t total;
-    const int64_t at = carry + scan_before(v, warp_sums, total);
+    const int64_t at = carry + scan_before<kThreads>(v, warp_sums, total);
     if (x >= at && x < at + v) found[0] = mine, found[1] = x - at;
     carry += total;
     if (x < carry) break;
@@ -137,16 +143,40 @@ __device__ __forceinline__ void advance(const PagedAttnArgs& a, Cursor& c) {
   } while (c.tiles == 0);
 }
 
-__device__ __forceinline__ void copy_async16(uint32_t dst, const void* src, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+// 2-D tile load: rows `y` ... of a [rows, bytes] tensor, bytes from `x` on.
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+      : "memory");
 }
-__device__ __forceinline__ void copy_async4(uint32_t dst, const void* src, bool ok) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(ok ? 4 : 0) : "memory");
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
 }
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+
+__device__ __forceinline__ void arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// Bounded wait for a phase of a stage barrier.  Unlike mbar_wait it does not give up on an error that stands in the
+// status word: a bad page of one sequence leaves the others' work as it is.
+__device__ __forceinline__ bool wait_stage(uint64_t* bar, uint32_t parity, volatile int* given_up, int* status) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+  for (uint32_t i = 1; !mbar_try_wait(bar, parity); ++i) {
+    if ((i & 63u) != 0) continue;
+    if (*given_up != 0) return false;
+    if (global_timer_ns() - t0 > kWaitLimitNs) {
+      *given_up = 1;
+      *const_cast<volatile int*>(status) = kStatusTimeout;
+      return false;
+    }
+  }
+  return true;
 }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -180,47 +210,78 @@ __device__ __forceinline__ uint32_t e4m3_to_f16(uint16_t v) {
   return r;
 }
 
-// Shared-memory tiles.  A warp works on groups of 16 keys; lane (n = lane / 4, c = lane % 4) owns keys 4c .. 4c + 3 of a
-// group in the products with V, which is what the accumulator layout of the first product leaves it with when column n
-// of its tile j stands for key 4 (n / 2) + 2 j + n % 2.  K rows lie in order; lane c reads the 16-byte chunks c, c + 4,
-// ... of row n.  V rows lie transposed within the group (key 4c + k at slot 4k + c); lane n reads the d channels that it
-// holds as columns, D / 8 consecutive ones (256: two runs of 16).  Chunks are permuted so that the eight lanes of a
-// 16-byte shared load (sixteen of an 8-byte one) touch different banks (96: up to two-way conflicts are left).
+// Transposes an 8 x 8 tile of 16-bit values across the warp (row lane / 4, columns 2 (lane % 4) and the next).
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// Shared-memory tiles, as TMA writes them: 64 rows of K, 64 rows of V, of 128 swizzled bytes (D 256: two such halves), 64
+// swizzled bytes (D 64) or 96 plain ones.  A warp works on groups of 16 keys; lane (n = lane / 4, c = lane % 4) takes the
+// scores of the keys in slots n and n + 8 for the columns 2c and 2c + 1, and after the transposition the weights of the
+// keys in slots 2c, 2c + 1, 2c + 8, 2c + 9 for column n.  slot_key() and first_channel() are chosen so that the lanes of one
+// phase of a shared load touch different banks (D 64 and 96: two-way conflicts are left in V).
 template <int D>
 struct Tile {
-  static constexpr int CH = D / 16;                       // 16-byte chunks of a row
-  static constexpr int kBytes = kTileKeys * D;
-  static constexpr int kStage = 2 * kBytes + 2 * kTileKeys * 4;
-  __device__ static int k_at(int row, int ch) { return row * D + ((D % 128 == 0 ? ch ^ ((row & 1) << 2) : ch) << 4); }
-  __device__ static int v_at(int row, int ch) {
-    const int c = (row >> 2) & 3, slot = (row & ~15) | ((row & 3) << 2) | c;
-    return slot * D + ((D % 128 == 0 ? ch ^ (c << 1) : D == 64 ? ch ^ (c & 2) : ch) << 4);
+  static constexpr bool kWide = D % 128 == 0;
+  static constexpr int kBox = kWide ? 128 : D;            // bytes of a row in a box
+  static constexpr int kHalves = D / kBox;
+  static constexpr int kBytes = kTileKeys * D;            // of K, and of V
+  static constexpr int kStage = 2 * kBytes;
+  // where byte x of row `row` lies
+  __device__ static int at(int row, int x) {
+    if constexpr (kWide) return x / 128 * (kTileKeys * 128) + row * 128 + ((x % 128) ^ ((row & 7) << 4));
+    if constexpr (D == 64) return row * 64 + (x ^ ((row >> 1 & 3) << 4));
+    return row * D + x;
   }
+  __device__ static int slot_key(int slot) { return kWide ? (slot & 8) | (slot & 7) >> 1 | (slot & 1) << 2 : slot; }
+  // first of the D / 8 channels (D 256: of either half) whose output lane row n holds
+  __device__ static int first_channel(int n) { return kWide ? ((n >> 1) | (n & 1) << 2) * 16 : n * (D / 8); }
+  // channel of row n + 8 e of the output tile t
+  __device__ static int channel(int n, int t, int e) { return first_channel(n) + (kWide ? t / 8 * 128 + t % 8 * 2 : t * 2) + e; }
 };
 
-template <int D>
-constexpr int smem_bytes() {
-  return kStages * Tile<D>::kStage + 2 * kTileKeys * 16;
-}
+template <int D, int NR, int WM>
+struct Config {
+  // CTAs of an SM: as the registers of a thread allow (up to 128 for three CTAs, 200 for two)
+  static constexpr int kCtas = D * NR <= 128 ? 3 : 2;
+  static constexpr int kRows = 8 * NR * WM;               // of a row tile
+  static constexpr int kJoin = WM < kWarps ? kRows * (D + 4) * 4 : 0;
+  static constexpr int kPerStage = Tile<D>::kStage + 2 * kTileKeys * 4 + 16;
+  static constexpr int kFit = (232448 / kCtas - 2048 - 1024 - kJoin) / kPerStage;
+  static constexpr int kStages = kFit < 8 ? kFit : 8;
+  static constexpr int kSmem = 1024 + kStages * kPerStage + kJoin;
+  static_assert(kStages >= 2, "two stages at the least");
+};
 
-// First row of the d channels behind column n of the output tile t.
-template <int D>
-__device__ __forceinline__ int channel(int n, int t) {
-  return D == 256 ? (n + 8 * (t / 16)) * 16 + t % 16 : n * (D / 8) + t;
-}
-
-// WM row tiles of 16 rows, each with 4 / WM warps that share its keys.
-template <typename T, int D, int WM>
-__global__ void __launch_bounds__(kThreads) paged_attn_kernel(const PagedAttnArgs a) {
-  constexpr int WK = 4 / WM, CH = Tile<D>::CH, NS = D / 16, NT = D / 8, ROWS = 16 * WM;
-  extern __shared__ __align__(128) unsigned char smem[];
+// A row tile has 8 NR WM rows: WM groups of 4 / WM warps that share its keys, NR column tiles of 8 rows a warp.
+template <typename T, int D, int NR, int WM>
+__global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
+    paged_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap k_map,
+                      const __grid_constant__ CUtensorMap v_map) {
+  using C = Config<D, NR, WM>;
+  using S = Tile<D>;
+  constexpr int WK = kWarps / WM, NS = D / 16, NT = D / 16, kStages = C::kStages;
+  extern __shared__ unsigned char smem_raw[];
   __shared__ int64_t warp_sums[kThreads / 32], found[2];
-  unsigned char* stages = smem;
-  float4* params = reinterpret_cast<float4*>(smem + kStages * Tile<D>::kStage);          // [2][64]
-  __shared__ float2 join_ml[4 * 16];
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32, n = lane / 4, c = lane % 4;
-  const int wm = warp % WM, wk = warp / WM;
+  __shared__ float2 join_ml[kWarps][8 * NR];
+  __shared__ int given_up;
+  unsigned char* stages = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  float* scales = reinterpret_cast<float*>(stages + kStages * S::kStage);               // [stage][ks, vs][64]
+  uint64_t* full = reinterpret_cast<uint64_t*>(scales + kStages * 2 * kTileKeys);
+  uint64_t* empty = full + kStages;
+  float* join_o = reinterpret_cast<float*>(empty + kStages);                            // [rows][D + 4]
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (tid == 0) {
+    given_up = 0;
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(full + s, 1);
+      mbar_init(empty + s, kWarps);
+    }
+    fence_barrier_init();
+  }
 
   const int64_t list = list_length(a, warp_sums);
   const int share = sharers(a, list);
@@ -229,75 +290,76 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const PagedAttnArg
   Cursor now;
   {
     int64_t within;
-    find(a, first, warp_sums, found, now.b, within);
+    find(a, first, warp_sums, found, now.b, within);   // ends with a barrier of the CTA
     now.tiles = sequence(a, now.b, now.len, now.fresh);
     now.unit = (int)(within / now.tiles);
     now.tile = (int)(within - (int64_t)now.unit * now.tiles);
   }
-  Cursor ahead = now;
-  int64_t to_load = end - first, to_do = end - first;
+  int64_t todo = end - first;
+  int slot = 0;
+  uint32_t phase = 0;
 
-  // lane g < 4: cache row of the first key of group g of the tile to be loaded next, or -1
-  auto lookup = [&](const Cursor& t) -> int64_t {
-    const int64_t at = (int64_t)t.tile * kTileKeys + lane * 16;
-    return lane < 4 && at < t.len + t.fresh ? paged_row(a.p, t.b, t.unit / a.row_tiles, at) : -1;
-  };
-  int64_t base = lookup(ahead);
-  int load_slot = 0;
-  auto load = [&]() {
-    if (to_load > 0) {
-      const uint32_t dst = smem_u32(stages) + load_slot * Tile<D>::kStage;
-      const int total = ahead.len + ahead.fresh, key0 = ahead.tile * kTileKeys;
+  if (warp == kWarps) {
+    // ------------------------------------------------------------------ producer: a lane per page of the tile
+    const int box_rows = min(kTileKeys, 1 << a.p.page_shift), boxes = kTileKeys / box_rows;
+    auto lookup = [&](const Cursor& t) -> int64_t {   // cache row of the lane's first key, or -1
+      const int64_t at = (int64_t)t.tile * kTileKeys + lane * box_rows;
+      return lane < boxes && at < t.len + t.fresh ? paged_row(a.p, t.b, t.unit / a.row_tiles, at) : -1;
+    };
+    int64_t row = lookup(now);
+    for (; todo > 0; --todo) {
+      if (!wait_stage(empty + slot, phase ^ 1, &given_up, a.p.status)) break;
+      const int there = __popc(__ballot_sync(0xffffffffu, row >= 0));
+      const uint32_t bar = smem_u32(full + slot);
+      if (lane == 0)
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar),
+                     "r"(there * box_rows * (2 * D + 8))
+                     : "memory");
+      __syncwarp();
+      if (row >= 0) {
+        const uint32_t k = smem_u32(stages + slot * S::kStage) + lane * box_rows * S::kBox;
+        const uint32_t scale = smem_u32(scales + slot * 2 * kTileKeys + lane * box_rows);
 #pragma unroll
-      for (int i = 0; i < kTileKeys * CH / kThreads; ++i) {
-        const int id = tid + i * kThreads, row = id / CH, ch = id % CH;
-        const int64_t from = __shfl_sync(0xffffffffu, base, row / 16);
-        const bool ok = from >= 0 && key0 + row < total;
-        const int64_t off = ok ? (from + row % 16) * D + ch * 16 : 0;
-        copy_async16(dst + Tile<D>::k_at(row, ch), a.p.k8 + off, ok);
-        copy_async16(dst + Tile<D>::kBytes + Tile<D>::v_at(row, ch), a.p.v8 + off, ok);
+        for (int h = 0; h < S::kHalves; ++h) {
+          tma_load_2d(k + h * (kTileKeys * 128), &k_map, bar, h * 128, (int)row);
+          tma_load_2d(k + S::kBytes + h * (kTileKeys * 128), &v_map, bar, h * 128, (int)row);
+        }
+        bulk_load(scale, a.p.ks + row, box_rows * 4, bar);
+        bulk_load(scale + kTileKeys * 4, a.p.vs + row, box_rows * 4, bar);
       }
-      const int row = tid % kTileKeys;   // a thread below 64 loads both scales of a key and prepares them itself
-      const int64_t from = __shfl_sync(0xffffffffu, base, row / 16);
-      const bool ok = from >= 0 && key0 + row < total;
-      const int64_t off = ok ? from + row % 16 : 0;
-      if (tid < kTileKeys) {
-        copy_async4(dst + 2 * Tile<D>::kBytes + row * 4, a.p.ks + off, ok);
-        copy_async4(dst + 2 * Tile<D>::kBytes + (kTileKeys + row) * 4, a.p.vs + off, ok);
+      if (todo > 1) {
+        advance(a, now);
+        row = lookup(now);
       }
-      load_slot = load_slot + 1 == kStages ? 0 : load_slot + 1;
-      if (--to_load > 0) {
-        advance(a, ahead);
-        base = lookup(ahead);
-      }
+      if (++slot == kStages) slot = 0, phase ^= 1;
     }
-    copy_commit();
-  };
-#pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) load();
+    if (given_up != 0)   // leave no copy in flight behind
+      for (int s = 0; s < kStages; ++s) mbar_drain(full + s, s < slot ? phase : phase ^ 1);
+    return;
+  }
 
-  uint32_t qf[NS][4];
-  float o[NT][4], m[2], l[2], row_scale[2];
-  int token[2], head[2];
+  // -------------------------------------------------------------------- consumers
+  const int n = lane / 4, c = lane % 4, wm = warp % WM, wk = warp / WM;
+  uint32_t qf[NR][NS][2];
+  float o[NR][NT][4], m[NR][2], l[NR][2], row_scale[NR][2];
   bool fresh_unit = true;
-  int slot = 0, parity = 0;
   int segment = 0;                    // 0 for the first row tile that this CTA works on
   int first_tile = now.tile;          // of the row tile, by this CTA
-  for (; to_do > 0; --to_do) {
+  for (; todo > 0; --todo) {
+    const int row0 = now.unit % a.row_tiles * C::kRows + wm * 8 * NR;   // first query row of this warp
+    const int head0 = now.unit / a.row_tiles * a.group;
     if (fresh_unit) {
       fresh_unit = false;
       first_tile = now.tile;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.0f;
-      m[0] = m[1] = -3.402823466e38f;
-      l[0] = l[1] = 0.0f;
-      const int row0 = now.unit % a.row_tiles * ROWS + wm * 16 + n;
+      for (int r = 0; r < NR; ++r) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        token[r] = (row0 + 8 * r) / a.group;
-        head[r] = now.unit / a.row_tiles * a.group + (row0 + 8 * r) % a.group;
-        const bool live = token[r] < now.fresh;
-        const T* src = static_cast<const T*>(a.q) + now.b * a.q_st.b + token[r] * a.q_st.s + head[r] * a.q_st.h;
+        for (int t = 0; t < NT; ++t) o[r][t][0] = o[r][t][1] = o[r][t][2] = o[r][t][3] = 0.0f;
+        m[r][0] = m[r][1] = -3.402823466e38f;
+        l[r][0] = l[r][1] = 0.0f;
+        const int row = row0 + 8 * r + n, token = row / a.group;
+        const bool live = token < now.fresh;
+        const T* src = static_cast<const T*>(a.q) + now.b * a.q_st.b + token * a.q_st.s + (head0 + row % a.group) * a.q_st.h;
         // channels of step s: four consecutive ones, as a word of four codes holds them
         uint2 w[NS];
 #pragma unroll
@@ -305,10 +367,9 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const PagedAttnArg
           const int d = D % 64 == 0 ? (c + 4 * (s / 4)) * 16 + s % 4 * 4 : (c + 4 * (s / 2)) * 8 + s % 2 * 4;
           w[s] = live ? *reinterpret_cast<const uint2*>(src + d) : make_uint2(0, 0);
         }
-        row_scale[r] = 1.0f;
         if constexpr (std::is_same<T, __half>::value) {
 #pragma unroll
-          for (int s = 0; s < NS; ++s) qf[s][r] = w[s].x, qf[s][2 + r] = w[s].y;
+          for (int s = 0; s < NS; ++s) qf[r][s][0] = w[s].x, qf[r][s][1] = w[s].y;
         } else {
           uint32_t top = 0;
 #pragma unroll
@@ -319,248 +380,281 @@ __global__ void __launch_bounds__(kThreads) paged_attn_kernel(const PagedAttnArg
           top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
           // 2^e with e the exponent of the row's largest value (zero, infinite and NaN rows: 1; tiny ones: 2^-100)
           const int e = top == 0 || top >= 0x7f80u ? 127 : max((int)(top >> 7), 27);
-          row_scale[r] = __int_as_float(e << 23);
           const float inverse = __int_as_float((254 - e) << 23);
 #pragma unroll
           for (int s = 0; s < NS; ++s) {
-            qf[s][r] = pack2(__uint_as_float(w[s].x << 16) * inverse, __uint_as_float(w[s].x & 0xffff0000u) * inverse,
-                             __half());
-            qf[s][2 + r] = pack2(__uint_as_float(w[s].y << 16) * inverse,
-                                 __uint_as_float(w[s].y & 0xffff0000u) * inverse, __half());
+            qf[r][s][0] = pack2(__uint_as_float(w[s].x << 16) * inverse, __uint_as_float(w[s].x & 0xffff0000u) * inverse,
+                                __half());
+            qf[r][s][1] = pack2(__uint_as_float(w[s].y << 16) * inverse, __uint_as_float(w[s].y & 0xffff0000u) * inverse,
+                                __half());
           }
+          row_scale[r][0] = __int_as_float(__shfl_sync(0xffffffffu, e, 8 * c) << 23);
+          row_scale[r][1] = __int_as_float(__shfl_sync(0xffffffffu, e, 8 * c + 4) << 23);
         }
       }
     }
 
-    copy_wait<kStages - 2>();
-    unsigned char* stage = stages + slot * Tile<D>::kStage;
+    wait_stage(full + slot, phase, &given_up, a.p.status);   // after a timeout the rest runs through on what is there
+    const unsigned char* kt = stages + slot * S::kStage;
+    unsigned char* vt = stages + slot * S::kStage + S::kBytes;
+    const float* ks = scales + slot * 2 * kTileKeys;
     const int key0 = now.tile * kTileKeys, total = now.len + now.fresh;
-    const bool drafts = key0 + kTileKeys > now.len;   // the tile holds keys that some rows do not see
-    if (drafts) {
-      // a NaN code in a drafted row that its reader does not see must not reach it through 0 * NaN
-#pragma unroll
-      for (int i = 0; i < kTileKeys * CH / kThreads; ++i) {
-        const int id = tid + i * kThreads, row = id / CH, ch = id % CH;
-        if (key0 + row >= now.len) {
-          uint4* at = reinterpret_cast<uint4*>(stage + Tile<D>::kBytes + Tile<D>::v_at(row, ch));
-          uint4 v = *at;
-          v.x &= ~__vcmpeq4(v.x & 0x7f7f7f7fu, 0x7f7f7f7fu);
-          v.y &= ~__vcmpeq4(v.y & 0x7f7f7f7fu, 0x7f7f7f7fu);
-          v.z &= ~__vcmpeq4(v.z & 0x7f7f7f7fu, 0x7f7f7f7fu);
-          v.w &= ~__vcmpeq4(v.w & 0x7f7f7f7fu, 0x7f7f7f7fu);
-          *at = v;
-        }
-      }
-    }
-    bool zeros = false;
-    if (tid < kTileKeys) {
-      // what the rows need of a key: factor of its score, log2 of its V scale, the inverse of that scale, and what the
-      // exponent of a zero row gains over its part in the maximum
-      const float* scales = reinterpret_cast<const float*>(stage + 2 * Tile<D>::kBytes);
-      const float vs = scales[kTileKeys + tid];
-      zeros = vs == 0.0f && key0 + tid < total;
-      params[parity * kTileKeys + tid] =
-          key0 + tid >= total ? make_float4(0.0f, -INFINITY, 0.0f, 0.0f)
-          : zeros             ? make_float4(scales[tid] * a.scale, kZeroLog, 1.0f, -kZeroLog)
-                              : make_float4(scales[tid] * a.scale, __log2f(vs), __fdividef(1.0f, vs), 0.0f);
-    }
-    const bool special = __syncthreads_or(drafts || zeros);
-    load();
 
 #pragma unroll 1
-    for (int g = wk; g < 4; g += WK) {
-      float s[2][4] = {};
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int row = g * 16 + 4 * (n / 2) + 2 * j + n % 2;
-        uint32_t kw[NS];
-        if constexpr (D % 64 == 0) {
-#pragma unroll
-          for (int i = 0; i < NS / 4; ++i) {
-            const uint4 v = *reinterpret_cast<const uint4*>(stage + Tile<D>::k_at(row, c + 4 * i));
-            kw[4 * i] = v.x, kw[4 * i + 1] = v.y, kw[4 * i + 2] = v.z, kw[4 * i + 3] = v.w;
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < NS / 2; ++i) {
-            const uint2 v = *reinterpret_cast<const uint2*>(stage + row * D + (c + 4 * i) * 8);
-            kw[2 * i] = v.x, kw[2 * i + 1] = v.y;
+    for (int g = wk * 16; g < kTileKeys; g += WK * 16) {
+      const bool drafts = key0 + g + 16 > now.len;   // the group holds keys that some rows do not see
+      if (drafts) {
+        // codes behind the last key are anything, and a NaN code of a draft that its reader does not see must not reach
+        // it through 0 * NaN: both are cleared (by each warp that reads the group)
+        for (int i = lane; i < D; i += 32) {
+          const int row = g + i % 16;
+          uint4* at = reinterpret_cast<uint4*>(vt + S::at(row, i / 16 * 16));
+          if (key0 + row >= total) {
+            *at = make_uint4(0, 0, 0, 0);
+          } else if (key0 + row >= now.len) {
+            uint4 v = *at;
+            v.x &= ~__vcmpeq4(v.x & 0x7f7f7f7fu, 0x7f7f7f7fu);
+            v.y &= ~__vcmpeq4(v.y & 0x7f7f7f7fu, 0x7f7f7f7fu);
+            v.z &= ~__vcmpeq4(v.z & 0x7f7f7f7fu, 0x7f7f7f7fu);
+            v.w &= ~__vcmpeq4(v.w & 0x7f7f7f7fu, 0x7f7f7f7fu);
+            *at = v;
           }
         }
+        fence_proxy_async_smem();   // before the stage's next load
+        __syncwarp();
+      }
+      float s[NR][4] = {};          // [2 h + e]: key in slot n + 8 h, row 2c + e of the column tile
+      const int keys[2] = {g + S::slot_key(n), g + S::slot_key(n + 8)};
+      auto step = [&](int i, uint32_t w0, uint32_t w1) {
+        uint32_t x[4];
+        int8_to_f16(w0, x[0], x[2]);
+        int8_to_f16(w1, x[1], x[3]);
 #pragma unroll
-        for (int i = 0; i < NS; ++i) {
-          uint32_t b0, b1;
-          int8_to_f16(kw[i], b0, b1);
-          mma_f16(s[j], qf[i], b0, b1);
+        for (int r = 0; r < NR; ++r) mma_f16(s[r], x, qf[r][i][0], qf[r][i][1]);
+      };
+      if constexpr (D % 64 == 0) {
+#pragma unroll
+        for (int i = 0; i < NS / 4; ++i) {
+          const uint4 u = *reinterpret_cast<const uint4*>(kt + S::at(keys[0], (c + 4 * i) * 16));
+          const uint4 v = *reinterpret_cast<const uint4*>(kt + S::at(keys[1], (c + 4 * i) * 16));
+          step(4 * i, u.x, v.x), step(4 * i + 1, u.y, v.y), step(4 * i + 2, u.z, v.z), step(4 * i + 3, u.w, v.w);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NS / 2; ++i) {
+          const uint2 u = *reinterpret_cast<const uint2*>(kt + S::at(keys[0], (c + 4 * i) * 8));
+          const uint2 v = *reinterpret_cast<const uint2*>(kt + S::at(keys[1], (c + 4 * i) * 8));
+          step(2 * i, u.x, v.x), step(2 * i + 1, u.y, v.y);
         }
       }
-      // s[j][2 r + e]: row n + 8 r, key 4c + 2j + e of the group
-      float4 key[4];
+      // of the lane's two keys: factor of the score, log2 of the V scale, its inverse, and what the exponent of a zero row
+      // gains over its part in the maximum
+      float factor[2], log_v[2], inverse_v[2], gain[2];
+      bool zero = false;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) key[k] = params[parity * kTileKeys + g * 16 + 4 * c + k];
-      float top[2] = {-INFINITY, -INFINITY};
+      for (int h = 0; h < 2; ++h) {
+        const float vs = ks[kTileKeys + keys[h]];
+        factor[h] = ks[keys[h]] * a.scale;
+        log_v[h] = __log2f(vs);
+        inverse_v[h] = __fdividef(1.0f, vs);
+        gain[h] = 0.0f;
+        if (vs == 0.0f) zero = true, log_v[h] = kZeroLog, inverse_v[h] = 1.0f, gain[h] = -kZeroLog;
+      }
+      const bool special = drafts || __any_sync(0xffffffffu, zero);
+      bool more = false;
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int r = 0; r < NR; ++r)
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float& x = s[j][2 * r + e];
-            const float4& y = key[2 * j + e];
-            x = fmaf(x * row_scale[r], y.x, y.y);
+            float& x = s[r][2 * h + e];
+            if constexpr (!std::is_same<T, __half>::value) x *= row_scale[r][e];
+            x = fmaf(x, factor[h], log_v[h]);
             if (drafts) {
-              const int t = key0 + g * 16 + 4 * c + 2 * j + e - now.len;
-              const bool seen = t < 0 || (t < now.fresh && token[r] < now.fresh &&
-                                          (a.mask != nullptr ? a.mask[now.b * a.mask_b + token[r] * a.mask_i + t] != 0
-                                                             : t <= token[r]));
+              const int t = key0 + keys[h] - now.len, token = (row0 + 8 * r + 2 * c + e) / a.group;
+              const bool seen = t < 0 || (t < now.fresh && token < now.fresh &&
+                                          (a.mask != nullptr ? a.mask[now.b * a.mask_b + token * a.mask_i + t] != 0
+                                                             : t <= token));
               if (!seen) x = -INFINITY;
             }
-            top[r] = fmaxf(top[r], x);
+            more |= x > m[r][e] + 8.0f;
+          }
+      if (__any_sync(0xffffffffu, more)) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+          float keep[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float top = fmaxf(s[r][e], s[r][2 + e]);
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+            const float next = top > m[r][e] + 8.0f ? top : m[r][e];
+            keep[e] = next == m[r][e] ? 1.0f : fast_exp2(m[r][e] - next);
+            m[r][e] = next;
+            l[r][e] *= keep[e];
           }
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-      }
-      if (__any_sync(0xffffffffu, top[0] > m[0] + 8.0f || top[1] > m[1] + 8.0f)) {
-        float keep[2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float next = top[r] > m[r] + 8.0f ? top[r] : m[r];
-          keep[r] = next == m[r] ? 1.0f : fast_exp2(m[r] - next);
-          m[r] = next;
-          l[r] *= keep[r];
+          for (int t = 0; t < NT; ++t) o[r][t][0] *= keep[0], o[r][t][1] *= keep[1], o[r][t][2] *= keep[0], o[r][t][3] *= keep[1];
         }
-#pragma unroll
-        for (int t = 0; t < NT; ++t) o[t][0] *= keep[0], o[t][1] *= keep[0], o[t][2] *= keep[1], o[t][3] *= keep[1];
       }
-      uint32_t pf[4];
+      uint32_t pf[NR][2];
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int r = 0; r < NR; ++r)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
+        for (int h = 0; h < 2; ++h) {
           float p[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float x = s[j][2 * r + e];
-            p[e] = fast_exp2(special ? x - m[r] + key[2 * j + e].w : x - m[r]);
+            const float x = s[r][2 * h + e];
+            p[e] = fast_exp2(special ? x - m[r][e] + gain[h] : x - m[r][e]);
             // an unseen key's inverse scale may be NaN
-            if (!special || x != -INFINITY) l[r] = fmaf(p[e], key[2 * j + e].z, l[r]);
+            if (!special || x != -INFINITY) l[r][e] = fmaf(p[e], inverse_v[h], l[r][e]);
           }
-          pf[2 * j + r] = pack_weights(p[0], p[1]);
+          pf[r][h] = transposed(pack_weights(p[0], p[1]));
         }
-      const unsigned char* vt = stage + Tile<D>::kBytes;
+      // four keys a lane; a word of four channels of each is two output tiles
+      auto product = [&](int i, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
 #pragma unroll
-      for (int i = 0; i < NT / 4; ++i) {   // four output tiles at a time: a word of four channels of each of four keys
-        uint32_t w[4];
+        for (int x = 0; x < 2; ++x) {
+          const uint32_t u = __byte_perm(w0, w1, x ? 0x7362 : 0x5140), v = __byte_perm(w2, w3, x ? 0x7362 : 0x5140);
+          const uint32_t f[4] = {e4m3_to_f16((uint16_t)u), e4m3_to_f16((uint16_t)(u >> 16)), e4m3_to_f16((uint16_t)v),
+                                 e4m3_to_f16((uint16_t)(v >> 16))};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int row = g * 16 + 4 * c + k;
-          const int byte = D == 256 ? n * 16 + i % 4 * 4 + i / 4 * 128 : n * (D / 8) + i * 4;
-          w[k] = *reinterpret_cast<const uint32_t*>(vt + Tile<D>::v_at(row, byte / 16) + byte % 16);
+          for (int r = 0; r < NR; ++r) mma_f16(o[r][2 * i + x], f, pf[r][0], pf[r][1]);
         }
-        const uint32_t x01 = __byte_perm(w[0], w[1], 0x5140), y01 = __byte_perm(w[0], w[1], 0x7362);
-        const uint32_t x23 = __byte_perm(w[2], w[3], 0x5140), y23 = __byte_perm(w[2], w[3], 0x7362);
-        mma_f16(o[4 * i], pf, e4m3_to_f16((uint16_t)x01), e4m3_to_f16((uint16_t)x23));
-        mma_f16(o[4 * i + 1], pf, e4m3_to_f16((uint16_t)(x01 >> 16)), e4m3_to_f16((uint16_t)(x23 >> 16)));
-        mma_f16(o[4 * i + 2], pf, e4m3_to_f16((uint16_t)y01), e4m3_to_f16((uint16_t)y23));
-        mma_f16(o[4 * i + 3], pf, e4m3_to_f16((uint16_t)(y01 >> 16)), e4m3_to_f16((uint16_t)(y23 >> 16)));
+      };
+      int vkeys[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) vkeys[k] = g + S::slot_key(2 * c + k % 2 + k / 2 * 8);
+      if constexpr (S::kWide) {
+#pragma unroll
+        for (int i = 0; i < S::kHalves; ++i) {
+          uint4 v[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            v[k] = *reinterpret_cast<const uint4*>(vt + S::at(vkeys[k], i * 128 + S::first_channel(n)));
+          product(4 * i, v[0].x, v[1].x, v[2].x, v[3].x), product(4 * i + 1, v[0].y, v[1].y, v[2].y, v[3].y);
+          product(4 * i + 2, v[0].z, v[1].z, v[2].z, v[3].z), product(4 * i + 3, v[0].w, v[1].w, v[2].w, v[3].w);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          uint32_t v[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            v[k] = *reinterpret_cast<const uint32_t*>(vt + S::at(vkeys[k], S::first_channel(n) + 4 * i));
+          product(i, v[0], v[1], v[2], v[3]);
+        }
       }
     }
-    slot = slot + 1 == kStages ? 0 : slot + 1;
-    parity ^= 1;
+    __syncwarp();
+    if (lane == 0) arrive(empty + slot);
+    if (++slot == kStages) slot = 0, phase ^= 1;
 
     const bool last_tile = now.tile + 1 == now.tiles;
-    if (last_tile || to_do == 1) {
+    if (last_tile || todo == 1) {
       // the row tile ends here, or this CTA's part of it does
       const bool whole = last_tile && first_tile == 0;
-      const int64_t part = (2 * (int64_t)blockIdx.x + (segment > 0)) * ROWS;
+      const int64_t part = (2 * (int64_t)blockIdx.x + (segment > 0)) * C::kRows;
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-      }
-      float factor[2] = {1.0f, 1.0f};
-      if constexpr (WK > 1) {
-        // the warps of a row tile join in their order, through the stage that they have just read
-        static_assert(WM == 4 || ROWS * (D + 4) * 4 <= Tile<D>::kStage, "a joined row tile must fit a stage");
-        float* join_o = reinterpret_cast<float*>(stage);   // [ROWS][D + 4]
-        if (c == 0) join_ml[warp * 16 + n] = make_float2(m[0], l[0]), join_ml[warp * 16 + n + 8] = make_float2(m[1], l[1]);
-        __syncthreads();
+      for (int r = 0; r < NR; ++r)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          float top = -3.402823466e38f, sum = 0.0f;
-#pragma unroll
-          for (int w = 0; w < WK; ++w) top = fmaxf(top, join_ml[(w * WM + wm) * 16 + n + 8 * r].x);
-#pragma unroll
-          for (int w = 0; w < WK; ++w) {
-            const float2 x = join_ml[(w * WM + wm) * 16 + n + 8 * r];
-            sum += fast_exp2(x.x - top) * x.y;
-          }
-          factor[r] = fast_exp2(m[r] - top);
-          m[r] = top, l[r] = sum;
+        for (int e = 0; e < 2; ++e) {
+          l[r][e] += __shfl_xor_sync(0xffffffffu, l[r][e], 4);
+          l[r][e] += __shfl_xor_sync(0xffffffffu, l[r][e], 8);
+          l[r][e] += __shfl_xor_sync(0xffffffffu, l[r][e], 16);
         }
+      if constexpr (WK > 1) {
+        // the warps of a row tile join through shared memory, in their order
+        auto consumers_sync = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
+        if (n == 0) {
+#pragma unroll
+          for (int r = 0; r < NR; ++r)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) join_ml[warp][8 * r + 2 * c + e] = make_float2(m[r][e], l[r][e]);
+        }
+        consumers_sync();
+        float factor[NR][2];
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float top = -3.402823466e38f, sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < WK; ++w) top = fmaxf(top, join_ml[w * WM + wm][8 * r + 2 * c + e].x);
+#pragma unroll
+            for (int w = 0; w < WK; ++w) {
+              const float2 x = join_ml[w * WM + wm][8 * r + 2 * c + e];
+              sum += fast_exp2(x.x - top) * x.y;
+            }
+            factor[r][e] = fast_exp2(m[r][e] - top);
+            m[r][e] = top, l[r][e] = sum;
+          }
 #pragma unroll 1
         for (int w = 0; w < WK; ++w) {
           if (w == wk) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+            for (int r = 0; r < NR; ++r)
 #pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                float* at = join_o + (wm * 16 + n + 8 * (x / 2)) * (D + 4) + channel<D>(2 * c + x % 2, t);
-                const float y = o[t][x] * factor[x / 2];
-                o[t][x] = w == 0 ? y : *at + y;
-                if (w < WK - 1) *at = o[t][x];
-              }
+              for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  // channels 2t and 2t + 1 of the lane lie next to each other
+                  float2* at = reinterpret_cast<float2*>(join_o + (wm * 8 * NR + 8 * r + 2 * c + e) * (D + 4) +
+                                                         S::channel(n, t, 0));
+                  float2 x = make_float2(o[r][t][e] * factor[r][e], o[r][t][2 + e] * factor[r][e]);
+                  if (w > 0) x.x += at->x, x.y += at->y;
+                  if (w < WK - 1) *at = x;
+                  o[r][t][e] = x.x, o[r][t][2 + e] = x.y;
+                }
           }
-          __syncthreads();
+          consumers_sync();
         }
       }
       if (wk == WK - 1) {
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const int row = now.unit % a.row_tiles * ROWS + wm * 16 + n + 8 * r;
-          if (row >= a.T * a.group) continue;
-          const bool live = token[r] < now.fresh;
-          if (whole) {
-            T* dst = static_cast<T*>(a.out) + now.b * a.out_st.b + token[r] * a.out_st.s + head[r] * a.out_st.h;
-            const float inverse = !live || l[r] == 0.0f ? 0.0f : 1.0f / l[r];
+        for (int r = 0; r < NR; ++r)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+          for (int e = 0; e < 2; ++e) {
+            const int row = row0 + 8 * r + 2 * c + e, token = row / a.group, head = head0 + row % a.group;
+            if (row >= a.T * a.group) continue;
+            const bool live = token < now.fresh;
+            if (whole) {
+              T* dst = static_cast<T*>(a.out) + now.b * a.out_st.b + token * a.out_st.s + head * a.out_st.h;
+              const float inverse = !live || l[r][e] == 0.0f ? 0.0f : 1.0f / l[r][e];
 #pragma unroll
-              for (int t = 0; t < NT; t += 4)
-                *reinterpret_cast<uint2*>(dst + channel<D>(2 * c + e, t)) =
-                    live ? make_uint2(pack2(o[t][2 * r + e] * inverse, o[t + 1][2 * r + e] * inverse, T()),
-                                      pack2(o[t + 2][2 * r + e] * inverse, o[t + 3][2 * r + e] * inverse, T()))
+              for (int t = 0; t < NT; t += 2)
+                *reinterpret_cast<uint2*>(dst + S::channel(n, t, 0)) =
+                    live ? make_uint2(pack2(o[r][t][e] * inverse, o[r][t][2 + e] * inverse, T()),
+                                      pack2(o[r][t + 1][e] * inverse, o[r][t + 1][2 + e] * inverse, T()))
                          : make_uint2(0, 0);
-            if (a.lse != nullptr && c == 0)
-              a.lse[((int64_t)now.b * a.H + head[r]) * a.T + token[r]] =
-                  !live || l[r] == 0.0f ? -INFINITY : (m[r] + log2f(l[r])) * 0.69314718055994531f;
-          } else {
-            const int64_t at = part + wm * 16 + n + 8 * r;
+              if (a.lse != nullptr && n == 0)
+                a.lse[((int64_t)now.b * a.H + head) * a.T + token] =
+                    !live || l[r][e] == 0.0f ? -INFINITY : (m[r][e] + log2f(l[r][e])) * 0.69314718055994531f;
+            } else {
+              const int64_t at = part + wm * 8 * NR + 8 * r + 2 * c + e;
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-              for (int t = 0; t < NT; t += 4)
-                *reinterpret_cast<float4*>(a.part_o + at * D + channel<D>(2 * c + e, t)) = make_float4(
-                    o[t][2 * r + e], o[t + 1][2 * r + e], o[t + 2][2 * r + e], o[t + 3][2 * r + e]);
-            if (c == 0) a.part_ml[at] = make_float2(m[r], l[r]);
+              for (int t = 0; t < NT; t += 2)
+                *reinterpret_cast<float4*>(a.part_o + at * D + S::channel(n, t, 0)) =
+                    make_float4(o[r][t][e], o[r][t][2 + e], o[r][t + 1][e], o[r][t + 1][2 + e]);
+              if (n == 0) a.part_ml[at] = make_float2(m[r][e], l[r][e]);
+            }
           }
-        }
       }
       ++segment;
       fresh_unit = true;
     }
-    if (to_do > 1) advance(a, now);
+    if (todo > 1) advance(a, now);
   }
-  copy_wait<0>();
 }
 
 // Joins the partial rows of the row tiles that fell to several CTAs, and writes the rows that see nothing at all.  A warp
 // takes a row; the CTAs of a row tile are joined in the order of its keys.
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) paged_join_kernel(const PagedAttnArgs a, int tile_rows, int blocks_per_unit) {
-  __shared__ int64_t warp_sums[kThreads / 32];
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAttnArgs a, int tile_rows, int blocks_per_unit) {
+  __shared__ int64_t warp_sums[kJoinThreads / 32];
   const int64_t id = blockIdx.x / blocks_per_unit;
   const int per = a.p.Hkv * a.row_tiles, b = (int)(id / per), unit = (int)(id - (int64_t)b * per);
   int len, fresh;
@@ -568,15 +662,15 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const PagedAttnArg
   int64_t mine = 0, before = 0;
   {
     int x, y;
-    for (int s = threadIdx.x; s < a.B; s += kThreads) {
+    for (int s = threadIdx.x; s < a.B; s += kJoinThreads) {
       const int t = sequence(a, s, x, y);
       mine += t;
       if (s < b) before += t;
     }
   }
   int64_t list, start;
-  scan_before(mine, warp_sums, list);
-  scan_before(before, warp_sums, start);
+  scan_before<kJoinThreads>(mine, warp_sums, list);
+  scan_before<kJoinThreads>(before, warp_sums, start);
   list *= per;
   start = start * per + (int64_t)unit * tiles;
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -589,8 +683,8 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const PagedAttnArg
     slot = (int64_t)c0 * list / share < start ? 1 : 0;          // not the first row tile of CTA c0
   }
   const int lane = threadIdx.x % 32;
-  for (int row = blockIdx.x % blocks_per_unit * (kThreads / 32) + threadIdx.x / 32; row < tile_rows;
-       row += blocks_per_unit * (kThreads / 32)) {
+  for (int row = blockIdx.x % blocks_per_unit * (kJoinThreads / 32) + threadIdx.x / 32; row < tile_rows;
+       row += blocks_per_unit * (kJoinThreads / 32)) {
     const int r = unit % a.row_tiles * tile_rows + row;
     if (r >= a.T * a.group) break;
     const int token = r / a.group, head = unit / a.row_tiles * a.group + r % a.group;
@@ -635,8 +729,17 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const PagedAttnArg
   }
 }
 
-// Row tiles of 16, 32 or 64 rows: the smallest that holds the rows of a kv head, 64 at the most.
-static int row_warps(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+// Row tiles: the smallest that hold the rows of a kv head, 64 rows (D 256: 32) at the most.  Columns come in eights, so a
+// single token of up to eight heads a group takes one column tile; two a warp share the converted codes, four do not fit
+// the registers, and D 256 has room for one.
+struct Shape {
+  int nr, wm;
+};
+static Shape row_tile(int64_t rows, int D) {
+  if (rows <= 8) return {1, 1};
+  if (D == 256) return rows <= 16 ? Shape{1, 2} : Shape{1, 4};
+  return rows <= 16 ? Shape{2, 1} : rows <= 32 ? Shape{2, 2} : Shape{2, 4};
+}
 
 static int sm_count() {
   int dev = 0, n = 0;
@@ -645,39 +748,76 @@ static int sm_count() {
   return n;
 }
 
-static int shared_ctas(int D) { return sm_count() * (D == 256 ? 2 : 3); }
+static int shared_ctas(int D, Shape s) { return sm_count() * (D * s.nr <= 128 ? 3 : 2); }
 
-template <typename T, int D, int WM>
+// The codes as [rows, D] bytes; a box is the rows of a page that a tile of keys takes, 128 bytes of each (or all of them).
+template <int D>
+static bool code_map(CUtensorMap* map, const void* base, uint64_t rows, int page_size) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) {
+    set_error("cuTensorMapEncodeTiled is not available from the CUDA driver");
+    return false;
+  }
+  const cuuint64_t dims[2] = {(cuuint64_t)D, rows}, strides[1] = {(cuuint64_t)D};
+  const cuuint32_t box[2] = {(cuuint32_t)Tile<D>::kBox, (cuuint32_t)std::min(page_size, kTileKeys)}, steps[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, steps,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        Tile<D>::kWide ? CU_TENSOR_MAP_SWIZZLE_128B
+                                       : D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r == CUDA_SUCCESS) return true;
+  set_error("cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return false;
+}
+
+template <typename T, int D, int NR, int WM>
 static int launch_paged_attn(const PagedAttnArgs& a, cudaStream_t st) {
-  constexpr int kSmem = smem_bytes<D>();
+  using C = Config<D, NR, WM>;
+  CUtensorMap k_map, v_map;
+  const uint64_t rows = (uint64_t)a.p.num_pages * a.p.Hkv << a.p.page_shift;
+  if (!code_map<D>(&k_map, a.p.k8, rows, 1 << a.p.page_shift) || !code_map<D>(&v_map, a.p.v8, rows, 1 << a.p.page_shift))
+    return SAGE_ERR_LAUNCH;
   static std::atomic<uint64_t> prepared{0};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev >= 64 || !(prepared.load() >> dev & 1))) {
-    e = cudaFuncSetAttribute(paged_attn_kernel<T, D, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    e = cudaFuncSetAttribute(paged_attn_kernel<T, D, NR, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
     if (e == cudaSuccess && dev < 64) prepared.fetch_or(uint64_t(1) << dev);
   }
   if (e == cudaSuccess) {
-    paged_attn_kernel<T, D, WM><<<a.ctas, kThreads, kSmem, st>>>(a);
+    paged_attn_kernel<T, D, NR, WM><<<a.ctas, kThreads, C::kSmem, st>>>(a, k_map, v_map);
     e = cudaGetLastError();
   }
   if (e == cudaSuccess) {
-    const int rows = std::min(16 * WM, a.T * a.group);
-    const int blocks = (rows + kThreads / 32 - 1) / (kThreads / 32);
+    const int used = std::min(C::kRows, a.T * a.group);
+    const int blocks = (used + kJoinThreads / 32 - 1) / (kJoinThreads / 32);
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(a.B * a.p.Hkv * a.row_tiles * blocks));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(kJoinThreads);
     cfg.stream = st;
     cudaLaunchAttribute attr{};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, paged_join_kernel<T, D>, a, 16 * WM, blocks);
+    e = cudaLaunchKernelEx(&cfg, paged_join_kernel<T, D>, a, C::kRows, blocks);
   }
   if (e == cudaSuccess) return SAGE_OK;
   set_error("paged attention: %s", cudaGetErrorString(e));
   return SAGE_ERR_LAUNCH;
+}
+
+template <typename T, int D>
+static int launch_paged_attn(const PagedAttnArgs& a, Shape s, cudaStream_t st) {
+  if constexpr (D == 256)
+    return s.wm == 1   ? launch_paged_attn<T, D, 1, 1>(a, st)
+           : s.wm == 2 ? launch_paged_attn<T, D, 1, 2>(a, st)
+                       : launch_paged_attn<T, D, 1, 4>(a, st);
+  else
+    return s.nr == 1   ? launch_paged_attn<T, D, 1, 1>(a, st)
+           : s.wm == 1 ? launch_paged_attn<T, D, 2, 1>(a, st)
+           : s.wm == 2 ? launch_paged_attn<T, D, 2, 2>(a, st)
+                       : launch_paged_attn<T, D, 2, 4>(a, st);
 }
 
 }  // namespace sage
@@ -686,8 +826,8 @@ using namespace sage;
 
 extern "C" size_t sage_paged_attention_workspace_bytes(int B, int T, int H, int Hkv, int D) {
   if (B <= 0 || T <= 0 || H <= 0 || Hkv <= 0 || H % Hkv != 0 || sage_qk_row_bytes(D) == 0) return 0;
-  const int64_t rows = (int64_t)T * (H / Hkv);
-  const size_t slots = (size_t)2 * shared_ctas(D) * 16 * row_warps(rows > 64 ? 64 : (int)rows);
+  const Shape s = row_tile((int64_t)T * (H / Hkv), D);
+  const size_t slots = (size_t)2 * shared_ctas(D, s) * 8 * s.nr * s.wm;
   return slots * (D * sizeof(float) + sizeof(float2));
 }
 
@@ -716,6 +856,14 @@ extern "C" int sage_paged_attention(const void* q, int dtype, int B, int T, int 
     set_error("%d pages of %d keys: positions must fit 32 bits", max_pages, page_size);
     rc = SAGE_ERR_UNSUPPORTED;
   }
+  if (rc == SAGE_OK && (((reinterpret_cast<uintptr_t>(ks) | reinterpret_cast<uintptr_t>(vs)) & 15u) != 0)) {
+    set_error("ks and vs must be 16-byte aligned");
+    rc = SAGE_ERR_INVALID;
+  }
+  if (rc == SAGE_OK && (int64_t)num_pages * page_size > (int64_t)INT_MAX / Hkv) {
+    set_error("%d pages of %d keys and %d heads: cache rows must fit 32 bits", num_pages, page_size, Hkv);
+    rc = SAGE_ERR_UNSUPPORTED;
+  }
   if (rc == SAGE_OK && (int64_t)B * T * H > INT_MAX / 64) {
     set_error("%d sequences of %d tokens and %d heads are too many for one call", B, T, H);
     rc = SAGE_ERR_UNSUPPORTED;
@@ -731,19 +879,16 @@ extern "C" int sage_paged_attention(const void* q, int dtype, int B, int T, int 
   a.lse = lse, a.counts = counts;
   a.mask = mask, a.mask_b = mask_b, a.mask_i = mask_i;
   a.B = B, a.T = T, a.H = H, a.group = H / Hkv;
-  const int rows = T * a.group, wm = row_warps(rows);
-  a.row_tiles = (rows + 16 * wm - 1) / (16 * wm);
-  a.ctas = shared_ctas(D);
+  const Shape shape = row_tile((int64_t)T * a.group, D);
+  const int tile_rows = 8 * shape.nr * shape.wm;
+  a.row_tiles = (T * a.group + tile_rows - 1) / tile_rows;
+  a.ctas = shared_ctas(D, shape);
   a.scale = (float)((sm_scale > 0.0 ? sm_scale : 1.0 / std::sqrt((double)D)) * 1.4426950408889634);
   a.part_o = static_cast<float*>(workspace);
-  a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)2 * a.ctas * 16 * wm * D);
+  a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)2 * a.ctas * tile_rows * D);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return by_head_dim(D, [&](auto d) {
     constexpr int kD = decltype(d)::value;
-    if (dtype == SAGE_BF16)
-      return wm == 1 ? launch_paged_attn<__nv_bfloat16, kD, 1>(a, st)
-                     : wm == 2 ? launch_paged_attn<__nv_bfloat16, kD, 2>(a, st) : launch_paged_attn<__nv_bfloat16, kD, 4>(a, st);
-    return wm == 1 ? launch_paged_attn<__half, kD, 1>(a, st)
-                   : wm == 2 ? launch_paged_attn<__half, kD, 2>(a, st) : launch_paged_attn<__half, kD, 4>(a, st);
+    return dtype == SAGE_BF16 ? launch_paged_attn<__nv_bfloat16, kD>(a, shape, st) : launch_paged_attn<__half, kD>(a, shape, st);
   });
 }
