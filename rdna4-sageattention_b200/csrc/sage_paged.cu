@@ -61,11 +61,9 @@ template <typename T, int D>
 __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
   constexpr int LPR = D == 64 ? 8 : D == 256 ? 32 : 16;
   const int lane = threadIdx.x % LPR;
-  const int64_t row = (int64_t)blockIdx.x * (256 / LPR) + threadIdx.x / LPR;
-  const int64_t bh = row / a.S;
-  const int s = (int)(row - bh * a.S);
-  const int b = (int)(bh / a.p.Hkv), h = (int)(bh - (int64_t)b * a.p.Hkv);
-  bool live = b < a.B;
+  const uint32_t row = blockIdx.x * (256u / LPR) + threadIdx.x / LPR;   // token and head of the sequence
+  const int h = (int)(row / a.S), s = (int)(row - h * (uint32_t)a.S), b = blockIdx.y;
+  bool live = h < a.p.Hkv;
   int64_t dst = -1;
   if (live) {
     const int n = a.counts != nullptr ? a.counts[b] : a.S;
@@ -132,15 +130,10 @@ struct ReadArgs {
 template <typename T, int D>
 __global__ void __launch_bounds__(256) read_kernel(const ReadArgs a) {
   constexpr int LPR = D / 16;
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int c = (int)(id % LPR) * 16;
-  int64_t row = id / LPR;
-  const int h = (int)(row % a.p.Hkv);
-  row /= a.p.Hkv;
-  const int s = (int)(row % a.S);
-  const int64_t b64 = row / a.S;
-  if (b64 >= a.B) return;
-  const int b = (int)b64;
+  const uint32_t id = blockIdx.x * 256u + threadIdx.x, row = id / LPR;   // token and head of the sequence
+  const int c = (int)(id % LPR) * 16, b = blockIdx.y;
+  const int s = (int)(row / a.p.Hkv), h = (int)(row - s * (uint32_t)a.p.Hkv);
+  if (s >= a.S) return;
   const int n = a.p.lens[b];
   if (n < 0 || n > (int64_t)a.p.max_pages << a.p.page_shift) raise_invalid(a.p);
   const int64_t src = s < n ? paged_row(a.p, b, h, s) : -1;
@@ -243,17 +236,18 @@ int sage_paged_append(const void* k, const void* v, int dtype, int B, int S, int
   a.counts = counts;
   a.B = B, a.S = S;
   const int per_block = 256 / (D == 64 ? 8 : D == 256 ? 32 : 16);
-  const int64_t blocks = ((int64_t)B * S * Hkv + per_block - 1) / per_block;
-  if (blocks > INT_MAX) {
-    set_error("append: %lld rows are too many for one call", (long long)B * S * Hkv);
+  const int64_t blocks = ((int64_t)S * Hkv + per_block - 1) / per_block;
+  if (blocks > (1 << 23) || B > 65535) {   // 32-bit thread numbers, grid limit
+    set_error("append: %d sequences of %d tokens and %d heads are too many for one call", B, S, Hkv);
     return SAGE_ERR_UNSUPPORTED;
   }
+  const dim3 grid((unsigned)blocks, (unsigned)B);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return by_head_dim(D, [&](auto d) {
     if (dtype == SAGE_BF16)
-      append_kernel<__nv_bfloat16, decltype(d)::value><<<(int)blocks, 256, 0, st>>>(a);
+      append_kernel<__nv_bfloat16, decltype(d)::value><<<grid, 256, 0, st>>>(a);
     else
-      append_kernel<__half, decltype(d)::value><<<(int)blocks, 256, 0, st>>>(a);
+      append_kernel<__half, decltype(d)::value><<<grid, 256, 0, st>>>(a);
     return launch_result("append");
   });
 }
@@ -276,17 +270,18 @@ int sage_paged_read(const int8_t* k8, const float* ks, const uint8_t* v8, const 
   a.out[0] = k, a.out[1] = v;
   a.st[0] = {ksb, kss, ksh}, a.st[1] = {vsb, vss, vsh};
   a.B = B, a.S = S;
-  const int64_t blocks = ((int64_t)B * S * Hkv * (D / 16) + 255) / 256;
-  if (blocks > INT_MAX) {
-    set_error("read: %lld rows are too many for one call", (long long)B * S * Hkv);
+  const int64_t blocks = ((int64_t)S * Hkv * (D / 16) + 255) / 256;
+  if (blocks > (1 << 23) || B > 65535) {   // 32-bit thread numbers, grid limit
+    set_error("read: %d sequences of %d tokens and %d heads are too many for one call", B, S, Hkv);
     return SAGE_ERR_UNSUPPORTED;
   }
+  const dim3 grid((unsigned)blocks, (unsigned)B);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return by_head_dim(D, [&](auto d) {
     if (dtype == SAGE_BF16)
-      read_kernel<__nv_bfloat16, decltype(d)::value><<<(int)blocks, 256, 0, st>>>(a);
+      read_kernel<__nv_bfloat16, decltype(d)::value><<<grid, 256, 0, st>>>(a);
     else
-      read_kernel<__half, decltype(d)::value><<<(int)blocks, 256, 0, st>>>(a);
+      read_kernel<__half, decltype(d)::value><<<grid, 256, 0, st>>>(a);
     return launch_result("read");
   });
 }

@@ -7,6 +7,8 @@
 // The angle is reduced in integers: a frequency is held in turns (w / 2 pi) as a 64-bit fixed-point fraction, so the
 // fraction of a turn at position p is the low 64 bits of p * turns, exact for any position (a product in 32-bit
 // floats is off by 0.06 radians at p = 10^6).  Its upper 32 bits go to sincospi.
+#include <algorithm>
+
 #include "../../include/sage_b200.h"
 #include "sage_internal.h"
 #include "sage_ptx.cuh"
@@ -19,7 +21,7 @@ struct RotaryArgs {
   void* out[2];
   Strides3 in_st[2], out_st[2];
   int heads[2];
-  int S, D, R, interleaved;
+  int S, D, R;
   int64_t tokens;      // B * S
   const void* positions;
   int pos64;
@@ -27,59 +29,81 @@ struct RotaryArgs {
   const uint64_t* turns;
   float magnitude;     // factor of both cosine and sine
   float sine_sign;     // -1 in the gradient
-  int slices;          // threads that share the heads of one token
 };
 
-// One thread holds 16 channels (8 pairs) of one token and walks over the heads, so each sine is computed once
-// for all of its heads.
-template <typename T>
+// One thread holds 16 channels (8 pairs) of one token and walks over the heads, so each sine is computed once for all of
+// its heads; kBatch heads are loaded before the first is turned.
+constexpr int kBatch = 4;
+
+template <typename T, bool INTERLEAVED>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
-  const int units = a.D / 16;
-  const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int u = (int)(id % units);
-  const int64_t rest = id / units;
-  const int64_t token = rest % a.tokens;
-  const int slice = (int)(rest / a.tokens);
-  if (slice >= a.slices) return;
-  const int64_t b = token / a.S, s = token - b * a.S;
-  const bool turned = u * 16 < a.R;
-  const int c0 = turned && !a.interleaved ? u * 8 : u * 16;          // first channel of each 8-channel part
-  const int c1 = turned && !a.interleaved ? a.R / 2 + u * 8 : u * 16 + 8;
-  float cs[8], sn[8];
-  if (turned) {
-    const int64_t at = b * a.pos_b + s * a.pos_s;
-    const uint64_t p = a.pos64 ? (uint64_t) static_cast<const int64_t*>(a.positions)[at]
-                               : (uint64_t)(int64_t) static_cast<const int*>(a.positions)[at];
+  const uint32_t units = a.D / 16;
+  const uint32_t id = blockIdx.x * 256u + threadIdx.x;
+  const uint32_t u = id % units, token = id / units;
+  if (token >= (uint32_t)a.tokens) return;
+  const uint32_t b = token / a.S, s = token - b * a.S;
+  const bool turned = u * 16 < (uint32_t)a.R;
+  const int c0 = turned && !INTERLEAVED ? u * 8 : u * 16;          // first channel of each 8-channel part
+  const int c1 = turned && !INTERLEAVED ? a.R / 2 + u * 8 : u * 16 + 8;
+  const T* src[2];
+  T* dst[2];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint64_t turn = p * a.turns[u * 8 + e];
-      const int half_turns = (int)(uint32_t)((turn + 0x80000000ull) >> 32);   // units of 2^-31 half turns
-      sincospif((float)half_turns * 0x1p-31f, &sn[e], &cs[e]);
-      cs[e] *= a.magnitude;
-      sn[e] *= a.magnitude * a.sine_sign;
-    }
+  for (int w = 0; w < 2; ++w) {
+    src[w] = static_cast<const T*>(a.in[w]) + b * a.in_st[w].b + s * a.in_st[w].s;
+    dst[w] = static_cast<T*>(a.out[w]) + b * a.out_st[w].b + s * a.out_st[w].s;
   }
-  const int total = a.heads[0] + a.heads[1];
-  for (int h = slice; h < total; h += a.slices) {
-    const int w = h >= a.heads[0];
-    const int hh = h - (w ? a.heads[0] : 0);
-    const T* src = static_cast<const T*>(a.in[w]) + b * a.in_st[w].b + s * a.in_st[w].s + hh * a.in_st[w].h;
-    T* dst = static_cast<T*>(a.out[w]) + b * a.out_st[w].b + s * a.out_st[w].s + hh * a.out_st[w].h;
-    float x[16];
-    load8(src + c0, x);
-    load8(src + c1, x + 8);
-    if (turned) {
+  const int total = a.heads[0] + a.heads[1], step = gridDim.y * kBatch;
+  float cs[8], sn[8];
+  for (int h0 = blockIdx.y * kBatch; h0 < total; h0 += step) {
+    uint4 x[kBatch][2];
+    int64_t at[kBatch];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float& p1 = a.interleaved ? x[2 * e] : x[e];
-        float& p2 = a.interleaved ? x[2 * e + 1] : x[8 + e];
-        const float x1 = p1, x2 = p2;
-        p1 = x1 * cs[e] - x2 * sn[e];
-        p2 = x2 * cs[e] + x1 * sn[e];
+    for (int i = 0; i < kBatch; ++i) {
+      const int h = h0 + i, w = h >= a.heads[0], hh = h - (w ? a.heads[0] : 0);
+      at[i] = hh * a.out_st[w].h;
+      if (h < total) {
+        const T* p = src[w] + hh * a.in_st[w].h;
+        x[i][0] = *reinterpret_cast<const uint4*>(p + c0);
+        x[i][1] = *reinterpret_cast<const uint4*>(p + c1);
       }
     }
-    store8(dst + c0, x);
-    store8(dst + c1, x + 8);
+    if (h0 == (int)blockIdx.y * kBatch && turned) {   // beside the first loads
+      const int64_t place = b * a.pos_b + s * a.pos_s;
+      const uint64_t pos = a.pos64 ? (uint64_t) static_cast<const int64_t*>(a.positions)[place]
+                                   : (uint64_t)(int64_t) static_cast<const int*>(a.positions)[place];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint64_t turn = pos * a.turns[u * 8 + e];
+        const int half_turns = (int)(uint32_t)((turn + 0x80000000ull) >> 32);   // units of 2^-31 half turns
+        sincospif((float)half_turns * 0x1p-31f, &sn[e], &cs[e]);
+        cs[e] *= a.magnitude;
+        sn[e] *= a.magnitude * a.sine_sign;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int h = h0 + i;
+      if (h >= total) break;
+      T* p = dst[h >= a.heads[0]] + at[i];
+      if (turned) {
+        float y[2][8];
+        unpack8(x[i][0], y[0], T());
+        unpack8(x[i][1], y[1], T());
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float& p1 = INTERLEAVED ? y[e / 4][2 * e % 8] : y[0][e];
+          float& p2 = INTERLEAVED ? y[e / 4][2 * e % 8 + 1] : y[1][e];
+          const float x1 = p1, x2 = p2;
+          p1 = x1 * cs[e] - x2 * sn[e];
+          p2 = x2 * cs[e] + x1 * sn[e];
+        }
+        store8(p + c0, y[0]);
+        store8(p + c1, y[1]);
+      } else {
+        *reinterpret_cast<uint4*>(p + c0) = x[i][0];
+        *reinterpret_cast<uint4*>(p + c1) = x[i][1];
+      }
+    }
   }
 }
 
@@ -116,23 +140,27 @@ extern "C" int sage_rotary(const void* q, const void* k, int dtype, int B, int S
   a.in_st[0] = {qsb, qss, qsh}, a.in_st[1] = {ksb, kss, ksh};
   a.out_st[0] = {qosb, qoss, qosh}, a.out_st[1] = {kosb, koss, kosh};
   a.heads[0] = H, a.heads[1] = Hkv;
-  a.S = S, a.D = D, a.R = R, a.interleaved = interleaved != 0;
+  a.S = S, a.D = D, a.R = R;
   a.tokens = (int64_t)B * S;
   a.positions = positions, a.pos64 = position_bits == 64, a.pos_b = psb, a.pos_s = pss;
   a.turns = turns;
   a.magnitude = magnitude;
   a.sine_sign = backward ? -1.0f : 1.0f;
-  a.slices = 1;
-  const int64_t threads = a.tokens * (D / 16) * a.slices;
-  const int64_t blocks = (threads + 255) / 256;
-  if (blocks > INT_MAX) {
+  const int64_t blocks = (a.tokens * (D / 16) + 255) / 256;
+  if (blocks > (1 << 23)) {   // 32-bit thread numbers
     set_error("rotary: %lld tokens are too many for one call", (long long)a.tokens);
     return SAGE_ERR_UNSUPPORTED;
   }
+  // few tokens: their heads are shared by several threads, so that the GPU is filled
+  const int batches = (H + Hkv + kBatch - 1) / kBatch;
+  const int64_t share = blocks >= 2048 ? 1 : (2048 + blocks - 1) / blocks;
+  const dim3 grid((unsigned)blocks, (unsigned)std::min<int64_t>(batches, share));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == SAGE_BF16)
-    rotary_kernel<__nv_bfloat16><<<(int)blocks, 256, 0, st>>>(a);
+    interleaved ? rotary_kernel<__nv_bfloat16, true><<<grid, 256, 0, st>>>(a)
+                : rotary_kernel<__nv_bfloat16, false><<<grid, 256, 0, st>>>(a);
   else
-    rotary_kernel<__half><<<(int)blocks, 256, 0, st>>>(a);
+    interleaved ? rotary_kernel<__half, true><<<grid, 256, 0, st>>>(a)
+                : rotary_kernel<__half, false><<<grid, 256, 0, st>>>(a);
   return launch_result("rotary");
 }

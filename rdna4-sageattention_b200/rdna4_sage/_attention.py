@@ -124,7 +124,7 @@ def _raise_pending(device: torch.device) -> None:
 
 # The step calls of the paged cache report through a word in pinned host memory instead, which their kernels write only
 # on an error: nothing has to be copied behind each call, and reading it costs the host one load.
-_host_words: dict[int, tuple[torch.Tensor, ctypes.c_int32]] = {}
+_host_words: dict[int, tuple[torch.Tensor, ctypes.c_int32, int]] = {}
 
 
 def host_word(device: torch.device) -> int:
@@ -132,8 +132,8 @@ def host_word(device: torch.device) -> int:
     w = _host_words.get(device.index)
     if w is None:
         t = torch.zeros(1, dtype=torch.int32, pin_memory=True)
-        w = _host_words.setdefault(device.index, (t, ctypes.c_int32.from_address(t.data_ptr())))
-    return w[0].data_ptr()
+        w = _host_words.setdefault(device.index, (t, ctypes.c_int32.from_address(t.data_ptr()), t.data_ptr()))
+    return w[2]
 
 
 def _raise_host_word(device: torch.device) -> None:
@@ -144,10 +144,48 @@ def _raise_host_word(device: torch.device) -> None:
                            f"{_lib.STATUS_NAMES.get(code, code)} (lengths, counts or page table of a paged K/V call)")
 
 
-def _checked(device: torch.device) -> None:
-    """RDNA4_SAGE_CHECK=1: raise at once what the call just enqueued reports."""
+_ready: dict[int, torch.device] = {}   # GPUs that step() has checked
+
+
+def step(tensors) -> torch.device:
+    """The prelude of a step call (paged cache, rotary positions), whose host time counts: all tensors on one supported
+    GPU, and nothing reported there by earlier calls.  Returns the device."""
+    index = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != index or index < 0:
+            raise Unsupported("tensors must be on one CUDA GPU")
+    dev = _ready.get(index)
+    if dev is None:
+        dev = torch.device("cuda", index)
+        _check_arch(dev)
+        host_word(dev)
+        _ready[index] = dev
+    _raise_pending(dev)
+    return dev
+
+
+def launch(dev: torch.device, what: str, entry, *args) -> None:
+    """entry(*args, status word, stream) on dev's current stream, with dev as the current device."""
+    index = dev.index
+    if torch._C._cuda_getDevice() == index:
+        rc = entry(*args, _host_words[index][2], torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(dev):
+            rc = entry(*args, _host_words[index][2], torch._C._cuda_getCurrentRawStream(index))
+    if rc != 0:
+        _lib.check(rc, what)
     if _CHECK and not torch.cuda.is_current_stream_capturing():
-        check_status(device)
+        check_status(dev)
+
+
+def step_rows(t: torch.Tensor, layout: str):
+    """(tensor, address, (batch, seq, head) strides) of 4-D rows the kernels take: _bsh without its cost where it has
+    nothing to do."""
+    st, at = t.stride(), t.data_ptr()
+    if st[3] == 1 and not (st[0] | st[1] | st[2]) & 7 and not at & 15:
+        return t, at, ((st[0], st[2], st[1]) if layout == "HND" else st[:3])
+    t, st = _bsh(t, layout)
+    return t, t.data_ptr(), st
 
 
 def _watch_status(device: torch.device) -> None:

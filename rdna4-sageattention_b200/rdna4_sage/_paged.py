@@ -18,8 +18,7 @@ from __future__ import annotations
 import torch
 
 from . import _attention, _lib
-from ._attention import DTYPES, HEAD_DIMS, Unsupported, _bsh
-from ._rotary import _check_devices
+from ._attention import DTYPES, HEAD_DIMS, Unsupported, launch, step, step_rows
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 
@@ -59,8 +58,13 @@ class PagedKV:
     def device(self):
         return self.k8.device
 
-    def _buffers(self):
-        return self.k8.data_ptr(), self.ks.data_ptr(), self.v8.data_ptr(), self.vs.data_ptr()
+    def _pool(self):
+        return (self.k8.data_ptr(), self.ks.data_ptr(), self.v8.data_ptr(), self.vs.data_ptr(), self.num_pages,
+                self.page_size)
+
+
+def _table(page_table):
+    return page_table.data_ptr(), page_table.stride(0), page_table.shape[1]
 
 
 def _check_table(kv, page_table, lens, counts, B):
@@ -97,20 +101,13 @@ def paged_kv_append(kv, k, v, page_table, lens, counts=None, tensor_layout="HND"
         raise Unsupported("k and v must match in shape and dtype")
     _check_rows(kv, v, tensor_layout)
     _check_table(kv, page_table, lens, counts, B)
-    dev = _check_devices([kv.k8, k, v, page_table, lens] + ([] if counts is None else [counts]))
+    dev = step((kv.k8, k, v, page_table, lens) if counts is None else (kv.k8, k, v, page_table, lens, counts))
     if B == 0 or S == 0:
         return
-    _attention._raise_pending(dev)
-    k, ks = _bsh(k, tensor_layout)
-    v, vs = _bsh(v, tensor_layout)
-    with torch.cuda.device(dev):
-        rc = _lib.lib().sage_paged_append(k.data_ptr(), v.data_ptr(), DTYPES[k.dtype], B, S, Hkv, kv.head_dim, *ks, *vs,
-                                          *kv._buffers(), kv.num_pages, kv.page_size, page_table.data_ptr(),
-                                          page_table.stride(0), page_table.shape[1], lens.data_ptr(),
-                                          None if counts is None else counts.data_ptr(), _attention.host_word(dev),
-                                          torch.cuda.current_stream(dev).cuda_stream)
-    _lib.check(rc, "sage_paged_append")
-    _attention._checked(dev)
+    k, kp, ks = step_rows(k, tensor_layout)
+    v, vp, vs = step_rows(v, tensor_layout)
+    launch(dev, "sage_paged_append", _lib.lib().sage_paged_append, kp, vp, DTYPES[k.dtype], B, S, Hkv, kv.head_dim, *ks,
+           *vs, *kv._pool(), *_table(page_table), lens.data_ptr(), None if counts is None else counts.data_ptr())
 
 
 def paged_kv_read(kv, page_table, lens, max_len, dtype=torch.bfloat16, tensor_layout="HND"):
@@ -124,21 +121,15 @@ def paged_kv_read(kv, page_table, lens, max_len, dtype=torch.bfloat16, tensor_la
         raise ValueError(f"max_len {max_len}")
     B = lens.shape[0] if lens.dim() == 1 else -1
     _check_table(kv, page_table, lens, None, B)
-    dev = _check_devices((kv.k8, page_table, lens))
+    dev = step((kv.k8, page_table, lens))
     Hkv, D = kv.kv_heads, kv.head_dim
-    k, v = (torch.empty((B, Hkv, max_len, D) if tensor_layout == "HND" else (B, max_len, Hkv, D), device=dev, dtype=dtype)
-            for _ in range(2))
-    if k.numel() == 0:
+    shape = (B, Hkv, max_len, D) if tensor_layout == "HND" else (B, max_len, Hkv, D)
+    k, v = torch.empty(shape, device=dev, dtype=dtype), torch.empty(shape, device=dev, dtype=dtype)
+    if 0 in shape:
         return k, v
-    _attention._raise_pending(dev)
-    st = (k.stride(0), k.stride(2), k.stride(1)) if tensor_layout == "HND" else k.stride()[:3]
-    with torch.cuda.device(dev):
-        rc = _lib.lib().sage_paged_read(*kv._buffers(), kv.num_pages, kv.page_size, Hkv, D, page_table.data_ptr(),
-                                        page_table.stride(0), page_table.shape[1], lens.data_ptr(), B, max_len,
-                                        k.data_ptr(), v.data_ptr(), DTYPES[dtype], *st, *st, _attention.host_word(dev),
-                                        torch.cuda.current_stream(dev).cuda_stream)
-    _lib.check(rc, "sage_paged_read")
-    _attention._checked(dev)
+    _, kp, st = step_rows(k, tensor_layout)
+    launch(dev, "sage_paged_read", _lib.lib().sage_paged_read, *kv._pool(), Hkv, D, *_table(page_table), lens.data_ptr(), B,
+           max_len, kp, v.data_ptr(), DTYPES[dtype], *st, *st)
     return k, v
 
 
@@ -150,18 +141,12 @@ def paged_kv_keep(kv, page_table, lens, keep, counts=None):
     _check_table(kv, page_table, lens, counts, B)
     if keep.dim() != 2 or keep.shape[0] != B or keep.dtype != torch.int32 or (keep.shape[1] > 1 and keep.stride(1) != 1):
         raise Unsupported(f"keep must be int32 [{B}, N] with contiguous rows")
-    dev = _check_devices([kv.k8, page_table, lens, keep] + ([] if counts is None else [counts]))
+    dev = step((kv.k8, page_table, lens, keep) if counts is None else (kv.k8, page_table, lens, keep, counts))
     if keep.numel() == 0:
         return
-    _attention._raise_pending(dev)
-    with torch.cuda.device(dev):
-        rc = _lib.lib().sage_paged_keep(*kv._buffers(), kv.num_pages, kv.page_size, kv.kv_heads, kv.head_dim,
-                                        page_table.data_ptr(), page_table.stride(0), page_table.shape[1],
-                                        lens.data_ptr(), keep.data_ptr(), keep.stride(0), keep.shape[1],
-                                        None if counts is None else counts.data_ptr(), B, _attention.host_word(dev),
-                                        torch.cuda.current_stream(dev).cuda_stream)
-    _lib.check(rc, "sage_paged_keep")
-    _attention._checked(dev)
+    launch(dev, "sage_paged_keep", _lib.lib().sage_paged_keep, *kv._pool(), kv.kv_heads, kv.head_dim, *_table(page_table),
+           lens.data_ptr(), keep.data_ptr(), keep.stride(0), keep.shape[1],
+           None if counts is None else counts.data_ptr(), B)
 
 
 def attention_paged_kv(q, kv, page_table, lens, tree_mask=None, counts=None, tensor_layout="HND", sm_scale=None,
@@ -174,34 +159,30 @@ def attention_paged_kv(q, kv, page_table, lens, tree_mask=None, counts=None, ten
     log-sum-exp -inf."""
     B, T, H = _check_rows(kv, q, tensor_layout)
     _check_table(kv, page_table, lens, counts, B)
-    tensors = [kv.k8, q, page_table, lens] + ([] if counts is None else [counts])
-    mask, mask_b, mask_i = None, 0, 0
+    tensors = [kv.k8, q, page_table, lens]
+    if counts is not None:
+        tensors.append(counts)
     if tree_mask is not None:
         if tree_mask.dtype != torch.bool or tree_mask.shape not in ((T, T), (1, T, T), (B, T, T)):
             raise Unsupported(f"tree_mask must be bool [{T}, {T}] or [{B}, {T}, {T}]")
         tensors.append(tree_mask)
-    dev = _check_devices(tensors)
-    out = torch.empty((B, T, H, kv.head_dim), device=dev, dtype=q.dtype)
+    dev = step(tensors)
+    D = kv.head_dim
+    out = torch.empty((B, T, H, D), device=dev, dtype=q.dtype)
     lse = torch.empty((B, H, T), device=dev, dtype=torch.float32) if return_lse else None
-    if out.numel() > 0:
-        _attention._raise_pending(dev)
-        L = _lib.lib()
+    if B and T:
+        mask, mask_b, mask_i = None, 0, 0
         if tree_mask is not None:
             tree_mask = tree_mask if tree_mask.stride(-1) == 1 else tree_mask.contiguous()
             mask, mask_i = tree_mask.data_ptr(), tree_mask.stride(-2)
             mask_b = tree_mask.stride(0) if tree_mask.dim() == 3 and tree_mask.shape[0] == B else 0
-        q, qs = _bsh(q, tensor_layout)
-        ws_bytes = L.sage_paged_attention_workspace_bytes(B, T, H, kv.kv_heads, kv.head_dim)
+        q, qp, qs = step_rows(q, tensor_layout)
+        L = _lib.lib()
+        ws_bytes = L.sage_paged_attention_workspace_bytes(B, T, H, kv.kv_heads, D)
         ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
-        with torch.cuda.device(dev):
-            rc = L.sage_paged_attention(q.data_ptr(), DTYPES[q.dtype], B, T, H, kv.kv_heads, kv.head_dim, *qs,
-                                        *kv._buffers(), kv.num_pages, kv.page_size, page_table.data_ptr(),
-                                        page_table.stride(0), page_table.shape[1], lens.data_ptr(),
-                                        None if counts is None else counts.data_ptr(), mask, mask_b, mask_i,
-                                        float(sm_scale or 0.0), out.data_ptr(), *out.stride()[:3],
-                                        lse.data_ptr() if return_lse else None, ws.data_ptr(), ws_bytes,
-                                        _attention.host_word(dev), torch.cuda.current_stream(dev).cuda_stream)
-        _lib.check(rc, "sage_paged_attention")
-        _attention._checked(dev)
+        launch(dev, "sage_paged_attention", L.sage_paged_attention, qp, DTYPES[q.dtype], B, T, H, kv.kv_heads, D, *qs,
+               *kv._pool(), *_table(page_table), lens.data_ptr(), None if counts is None else counts.data_ptr(), mask,
+               mask_b, mask_i, float(sm_scale or 0.0), out.data_ptr(), T * H * D, H * D, D,
+               lse.data_ptr() if return_lse else None, ws.data_ptr(), ws_bytes)
     out = out.transpose(1, 2) if tensor_layout == "HND" else out
     return (out, lse) if return_lse else out

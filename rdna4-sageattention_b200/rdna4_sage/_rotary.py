@@ -9,8 +9,8 @@ import math
 
 import torch
 
-from . import _attention, _lib
-from ._attention import DTYPES, HEAD_DIMS, Unsupported, _bsh
+from . import _lib
+from ._attention import DTYPES, HEAD_DIMS, Unsupported, launch, step, step_rows
 
 SCALINGS = (None, "linear", "ntk", "ramp")
 
@@ -94,41 +94,36 @@ def _check(q, k, positions, rope, layout):
         raise Unsupported(f"positions {tuple(positions.shape)}: (S,) or (B, S) of ({B}, {S}) tokens required")
 
 
-def _check_devices(tensors):
-    dev = tensors[0].device
-    if dev.type != "cuda" or any(t.device != dev for t in tensors):
-        raise Unsupported("tensors must be on one CUDA GPU")
-    _attention._check_arch(dev)
-    return dev
-
-
-def _launch(q, k, positions, rope, layout, backward):
+def _launch(dev, q, k, positions, rope, layout, backward):
     """(q, k) turned, new tensors in the inputs' layout (k may be None)."""
-    dev = q.device
     if q.numel() == 0 or k is not None and k.numel() == 0:
         if q.numel() != 0 or k is not None and k.numel() != 0:
             raise Unsupported("q and k must both hold heads")
         return torch.empty_like(q), None if k is None else torch.empty_like(k)
-    B, S, H = (q.shape[0], q.shape[2], q.shape[1]) if layout == "HND" else q.shape[:3]
-    bsh = (0, 2, 1) if layout == "HND" else (0, 1, 2)
-    q, qs = _bsh(q, layout)
+    q, qp, qs = step_rows(q, layout)
     q_out = torch.empty_like(q)   # of a tensor that the kernels take, so it is one too
-    qos = [q_out.stride(i) for i in bsh]
+    B, S, H = (q.shape[0], q.shape[2], q.shape[1]) if layout == "HND" else q.shape[:3]
+    _, qop, qos = step_rows(q_out, layout)
     if k is None:
         k_out, Hkv, kp, kop, ks, kos = None, 0, None, None, (0, 0, 0), (0, 0, 0)
     else:
-        k, ks = _bsh(k, layout)
+        k, kp, ks = step_rows(k, layout)
         k_out = torch.empty_like(k)
-        kos = [k_out.stride(i) for i in bsh]
-        Hkv, kp, kop = k.shape[1 if layout == "HND" else 2], k.data_ptr(), k_out.data_ptr()
-    at = positions.expand(B, S)
-    with torch.cuda.device(dev):
-        rc = _lib.lib().sage_rotary(q.data_ptr(), kp, DTYPES[q.dtype], B, S, H, Hkv, rope.head_dim, rope.rotary_dim,
-                                    rope.interleaved, *qs, *ks, q_out.data_ptr(), kop, *qos, *kos, at.data_ptr(),
-                                    32 if at.dtype == torch.int32 else 64, *at.stride(), rope.turns.data_ptr(),
-                                    rope.magnitude, backward, torch.cuda.current_stream(dev).cuda_stream)
-    _lib.check(rc, "sage_rotary")
+        _, kop, kos = step_rows(k_out, layout)
+        Hkv = k.shape[1 if layout == "HND" else 2]
+    if positions.dim() == 1:
+        pb, ps = 0, positions.stride(0)
+    else:
+        pb, ps = positions.stride()
+        pb = 0 if positions.shape[0] == 1 else pb
+    launch(dev, "sage_rotary", _rotary_entry, qp, kp, DTYPES[q.dtype], B, S, H, Hkv, rope.head_dim, rope.rotary_dim,
+           rope.interleaved, *qs, *ks, qop, kop, *qos, *kos, positions.data_ptr(),
+           32 if positions.dtype == torch.int32 else 64, pb, ps, rope.turns.data_ptr(), rope.magnitude, backward)
     return q_out, k_out
+
+
+def _rotary_entry(*args):
+    return _lib.lib().sage_rotary(*args[:-2], args[-1])   # it reports nothing from the device
 
 
 class _RotaryFunction(torch.autograd.Function):
@@ -139,7 +134,7 @@ class _RotaryFunction(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(positions)
         ctx.rope, ctx.layout, ctx.turn_back = rope, layout, not backward
-        q_out, k_out = _launch(q, k, positions, rope, layout, backward)
+        q_out, k_out = _launch(q.device, q, k, positions, rope, layout, backward)
         return q_out if k is None else (q_out, k_out)
 
     @staticmethod
@@ -148,7 +143,12 @@ class _RotaryFunction(torch.autograd.Function):
         dq = dq if ctx.needs_input_grad[0] else None
         dk = dk if ctx.needs_input_grad[1] else None
         args = (positions, ctx.rope, ctx.layout, ctx.turn_back)
-        if dq is not None and dk is not None:
+        if not torch.is_grad_enabled():
+            if dq is not None:
+                dq, dk = _launch(dq.device, dq, dk, *args)
+            elif dk is not None:
+                dk, _ = _launch(dk.device, dk, None, *args)
+        elif dq is not None and dk is not None:
             dq, dk = _RotaryFunction.apply(dq, dk, *args)
         elif dq is not None:
             dq = _RotaryFunction.apply(dq, None, *args)
@@ -163,8 +163,8 @@ def rotary(q, k, positions, rope, tensor_layout="HND"):
     alone.  positions: int32 or int64 of any value, (S,) for all sequences or (B, S), on the GPU.  rope: a Rotary.
     Differentiable in q and k.  Raises Unsupported for inputs the kernel does not take."""
     _check(q, k, positions, rope, tensor_layout)
-    _check_devices((q, positions, rope.turns) if k is None else (q, k, positions, rope.turns))
-    if torch.is_grad_enabled() and (q.requires_grad or k is not None and k.requires_grad):
+    dev = step((q, positions, rope.turns) if k is None else (q, k, positions, rope.turns))
+    if (q.requires_grad or k is not None and k.requires_grad) and torch.is_grad_enabled():
         return _RotaryFunction.apply(q, k, positions, rope, tensor_layout, False)
-    q_out, k_out = _launch(q, k, positions, rope, tensor_layout, False)
+    q_out, k_out = _launch(dev, q, k, positions, rope, tensor_layout, False)
     return q_out if k is None else (q_out, k_out)
