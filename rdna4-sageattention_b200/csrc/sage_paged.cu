@@ -55,66 +55,70 @@ struct AppendArgs {
   int B, S;
 };
 
-// A group of LPR lanes (a power of two, D / 8 of them with data) holds one row of K and the same row of V, 8 channels a
-// lane; tokens of one head follow one another, as their rows do in a page.
+// A group of LPR lanes (a power of two, D / 8 of them with data) holds kTokens consecutive tokens of one head of K and of V,
+// 8 channels a lane.  The rows are loaded before their places in the cache are looked up: the chain of dependent loads
+// (length, page, row) would otherwise leave the memory idle (one token a lane, looked up first: 55 us for 4 x 8190
+// tokens of 8 heads, D 128).
+constexpr int kTokens = 4;
+
 template <typename T, int D>
 __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
   constexpr int LPR = D == 64 ? 8 : D == 256 ? 32 : 16;
   const int lane = threadIdx.x % LPR;
-  const uint32_t row = blockIdx.x * (256u / LPR) + threadIdx.x / LPR;   // token and head of the sequence
-  const int h = (int)(row / a.S), s = (int)(row - h * (uint32_t)a.S), b = blockIdx.y;
-  bool live = h < a.p.Hkv;
-  int64_t dst = -1;
-  if (live) {
-    const int n = a.counts != nullptr ? a.counts[b] : a.S;
-    if (n < 0 || n > a.S) raise_invalid(a.p);
-    live = s < min(n, a.S);
-    if (live) dst = paged_row(a.p, b, h, (int64_t)a.p.lens[b] + s);
-    live = dst >= 0;
-  }
-  const bool data = live && lane * 8 < D;
-  float x[2][8];
+  const uint32_t id = blockIdx.x * (256u / LPR) + threadIdx.x / LPR, run = id / a.p.Hkv;
+  const int h = (int)(id - run * a.p.Hkv), s0 = (int)run * kTokens, b = blockIdx.y;
+  uint4 x[2][kTokens];
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
+    const T* src = static_cast<const T*>(a.x[w]) + b * a.st[w].b + s0 * a.st[w].s + h * a.st[w].h + lane * 8;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[w][i] = 0.0f;
-    if (data)
-      load8(static_cast<const T*>(a.x[w]) + b * a.st[w].b + s * a.st[w].s + h * a.st[w].h + lane * 8, x[w]);
+    for (int r = 0; r < kTokens; ++r)
+      x[w][r] = s0 + r < a.S && lane * 8 < D ? *reinterpret_cast<const uint4*>(src + r * a.st[w].s)
+                                             : make_uint4(0, 0, 0, 0);
   }
+  const int n = a.counts != nullptr ? a.counts[b] : a.S, len = a.p.lens[b];
+  if (n < 0 || n > a.S) raise_invalid(a.p);
 #pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    // the largest magnitude as bits: NaN and infinity compare above every finite value
-    uint32_t top = 0;
+  for (int r = 0; r < kTokens; ++r) {
+    const bool live = s0 + r < min(n, a.S);
+    const int64_t dst = live ? paged_row(a.p, b, h, (int64_t)len + s0 + r) : -1;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[w][i]) & 0x7fffffffu);
+    for (int w = 0; w < 2; ++w) {
+      float y[8];
+      unpack8(x[w][r], y, T());
+      // the largest magnitude as bits: NaN and infinity compare above every finite value
+      uint32_t top = 0;
 #pragma unroll
-    for (int o = LPR / 2; o > 0; o /= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const bool finite = top < 0x7f800000u;
-    const float amax = __uint_as_float(top);
-    const bool kept = finite && amax >= kTiny;
-    const float most = w == 0 ? 127.0f : 448.0f;
-    const float mul = __fdiv_rn(most, kept ? amax : most) * kOutwards;
-    const float scale = kept ? __fdiv_rn(amax, most) : finite ? 0.0f : __uint_as_float(0x7fc00000u);
-    uint32_t code[2];
+      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(y[i]) & 0x7fffffffu);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if (w == 0) {
-        uint32_t c = 0;
+      for (int o = LPR / 2; o > 0; o /= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const bool finite = top < 0x7f800000u;
+      const float amax = __uint_as_float(top);
+      const bool kept = finite && amax >= kTiny;
+      const float most = w == 0 ? 127.0f : 448.0f;
+      const float mul = __fdiv_rn(most, kept ? amax : most) * kOutwards;
+      uint32_t code[2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          c |= (uint32_t)(uint8_t)(int8_t)__float2int_rn(kept ? x[w][4 * i + e] * mul : 0.0f) << (8 * e);
-        code[i] = c;
-      } else {
-        const float* y = x[w] + 4 * i;
-        code[i] = kept ? (uint32_t)pack_e4m3x2(y[0] * mul, y[1] * mul) |
-                               (uint32_t)pack_e4m3x2(y[2] * mul, y[3] * mul) << 16
-                         : 0u;
+      for (int i = 0; i < 2; ++i) {
+        const float* z = y + 4 * i;
+        if (w == 0) {
+          uint32_t c = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)   // 1.5 * 2^23 + x rounds x to a whole number, whose low byte is the code
+            c |= (__float_as_uint(z[e] * mul + kMagicF) & 0xffu) << (8 * e);
+          code[i] = c;
+        } else {
+          code[i] = (uint32_t)pack_e4m3x2(z[0] * mul, z[1] * mul) | (uint32_t)pack_e4m3x2(z[2] * mul, z[3] * mul) << 16;
+        }
+        if (!kept) code[i] = 0;
       }
-    }
-    if (data) {
-      uint8_t* to = w == 0 ? reinterpret_cast<uint8_t*>(a.p.k8) : a.p.v8;
-      *reinterpret_cast<uint2*>(to + dst * D + lane * 8) = make_uint2(code[0], code[1]);
-      if (lane == 0) (w == 0 ? a.p.ks : a.p.vs)[dst] = scale;
+      if (dst >= 0 && lane * 8 < D) {
+        uint8_t* to = w == 0 ? reinterpret_cast<uint8_t*>(a.p.k8) : a.p.v8;
+        *reinterpret_cast<uint2*>(to + dst * D + lane * 8) = make_uint2(code[0], code[1]);
+        if (lane == 0)
+          (w == 0 ? a.p.ks : a.p.vs)[dst] =
+              kept ? __fdiv_rn(amax, most) : finite ? 0.0f : __uint_as_float(0x7fc00000u);
+      }
     }
   }
 }
@@ -126,39 +130,55 @@ struct ReadArgs {
   int B, S;
 };
 
-// A thread reads 16 codes of K and of V and writes 16 channels of each.
+// A thread reads 8 codes of kRun consecutive tokens (a run never leaves its page) of K and of V, all of them under way at
+// once, and writes 8 channels of each, so that a warp's stores are whole lines.
+constexpr int kRun = 4;
+
 template <typename T, int D>
 __global__ void __launch_bounds__(256) read_kernel(const ReadArgs a) {
-  constexpr int LPR = D / 16;
-  const uint32_t id = blockIdx.x * 256u + threadIdx.x, row = id / LPR;   // token and head of the sequence
-  const int c = (int)(id % LPR) * 16, b = blockIdx.y;
-  const int s = (int)(row / a.p.Hkv), h = (int)(row - s * (uint32_t)a.p.Hkv);
-  if (s >= a.S) return;
+  constexpr int LPR = D / 8;
+  const uint32_t id = blockIdx.x * 256u + threadIdx.x, row = id / LPR;   // run of tokens and head of the sequence
+  const int c = (int)(id % LPR) * 8, b = blockIdx.y;
+  const int run = (int)(row / a.p.Hkv), h = (int)(row - run * (uint32_t)a.p.Hkv), s0 = run * kRun;
+  if (s0 >= a.S) return;
   const int n = a.p.lens[b];
   if (n < 0 || n > (int64_t)a.p.max_pages << a.p.page_shift) raise_invalid(a.p);
-  const int64_t src = s < n ? paged_row(a.p, b, h, s) : -1;
-  float x[2][16];
-#pragma unroll
-  for (int w = 0; w < 2; ++w)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) x[w][i] = 0.0f;
-  if (src >= 0) {
-    const uint4 k = *reinterpret_cast<const uint4*>(a.p.k8 + src * D + c);
-    const uint4 v = *reinterpret_cast<const uint4*>(a.p.v8 + src * D + c);
-    const float ks = a.p.ks[src], vs = a.p.vs[src];
-    const uint32_t kw[4] = {k.x, k.y, k.z, k.w}, vw[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      x[0][i] = (float)(int8_t)(kw[i / 4] >> (8 * (i % 4))) * ks;
-      const __nv_fp8_storage_t code = (__nv_fp8_storage_t)(vw[i / 4] >> (8 * (i % 4)));
-      x[1][i] = __half2float(__half(__nv_cvt_fp8_to_halfraw(code, __NV_E4M3))) * vs;
-    }
-  }
+  const int64_t src = s0 < n ? paged_row(a.p, b, h, s0) : -1;
+  uint2 code[2][kRun];
+  float4 scale[2];
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
-    T* dst = static_cast<T*>(a.out[w]) + b * a.st[w].b + s * a.st[w].s + h * a.st[w].h + c;
-    store8(dst, x[w]);
-    store8(dst + 8, x[w] + 8);
+    const uint8_t* from = w == 0 ? reinterpret_cast<const uint8_t*>(a.p.k8) : a.p.v8;
+    const float* scales = w == 0 ? a.p.ks : a.p.vs;
+#pragma unroll
+    for (int r = 0; r < kRun; ++r)
+      code[w][r] = src >= 0 && s0 + r < min(n, a.S) ? *reinterpret_cast<const uint2*>(from + (src + r) * D + c)
+                                                    : make_uint2(0, 0);
+    scale[w] = src >= 0 ? make_float4(scales[src], scales[src + 1], scales[src + 2], scales[src + 3])
+                        : make_float4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int r = 0; r < kRun; ++r) {
+    if (s0 + r >= a.S) break;
+    const bool held = src >= 0 && s0 + r < n;   // what lies behind may be anything, a NaN scale too
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const float f = !held ? 0.0f : r == 0 ? scale[w].x : r == 1 ? scale[w].y : r == 2 ? scale[w].z : scale[w].w;
+      const uint32_t q[2] = {code[w][r].x, code[w][r].y};
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        uint32_t lo, hi;
+        if (w == 0)
+          int8_to_f16(q[i], lo, hi);
+        else
+          lo = e4m3_to_f16((uint16_t)q[i]), hi = e4m3_to_f16((uint16_t)(q[i] >> 16));
+        const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+        const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+        x[4 * i] = u.x * f, x[4 * i + 1] = u.y * f, x[4 * i + 2] = v.x * f, x[4 * i + 3] = v.y * f;
+      }
+      store8(static_cast<T*>(a.out[w]) + b * a.st[w].b + (s0 + r) * a.st[w].s + h * a.st[w].h + c, x);
+    }
   }
 }
 
@@ -236,7 +256,7 @@ int sage_paged_append(const void* k, const void* v, int dtype, int B, int S, int
   a.counts = counts;
   a.B = B, a.S = S;
   const int per_block = 256 / (D == 64 ? 8 : D == 256 ? 32 : 16);
-  const int64_t blocks = ((int64_t)S * Hkv + per_block - 1) / per_block;
+  const int64_t blocks = ((int64_t)((S + kTokens - 1) / kTokens) * Hkv + per_block - 1) / per_block;
   if (blocks > (1 << 23) || B > 65535) {   // 32-bit thread numbers, grid limit
     set_error("append: %d sequences of %d tokens and %d heads are too many for one call", B, S, Hkv);
     return SAGE_ERR_UNSUPPORTED;
@@ -270,7 +290,7 @@ int sage_paged_read(const int8_t* k8, const float* ks, const uint8_t* v8, const 
   a.out[0] = k, a.out[1] = v;
   a.st[0] = {ksb, kss, ksh}, a.st[1] = {vsb, vss, vsh};
   a.B = B, a.S = S;
-  const int64_t blocks = ((int64_t)S * Hkv * (D / 16) + 255) / 256;
+  const int64_t blocks = ((int64_t)((S + kRun - 1) / kRun) * Hkv * (D / 8) + 255) / 256;
   if (blocks > (1 << 23) || B > 65535) {   // 32-bit thread numbers, grid limit
     set_error("read: %d sequences of %d tokens and %d heads are too many for one call", B, S, Hkv);
     return SAGE_ERR_UNSUPPORTED;

@@ -186,27 +186,10 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Four int8 codes -> two fp16 pairs, exactly: 0x6400 + u is the fp16 number 1024 + u, and u = code + 128.
-__device__ __forceinline__ void int8_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  w ^= 0x80808080u;
-  const __half2 off = __half2half2(__ushort_as_half(0x6480));   // 1152
-  uint32_t x = __byte_perm(w, 0x64646464u, 0x4140), y = __byte_perm(w, 0x64646464u, 0x4342);
-  const __half2 p = __hsub2(*reinterpret_cast<__half2*>(&x), off), q = __hsub2(*reinterpret_cast<__half2*>(&y), off);
-  lo = *reinterpret_cast<const uint32_t*>(&p);
-  hi = *reinterpret_cast<const uint32_t*>(&q);
-}
-
 // Two weights -> an fp16 pair, the largest finite number for what is above it (only weights of zero rows are).
 __device__ __forceinline__ uint32_t pack_weights(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-
-// Two e4m3 codes -> an fp16 pair (exact).
-__device__ __forceinline__ uint32_t e4m3_to_f16(uint16_t v) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
   return r;
 }
 

@@ -31,8 +31,9 @@ struct RotaryArgs {
   float sine_sign;     // -1 in the gradient
 };
 
-// One thread holds 16 channels (8 pairs) of one token and walks over the heads, so each sine is computed once for all of
-// its heads; kBatch heads are loaded before the first is turned.
+// One thread holds two runs of 8 channels (8 pairs in all) of one token and walks over the heads, so each sine is computed
+// once for all of its heads; kBatch heads are loaded before the first is turned.  Half layout: the runs are the partners
+// of one another; interleaved: each holds four pairs.  Neighbouring threads hold neighbouring runs.
 constexpr int kBatch = 4;
 
 template <typename T, bool INTERLEAVED>
@@ -42,9 +43,17 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
   const uint32_t u = id % units, token = id / units;
   if (token >= (uint32_t)a.tokens) return;
   const uint32_t b = token / a.S, s = token - b * a.S;
-  const bool turned = u * 16 < (uint32_t)a.R;
-  const int c0 = turned && !INTERLEAVED ? u * 8 : u * 16;          // first channel of each 8-channel part
-  const int c1 = turned && !INTERLEAVED ? a.R / 2 + u * 8 : u * 16 + 8;
+  // first channel of either run, and whether it is turned
+  int c0, c1;
+  bool turned, turned1;
+  if (INTERLEAVED) {
+    c0 = u * 8, c1 = a.D / 2 + u * 8;
+    turned = c0 < a.R, turned1 = c1 < a.R;
+  } else {
+    const int v = (int)u - a.R / 16;   // past the turned runs
+    turned = turned1 = v < 0;
+    c0 = turned ? u * 8 : a.R + v * 8, c1 = turned ? a.R / 2 + u * 8 : a.R + (a.D - a.R) / 2 + v * 8;
+  }
   const T* src[2];
   T* dst[2];
 #pragma unroll
@@ -73,7 +82,9 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
                                    : (uint64_t)(int64_t) static_cast<const int*>(a.positions)[place];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const uint64_t turn = pos * a.turns[u * 8 + e];
+        const int pair = !INTERLEAVED ? u * 8 + e : (e < 4 ? c0 : c1) / 2 + e % 4;
+        if (INTERLEAVED && e >= 4 && !turned1) break;
+        const uint64_t turn = pos * a.turns[pair];
         const int half_turns = (int)(uint32_t)((turn + 0x80000000ull) >> 32);   // units of 2^-31 half turns
         sincospif((float)half_turns * 0x1p-31f, &sn[e], &cs[e]);
         cs[e] *= a.magnitude;
@@ -91,6 +102,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
         unpack8(x[i][1], y[1], T());
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
+          if (INTERLEAVED && e >= 4 && !turned1) break;
           float& p1 = INTERLEAVED ? y[e / 4][2 * e % 8] : y[0][e];
           float& p2 = INTERLEAVED ? y[e / 4][2 * e % 8 + 1] : y[1][e];
           const float x1 = p1, x2 = p2;
@@ -98,7 +110,10 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
           p2 = x2 * cs[e] + x1 * sn[e];
         }
         store8(p + c0, y[0]);
-        store8(p + c1, y[1]);
+        if (turned1)
+          store8(p + c1, y[1]);
+        else
+          *reinterpret_cast<uint4*>(p + c1) = x[i][1];
       } else {
         *reinterpret_cast<uint4*>(p + c0) = x[i][0];
         *reinterpret_cast<uint4*>(p + c1) = x[i][1];
