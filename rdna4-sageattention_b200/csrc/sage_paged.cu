@@ -3,8 +3,9 @@
 // A row (one token of one kv head) is stored on its own, so the cache grows by single tokens:
 //   K: int8 codes round(127 x / a), scale a / 127;   V: e4m3 codes of 448 x / a, scale a / 448;   a = max |x|.
 // Both roundings are to nearest, ties away from zero.  For 16-bit x the quotient is a ratio of small integers: it is a
-// tie exactly, or at least 2^-16 (relative, e4m3) resp. 2^-12 (absolute, int8) away from one.  So the product with the
-// reciprocal, pushed outwards by 2^-21, falls on the right side of every border and no division per element is needed.
+// tie exactly, or at least 2^-16 (relative, e4m3) resp. 2^-(12 + d) (absolute, int8, for a quotient below 2^(8 - d)) away
+// from one.  The product with 127 / a resp. 448 / a is off by less than 2^-21 (the reciprocal by 2^-23, three roundings by
+// 2^-24), so pushed outwards by 2^-21 it falls on the right side of every border, and no division per element is needed.
 // Rows with an infinity or NaN store scale NaN and codes 0; rows with a < 2^-100 store zeros.
 #include "../../include/sage_b200.h"
 #include "sage_internal.h"
@@ -47,6 +48,12 @@ int paged_args(PagedArgs* out, void* k8, float* ks, void* v8, float* vs, int num
 constexpr float kTiny = 0x1p-100f;
 constexpr float kOutwards = 1.0f + 0x1p-21f;
 
+template <typename T>
+constexpr uint32_t kInfBits = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+
+__device__ __forceinline__ float from_bits(uint32_t bits, __nv_bfloat16) { return __uint_as_float(bits << 16); }
+__device__ __forceinline__ float from_bits(uint32_t bits, __half) { return __half2float(__ushort_as_half((uint16_t)bits)); }
+
 struct AppendArgs {
   PagedArgs p;
   const void* x[2];   // K, V
@@ -82,42 +89,47 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
   for (int r = 0; r < kTokens; ++r) {
     const bool live = s0 + r < min(n, a.S);
     const int64_t dst = live ? paged_row(a.p, b, h, (int64_t)len + s0 + r) : -1;
+    // The largest magnitudes of the K row (low half) and of the V row, as 16-bit patterns: without the sign they order as
+    // the numbers do, with infinity and NaN above every finite one.
+    uint32_t top = 0;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const uint4 v = x[w][r];
+      const uint32_t m = __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
+                                  __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
+      top |= max(m & 0xffffu, m >> 16) << (16 * w);
+    }
+#pragma unroll
+    for (int o = LPR / 2; o > 0; o /= 2) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
       float y[8];
       unpack8(x[w][r], y, T());
-      // the largest magnitude as bits: NaN and infinity compare above every finite value
-      uint32_t top = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(y[i]) & 0x7fffffffu);
-#pragma unroll
-      for (int o = LPR / 2; o > 0; o /= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const bool finite = top < 0x7f800000u;
-      const float amax = __uint_as_float(top);
+      const uint32_t bits = w == 0 ? top & 0xffffu : top >> 16;
+      const bool finite = bits < kInfBits<T>;
+      const float amax = from_bits(bits, T());
       const bool kept = finite && amax >= kTiny;
       const float most = w == 0 ? 127.0f : 448.0f;
-      const float mul = __fdiv_rn(most, kept ? amax : most) * kOutwards;
+      float inverse;   // of amax / 4, which is normal for every amax that is kept
+      asm("rcp.approx.f32 %0, %1;" : "=f"(inverse) : "f"(kept ? amax * 0.25f : 1.0f));
+      const float mul = inverse * (most * 0.25f) * kOutwards;
       uint32_t code[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const float* z = y + 4 * i;
-        if (w == 0) {
-          uint32_t c = 0;
-#pragma unroll
-          for (int e = 0; e < 4; ++e)   // 1.5 * 2^23 + x rounds x to a whole number, whose low byte is the code
-            c |= (__float_as_uint(z[e] * mul + kMagicF) & 0xffu) << (8 * e);
-          code[i] = c;
+        if (w == 0) {   // 1.5 * 2^23 + x rounds x to a whole number, whose low byte is the code
+          const uint32_t lo = __byte_perm(__float_as_uint(fmaf(z[0], mul, kMagicF)), __float_as_uint(fmaf(z[1], mul, kMagicF)), 0x0040);
+          const uint32_t hi = __byte_perm(__float_as_uint(fmaf(z[2], mul, kMagicF)), __float_as_uint(fmaf(z[3], mul, kMagicF)), 0x0040);
+          code[i] = __byte_perm(lo, hi, 0x5410);
         } else {
-          code[i] = (uint32_t)pack_e4m3x2(z[0] * mul, z[1] * mul) | (uint32_t)pack_e4m3x2(z[2] * mul, z[3] * mul) << 16;
+          code[i] = __byte_perm(pack_e4m3x2(z[0] * mul, z[1] * mul), pack_e4m3x2(z[2] * mul, z[3] * mul), 0x5410);
         }
-        if (!kept) code[i] = 0;
       }
       if (dst >= 0 && lane * 8 < D) {
         uint8_t* to = w == 0 ? reinterpret_cast<uint8_t*>(a.p.k8) : a.p.v8;
-        *reinterpret_cast<uint2*>(to + dst * D + lane * 8) = make_uint2(code[0], code[1]);
+        *reinterpret_cast<uint2*>(to + dst * D + lane * 8) = kept ? make_uint2(code[0], code[1]) : make_uint2(0, 0);
         if (lane == 0)
-          (w == 0 ? a.p.ks : a.p.vs)[dst] =
-              kept ? __fdiv_rn(amax, most) : finite ? 0.0f : __uint_as_float(0x7fc00000u);
+          (w == 0 ? a.p.ks : a.p.vs)[dst] = kept ? amax * (1.0f / most) : finite ? 0.0f : __uint_as_float(0x7fc00000u);
       }
     }
   }
