@@ -1,0 +1,284 @@
+// Shared by the two kernels of paged attention (sage_paged_attn.cu for few query rows of a kv head, sage_paged_wide.cu for
+// many): the list of work, the places in it, the tiles that TMA writes, and small device helpers.
+#pragma once
+
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+
+#include "../../include/sage_b200.h"
+#include "sage_internal.h"
+#include "sage_paged.cuh"
+#include "sage_ptx.cuh"
+
+namespace sage {
+
+constexpr int kTileKeys = 64;
+constexpr int kMinTiles = 2;               // tiles a CTA takes at the least
+constexpr float kZeroLog = -100.0f;        // log2 of a zero V scale in the running maximum
+
+struct PagedAttnArgs {
+  PagedArgs p;
+  const void* q;
+  Strides3 q_st;
+  void* out;
+  Strides3 out_st;
+  float* lse;          // [B, H, T] or null
+  const int* counts;
+  const uint8_t* mask;
+  int64_t mask_b, mask_i;
+  int B, T, H, group;  // group = H / Hkv
+  int row_tiles;       // row tiles of one kv head
+  int ctas;            // CTAs that share the list
+  float scale;         // sm_scale * log2(e)
+  float* part_o;       // [2 * ctas][rows of a tile][D]
+  float2* part_ml;     // [2 * ctas][rows of a tile]
+};
+
+// Context length and fresh tokens of sequence b; returns its key tiles (0 where no row has anything to see).
+__device__ __forceinline__ int sequence(const PagedAttnArgs& a, int b, int& len, int& fresh) {
+  len = a.p.lens[b];
+  fresh = a.counts != nullptr ? a.counts[b] : a.T;
+  if (len < 0 || fresh < 0 || fresh > a.T || (int64_t)len + fresh > ((int64_t)a.p.max_pages << a.p.page_shift)) {
+    raise_invalid(a.p);
+    len = fresh = 0;
+  }
+  return fresh > 0 ? (len + fresh + kTileKeys - 1) / kTileKeys : 0;
+}
+
+// Sum over the CTA's threads before this one; `total` receives the sum over all.
+template <int THREADS>
+__device__ __forceinline__ int64_t scan_before(int64_t v, int64_t* warp_sums, int64_t& total) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  int64_t x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o *= 2) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  total = 0;
+  int64_t before = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) before += warp_sums[w];
+    total += warp_sums[w];
+  }
+  return before + x - v;
+}
+
+// The list's length: key tiles over all sequences, kv heads and row tiles.
+template <int THREADS>
+__device__ __forceinline__ int64_t list_length(const PagedAttnArgs& a, int64_t* warp_sums) {
+  int64_t mine = 0;
+  int len, fresh;
+  for (int b = threadIdx.x; b < a.B; b += THREADS) mine += sequence(a, b, len, fresh);
+  int64_t total;
+  scan_before<THREADS>(mine, warp_sums, total);
+  return total * (a.p.Hkv * a.row_tiles);
+}
+
+__device__ __forceinline__ int sharers(const PagedAttnArgs& a, int64_t list) {
+  return (int)min((int64_t)a.ctas, (list + kMinTiles - 1) / kMinTiles);
+}
+
+// Where the list's element x lies: sequence b and the element's number within the sequence.
+template <int THREADS>
+__device__ __forceinline__ void find(const PagedAttnArgs& a, int64_t x, int64_t* warp_sums, int64_t* found, int& b,
+                                     int64_t& within) {
+  int64_t carry = 0;
+  int len, fresh;
+  const int per = a.p.Hkv * a.row_tiles;
+  for (int base = 0; base < a.B; base += THREADS) {
+    const int mine = base + threadIdx.x;
+    const int64_t v = mine < a.B ? (int64_t)sequence(a, mine, len, fresh) * per : 0;
+    int64_t total;
+    const int64_t at = carry + scan_before<THREADS>(v, warp_sums, total);
+    if (x >= at && x < at + v) found[0] = mine, found[1] = x - at;
+    carry += total;
+    if (x < carry) break;
+  }
+  __syncthreads();
+  b = (int)found[0];
+  within = found[1];
+}
+
+// A place in the list.
+struct Cursor {
+  int b, unit, tile;        // sequence, kv head * row_tiles + row tile, key tile
+  int tiles, len, fresh;    // of the sequence
+};
+
+__device__ __forceinline__ void advance(const PagedAttnArgs& a, Cursor& c) {
+  if (++c.tile < c.tiles) return;
+  c.tile = 0;
+  if (++c.unit < a.p.Hkv * a.row_tiles) return;
+  c.unit = 0;
+  do {
+    ++c.b;
+    c.tiles = c.b < a.B ? sequence(a, c.b, c.len, c.fresh) : 1;
+  } while (c.tiles == 0);
+}
+
+// 2-D tile load: rows `y` ... of a [rows, bytes] tensor, bytes from `x` on.
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+__device__ __forceinline__ void arrive(uint64_t* bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// Bounded wait for a phase of a stage barrier.  Unlike mbar_wait it does not give up on an error that stands in the
+// status word: a bad page of one sequence leaves the others' work as it is.
+__device__ __forceinline__ bool wait_stage(uint64_t* bar, uint32_t parity, volatile int* given_up, int* status) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+  for (uint32_t i = 1; !mbar_try_wait(bar, parity); ++i) {
+    if ((i & 63u) != 0) continue;
+    if (*given_up != 0) return false;
+    if (global_timer_ns() - t0 > kWaitLimitNs) {
+      *given_up = 1;
+      *const_cast<volatile int*>(status) = kStatusTimeout;
+      return false;
+    }
+  }
+  return true;
+}
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Two weights -> an fp16 pair, the largest finite number for what is above it (only weights of zero rows are).
+__device__ __forceinline__ uint32_t pack_weights(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// Transposes an 8 x 8 tile of 16-bit values across the warp (row lane / 4, columns 2 (lane % 4) and the next).
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// Shared-memory tiles, as TMA writes them: 64 rows of K, 64 rows of V, of 128 swizzled bytes (D 256: two such halves), 64
+// swizzled bytes (D 64) or 96 plain ones.  A warp works on groups of 16 keys; lane (n = lane / 4, c = lane % 4) takes the
+// scores of the keys in slots n and n + 8 for the columns 2c and 2c + 1, and after the transposition the weights of the
+// keys in slots 2c, 2c + 1, 2c + 8, 2c + 9 for column n.  slot_key() and first_channel() are chosen so that the lanes of one
+// phase of a shared load touch different banks (D 64 and 96: two-way conflicts are left in V).
+template <int D>
+struct Tile {
+  static constexpr bool kWide = D % 128 == 0;
+  static constexpr int kBox = kWide ? 128 : D;            // bytes of a row in a box
+  static constexpr int kHalves = D / kBox;
+  static constexpr int kBytes = kTileKeys * D;            // of K, and of V
+  static constexpr int kStage = 2 * kBytes;
+  // where byte x of row `row` lies
+  __device__ static int at(int row, int x) {
+    if constexpr (kWide) return x / 128 * (kTileKeys * 128) + row * 128 + ((x % 128) ^ ((row & 7) << 4));
+    if constexpr (D == 64) return row * 64 + (x ^ ((row >> 1 & 3) << 4));
+    return row * D + x;
+  }
+  __device__ static int slot_key(int slot) { return kWide ? (slot & 8) | (slot & 7) >> 1 | (slot & 1) << 2 : slot; }
+  // first of the D / 8 channels (D 256: of either half) whose output lane row n holds
+  __device__ static int first_channel(int n) { return kWide ? ((n >> 1) | (n & 1) << 2) * 16 : n * (D / 8); }
+  // channel of row n + 8 e of the output tile t
+  __device__ static int channel(int n, int t, int e) { return first_channel(n) + (kWide ? t / 8 * 128 + t % 8 * 2 : t * 2) + e; }
+};
+
+// The producer warp's part: loads `todo` tiles from `now` on into a ring of raw stages (K rows, V rows) and their scales
+// (64 of K, 64 of V a stage); a lane per page of the tile.
+template <int D>
+__device__ __forceinline__ void load_tiles(const PagedAttnArgs& a, const CUtensorMap* k_map, const CUtensorMap* v_map,
+                                           Cursor now, int64_t todo, unsigned char* stages, float* scales,
+                                           uint64_t* full, uint64_t* empty, int count, volatile int* given_up) {
+  using S = Tile<D>;
+  const int lane = threadIdx.x % 32;
+  const int box_rows = min(kTileKeys, 1 << a.p.page_shift), boxes = kTileKeys / box_rows;
+  auto lookup = [&](const Cursor& t) -> int64_t {   // cache row of the lane's first key, or -1
+    const int64_t at = (int64_t)t.tile * kTileKeys + lane * box_rows;
+    return lane < boxes && at < t.len + t.fresh ? paged_row(a.p, t.b, t.unit / a.row_tiles, at) : -1;
+  };
+  int64_t row = lookup(now);
+  int slot = 0;
+  uint32_t phase = 0;
+  for (; todo > 0; --todo) {
+    if (!wait_stage(empty + slot, phase ^ 1, given_up, a.p.status)) break;
+    const int there = __popc(__ballot_sync(0xffffffffu, row >= 0));
+    const uint32_t bar = smem_u32(full + slot);
+    if (lane == 0)
+      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(there * box_rows * (2 * D + 8))
+                   : "memory");
+    __syncwarp();
+    if (row >= 0) {
+      const uint32_t k = smem_u32(stages + slot * S::kStage) + lane * box_rows * S::kBox;
+      const uint32_t scale = smem_u32(scales + slot * 2 * kTileKeys + lane * box_rows);
+#pragma unroll
+      for (int h = 0; h < S::kHalves; ++h) {
+        tma_load_2d(k + h * (kTileKeys * 128), k_map, bar, h * 128, (int)row);
+        tma_load_2d(k + S::kBytes + h * (kTileKeys * 128), v_map, bar, h * 128, (int)row);
+      }
+      bulk_load(scale, a.p.ks + row, box_rows * 4, bar);
+      bulk_load(scale + kTileKeys * 4, a.p.vs + row, box_rows * 4, bar);
+    }
+    if (todo > 1) {
+      advance(a, now);
+      row = lookup(now);
+    }
+    if (++slot == count) slot = 0, phase ^= 1;
+  }
+  if (*given_up != 0)   // leave no copy in flight behind
+    for (int s = 0; s < count; ++s) mbar_drain(full + s, s < slot ? phase : phase ^ 1);
+}
+
+inline int sm_count() {
+  int dev = 0, n = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return 148;
+  return n;
+}
+
+// The codes as [rows, D] bytes; a box is the rows of a page that a tile of keys takes, 128 bytes of each (or all of them).
+template <int D>
+inline bool code_map(CUtensorMap* map, const void* base, uint64_t rows, int page_size) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) {
+    set_error("cuTensorMapEncodeTiled is not available from the CUDA driver");
+    return false;
+  }
+  const cuuint64_t dims[2] = {(cuuint64_t)D, rows}, strides[1] = {(cuuint64_t)D};
+  const cuuint32_t box[2] = {(cuuint32_t)Tile<D>::kBox, (cuuint32_t)std::min(page_size, kTileKeys)}, steps[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, steps,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        Tile<D>::kWide ? CU_TENSOR_MAP_SWIZZLE_128B
+                                       : D == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r == CUDA_SUCCESS) return true;
+  set_error("cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return false;
+}
+
+// The kernel for many rows: its CTAs, the rows of its row tiles, and its launch (the join follows by the caller).
+int wide_ctas();
+int wide_rows(int D);
+int launch_paged_wide(const PagedAttnArgs& a, int dtype, cudaStream_t st);
+
+}  // namespace sage

@@ -1,0 +1,545 @@
+// Paged attention for many query rows of a kv head (a tree of drafts, a run of tokens): the arithmetic of
+// sage_paged_attn.cu on tcgen05.
+//
+// A CTA (one per SM) owns QT row tiles of 128 query rows of one kv head and walks its stretch of the list:
+//   softmax warps   one warpgroup per row tile, one thread per row: q to TMEM (fp16), then per key tile S from TMEM,
+//                   weights (fp16) back over S, O rescaled in TMEM when the maximum moves, epilogue
+//   producer warp   TMA of the raw codes and scales into a ring
+//   MMA warp        S_t = Q_t K^T (A from TMEM, fp16), O_t += P_t V (A from TMEM); while row tile 0 is in its softmax,
+//                   row tile 1 is in its products
+//   4 converter warps   int8 and e4m3 codes to fp16 operand tiles in shared memory, once for all QT * 128 rows, and what
+//                   the rows need of each key (factor of its score, log2 of its V scale, the inverse of that)
+// Codes convert exactly, so there is nothing to choose there; with Q and P in TMEM the products read only K and V from
+// shared memory (64 KB a key tile of 64 for D 128 and 256 rows, beside 48 KB that the converters write).
+// TMEM (512 columns): O_t at t D, S_t / P_t at QT D + 64 t, Q_t at QT (D + 64) + t D / 2.
+#include "sage_paged_attn.cuh"
+
+namespace sage {
+
+template <int D>
+struct Wide {
+  static constexpr int QT = D == 256 ? 1 : 2;
+  static constexpr int kSoftmaxWarps = 4 * QT, kConverters = 4;
+  static constexpr int kThreads = 32 * (kSoftmaxWarps + 2 + kConverters);
+  static constexpr int kRows = 128 * QT;
+  static constexpr int kPanels = (D + 63) / 64;            // of 64 channels: 128 bytes a key
+  static constexpr int kPanel = kTileKeys * 128;
+  static constexpr int kOperand = kPanels * kPanel;        // K or V of a tile in fp16
+  static constexpr int kRaw = D == 256 ? 2 : 3;            // ring of raw stages
+  static constexpr int kBufs = D == 256 ? 2 : 3;           // ring of operand tiles
+  static constexpr int kO = 0, kS = QT * D, kQ = kS + QT * kTileKeys;
+  static_assert(kQ + QT * D / 2 <= 512, "TMEM columns");
+  static constexpr int kParams = 4 * kTileKeys;            // floats of a tile: factor, log2 V scale, inverse, gain
+  static constexpr int kSmem = 1024 + kBufs * 2 * kOperand + kRaw * (Tile<D>::kStage + 2 * kTileKeys * 4) +
+                               kBufs * kParams * 4;
+};
+
+// D(tmem) (+)= A(tmem) * B(smem), fp16 operands, fp32 accumulator.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      "}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Instruction descriptor, kind::f16: fp16 A and B, fp32 D; b_mn: B is stored with N contiguous.
+__host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool b_mn) {
+  return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+// Descriptor of an operand stored with N contiguous, 128-byte swizzle: panels of 64 columns `panel` bytes apart, groups of
+// 8 rows (of K) 1024 bytes apart.
+__device__ __forceinline__ uint64_t smem_desc_nmajor(uint32_t smem_addr, uint32_t panel) {
+  return (uint64_t)((smem_addr >> 4) & 0x3FFFu) | ((uint64_t)(panel >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         (1ull << 46) | (2ull << 61);
+}
+
+// Byte of 16-byte chunk `ch` (8 fp16 channels) of key `row` in an operand tile.
+__device__ __forceinline__ int operand_at(int row, int ch) {
+  return ch / 8 * (kTileKeys * 128) + row * 128 + (((ch % 8) ^ (row & 7)) << 4);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(Wide<D>::kThreads, 1)
+    paged_wide_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap k_map,
+                      const __grid_constant__ CUtensorMap v_map) {
+  using W = Wide<D>;
+  using S = Tile<D>;
+  constexpr int QT = W::QT;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ int64_t warp_sums[W::kThreads / 32], found[2];
+  __shared__ uint64_t raw_full[W::kRaw], raw_empty[W::kRaw], k_full[W::kBufs], v_full[W::kBufs], buf_empty[W::kBufs];
+  __shared__ uint64_t s_full[QT], p_full[QT], q_full[QT], o_full[QT], all_done;
+  __shared__ uint32_t tmem_base;
+  __shared__ int given_up, zero_rows[W::kBufs][2];
+  unsigned char* operands = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  unsigned char* stages = operands + W::kBufs * 2 * W::kOperand;
+  float* scales = reinterpret_cast<float*>(stages + W::kRaw * S::kStage);
+  float* params = scales + W::kRaw * 2 * kTileKeys;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (tid == 0) {
+    given_up = 0;
+    for (int i = 0; i < W::kRaw; ++i) mbar_init(raw_full + i, 1), mbar_init(raw_empty + i, W::kConverters);
+    for (int i = 0; i < W::kBufs; ++i) {
+      mbar_init(k_full + i, W::kConverters);
+      mbar_init(v_full + i, W::kConverters);
+      mbar_init(buf_empty + i, 1);
+    }
+    for (int t = 0; t < QT; ++t) {
+      mbar_init(s_full + t, 1);
+      mbar_init(p_full + t, 4);
+      mbar_init(q_full + t, 4);
+      mbar_init(o_full + t, 1);
+    }
+    mbar_init(&all_done, 1);
+    fence_barrier_init();
+  }
+
+  const int64_t list = list_length<W::kThreads>(a, warp_sums);
+  const int share = sharers(a, list);
+  if ((int)blockIdx.x >= share) return;
+  if (warp == 0) {
+    tmem_alloc(&tmem_base, 512);
+    tmem_relinquish();
+  }
+  const int64_t first = (int64_t)blockIdx.x * list / share, end = (int64_t)(blockIdx.x + 1) * list / share;
+  Cursor now;
+  {
+    int64_t within;
+    tc_fence_before();
+    find<W::kThreads>(a, first, warp_sums, found, now.b, within);   // ends with a barrier of the CTA
+    tc_fence_after();
+    now.tiles = sequence(a, now.b, now.len, now.fresh);
+    now.unit = (int)(within / now.tiles);
+    now.tile = (int)(within - (int64_t)now.unit * now.tiles);
+  }
+  int64_t todo = end - first;
+  const uint32_t tmem = tmem_base;
+  // whether row tile t of the unit holds a live row
+  auto active = [&](const Cursor& c, int t) { return c.unit % a.row_tiles * W::kRows + t * 128 < c.fresh * a.group; };
+
+  if (warp == W::kSoftmaxWarps) {
+    load_tiles<D>(a, &k_map, &v_map, now, todo, stages, scales, raw_full, raw_empty, W::kRaw, &given_up);
+  } else if (warp == W::kSoftmaxWarps + 1) {
+    // ------------------------------------------------------------------------------------------------ products
+    if (lane == 0) {
+      constexpr uint32_t kScores = idesc_f16(128, kTileKeys, false), kValues = idesc_f16(128, D, true);
+      int buf = 0;
+      uint32_t phase = 0, p_phase[QT] = {}, q_phase[QT] = {};
+      bool begins = true;
+      auto scores = [&](int t, int b) {
+        const uint32_t k = smem_u32(operands + b * 2 * W::kOperand);
+#pragma unroll
+        for (int s = 0; s < D / 16; ++s)
+          mma_f16_ts(tmem + W::kS + t * kTileKeys, tmem + W::kQ + t * (D / 2) + s * 8,
+                     smem_desc_kmajor(k + s / 4 * W::kPanel + s % 4 * 32, 128), kScores, s > 0);
+        tc_commit(s_full + t);
+      };
+      for (; todo > 0; --todo) {
+        bool act[QT];
+        int last = -1;
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+          act[t] = active(now, t);
+          if (act[t]) last = t;
+        }
+        if (begins) {
+          wait_stage(k_full + buf, phase, &given_up, a.p.status);
+#pragma unroll
+          for (int t = 0; t < QT; ++t)
+            if (act[t]) {
+              wait_stage(q_full + t, q_phase[t], &given_up, a.p.status);
+              q_phase[t] ^= 1;
+              tc_fence_after();
+              scores(t, buf);
+            }
+        }
+        const bool more = todo > 1 && now.tile + 1 < now.tiles;
+        const int next = buf + 1 == W::kBufs ? 0 : buf + 1;
+        const uint32_t next_phase = next == 0 ? phase ^ 1 : phase;
+        wait_stage(v_full + buf, phase, &given_up, a.p.status);
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+          if (act[t]) {
+            wait_stage(p_full + t, p_phase[t], &given_up, a.p.status);
+            p_phase[t] ^= 1;
+            tc_fence_after();
+            const uint32_t v = smem_u32(operands + buf * 2 * W::kOperand + W::kOperand);
+#pragma unroll
+            for (int s = 0; s < kTileKeys / 16; ++s)
+              mma_f16_ts(tmem + W::kO + t * D, tmem + W::kS + t * kTileKeys + s * 8,
+                         smem_desc_nmajor(v + s * 2048, W::kPanel), kValues, !begins || s > 0);
+            if (t == last) tc_commit(buf_empty + buf);
+            if (more) {
+              if (wait_stage(k_full + next, next_phase, &given_up, a.p.status)) tc_fence_after();
+              scores(t, next);
+            } else {
+              tc_commit(o_full + t);
+            }
+          }
+        if (last < 0) tc_commit(buf_empty + buf);   // no row of this row tile is live
+        begins = !more;
+        buf = next, phase = next_phase;
+        if (todo > 1) advance(a, now);
+      }
+      tc_commit(&all_done);   // nothing is in flight when the CTA ends
+      wait_stage(&all_done, 0, &given_up, a.p.status);
+    }
+    __syncwarp();
+  } else if (warp >= W::kSoftmaxWarps + 2) {
+    // ------------------------------------------------------------------------------------------------ converters
+    const int ct = tid - 32 * (W::kSoftmaxWarps + 2), cw = ct / 32;
+    int raw = 0, buf = 0;
+    uint32_t raw_phase = 0, phase = 0;
+    // The eight lanes of a phase of a 16-byte access take four neighbouring chunks of a raw row and of the row that
+    // differs in bits 0 and 2: different banks in the raw tile (bit 2) and in the operand tile (bit 0), whose rows are
+    // twice as long.
+    constexpr int kItems = kTileKeys * (D / 16) / 128;
+    auto place = [&](int i, int& row, int& ch) {
+      const int item = ct + i * 128;
+      if constexpr (D == 96) {
+        row = item / 6, ch = item % 6;
+      } else {
+        constexpr int kQuads = D / 64;
+        const int g = item / 8, pair = g / kQuads;
+        ch = g % kQuads * 4 + item % 4;
+        row = (pair / 4 * 8 + pair % 4) ^ (item / 4 % 2 * 5);
+      }
+    };
+    for (; todo > 0; --todo) {
+      const int key0 = now.tile * kTileKeys, total = now.len + now.fresh;
+      wait_stage(raw_full + raw, raw_phase, &given_up, a.p.status);
+      wait_stage(buf_empty + buf, phase ^ 1, &given_up, a.p.status);
+      const unsigned char* kt = stages + raw * S::kStage;
+      unsigned char* to = operands + buf * 2 * W::kOperand;
+      if (ct < kTileKeys) {
+        const float* sc = scales + raw * 2 * kTileKeys;
+        float* out = params + buf * W::kParams;
+        const float vs = sc[kTileKeys + ct];
+        const bool there = key0 + ct < total, zero = there && vs == 0.0f;
+        out[ct] = there ? sc[ct] * a.scale : 0.0f;
+        out[kTileKeys + ct] = !there ? -INFINITY : zero ? kZeroLog : __log2f(vs);
+        out[2 * kTileKeys + ct] = !there ? 0.0f : zero ? 1.0f : __fdividef(1.0f, vs);
+        out[3 * kTileKeys + ct] = zero ? -kZeroLog : 0.0f;
+        const bool any = __any_sync(0xffffffffu, zero);
+        if (lane == 0) zero_rows[buf][cw] = any;
+      }
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) {
+        int row, ch;
+        place(i, row, ch);
+        const uint4 v = *reinterpret_cast<const uint4*>(kt + S::at(row, ch * 16));
+        uint4 x, y;
+        int8_to_f16(v.x, x.x, x.y), int8_to_f16(v.y, x.z, x.w), int8_to_f16(v.z, y.x, y.y), int8_to_f16(v.w, y.z, y.w);
+        *reinterpret_cast<uint4*>(to + operand_at(row, 2 * ch)) = x;
+        *reinterpret_cast<uint4*>(to + operand_at(row, 2 * ch + 1)) = y;
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) arrive(k_full + buf);
+      const bool drafts = key0 + kTileKeys > now.len;
+#pragma unroll
+      for (int i = 0; i < kItems; ++i) {
+        int row, ch;
+        place(i, row, ch);
+        uint4 v = *reinterpret_cast<const uint4*>(kt + S::kBytes + S::at(row, ch * 16));
+        if (drafts) {
+          // codes behind the last key are anything, and a NaN code of a draft that its reader does not see must not
+          // reach it through 0 * NaN: both are cleared
+          if (key0 + row >= total) v = make_uint4(0, 0, 0, 0);
+          if (key0 + row >= now.len) {
+            v.x &= ~__vcmpeq4(v.x & 0x7f7f7f7fu, 0x7f7f7f7fu);
+            v.y &= ~__vcmpeq4(v.y & 0x7f7f7f7fu, 0x7f7f7f7fu);
+            v.z &= ~__vcmpeq4(v.z & 0x7f7f7f7fu, 0x7f7f7f7fu);
+            v.w &= ~__vcmpeq4(v.w & 0x7f7f7f7fu, 0x7f7f7f7fu);
+          }
+        }
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        uint32_t x[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[2 * k] = e4m3_to_f16((uint16_t)w[k]), x[2 * k + 1] = e4m3_to_f16((uint16_t)(w[k] >> 16));
+        *reinterpret_cast<uint4*>(to + W::kOperand + operand_at(row, 2 * ch)) = make_uint4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<uint4*>(to + W::kOperand + operand_at(row, 2 * ch + 1)) = make_uint4(x[4], x[5], x[6], x[7]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) arrive(v_full + buf), arrive(raw_empty + raw);
+      if (++raw == W::kRaw) raw = 0, raw_phase ^= 1;
+      if (++buf == W::kBufs) buf = 0, phase ^= 1;
+      if (todo > 1) advance(a, now);
+    }
+  } else {
+    // ------------------------------------------------------------------------------------------------ softmax
+    const int t = warp / 4;
+    const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;   // of TMEM
+    const uint32_t s_at = tmem + lanes + W::kS + t * kTileKeys, o_at = tmem + lanes + W::kO + t * D;
+    int buf = 0, token = 0, head = 0, row = 0, segment = 0, first_tile = 0;
+    uint32_t phase = 0, s_phase = 0, o_phase = 0;
+    float m = 0.0f, l = 0.0f, row_scale = 1.0f;
+    bool begins = true, act = false, warp_live = false;
+    for (; todo > 0; --todo) {
+      if (begins) {
+        first_tile = now.tile;
+        act = active(now, t);
+        row = now.unit % a.row_tiles * W::kRows + t * 128 + warp % 4 * 32 + lane;
+        token = row / a.group;
+        head = now.unit / a.row_tiles * a.group + row % a.group;
+        warp_live = row - lane < now.fresh * a.group;
+        m = -3.402823466e38f, l = 0.0f;
+        if (act) {
+          if (warp_live) {
+            // the row in fp16, scaled by a power of two of its largest value, as D / 2 TMEM columns
+            const bool live = token < now.fresh;
+            const T* src = static_cast<const T*>(a.q) + now.b * a.q_st.b + token * a.q_st.s + head * a.q_st.h;
+            float inverse = 1.0f;
+            if constexpr (!std::is_same<T, __half>::value) {
+              uint32_t top = 0;
+              if (live) {
+#pragma unroll 4
+                for (int i = 0; i < D / 8; ++i) {
+                  const uint4 v = *reinterpret_cast<const uint4*>(src + 8 * i);
+                  top = __vmaxu2(top, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
+                                               __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
+                }
+              }
+              top = max(top & 0xffffu, top >> 16);
+              // 2^e with e the exponent of that value (zero, infinite and NaN rows: 1; tiny ones: 2^-100)
+              const int e = top == 0 || top >= 0x7f80u ? 127 : max((int)(top >> 7), 27);
+              row_scale = __int_as_float(e << 23);
+              inverse = __int_as_float((254 - e) << 23);
+            }
+#pragma unroll 1
+            for (int i = 0; i < D / 32; ++i) {   // 32 channels: 16 columns
+              uint32_t w[16];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const uint4 v = live ? *reinterpret_cast<const uint4*>(src + 32 * i + 8 * k) : make_uint4(0, 0, 0, 0);
+                if constexpr (std::is_same<T, __half>::value) {
+                  w[4 * k] = v.x, w[4 * k + 1] = v.y, w[4 * k + 2] = v.z, w[4 * k + 3] = v.w;
+                } else {
+                  float x[8];
+                  unpack8(v, x, T());
+#pragma unroll
+                  for (int z = 0; z < 4; ++z) w[4 * k + z] = pack2(x[2 * z] * inverse, x[2 * z + 1] * inverse, __half());
+                }
+              }
+              asm volatile(
+                  "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+                  "%15, %16};" ::"r"(tmem + lanes + W::kQ + t * (D / 2) + i * 16),
+                  "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "r"(w[8]),
+                  "r"(w[9]), "r"(w[10]), "r"(w[11]), "r"(w[12]), "r"(w[13]), "r"(w[14]), "r"(w[15])
+                  : "memory");
+            }
+            tmem_wait_st();
+            tc_fence_before();
+          }
+          __syncwarp();
+          if (lane == 0) arrive(q_full + t);
+        }
+      }
+      const bool last_tile = now.tile + 1 == now.tiles, ends = last_tile || todo == 1;
+      if (act) {
+        wait_stage(s_full + t, s_phase, &given_up, a.p.status);
+        s_phase ^= 1;
+        if (warp_live) {
+          wait_stage(k_full + buf, phase, &given_up, a.p.status);   // long there: orders the reads of params and zero_rows
+          tc_fence_after();
+          const float* factor = params + buf * W::kParams;
+          const int key0 = now.tile * kTileKeys;
+          const bool drafts = key0 + kTileKeys > now.len;
+          const bool special = drafts || (zero_rows[buf][0] | zero_rows[buf][1]) != 0;
+          uint64_t x[kTileKeys / 2];   // two scores each
+          {
+            uint32_t r[2][32];
+            tmem_ld32(s_at, r[0]);
+            tmem_ld32(s_at + 32, r[1]);
+            tmem_wait_ld();
+            const uint64_t scale2 = f2_pack(row_scale, row_scale);
+#pragma unroll
+            for (int i = 0; i < kTileKeys / 4; ++i) {
+              const float4 f = *reinterpret_cast<const float4*>(factor + 4 * i);
+              const float4 g = *reinterpret_cast<const float4*>(factor + kTileKeys + 4 * i);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int c = 4 * i + 2 * h;
+                uint64_t v = f2_pack(__uint_as_float(r[c / 32][c % 32]), __uint_as_float(r[c / 32][c % 32 + 1]));
+                if constexpr (!std::is_same<T, __half>::value) v = f2_mul(v, scale2);
+                x[c / 2] = f2_fma(v, h ? f2_pack(f.z, f.w) : f2_pack(f.x, f.y), h ? f2_pack(g.z, g.w) : f2_pack(g.x, g.y));
+              }
+            }
+          }
+          if (drafts) {
+            const uint8_t* mask = a.mask != nullptr && token < now.fresh ? a.mask + now.b * a.mask_b + token * a.mask_i : nullptr;
+#pragma unroll
+            for (int i = 0; i < kTileKeys / 2; ++i) {
+              float v[2];
+              f2_unpack(x[i], v[0], v[1]);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int d = key0 + 2 * i + e - now.len;
+                const bool seen = d < 0 || (d < now.fresh && token < now.fresh && (mask != nullptr ? mask[d] != 0 : d <= token));
+                if (!seen) v[e] = -INFINITY;
+              }
+              x[i] = f2_pack(v[0], v[1]);
+            }
+          }
+          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < kTileKeys / 2; ++i) {
+            float u, v;
+            f2_unpack(x[i], u, v);
+            top[i % 4] = fmaxf(fmaxf(top[i % 4], u), v);
+          }
+          const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+          if (__any_sync(0xffffffffu, most > m + 8.0f)) {
+            const float next = most > m + 8.0f ? most : m;
+            const float keep = next == m ? 1.0f : fast_exp2(m - next);
+            m = next;
+            l *= keep;
+            if (now.tile != first_tile) {   // the first product of a row tile overwrites O
+              const uint64_t keep2 = f2_pack(keep, keep);
+#pragma unroll 1
+              for (int i = 0; i < D / 32; ++i) {
+                uint32_t r[32];
+                tmem_ld32(o_at + 32 * i, r);
+                tmem_wait_ld();
+#pragma unroll
+                for (int k = 0; k < 32; k += 2) {
+                  float u, v;
+                  f2_unpack(f2_mul(f2_pack(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), keep2), u, v);
+                  r[k] = __float_as_uint(u), r[k + 1] = __float_as_uint(v);
+                }
+                tmem_st32(o_at + 32 * i, r);
+              }
+            }
+          }
+          const uint64_t minus_m = f2_pack(-m, -m);
+          uint64_t sum = f2_pack(l, 0.0f);
+          uint32_t packed[32];
+#pragma unroll
+          for (int i = 0; i < kTileKeys / 4; ++i) {
+            const float4 inv = *reinterpret_cast<const float4*>(factor + 2 * kTileKeys + 4 * i);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int c = 2 * i + h;
+              float u, v;
+              f2_unpack(f2_add(x[c], minus_m), u, v);
+              uint64_t w = h ? f2_pack(inv.z, inv.w) : f2_pack(inv.x, inv.y);
+              if (special) {
+                u += factor[3 * kTileKeys + 2 * c], v += factor[3 * kTileKeys + 2 * c + 1];
+                // an unseen key's inverse scale may be NaN
+                float p, q, wu, wv;
+                f2_unpack(x[c], p, q);
+                f2_unpack(w, wu, wv);
+                w = f2_pack(p == -INFINITY ? 0.0f : wu, q == -INFINITY ? 0.0f : wv);
+              }
+              u = fast_exp2(u), v = fast_exp2(v);
+              sum = f2_fma(f2_pack(u, v), w, sum);
+              packed[c] = pack_weights(u, v);
+            }
+          }
+          float u, v;
+          f2_unpack(sum, u, v);
+          l = u + v;
+          tmem_st32(s_at, packed);
+          tmem_wait_st();
+          tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) arrive(p_full + t);
+      }
+      if (ends) {
+        // the row tile ends here, or this CTA's part of it does
+        const bool whole = last_tile && first_tile == 0, mine = row < a.T * a.group, live = token < now.fresh;
+        if (act) {
+          wait_stage(o_full + t, o_phase, &given_up, a.p.status);
+          o_phase ^= 1;
+          tc_fence_after();
+        }
+        T* dst = static_cast<T*>(a.out) + now.b * a.out_st.b + token * a.out_st.s + head * a.out_st.h;
+        const int64_t at = (2 * (int64_t)blockIdx.x + (segment > 0)) * W::kRows + t * 128 + warp % 4 * 32 + lane;
+        const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+        if (act && warp_live) {
+#pragma unroll 1
+          for (int i = 0; i < D / 32; ++i) {
+            uint32_t r[32];
+            tmem_ld32(o_at + 32 * i, r);
+            tmem_wait_ld();
+            if (mine && whole) {
+#pragma unroll
+              for (int k = 0; k < 32; k += 8) {
+                float x[8];
+#pragma unroll
+                for (int z = 0; z < 8; ++z) x[z] = live && l != 0.0f ? __uint_as_float(r[k + z]) * inverse : 0.0f;
+                store8(dst + 32 * i + k, x);
+              }
+            } else if (mine && live) {
+#pragma unroll
+              for (int k = 0; k < 32; k += 4)
+                *reinterpret_cast<uint4*>(a.part_o + at * D + 32 * i + k) = make_uint4(r[k], r[k + 1], r[k + 2], r[k + 3]);
+            }
+          }
+          tc_fence_before();
+        } else if (mine && whole) {
+          for (int i = 0; i < D / 8; ++i) *reinterpret_cast<uint4*>(dst + 8 * i) = make_uint4(0, 0, 0, 0);
+        }
+        if (mine && whole) {
+          if (a.lse != nullptr)
+            a.lse[((int64_t)now.b * a.H + head) * a.T + token] =
+                !live || l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+        } else if (mine && live) {
+          a.part_ml[at] = make_float2(m, l);
+        }
+        ++segment;
+      }
+      begins = ends;
+      if (++buf == W::kBufs) buf = 0, phase ^= 1;
+      if (todo > 1) advance(a, now);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 0) tmem_dealloc(tmem, 512);
+}
+
+int wide_ctas() { return sm_count(); }
+int wide_rows(int D) { return D == 256 ? 128 : 256; }
+
+template <typename T, int D>
+static int launch_wide(const PagedAttnArgs& a, cudaStream_t st) {
+  using W = Wide<D>;
+  CUtensorMap k_map, v_map;
+  const uint64_t rows = (uint64_t)a.p.num_pages * a.p.Hkv << a.p.page_shift;
+  if (!code_map<D>(&k_map, a.p.k8, rows, 1 << a.p.page_shift) || !code_map<D>(&v_map, a.p.v8, rows, 1 << a.p.page_shift))
+    return SAGE_ERR_LAUNCH;
+  static std::atomic<uint64_t> prepared{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !(prepared.load() >> dev & 1))) {
+    e = cudaFuncSetAttribute(paged_wide_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, W::kSmem);
+    if (e == cudaSuccess && dev < 64) prepared.fetch_or(uint64_t(1) << dev);
+  }
+  if (e == cudaSuccess) {
+    paged_wide_kernel<T, D><<<a.ctas, W::kThreads, W::kSmem, st>>>(a, k_map, v_map);
+    e = cudaGetLastError();
+  }
+  if (e == cudaSuccess) return SAGE_OK;
+  set_error("paged attention: %s", cudaGetErrorString(e));
+  return SAGE_ERR_LAUNCH;
+}
+
+int launch_paged_wide(const PagedAttnArgs& a, int dtype, cudaStream_t st) {
+  return by_head_dim(a.p.D, [&](auto d) {
+    constexpr int kD = decltype(d)::value;
+    return dtype == SAGE_BF16 ? launch_wide<__nv_bfloat16, kD>(a, st) : launch_wide<__half, kD>(a, st);
+  });
+}
+
+}  // namespace sage
