@@ -211,11 +211,12 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
         const float vs = ks[kTileKeys + keys[h]];
         factor[h] = ks[keys[h]] * a.scale;
         log_v[h] = __log2f(vs);
-        inverse_v[h] = __fdividef(1.0f, vs);
+        // finite whatever the scale is (unwritten memory): rows that see a NaN scale are NaN by its logarithm, and rows that do
+        // not see the key must not meet 0 * NaN or 0 * infinity here
+        inverse_v[h] = vs > 0x1p-120f ? __fdividef(1.0f, vs) : 0x1p120f;
         gain[h] = 0.0f;
         if (vs == 0.0f) zero = true, log_v[h] = kZeroLog, inverse_v[h] = 1.0f, gain[h] = -kZeroLog;
       }
-      const bool special = drafts || __any_sync(0xffffffffu, zero);
       bool more = false;
 #pragma unroll
       for (int r = 0; r < NR; ++r)
@@ -254,6 +255,12 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
           for (int t = 0; t < NT; ++t) o[r][t][0] *= keep[0], o[r][t][1] *= keep[1], o[r][t][2] *= keep[0], o[r][t][3] *= keep[1];
         }
       }
+      if (__any_sync(0xffffffffu, zero)) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) s[r][x] += gain[x / 2];
+      }
       uint32_t pf[NR][2];
 #pragma unroll
       for (int r = 0; r < NR; ++r)
@@ -262,10 +269,8 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
           float p[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float x = s[r][2 * h + e];
-            p[e] = fast_exp2(special ? x - m[r][e] + gain[h] : x - m[r][e]);
-            // an unseen key's inverse scale may be NaN
-            if (!special || x != -INFINITY) l[r][e] = fmaf(p[e], inverse_v[h], l[r][e]);
+            p[e] = fast_exp2(s[r][2 * h + e] - m[r][e]);
+            l[r][e] = fmaf(p[e], inverse_v[h], l[r][e]);
           }
           pf[r][h] = transposed(pack_weights(p[0], p[1]));
         }

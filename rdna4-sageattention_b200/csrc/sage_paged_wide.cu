@@ -225,7 +225,9 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
         const bool there = key0 + ct < total, zero = there && vs == 0.0f;
         out[ct] = there ? sc[ct] * a.scale : 0.0f;
         out[kTileKeys + ct] = !there ? -INFINITY : zero ? kZeroLog : __log2f(vs);
-        out[2 * kTileKeys + ct] = !there ? 0.0f : zero ? 1.0f : __fdividef(1.0f, vs);
+        // finite whatever the scale is (unwritten memory): rows that see a NaN scale are NaN by its logarithm, and rows that do
+        // not see the key must not meet 0 * NaN or 0 * infinity here
+        out[2 * kTileKeys + ct] = !there ? 0.0f : zero ? 1.0f : vs > 0x1p-120f ? __fdividef(1.0f, vs) : 0x1p120f;
         out[3 * kTileKeys + ct] = zero ? -kZeroLog : 0.0f;
         const bool any = __any_sync(0xffffffffu, zero);
         if (lane == 0) zero_rows[buf][cw] = any;
@@ -353,7 +355,6 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
           const float* factor = params + buf * W::kParams;
           const int key0 = now.tile * kTileKeys;
           const bool drafts = key0 + kTileKeys > now.len;
-          const bool special = drafts || (zero_rows[buf][0] | zero_rows[buf][1]) != 0;
           uint64_t x[kTileKeys / 2];   // two scores each
           {
             uint32_t r[2][32];
@@ -419,8 +420,15 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
               }
             }
           }
+          if ((zero_rows[buf][0] | zero_rows[buf][1]) != 0) {
+#pragma unroll
+            for (int i = 0; i < kTileKeys / 4; ++i) {
+              const float4 g = *reinterpret_cast<const float4*>(factor + 3 * kTileKeys + 4 * i);
+              x[2 * i] = f2_add(x[2 * i], f2_pack(g.x, g.y)), x[2 * i + 1] = f2_add(x[2 * i + 1], f2_pack(g.z, g.w));
+            }
+          }
           const uint64_t minus_m = f2_pack(-m, -m);
-          uint64_t sum = f2_pack(l, 0.0f);
+          uint64_t sum[2] = {f2_pack(l, 0.0f), f2_pack(0.0f, 0.0f)};
           uint32_t packed[32];
 #pragma unroll
           for (int i = 0; i < kTileKeys / 4; ++i) {
@@ -430,22 +438,13 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
               const int c = 2 * i + h;
               float u, v;
               f2_unpack(f2_add(x[c], minus_m), u, v);
-              uint64_t w = h ? f2_pack(inv.z, inv.w) : f2_pack(inv.x, inv.y);
-              if (special) {
-                u += factor[3 * kTileKeys + 2 * c], v += factor[3 * kTileKeys + 2 * c + 1];
-                // an unseen key's inverse scale may be NaN
-                float p, q, wu, wv;
-                f2_unpack(x[c], p, q);
-                f2_unpack(w, wu, wv);
-                w = f2_pack(p == -INFINITY ? 0.0f : wu, q == -INFINITY ? 0.0f : wv);
-              }
               u = fast_exp2(u), v = fast_exp2(v);
-              sum = f2_fma(f2_pack(u, v), w, sum);
+              sum[h] = f2_fma(f2_pack(u, v), h ? f2_pack(inv.z, inv.w) : f2_pack(inv.x, inv.y), sum[h]);
               packed[c] = pack_weights(u, v);
             }
           }
           float u, v;
-          f2_unpack(sum, u, v);
+          f2_unpack(f2_add(sum[0], sum[1]), u, v);
           l = u + v;
           tmem_st32(s_at, packed);
           tmem_wait_st();

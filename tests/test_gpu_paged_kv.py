@@ -259,22 +259,27 @@ def test_masks_that_leave_nothing_and_shared_masks():
     check_attention(q, cache, table, lens, torch.ones_like(mask))                # drafts may see what comes after them
 
 
-def test_masked_rows_may_hold_anything():
+@pytest.mark.parametrize("H", [2, 4, 16])                               # 24, 48 and 192 rows of a kv head
+def test_masked_rows_may_hold_anything(H):
     # NaN and infinities at drafts that nothing sees, and behind the last token, stay where they are
     T, lens, page = 24, [37, 0], 16
     cache, table = filled(lens, T, page, 2, 64)
     mask = trees(2, T)
     dead = 9
     mask[:, :, dead] = False
-    q = queries(2, T, 4, 64)
+    q = queries(2, T, H, 64)
     a, _ = check_attention(q, cache, table, lens, mask)
-    for b in range(2):
-        p, r = P.place(cache, table, b, [lens[b] + dead])
-        for name in ("ks", "vs"):
-            cache[name][p, :, r] = math.nan if b else math.inf
-        cache["v8"].view(torch.uint8)[p, :, r] = 0x7f
-    b_, _ = check_attention(q, cache, table, lens, mask)
-    assert torch.equal(a, b_)
+    for junk in (math.nan, math.inf, -math.inf, -1e-40, 1e-40, -3.0, 0.0, 3e38):
+        for b in range(2):
+            p, r = P.place(cache, table, b, [lens[b] + dead])
+            for name in ("ks", "vs"):
+                cache[name][p, :, r] = junk
+            cache["v8"].view(torch.uint8)[p, :, r] = 0x7f
+        # behind the last token too, in the rest of the page
+        p, r = P.place(cache, table, 1, range(T, 2 * page))
+        cache["vs"][p, :, r] = junk
+        b_, _ = check_attention(q, cache, table, lens, mask)
+        assert torch.equal(a, b_), junk
     # a visible NaN reaches the rows that see it, and only those
     p, r = P.place(cache, table, 0, [lens[0] + 2])
     cache["ks"][p, :, r] = math.nan
