@@ -410,38 +410,44 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
   }
 }
 
-// Joins the partial rows of the row tiles that fell to several CTAs, and writes the rows that see nothing at all.  A warp
-// takes a row; the CTAs of a row tile are joined in the order of its keys.
+// Which CTAs share row tile `unit` of sequence b, found by all threads of a join block: CTAs c0 .. c1, c0 with its partial
+// slot `slot`, the others with slot 0.  Returns its key tiles.
+__device__ __forceinline__ int sharing(const PagedAttnArgs& a, int b, int unit, int64_t* warp_sums, int& fresh, int& c0,
+                                       int& c1, int& slot) {
+  const int per = a.p.Hkv * a.row_tiles;
+  int len;
+  int64_t mine = 0, before = 0, list, start;
+  for (int s = threadIdx.x; s < a.B; s += kJoinThreads) {
+    const int t = sequence(a, s, len, fresh);
+    mine += t;
+    if (s < b) before += t;
+  }
+  scan_before<kJoinThreads>(mine, warp_sums, list);
+  scan_before<kJoinThreads>(before, warp_sums, start);
+  const int tiles = sequence(a, b, len, fresh);
+  list *= per;
+  start = start * per + (int64_t)unit * tiles;
+  c0 = c1 = slot = 0;
+  if (tiles > 0) {
+    const int share = sharers(a, list);
+    c0 = (int)(((start + 1) * share - 1) / list);
+    c1 = (int)(((start + tiles) * share - 1) / list);
+    slot = (int64_t)c0 * list / share < start ? 1 : 0;   // not the first row tile of CTA c0
+  }
+  return tiles;
+}
+
+// Joins the partial rows of the row tiles that fell to several CTAs, and writes the rows that see nothing at all; the CTAs
+// of a row tile are joined in the order of its keys.  A warp takes a row.
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAttnArgs a, int tile_rows, int blocks_per_unit) {
   __shared__ int64_t warp_sums[kJoinThreads / 32];
   const int64_t id = blockIdx.x / blocks_per_unit;
   const int per = a.p.Hkv * a.row_tiles, b = (int)(id / per), unit = (int)(id - (int64_t)b * per);
-  int len, fresh;
-  const int tiles = sequence(a, b, len, fresh);
-  int64_t mine = 0, before = 0;
-  {
-    int x, y;
-    for (int s = threadIdx.x; s < a.B; s += kJoinThreads) {
-      const int t = sequence(a, s, x, y);
-      mine += t;
-      if (s < b) before += t;
-    }
-  }
-  int64_t list, start;
-  scan_before<kJoinThreads>(mine, warp_sums, list);
-  scan_before<kJoinThreads>(before, warp_sums, start);
-  list *= per;
-  start = start * per + (int64_t)unit * tiles;
+  int fresh, c0, c1, slot;
+  const int tiles = sharing(a, b, unit, warp_sums, fresh, c0, c1, slot);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  int c0 = 0, c1 = 0, slot = 0;
-  if (tiles > 0) {
-    const int share = sharers(a, list);
-    c0 = (int)(((start + 1) * share - 1) / list);
-    c1 = (int)(((start + tiles) * share - 1) / list);
-    if (c0 == c1) return;                                       // the CTA wrote the rows itself
-    slot = (int64_t)c0 * list / share < start ? 1 : 0;          // not the first row tile of CTA c0
-  }
+  if (tiles > 0 && c0 == c1) return;   // the CTA wrote the rows itself
   const int lane = threadIdx.x % 32;
   for (int row = blockIdx.x % blocks_per_unit * (kJoinThreads / 32) + threadIdx.x / 32; row < tile_rows;
        row += blocks_per_unit * (kJoinThreads / 32)) {
@@ -489,6 +495,53 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAtt
   }
 }
 
+// The same for the partial rows of the kernel for many rows (four channels of all rows, then the next four): a block takes
+// 32 rows, a lane a row, a warp a quarter of its channels.
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads) wide_join_kernel(const PagedAttnArgs a, int tile_rows, int blocks_per_unit) {
+  __shared__ int64_t warp_sums[kJoinThreads / 32];
+  const int64_t id = blockIdx.x / blocks_per_unit;
+  const int per = a.p.Hkv * a.row_tiles, b = (int)(id / per), unit = (int)(id - (int64_t)b * per);
+  int fresh, c0, c1, slot;
+  const int tiles = sharing(a, b, unit, warp_sums, fresh, c0, c1, slot);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (tiles > 0 && c0 == c1) return;   // the CTA wrote the rows itself
+  constexpr int kChannels = D / 4;     // of a warp
+  const int lane = threadIdx.x % 32, d0 = threadIdx.x / 32 * kChannels;
+  const int row = blockIdx.x % blocks_per_unit * 32 + lane, r = unit % a.row_tiles * tile_rows + row;
+  if (r >= a.T * a.group) return;
+  const int token = r / a.group, head = unit / a.row_tiles * a.group + r % a.group;
+  const bool live = tiles > 0 && token < fresh;
+  float top = -3.402823466e38f, sum = 0.0f, o[kChannels];
+#pragma unroll
+  for (int i = 0; i < kChannels; ++i) o[i] = 0.0f;
+  if (live) {
+    for (int x = c0; x <= c1; ++x)
+      top = fmaxf(top, a.part_ml[(2 * (int64_t)x + (x == c0 ? slot : 0)) * tile_rows + row].x);
+    for (int x = c0; x <= c1; ++x) {
+      const int64_t first = (2 * (int64_t)x + (x == c0 ? slot : 0)) * tile_rows;
+      const float2 ml = a.part_ml[first + row];
+      const float f = fast_exp2(ml.x - top);
+      sum = fmaf(f, ml.y, sum);
+      const float* part = a.part_o + first * D + (int64_t)d0 * tile_rows + row * 4;
+#pragma unroll
+      for (int i = 0; i < kChannels; i += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(part + i * tile_rows);
+        o[i] = fmaf(f, v.x, o[i]), o[i + 1] = fmaf(f, v.y, o[i + 1]);
+        o[i + 2] = fmaf(f, v.z, o[i + 2]), o[i + 3] = fmaf(f, v.w, o[i + 3]);
+      }
+    }
+  }
+  const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+  for (int i = 0; i < kChannels; ++i) o[i] *= inverse;
+  T* dst = static_cast<T*>(a.out) + b * a.out_st.b + token * a.out_st.s + head * a.out_st.h + d0;
+#pragma unroll
+  for (int i = 0; i < kChannels; i += 8) store8(dst + i, o + i);
+  if (a.lse != nullptr && d0 == 0)
+    a.lse[((int64_t)b * a.H + head) * a.T + token] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+}
+
 // Row tiles: the smallest that hold the rows of a kv head, 64 rows (D 256: 32) at the most.  Columns come in eights, so a
 // single token of up to eight heads a group takes one column tile; two a warp share the converted codes, four do not fit
 // the registers, and D 256 has room for one.
@@ -530,9 +583,9 @@ static int launch_paged_attn(const PagedAttnArgs& a, cudaStream_t st) {
 }
 
 template <typename T, int D>
-static int launch_join(const PagedAttnArgs& a, int tile_rows, cudaStream_t st) {
-  const int used = std::min(tile_rows, a.T * a.group);
-  const int blocks = (used + kJoinThreads / 32 - 1) / (kJoinThreads / 32);
+static int launch_join(const PagedAttnArgs& a, int tile_rows, bool many, cudaStream_t st) {
+  const int used = std::min(tile_rows, a.T * a.group), per_block = many ? 32 : kJoinThreads / 32;
+  const int blocks = (used + per_block - 1) / per_block;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(a.B * a.p.Hkv * a.row_tiles * blocks));
   cfg.blockDim = dim3(kJoinThreads);
@@ -542,7 +595,7 @@ static int launch_join(const PagedAttnArgs& a, int tile_rows, cudaStream_t st) {
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, paged_join_kernel<T, D>, a, tile_rows, blocks);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, many ? wide_join_kernel<T, D> : paged_join_kernel<T, D>, a, tile_rows, blocks);
   if (e == cudaSuccess) return SAGE_OK;
   set_error("paged attention: %s", cudaGetErrorString(e));
   return SAGE_ERR_LAUNCH;
@@ -638,6 +691,7 @@ extern "C" int sage_paged_attention(const void* q, int dtype, int B, int T, int 
     else
       rc2 = dtype == SAGE_BF16 ? launch_paged_attn<__nv_bfloat16, kD>(a, shape, st) : launch_paged_attn<__half, kD>(a, shape, st);
     if (rc2 != SAGE_OK) return rc2;
-    return dtype == SAGE_BF16 ? launch_join<__nv_bfloat16, kD>(a, tile_rows, st) : launch_join<__half, kD>(a, tile_rows, st);
+    return dtype == SAGE_BF16 ? launch_join<__nv_bfloat16, kD>(a, tile_rows, many, st)
+                              : launch_join<__half, kD>(a, tile_rows, many, st);
   });
 }

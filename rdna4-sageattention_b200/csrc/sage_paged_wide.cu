@@ -5,8 +5,8 @@
 //   softmax warps   one warpgroup per row tile, one thread per row: q to TMEM (fp16), then per key tile S from TMEM,
 //                   weights (fp16) back over S, O rescaled in TMEM when the maximum moves, epilogue
 //   producer warp   TMA of the raw codes and scales into a ring
-//   MMA warp        S_t = Q_t K^T (A from TMEM, fp16), O_t += P_t V (A from TMEM); while row tile 0 is in its softmax,
-//                   row tile 1 is in its products
+//   MMA warps       one per row tile: S_t = Q_t K^T (A from TMEM, fp16), O_t += P_t V (A from TMEM); while row tile 0 is
+//                   in its softmax, row tile 1 is in its products
 //   4 converter warps   int8 and e4m3 codes to fp16 operand tiles in shared memory, once for all QT * 128 rows, and what
 //                   the rows need of each key (factor of its score, log2 of its V scale, the inverse of that)
 // Codes convert exactly, so there is nothing to choose there; with Q and P in TMEM the products read only K and V from
@@ -20,7 +20,7 @@ template <int D>
 struct Wide {
   static constexpr int QT = D == 256 ? 1 : 2;
   static constexpr int kSoftmaxWarps = 4 * QT, kConverters = 4;
-  static constexpr int kThreads = 32 * (kSoftmaxWarps + 2 + kConverters);
+  static constexpr int kThreads = 32 * (kSoftmaxWarps + 1 + QT + kConverters);
   static constexpr int kRows = 128 * QT;
   static constexpr int kPanels = (D + 63) / 64;            // of 64 channels: 128 bytes a key
   static constexpr int kPanel = kTileKeys * 128;
@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
   extern __shared__ unsigned char smem_raw[];
   __shared__ int64_t warp_sums[W::kThreads / 32], found[2];
   __shared__ uint64_t raw_full[W::kRaw], raw_empty[W::kRaw], k_full[W::kBufs], v_full[W::kBufs], buf_empty[W::kBufs];
-  __shared__ uint64_t s_full[QT], p_full[QT], q_full[QT], o_full[QT], all_done;
+  __shared__ uint64_t s_full[QT], p_full[QT], q_full[QT], o_full[QT], all_done[QT];
   __shared__ uint32_t tmem_base;
   __shared__ int given_up, zero_rows[W::kBufs][2];
   unsigned char* operands = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
@@ -89,15 +89,15 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
     for (int i = 0; i < W::kBufs; ++i) {
       mbar_init(k_full + i, W::kConverters);
       mbar_init(v_full + i, W::kConverters);
-      mbar_init(buf_empty + i, 1);
+      mbar_init(buf_empty + i, QT);
     }
     for (int t = 0; t < QT; ++t) {
       mbar_init(s_full + t, 1);
       mbar_init(p_full + t, 4);
       mbar_init(q_full + t, 4);
       mbar_init(o_full + t, 1);
+      mbar_init(all_done + t, 1);
     }
-    mbar_init(&all_done, 1);
     fence_barrier_init();
   }
 
@@ -126,75 +126,67 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
 
   if (warp == W::kSoftmaxWarps) {
     load_tiles<D>(a, &k_map, &v_map, now, todo, stages, scales, raw_full, raw_empty, W::kRaw, &given_up);
-  } else if (warp == W::kSoftmaxWarps + 1) {
+  } else if (warp > W::kSoftmaxWarps && warp <= W::kSoftmaxWarps + QT) {
     // ------------------------------------------------------------------------------------------------ products
     if (lane == 0) {
       constexpr uint32_t kScores = idesc_f16(128, kTileKeys, false), kValues = idesc_f16(128, D, true);
+      const int t = warp - W::kSoftmaxWarps - 1;
+      const uint64_t k_desc = smem_desc_kmajor(smem_u32(operands), 128);
+      const uint64_t v_desc = smem_desc_nmajor(smem_u32(operands) + W::kOperand, W::kPanel);
+      const uint32_t s_at = tmem + W::kS + t * kTileKeys, q_at = tmem + W::kQ + t * (D / 2), o_at = tmem + W::kO + t * D;
       int buf = 0;
-      uint32_t phase = 0, p_phase[QT] = {}, q_phase[QT] = {};
+      uint32_t phase = 0, p_phase = 0, q_phase = 0;
       bool begins = true;
-      auto scores = [&](int t, int b) {
-        const uint32_t k = smem_u32(operands + b * 2 * W::kOperand);
+      auto scores = [&](int b) {
+        const uint64_t k = k_desc + b * (2 * W::kOperand / 16);
 #pragma unroll
         for (int s = 0; s < D / 16; ++s)
-          mma_f16_ts(tmem + W::kS + t * kTileKeys, tmem + W::kQ + t * (D / 2) + s * 8,
-                     smem_desc_kmajor(k + s / 4 * W::kPanel + s % 4 * 32, 128), kScores, s > 0);
+          mma_f16_ts(s_at, q_at + s * 8, k + (s / 4 * W::kPanel + s % 4 * 32) / 16, kScores, s > 0);
         tc_commit(s_full + t);
       };
       for (; todo > 0; --todo) {
-        bool act[QT];
-        int last = -1;
-#pragma unroll
-        for (int t = 0; t < QT; ++t) {
-          act[t] = active(now, t);
-          if (act[t]) last = t;
-        }
-        if (begins) {
-          wait_stage(k_full + buf, phase, &given_up, a.p.status);
-#pragma unroll
-          for (int t = 0; t < QT; ++t)
-            if (act[t]) {
-              wait_stage(q_full + t, q_phase[t], &given_up, a.p.status);
-              q_phase[t] ^= 1;
-              tc_fence_after();
-              scores(t, buf);
-            }
-        }
-        const bool more = todo > 1 && now.tile + 1 < now.tiles;
+        const bool act = active(now, t), more = todo > 1 && now.tile + 1 < now.tiles;
         const int next = buf + 1 == W::kBufs ? 0 : buf + 1;
         const uint32_t next_phase = next == 0 ? phase ^ 1 : phase;
-        wait_stage(v_full + buf, phase, &given_up, a.p.status);
-#pragma unroll
-        for (int t = 0; t < QT; ++t)
-          if (act[t]) {
-            wait_stage(p_full + t, p_phase[t], &given_up, a.p.status);
-            p_phase[t] ^= 1;
+        if (act) {
+          if (begins) {
+            wait_stage(k_full + buf, phase, &given_up, a.p.status);
+            wait_stage(q_full + t, q_phase, &given_up, a.p.status);
+            q_phase ^= 1;
             tc_fence_after();
-            const uint32_t v = smem_u32(operands + buf * 2 * W::kOperand + W::kOperand);
-#pragma unroll
-            for (int s = 0; s < kTileKeys / 16; ++s)
-              mma_f16_ts(tmem + W::kO + t * D, tmem + W::kS + t * kTileKeys + s * 8,
-                         smem_desc_nmajor(v + s * 2048, W::kPanel), kValues, !begins || s > 0);
-            if (t == last) tc_commit(buf_empty + buf);
-            if (more) {
-              if (wait_stage(k_full + next, next_phase, &given_up, a.p.status)) tc_fence_after();
-              scores(t, next);
-            } else {
-              tc_commit(o_full + t);
-            }
+            scores(buf);
           }
-        if (last < 0) tc_commit(buf_empty + buf);   // no row of this row tile is live
+          wait_stage(v_full + buf, phase, &given_up, a.p.status);
+          wait_stage(p_full + t, p_phase, &given_up, a.p.status);
+          p_phase ^= 1;
+          tc_fence_after();
+          const uint64_t v = v_desc + buf * (2 * W::kOperand / 16);
+#pragma unroll
+          for (int s = 0; s < kTileKeys / 16; ++s)
+            mma_f16_ts(o_at, s_at + s * 8, v + s * (2048 / 16), kValues, !begins || s > 0);
+          tc_commit(buf_empty + buf);
+          if (more) {
+            wait_stage(k_full + next, next_phase, &given_up, a.p.status);
+            tc_fence_after();
+            scores(next);
+          } else {
+            tc_commit(o_full + t);
+          }
+        } else {   // no row of this row tile is live
+          wait_stage(v_full + buf, phase, &given_up, a.p.status);
+          arrive(buf_empty + buf);
+        }
         begins = !more;
         buf = next, phase = next_phase;
         if (todo > 1) advance(a, now);
       }
-      tc_commit(&all_done);   // nothing is in flight when the CTA ends
-      wait_stage(&all_done, 0, &given_up, a.p.status);
+      tc_commit(all_done + t);   // nothing is in flight when the CTA ends
+      wait_stage(all_done + t, 0, &given_up, a.p.status);
     }
     __syncwarp();
-  } else if (warp >= W::kSoftmaxWarps + 2) {
+  } else if (warp > W::kSoftmaxWarps) {
     // ------------------------------------------------------------------------------------------------ converters
-    const int ct = tid - 32 * (W::kSoftmaxWarps + 2), cw = ct / 32;
+    const int ct = tid - 32 * (W::kSoftmaxWarps + 1 + QT), cw = ct / 32;
     int raw = 0, buf = 0;
     uint32_t raw_phase = 0, phase = 0;
     // The eight lanes of a phase of a 16-byte access take four neighbouring chunks of a raw row and of the row that
@@ -299,16 +291,24 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
             // the row in fp16, scaled by a power of two of its largest value, as D / 2 TMEM columns
             const bool live = token < now.fresh;
             const T* src = static_cast<const T*>(a.q) + now.b * a.q_st.b + token * a.q_st.s + head * a.q_st.h;
+            constexpr int kPart = D == 256 ? 128 : D;   // channels held in registers at once
+            uint4 v[kPart / 8];
+            auto fetch = [&](int c0) {
+#pragma unroll
+              for (int i = 0; i < kPart / 8; ++i)
+                v[i] = live ? *reinterpret_cast<const uint4*>(src + c0 + 8 * i) : make_uint4(0, 0, 0, 0);
+            };
+            fetch(0);
             float inverse = 1.0f;
             if constexpr (!std::is_same<T, __half>::value) {
               uint32_t top = 0;
-              if (live) {
-#pragma unroll 4
-                for (int i = 0; i < D / 8; ++i) {
-                  const uint4 v = *reinterpret_cast<const uint4*>(src + 8 * i);
-                  top = __vmaxu2(top, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
-                                               __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
-                }
+#pragma unroll
+              for (int c0 = D - kPart; c0 >= 0; c0 -= kPart) {
+                if (D > kPart) fetch(c0);
+#pragma unroll
+                for (int i = 0; i < kPart / 8; ++i)
+                  top = __vmaxu2(top, __vmaxu2(__vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu),
+                                               __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu)));
               }
               top = max(top & 0xffffu, top >> 16);
               // 2^e with e the exponent of that value (zero, infinite and NaN rows: 1; tiny ones: 2^-100)
@@ -316,27 +316,31 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
               row_scale = __int_as_float(e << 23);
               inverse = __int_as_float((254 - e) << 23);
             }
-#pragma unroll 1
-            for (int i = 0; i < D / 32; ++i) {   // 32 channels: 16 columns
-              uint32_t w[16];
 #pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const uint4 v = live ? *reinterpret_cast<const uint4*>(src + 32 * i + 8 * k) : make_uint4(0, 0, 0, 0);
-                if constexpr (std::is_same<T, __half>::value) {
-                  w[4 * k] = v.x, w[4 * k + 1] = v.y, w[4 * k + 2] = v.z, w[4 * k + 3] = v.w;
-                } else {
-                  float x[8];
-                  unpack8(v, x, T());
+            for (int c0 = 0; c0 < D; c0 += kPart) {
+              if (c0 > 0) fetch(c0);
 #pragma unroll
-                  for (int z = 0; z < 4; ++z) w[4 * k + z] = pack2(x[2 * z] * inverse, x[2 * z + 1] * inverse, __half());
+              for (int i = 0; i < kPart / 32; ++i) {   // 32 channels: 16 columns
+                uint32_t w[16];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  const uint4 y = v[4 * i + k];
+                  if constexpr (std::is_same<T, __half>::value) {
+                    w[4 * k] = y.x, w[4 * k + 1] = y.y, w[4 * k + 2] = y.z, w[4 * k + 3] = y.w;
+                  } else {
+                    float x[8];
+                    unpack8(y, x, T());
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) w[4 * k + z] = pack2(x[2 * z] * inverse, x[2 * z + 1] * inverse, __half());
+                  }
                 }
+                asm volatile(
+                    "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+                    "%14, %15, %16};" ::"r"(tmem + lanes + W::kQ + t * (D / 2) + c0 / 2 + i * 16),
+                    "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "r"(w[8]),
+                    "r"(w[9]), "r"(w[10]), "r"(w[11]), "r"(w[12]), "r"(w[13]), "r"(w[14]), "r"(w[15])
+                    : "memory");
               }
-              asm volatile(
-                  "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-                  "%15, %16};" ::"r"(tmem + lanes + W::kQ + t * (D / 2) + i * 16),
-                  "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "r"(w[8]),
-                  "r"(w[9]), "r"(w[10]), "r"(w[11]), "r"(w[12]), "r"(w[13]), "r"(w[14]), "r"(w[15])
-                  : "memory");
             }
             tmem_wait_st();
             tc_fence_before();
@@ -462,7 +466,10 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
           tc_fence_after();
         }
         T* dst = static_cast<T*>(a.out) + now.b * a.out_st.b + token * a.out_st.s + head * a.out_st.h;
-        const int64_t at = (2 * (int64_t)blockIdx.x + (segment > 0)) * W::kRows + t * 128 + warp % 4 * 32 + lane;
+        // partial rows: four channels of all rows, then the next four, so that the lanes' stores are whole lines
+        const int64_t first_row = (2 * (int64_t)blockIdx.x + (segment > 0)) * W::kRows;
+        const int in_tile = t * 128 + warp % 4 * 32 + lane;
+        float* part = a.part_o + first_row * D + in_tile * 4;
         const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
         if (act && warp_live) {
 #pragma unroll 1
@@ -481,7 +488,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
             } else if (mine && live) {
 #pragma unroll
               for (int k = 0; k < 32; k += 4)
-                *reinterpret_cast<uint4*>(a.part_o + at * D + 32 * i + k) = make_uint4(r[k], r[k + 1], r[k + 2], r[k + 3]);
+                *reinterpret_cast<uint4*>(part + (32 * i + k) * W::kRows) = make_uint4(r[k], r[k + 1], r[k + 2], r[k + 3]);
             }
           }
           tc_fence_before();
@@ -493,7 +500,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
             a.lse[((int64_t)now.b * a.H + head) * a.T + token] =
                 !live || l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
         } else if (mine && live) {
-          a.part_ml[at] = make_float2(m, l);
+          a.part_ml[first_row + in_tile] = make_float2(m, l);
         }
         ++segment;
       }
