@@ -20,7 +20,11 @@ template <int D>
 struct Wide {
   static constexpr int QT = D == 256 ? 1 : 2;
   static constexpr int kSoftmaxWarps = 4 * QT, kConverters = 4;
-  static constexpr int kThreads = 32 * (kSoftmaxWarps + 1 + QT + kConverters);
+  // QT 2: 16 warps (one idle), so that the two warpgroups of the other roles hand registers to the two of softmax: 512
+  // threads of 128 at launch, then 256 of 168 and 256 of 80
+  static constexpr int kThreads = QT == 2 ? 512 : 32 * (kSoftmaxWarps + 1 + QT + kConverters);
+  static constexpr int kLaunchRegs = 128, kSoftmaxRegs = 168, kOtherRegs = 80;
+  static_assert(QT != 2 || 256 * (kSoftmaxRegs + kOtherRegs) <= 512 * kLaunchRegs, "register split");
   static constexpr int kRows = 128 * QT;
   static constexpr int kPanels = (D + 63) / 64;            // of 64 channels: 128 bytes a key
   static constexpr int kPanel = kTileKeys * 128;
@@ -63,6 +67,10 @@ __device__ __forceinline__ uint64_t smem_desc_nmajor(uint32_t smem_addr, uint32_
 __device__ __forceinline__ int operand_at(int row, int ch) {
   return ch / 8 * (kTileKeys * 128) + row * 128 + (((ch % 8) ^ (row & 7)) << 4);
 }
+
+// Turns of the two softmax warpgroups: each waits for its own named barrier, which the other arrives at.
+__device__ __forceinline__ void take_turn(int t) { asm volatile("bar.sync %0, 256;" ::"r"(2 + t) : "memory"); }
+__device__ __forceinline__ void pass_turn(int t) { asm volatile("bar.arrive %0, 256;" ::"r"(3 - t) : "memory"); }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
@@ -125,9 +133,11 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
   auto active = [&](const Cursor& c, int t) { return c.unit % a.row_tiles * W::kRows + t * 128 < c.fresh * a.group; };
 
   if (warp == W::kSoftmaxWarps) {
+    if constexpr (QT == 2) regs_decrease<W::kOtherRegs>();
     load_tiles<D>(a, &k_map, &v_map, now, todo, stages, scales, raw_full, raw_empty, W::kRaw, &given_up);
   } else if (warp > W::kSoftmaxWarps && warp <= W::kSoftmaxWarps + QT) {
     // ------------------------------------------------------------------------------------------------ products
+    if constexpr (QT == 2) regs_decrease<W::kOtherRegs>();
     if (lane == 0) {
       constexpr uint32_t kScores = idesc_f16(128, kTileKeys, false), kValues = idesc_f16(128, D, true);
       const int t = warp - W::kSoftmaxWarps - 1;
@@ -184,8 +194,11 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
       wait_stage(all_done + t, 0, &given_up, a.p.status);
     }
     __syncwarp();
+  } else if (warp > W::kSoftmaxWarps + QT + W::kConverters) {
+    if constexpr (QT == 2) regs_decrease<W::kOtherRegs>();   // idle
   } else if (warp > W::kSoftmaxWarps) {
     // ------------------------------------------------------------------------------------------------ converters
+    if constexpr (QT == 2) regs_decrease<W::kOtherRegs>();
     const int ct = tid - 32 * (W::kSoftmaxWarps + 1 + QT), cw = ct / 32;
     int raw = 0, buf = 0;
     uint32_t raw_phase = 0, phase = 0;
@@ -224,7 +237,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
         const bool any = __any_sync(0xffffffffu, zero);
         if (lane == 0) zero_rows[buf][cw] = any;
       }
-#pragma unroll
+#pragma unroll 2
       for (int i = 0; i < kItems; ++i) {
         int row, ch;
         place(i, row, ch);
@@ -238,7 +251,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
       __syncwarp();
       if (lane == 0) arrive(k_full + buf);
       const bool drafts = key0 + kTileKeys > now.len;
-#pragma unroll
+#pragma unroll 2
       for (int i = 0; i < kItems; ++i) {
         int row, ch;
         place(i, row, ch);
@@ -270,243 +283,259 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
     }
   } else {
     // ------------------------------------------------------------------------------------------------ softmax
+    if constexpr (QT == 2) regs_increase<W::kSoftmaxRegs>();
     const int t = warp / 4;
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;   // of TMEM
     const uint32_t s_at = tmem + lanes + W::kS + t * kTileKeys, o_at = tmem + lanes + W::kO + t * D;
-    int buf = 0, token = 0, head = 0, row = 0, segment = 0, first_tile = 0;
+    int buf = 0, segment = 0;
     uint32_t phase = 0, s_phase = 0, o_phase = 0;
-    float m = 0.0f, l = 0.0f, row_scale = 1.0f;
-    bool begins = true, act = false, warp_live = false;
-    for (; todo > 0; --todo) {
-      if (begins) {
-        first_tile = now.tile;
-        act = active(now, t);
-        row = now.unit % a.row_tiles * W::kRows + t * 128 + warp % 4 * 32 + lane;
-        token = row / a.group;
-        head = now.unit / a.row_tiles * a.group + row % a.group;
-        warp_live = row - lane < now.fresh * a.group;
-        m = -3.402823466e38f, l = 0.0f;
-        if (act) {
-          if (warp_live) {
-            // the row in fp16, scaled by a power of two of its largest value, as D / 2 TMEM columns
-            const bool live = token < now.fresh;
-            const T* src = static_cast<const T*>(a.q) + now.b * a.q_st.b + token * a.q_st.s + head * a.q_st.h;
-            constexpr int kPart = D == 256 ? 128 : D;   // channels held in registers at once
-            uint4 v[kPart / 8];
-            auto fetch = [&](int c0) {
+    // The two row tiles take turns in their exponentials, so that one is in its products while the other has the
+    // special-function unit (left alone they fall into step: both wait, then both want it).
+    if (QT == 2 && t == 1) asm volatile("bar.arrive 2, 256;" ::: "memory");
+    while (todo > 0) {
+      // ---- a row tile, or this CTA's part of it: key tiles first_tile ... last - 1
+      const int first_tile = now.tile, last = (int)min((int64_t)now.tiles, now.tile + todo);
+      const bool act = active(now, t), paired = QT == 2 && active(now, QT - 1);   // tile 0 is active where tile 1 is
+      const int row = now.unit % a.row_tiles * W::kRows + t * 128 + warp % 4 * 32 + lane, token = row / a.group;
+      const int head = now.unit / a.row_tiles * a.group + row % a.group;
+      const bool warp_live = act && row - lane < now.fresh * a.group, live = token < now.fresh;
+      float m = -3.402823466e38f, l = 0.0f, row_scale = 1.0f;
+      if (act) {
+        if (warp_live) {
+          // the row in fp16, scaled by a power of two of its largest value, as D / 2 TMEM columns
+          const T* src = static_cast<const T*>(a.q) + now.b * a.q_st.b + token * a.q_st.s + head * a.q_st.h;
+          constexpr int kPart = D == 256 ? 128 : D;   // channels held in registers at once
+          uint4 v[kPart / 8];
+          auto fetch = [&](int c0) {
+#pragma unroll
+            for (int i = 0; i < kPart / 8; ++i)
+              v[i] = live ? *reinterpret_cast<const uint4*>(src + c0 + 8 * i) : make_uint4(0, 0, 0, 0);
+          };
+          fetch(0);
+          float inverse = 1.0f;
+          if constexpr (!std::is_same<T, __half>::value) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int c0 = D - kPart; c0 >= 0; c0 -= kPart) {
+              if (D > kPart) fetch(c0);
 #pragma unroll
               for (int i = 0; i < kPart / 8; ++i)
-                v[i] = live ? *reinterpret_cast<const uint4*>(src + c0 + 8 * i) : make_uint4(0, 0, 0, 0);
-            };
-            fetch(0);
-            float inverse = 1.0f;
-            if constexpr (!std::is_same<T, __half>::value) {
-              uint32_t top = 0;
-#pragma unroll
-              for (int c0 = D - kPart; c0 >= 0; c0 -= kPart) {
-                if (D > kPart) fetch(c0);
-#pragma unroll
-                for (int i = 0; i < kPart / 8; ++i)
-                  top = __vmaxu2(top, __vmaxu2(__vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu),
-                                               __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu)));
-              }
-              top = max(top & 0xffffu, top >> 16);
-              // 2^e with e the exponent of that value (zero, infinite and NaN rows: 1; tiny ones: 2^-100)
-              const int e = top == 0 || top >= 0x7f80u ? 127 : max((int)(top >> 7), 27);
-              row_scale = __int_as_float(e << 23);
-              inverse = __int_as_float((254 - e) << 23);
+                top = __vmaxu2(top, __vmaxu2(__vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu),
+                                             __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu)));
             }
+            top = max(top & 0xffffu, top >> 16);
+            // 2^e with e the exponent of that value (zero, infinite and NaN rows: 1; tiny ones: 2^-100)
+            const int e = top == 0 || top >= 0x7f80u ? 127 : max((int)(top >> 7), 27);
+            row_scale = __int_as_float(e << 23);
+            inverse = __int_as_float((254 - e) << 23);
+          }
 #pragma unroll
-            for (int c0 = 0; c0 < D; c0 += kPart) {
-              if (c0 > 0) fetch(c0);
+          for (int c0 = 0; c0 < D; c0 += kPart) {
+            if (c0 > 0) fetch(c0);
 #pragma unroll
-              for (int i = 0; i < kPart / 32; ++i) {   // 32 channels: 16 columns
-                uint32_t w[16];
+            for (int i = 0; i < kPart / 32; ++i) {   // 32 channels: 16 columns
+              uint32_t w[16];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                  const uint4 y = v[4 * i + k];
-                  if constexpr (std::is_same<T, __half>::value) {
-                    w[4 * k] = y.x, w[4 * k + 1] = y.y, w[4 * k + 2] = y.z, w[4 * k + 3] = y.w;
-                  } else {
-                    float x[8];
-                    unpack8(y, x, T());
+              for (int k = 0; k < 4; ++k) {
+                const uint4 y = v[4 * i + k];
+                if constexpr (std::is_same<T, __half>::value) {
+                  w[4 * k] = y.x, w[4 * k + 1] = y.y, w[4 * k + 2] = y.z, w[4 * k + 3] = y.w;
+                } else {
+                  float x[8];
+                  unpack8(y, x, T());
 #pragma unroll
-                    for (int z = 0; z < 4; ++z) w[4 * k + z] = pack2(x[2 * z] * inverse, x[2 * z + 1] * inverse, __half());
-                  }
+                  for (int z = 0; z < 4; ++z) w[4 * k + z] = pack2(x[2 * z] * inverse, x[2 * z + 1] * inverse, __half());
                 }
-                asm volatile(
-                    "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
-                    "%14, %15, %16};" ::"r"(tmem + lanes + W::kQ + t * (D / 2) + c0 / 2 + i * 16),
-                    "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "r"(w[8]),
-                    "r"(w[9]), "r"(w[10]), "r"(w[11]), "r"(w[12]), "r"(w[13]), "r"(w[14]), "r"(w[15])
-                    : "memory");
               }
-            }
-            tmem_wait_st();
-            tc_fence_before();
-          }
-          __syncwarp();
-          if (lane == 0) arrive(q_full + t);
-        }
-      }
-      const bool last_tile = now.tile + 1 == now.tiles, ends = last_tile || todo == 1;
-      if (act) {
-        wait_stage(s_full + t, s_phase, &given_up, a.p.status);
-        s_phase ^= 1;
-        if (warp_live) {
-          wait_stage(k_full + buf, phase, &given_up, a.p.status);   // long there: orders the reads of params and zero_rows
-          tc_fence_after();
-          const float* factor = params + buf * W::kParams;
-          const int key0 = now.tile * kTileKeys;
-          const bool drafts = key0 + kTileKeys > now.len;
-          uint64_t x[kTileKeys / 2];   // two scores each
-          {
-            uint32_t r[2][32];
-            tmem_ld32(s_at, r[0]);
-            tmem_ld32(s_at + 32, r[1]);
-            tmem_wait_ld();
-            const uint64_t scale2 = f2_pack(row_scale, row_scale);
-#pragma unroll
-            for (int i = 0; i < kTileKeys / 4; ++i) {
-              const float4 f = *reinterpret_cast<const float4*>(factor + 4 * i);
-              const float4 g = *reinterpret_cast<const float4*>(factor + kTileKeys + 4 * i);
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const int c = 4 * i + 2 * h;
-                uint64_t v = f2_pack(__uint_as_float(r[c / 32][c % 32]), __uint_as_float(r[c / 32][c % 32 + 1]));
-                if constexpr (!std::is_same<T, __half>::value) v = f2_mul(v, scale2);
-                x[c / 2] = f2_fma(v, h ? f2_pack(f.z, f.w) : f2_pack(f.x, f.y), h ? f2_pack(g.z, g.w) : f2_pack(g.x, g.y));
-              }
+              asm volatile(
+                  "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+                  "%14, %15, %16};" ::"r"(tmem + lanes + W::kQ + t * (D / 2) + c0 / 2 + i * 16),
+                  "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "r"(w[8]),
+                  "r"(w[9]), "r"(w[10]), "r"(w[11]), "r"(w[12]), "r"(w[13]), "r"(w[14]), "r"(w[15])
+                  : "memory");
             }
           }
-          if (drafts) {
-            const uint8_t* mask = a.mask != nullptr && token < now.fresh ? a.mask + now.b * a.mask_b + token * a.mask_i : nullptr;
-#pragma unroll
-            for (int i = 0; i < kTileKeys / 2; ++i) {
-              float v[2];
-              f2_unpack(x[i], v[0], v[1]);
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int d = key0 + 2 * i + e - now.len;
-                const bool seen = d < 0 || (d < now.fresh && token < now.fresh && (mask != nullptr ? mask[d] != 0 : d <= token));
-                if (!seen) v[e] = -INFINITY;
-              }
-              x[i] = f2_pack(v[0], v[1]);
-            }
-          }
-          float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int i = 0; i < kTileKeys / 2; ++i) {
-            float u, v;
-            f2_unpack(x[i], u, v);
-            top[i % 4] = fmaxf(fmaxf(top[i % 4], u), v);
-          }
-          const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-          if (__any_sync(0xffffffffu, most > m + 8.0f)) {
-            const float next = most > m + 8.0f ? most : m;
-            const float keep = next == m ? 1.0f : fast_exp2(m - next);
-            m = next;
-            l *= keep;
-            if (now.tile != first_tile) {   // the first product of a row tile overwrites O
-              const uint64_t keep2 = f2_pack(keep, keep);
-#pragma unroll 1
-              for (int i = 0; i < D / 32; ++i) {
-                uint32_t r[32];
-                tmem_ld32(o_at + 32 * i, r);
-                tmem_wait_ld();
-#pragma unroll
-                for (int k = 0; k < 32; k += 2) {
-                  float u, v;
-                  f2_unpack(f2_mul(f2_pack(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), keep2), u, v);
-                  r[k] = __float_as_uint(u), r[k + 1] = __float_as_uint(v);
-                }
-                tmem_st32(o_at + 32 * i, r);
-              }
-            }
-          }
-          if ((zero_rows[buf][0] | zero_rows[buf][1]) != 0) {
-#pragma unroll
-            for (int i = 0; i < kTileKeys / 4; ++i) {
-              const float4 g = *reinterpret_cast<const float4*>(factor + 3 * kTileKeys + 4 * i);
-              x[2 * i] = f2_add(x[2 * i], f2_pack(g.x, g.y)), x[2 * i + 1] = f2_add(x[2 * i + 1], f2_pack(g.z, g.w));
-            }
-          }
-          const uint64_t minus_m = f2_pack(-m, -m);
-          uint64_t sum[2] = {f2_pack(l, 0.0f), f2_pack(0.0f, 0.0f)};
-          uint32_t packed[32];
-#pragma unroll
-          for (int i = 0; i < kTileKeys / 4; ++i) {
-            const float4 inv = *reinterpret_cast<const float4*>(factor + 2 * kTileKeys + 4 * i);
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int c = 2 * i + h;
-              float u, v;
-              f2_unpack(f2_add(x[c], minus_m), u, v);
-              u = fast_exp2(u), v = fast_exp2(v);
-              sum[h] = f2_fma(f2_pack(u, v), h ? f2_pack(inv.z, inv.w) : f2_pack(inv.x, inv.y), sum[h]);
-              packed[c] = pack_weights(u, v);
-            }
-          }
-          float u, v;
-          f2_unpack(f2_add(sum[0], sum[1]), u, v);
-          l = u + v;
-          tmem_st32(s_at, packed);
           tmem_wait_st();
           tc_fence_before();
         }
         __syncwarp();
-        if (lane == 0) arrive(p_full + t);
+        if (lane == 0) arrive(q_full + t);
       }
-      if (ends) {
-        // the row tile ends here, or this CTA's part of it does
-        const bool whole = last_tile && first_tile == 0, mine = row < a.T * a.group, live = token < now.fresh;
-        if (act) {
-          wait_stage(o_full + t, o_phase, &given_up, a.p.status);
-          o_phase ^= 1;
-          tc_fence_after();
-        }
-        T* dst = static_cast<T*>(a.out) + now.b * a.out_st.b + token * a.out_st.s + head * a.out_st.h;
-        // partial rows: four channels of all rows, then the next four, so that the lanes' stores are whole lines
-        const int64_t first_row = (2 * (int64_t)blockIdx.x + (segment > 0)) * W::kRows;
-        const int in_tile = t * 128 + warp % 4 * 32 + lane;
-        float* part = a.part_o + first_row * D + in_tile * 4;
-        const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
-        if (act && warp_live) {
 #pragma unroll 1
-          for (int i = 0; i < D / 32; ++i) {
-            uint32_t r[32];
-            tmem_ld32(o_at + 32 * i, r);
-            tmem_wait_ld();
-            if (mine && whole) {
-#pragma unroll
-              for (int k = 0; k < 32; k += 8) {
-                float x[8];
-#pragma unroll
-                for (int z = 0; z < 8; ++z) x[z] = live && l != 0.0f ? __uint_as_float(r[k + z]) * inverse : 0.0f;
-                store8(dst + 32 * i + k, x);
+      for (int tile = first_tile; tile < last; ++tile) {
+        if (act) {
+          wait_stage(s_full + t, s_phase, &given_up, a.p.status);
+          s_phase ^= 1;
+          if (warp_live) {
+            wait_stage(k_full + buf, phase, &given_up, a.p.status);   // long there: orders the reads of params, zero_rows
+            tc_fence_after();
+            const float* factor = params + buf * W::kParams;
+            const int key0 = tile * kTileKeys;
+            const bool drafts = key0 + kTileKeys > now.len;
+            uint64_t seen = ~uint64_t(0);
+            if (drafts) {
+              // bit j: the row sees key key0 + j (what is behind the last key has a factor of its own that hides it)
+              const int t0 = key0 - now.len;   // number of the first key as a draft
+              seen = t0 >= 0 ? 0 : (uint64_t(1) << -t0) - 1;
+              if (live) {
+                const int from = max(t0, 0);
+                if (a.mask != nullptr) {
+                  const uint8_t* mask = a.mask + now.b * a.mask_b + token * a.mask_i;
+                  const int to = min(t0 + kTileKeys, now.fresh);
+#pragma unroll 8
+                  for (int d = from; d < to; ++d) seen |= (uint64_t)(mask[d] != 0) << (d - t0);
+                } else if (token >= from) {
+                  const int count = min(token - t0 + 1, kTileKeys);
+                  seen |= count == kTileKeys ? ~uint64_t(0) : (uint64_t(1) << count) - 1;
+                }
               }
-            } else if (mine && live) {
-#pragma unroll
-              for (int k = 0; k < 32; k += 4)
-                *reinterpret_cast<uint4*>(part + (32 * i + k) * W::kRows) = make_uint4(r[k], r[k + 1], r[k + 2], r[k + 3]);
             }
+            uint64_t x[kTileKeys / 2];   // two scores each
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+              uint32_t r[32];
+              tmem_ld32(s_at + 32 * part, r);
+              tmem_wait_ld();
+              const uint64_t scale2 = f2_pack(row_scale, row_scale);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float4 f = *reinterpret_cast<const float4*>(factor + 32 * part + 4 * i);
+                const float4 g = *reinterpret_cast<const float4*>(factor + kTileKeys + 32 * part + 4 * i);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  const int c = 4 * i + 2 * h;
+                  uint64_t v = f2_pack(__uint_as_float(r[c]), __uint_as_float(r[c + 1]));
+                  if constexpr (!std::is_same<T, __half>::value) v = f2_mul(v, scale2);
+                  x[16 * part + c / 2] = f2_fma(v, h ? f2_pack(f.z, f.w) : f2_pack(f.x, f.y), h ? f2_pack(g.z, g.w) : f2_pack(g.x, g.y));
+                }
+              }
+            }
+            if (drafts) {
+#pragma unroll
+              for (int i = 0; i < kTileKeys / 2; ++i) {
+                float u, v;
+                f2_unpack(x[i], u, v);
+                x[i] = f2_pack(seen >> (2 * i) & 1 ? u : -INFINITY, seen >> (2 * i + 1) & 1 ? v : -INFINITY);
+              }
+            }
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int i = 0; i < kTileKeys / 2; ++i) {
+              float u, v;
+              f2_unpack(x[i], u, v);
+              top[i % 4] = fmaxf(fmaxf(top[i % 4], u), v);
+            }
+            const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            if (__any_sync(0xffffffffu, most > m + 8.0f)) {
+              const float next = most > m + 8.0f ? most : m;
+              const float keep = next == m ? 1.0f : fast_exp2(m - next);
+              m = next;
+              l *= keep;
+              if (tile != first_tile) {   // the first product of a row tile overwrites O
+                const uint64_t keep2 = f2_pack(keep, keep);
+#pragma unroll 1
+                for (int i = 0; i < D / 32; ++i) {
+                  uint32_t r[32];
+                  tmem_ld32(o_at + 32 * i, r);
+                  tmem_wait_ld();
+#pragma unroll
+                  for (int k = 0; k < 32; k += 2) {
+                    float u, v;
+                    f2_unpack(f2_mul(f2_pack(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), keep2), u, v);
+                    r[k] = __float_as_uint(u), r[k + 1] = __float_as_uint(v);
+                  }
+                  tmem_st32(o_at + 32 * i, r);
+                }
+              }
+            }
+            if ((zero_rows[buf][0] | zero_rows[buf][1]) != 0) {
+#pragma unroll
+              for (int i = 0; i < kTileKeys / 4; ++i) {
+                const float4 g = *reinterpret_cast<const float4*>(factor + 3 * kTileKeys + 4 * i);
+                x[2 * i] = f2_add(x[2 * i], f2_pack(g.x, g.y)), x[2 * i + 1] = f2_add(x[2 * i + 1], f2_pack(g.z, g.w));
+              }
+            }
+            const uint64_t minus_m = f2_pack(-m, -m);
+            if (paired) take_turn(t);
+            uint64_t sum[2] = {f2_pack(l, 0.0f), f2_pack(0.0f, 0.0f)};
+            uint32_t packed[32];
+#pragma unroll
+            for (int i = 0; i < kTileKeys / 4; ++i) {
+              const float4 inv = *reinterpret_cast<const float4*>(factor + 2 * kTileKeys + 4 * i);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int c = 2 * i + h;
+                float u, v;
+                f2_unpack(f2_add(x[c], minus_m), u, v);
+                u = fast_exp2(u), v = fast_exp2(v);
+                sum[h] = f2_fma(f2_pack(u, v), h ? f2_pack(inv.z, inv.w) : f2_pack(inv.x, inv.y), sum[h]);
+                packed[c] = pack_weights(u, v);
+              }
+            }
+            float u, v;
+            f2_unpack(f2_add(sum[0], sum[1]), u, v);
+            l = u + v;
+            tmem_st32(s_at, packed);
+            if (paired) pass_turn(t);
+            tmem_wait_st();
+            tc_fence_before();
+          } else if (paired) {
+            take_turn(t);
+            pass_turn(t);
           }
-          tc_fence_before();
-        } else if (mine && whole) {
-          for (int i = 0; i < D / 8; ++i) *reinterpret_cast<uint4*>(dst + 8 * i) = make_uint4(0, 0, 0, 0);
+          __syncwarp();
+          if (lane == 0) arrive(p_full + t);
         }
-        if (mine && whole) {
-          if (a.lse != nullptr)
-            a.lse[((int64_t)now.b * a.H + head) * a.T + token] =
-                !live || l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
-        } else if (mine && live) {
-          a.part_ml[first_row + in_tile] = make_float2(m, l);
-        }
-        ++segment;
+        if (++buf == W::kBufs) buf = 0, phase ^= 1;
       }
-      begins = ends;
-      if (++buf == W::kBufs) buf = 0, phase ^= 1;
-      if (todo > 1) advance(a, now);
+      // ---- its end
+      const bool whole = last == now.tiles && first_tile == 0, mine = row < a.T * a.group;
+      if (act) {
+        wait_stage(o_full + t, o_phase, &given_up, a.p.status);
+        o_phase ^= 1;
+        tc_fence_after();
+      }
+      T* dst = static_cast<T*>(a.out) + now.b * a.out_st.b + token * a.out_st.s + head * a.out_st.h;
+      // partial rows: four channels of all rows, then the next four, so that the lanes' stores are whole lines
+      const int64_t first_row = (2 * (int64_t)blockIdx.x + (segment > 0)) * W::kRows;
+      const int in_tile = t * 128 + warp % 4 * 32 + lane;
+      float* part = a.part_o + first_row * D + in_tile * 4;
+      const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+      if (warp_live) {
+#pragma unroll 1
+        for (int i = 0; i < D / 32; ++i) {
+          uint32_t r[32];
+          tmem_ld32(o_at + 32 * i, r);
+          tmem_wait_ld();
+          if (mine && whole) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 8) {
+              float x[8];
+#pragma unroll
+              for (int z = 0; z < 8; ++z) x[z] = live && l != 0.0f ? __uint_as_float(r[k + z]) * inverse : 0.0f;
+              store8(dst + 32 * i + k, x);
+            }
+          } else if (mine && live) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 4)
+              *reinterpret_cast<uint4*>(part + (32 * i + k) * W::kRows) = make_uint4(r[k], r[k + 1], r[k + 2], r[k + 3]);
+          }
+        }
+        tc_fence_before();
+      } else if (mine && whole) {
+        for (int i = 0; i < D / 8; ++i) *reinterpret_cast<uint4*>(dst + 8 * i) = make_uint4(0, 0, 0, 0);
+      }
+      if (mine && whole) {
+        if (a.lse != nullptr)
+          a.lse[((int64_t)now.b * a.H + head) * a.T + token] =
+              !live || l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+      } else if (mine && live) {
+        a.part_ml[first_row + in_tile] = make_float2(m, l);
+      }
+      ++segment;
+      todo -= last - first_tile;
+      now.tile = last - 1;
+      if (todo > 0) advance(a, now);
     }
   }
   tc_fence_before();
@@ -529,7 +558,16 @@ static int launch_wide(const PagedAttnArgs& a, cudaStream_t st) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev >= 64 || !(prepared.load() >> dev & 1))) {
-    e = cudaFuncSetAttribute(paged_wide_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, W::kSmem);
+    // setmaxnreg moves registers inside what the CTA was launched with: a build with fewer would wait forever
+    cudaFuncAttributes fa{};
+    e = cudaFuncGetAttributes(&fa, paged_wide_kernel<T, D>);
+    if (e == cudaSuccess && W::QT == 2 && fa.numRegs != W::kLaunchRegs) {
+      set_error("paged attention built with %d registers per thread; its setmaxnreg split needs %d", fa.numRegs,
+                W::kLaunchRegs);
+      return SAGE_ERR_LAUNCH;
+    }
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(paged_wide_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, W::kSmem);
     if (e == cudaSuccess && dev < 64) prepared.fetch_or(uint64_t(1) << dev);
   }
   if (e == cudaSuccess) {
