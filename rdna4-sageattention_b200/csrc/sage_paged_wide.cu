@@ -5,13 +5,13 @@
 //   softmax warps   one warpgroup per row tile, one thread per row: q to TMEM (fp16), then per key tile S from TMEM,
 //                   weights (fp16) back over S, O rescaled in TMEM when the maximum moves, epilogue
 //   producer warp   TMA of the raw codes and scales into a ring
-//   MMA warps       one per row tile: S_t = Q_t K^T (A from TMEM, fp16), O_t += P_t V (A from TMEM); while row tile 0 is
-//                   in its softmax, row tile 1 is in its products
+//   MMA warps       one per row tile: S_t = Q_t K^T, O_t += P_t V (A from TMEM); two score tiles a row tile, so that the
+//                   scores of the next key tile are there when the softmax of this one ends
 //   4 converter warps   int8 and e4m3 codes to fp16 operand tiles in shared memory, once for all QT * 128 rows, and what
 //                   the rows need of each key (factor of its score, log2 of its V scale, the inverse of that)
-// Codes convert exactly, so there is nothing to choose there; with Q and P in TMEM the products read only K and V from
-// shared memory (64 KB a key tile of 64 for D 128 and 256 rows, beside 48 KB that the converters write).
-// TMEM (512 columns): O_t at t D, S_t / P_t at QT D + 64 t, Q_t at QT (D + 64) + t D / 2.
+// Codes convert exactly, so there is nothing to choose there.
+// TMEM (512 columns): O_t at t D, the score tiles of t at QT D + 128 t, P over the first half of its scores; Q_t behind
+// them where it fits (D 64 and 256), else in shared memory (D 96 and 128).
 #include "sage_paged_attn.cuh"
 
 namespace sage {
@@ -21,9 +21,9 @@ struct Wide {
   static constexpr int QT = D == 256 ? 1 : 2;
   static constexpr int kSoftmaxWarps = 4 * QT, kConverters = 4;
   // QT 2: 16 warps (one idle), so that the two warpgroups of the other roles hand registers to the two of softmax: 512
-  // threads of 128 at launch, then 256 of 168 and 256 of 80
+  // threads of 128 at launch, then 256 of 152 and 256 of 104
   static constexpr int kThreads = QT == 2 ? 512 : 32 * (kSoftmaxWarps + 1 + QT + kConverters);
-  static constexpr int kLaunchRegs = 128, kSoftmaxRegs = 168, kOtherRegs = 80;
+  static constexpr int kLaunchRegs = 128, kSoftmaxRegs = 152, kOtherRegs = 104;
   static_assert(QT != 2 || 256 * (kSoftmaxRegs + kOtherRegs) <= 512 * kLaunchRegs, "register split");
   static constexpr int kRows = 128 * QT;
   static constexpr int kPanels = (D + 63) / 64;            // of 64 channels: 128 bytes a key
@@ -31,11 +31,15 @@ struct Wide {
   static constexpr int kOperand = kPanels * kPanel;        // K or V of a tile in fp16
   static constexpr int kRaw = D == 256 ? 2 : 3;            // ring of raw stages
   static constexpr int kBufs = D == 256 ? 2 : 3;           // ring of operand tiles
-  static constexpr int kO = 0, kS = QT * D, kQ = kS + QT * kTileKeys;
-  static_assert(kQ + QT * D / 2 <= 512, "TMEM columns");
+  // Q as fp16: in TMEM where there is room beside O and two score tiles a row tile, else in shared memory
+  static constexpr bool kQShared = QT * (D + 2 * kTileKeys + D / 2) > 512;
+  static constexpr int kO = 0, kS = QT * D, kQ = kS + QT * 2 * kTileKeys;
+  static_assert(kQ + (kQShared ? 0 : QT * D / 2) <= 512, "TMEM columns");
+  static constexpr int kQPanel = 128 * 128, kQTile = kPanels * kQPanel;   // bytes in shared memory: 64 channels, a row tile
   static constexpr int kParams = 4 * kTileKeys;            // floats of a tile: factor, log2 V scale, inverse, gain
   static constexpr int kSmem = 1024 + kBufs * 2 * kOperand + kRaw * (Tile<D>::kStage + 2 * kTileKeys * 4) +
-                               kBufs * kParams * 4;
+                               kBufs * kParams * 4 + (kQShared ? QT * kQTile : 0);
+  static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
 // D(tmem) (+)= A(tmem) * B(smem), fp16 operands, fp32 accumulator.
@@ -48,6 +52,19 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uin
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
       "}\n" ::"r"(d_tmem),
       "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// The same with A in shared memory.
+__device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "setp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+      "}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 
@@ -82,11 +99,12 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
   extern __shared__ unsigned char smem_raw[];
   __shared__ int64_t warp_sums[W::kThreads / 32], found[2];
   __shared__ uint64_t raw_full[W::kRaw], raw_empty[W::kRaw], k_full[W::kBufs], v_full[W::kBufs], buf_empty[W::kBufs];
-  __shared__ uint64_t s_full[QT], p_full[QT], q_full[QT], o_full[QT], all_done[QT];
+  __shared__ uint64_t s_full[QT][2], p_full[QT][2], q_full[QT], o_full[QT], pv_done[QT], all_done[QT];
   __shared__ uint32_t tmem_base;
   __shared__ int given_up, zero_rows[W::kBufs][2];
   unsigned char* operands = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
-  unsigned char* stages = operands + W::kBufs * 2 * W::kOperand;
+  unsigned char* queries = operands + W::kBufs * 2 * W::kOperand;   // kQShared
+  unsigned char* stages = queries + (W::kQShared ? QT * W::kQTile : 0);
   float* scales = reinterpret_cast<float*>(stages + W::kRaw * S::kStage);
   float* params = scales + W::kRaw * 2 * kTileKeys;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
@@ -100,10 +118,10 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
       mbar_init(buf_empty + i, QT);
     }
     for (int t = 0; t < QT; ++t) {
-      mbar_init(s_full + t, 1);
-      mbar_init(p_full + t, 4);
+      for (int i = 0; i < 2; ++i) mbar_init(s_full[t] + i, 1), mbar_init(p_full[t] + i, 4);
       mbar_init(q_full + t, 4);
       mbar_init(o_full + t, 1);
+      mbar_init(pv_done + t, 1);
       mbar_init(all_done + t, 1);
     }
     fence_barrier_init();
@@ -143,52 +161,65 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
       const int t = warp - W::kSoftmaxWarps - 1;
       const uint64_t k_desc = smem_desc_kmajor(smem_u32(operands), 128);
       const uint64_t v_desc = smem_desc_nmajor(smem_u32(operands) + W::kOperand, W::kPanel);
-      const uint32_t s_at = tmem + W::kS + t * kTileKeys, q_at = tmem + W::kQ + t * (D / 2), o_at = tmem + W::kO + t * D;
-      int buf = 0;
-      uint32_t phase = 0, p_phase = 0, q_phase = 0;
-      bool begins = true;
-      auto scores = [&](int b) {
-        const uint64_t k = k_desc + b * (2 * W::kOperand / 16);
+      const uint64_t q_desc = smem_desc_kmajor(smem_u32(queries) + t * W::kQTile, 128);
+      const uint32_t s_at = tmem + W::kS + t * 2 * kTileKeys, q_at = tmem + W::kQ + t * (D / 2), o_at = tmem + W::kO + t * D;
+      int buf = 0;               // of the tile whose values are next, and of the one whose scores are next
+      int ahead = 0;
+      uint32_t phase = 0, ahead_phase = 0, p_phase = 0, q_phase = 0;   // p_phase: a bit per score tile
+      // scores of the next tile into score tile i
+      auto scores = [&](int i) {
+        wait_stage(k_full + ahead, ahead_phase, &given_up, a.p.status);
+        tc_fence_after();
+        const uint64_t k = k_desc + ahead * (2 * W::kOperand / 16);
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s)
-          mma_f16_ts(s_at, q_at + s * 8, k + (s / 4 * W::kPanel + s % 4 * 32) / 16, kScores, s > 0);
-        tc_commit(s_full + t);
-      };
-      for (; todo > 0; --todo) {
-        const bool act = active(now, t), more = todo > 1 && now.tile + 1 < now.tiles;
-        const int next = buf + 1 == W::kBufs ? 0 : buf + 1;
-        const uint32_t next_phase = next == 0 ? phase ^ 1 : phase;
-        if (act) {
-          if (begins) {
-            wait_stage(k_full + buf, phase, &given_up, a.p.status);
-            wait_stage(q_full + t, q_phase, &given_up, a.p.status);
-            q_phase ^= 1;
-            tc_fence_after();
-            scores(buf);
-          }
-          wait_stage(v_full + buf, phase, &given_up, a.p.status);
-          wait_stage(p_full + t, p_phase, &given_up, a.p.status);
-          p_phase ^= 1;
-          tc_fence_after();
-          const uint64_t v = v_desc + buf * (2 * W::kOperand / 16);
-#pragma unroll
-          for (int s = 0; s < kTileKeys / 16; ++s)
-            mma_f16_ts(o_at, s_at + s * 8, v + s * (2048 / 16), kValues, !begins || s > 0);
-          tc_commit(buf_empty + buf);
-          if (more) {
-            wait_stage(k_full + next, next_phase, &given_up, a.p.status);
-            tc_fence_after();
-            scores(next);
-          } else {
-            tc_commit(o_full + t);
-          }
-        } else {   // no row of this row tile is live
-          wait_stage(v_full + buf, phase, &given_up, a.p.status);
-          arrive(buf_empty + buf);
+        for (int s = 0; s < D / 16; ++s) {
+          const uint64_t ks = k + (s / 4 * W::kPanel + s % 4 * 32) / 16;
+          if constexpr (W::kQShared)
+            mma_f16_ss(s_at + i * kTileKeys, q_desc + (s / 4 * W::kQPanel + s % 4 * 32) / 16, ks, kScores, s > 0);
+          else
+            mma_f16_ts(s_at + i * kTileKeys, q_at + s * 8, ks, kScores, s > 0);
         }
-        begins = !more;
-        buf = next, phase = next_phase;
-        if (todo > 1) advance(a, now);
+        tc_commit(s_full[t] + i);
+      };
+      auto next = [](int& b, uint32_t& p) {
+        if (++b == W::kBufs) b = 0, p ^= 1;
+      };
+      while (todo > 0) {
+        const int tiles = (int)min((int64_t)(now.tiles - now.tile), todo);
+        if (active(now, t)) {
+          wait_stage(q_full + t, q_phase, &given_up, a.p.status);
+          q_phase ^= 1;
+          scores(0), next(ahead, ahead_phase);
+          if (tiles > 1) scores(1), next(ahead, ahead_phase);
+#pragma unroll 1
+          for (int j = 0; j < tiles; ++j) {
+            const int i = j & 1;
+            wait_stage(v_full + buf, phase, &given_up, a.p.status);
+            wait_stage(p_full[t] + i, p_phase >> i & 1, &given_up, a.p.status);
+            p_phase ^= 1u << i;
+            tc_fence_after();
+            const uint64_t v = v_desc + buf * (2 * W::kOperand / 16);
+#pragma unroll
+            for (int s = 0; s < kTileKeys / 16; ++s)
+              mma_f16_ts(o_at, s_at + i * kTileKeys + s * 8, v + s * (2048 / 16), kValues, j > 0 || s > 0);
+            tc_commit(pv_done + t);
+            tc_commit(buf_empty + buf);
+            next(buf, phase);
+            if (j + 2 < tiles) scores(i), next(ahead, ahead_phase);
+          }
+          tc_commit(o_full + t);
+        } else {   // no row of this row tile is live
+#pragma unroll 1
+          for (int j = 0; j < tiles; ++j) {
+            wait_stage(v_full + buf, phase, &given_up, a.p.status);
+            arrive(buf_empty + buf);
+            next(buf, phase);
+          }
+          ahead = buf, ahead_phase = phase;
+        }
+        todo -= tiles;
+        now.tile += tiles - 1;
+        if (todo > 0) advance(a, now);
       }
       tc_commit(all_done + t);   // nothing is in flight when the CTA ends
       wait_stage(all_done + t, 0, &given_up, a.p.status);
@@ -217,6 +248,21 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
         row = (pair / 4 * 8 + pair % 4) ^ (item / 4 % 2 * 5);
       }
     };
+    constexpr int kTogether = kItems < 4 ? kItems : 4;   // chunks of a thread under way at once
+    auto fetch = [&](const unsigned char* from, int i0, uint4 (&v)[kTogether]) {
+#pragma unroll
+      for (int i = 0; i < kTogether; ++i) {
+        int row, ch;
+        place(i0 + i, row, ch);
+        v[i] = *reinterpret_cast<const uint4*>(from + S::at(row, ch * 16));
+      }
+    };
+    auto put = [&](unsigned char* to, int i, const uint4& x, const uint4& y) {
+      int row, ch;
+      place(i, row, ch);
+      *reinterpret_cast<uint4*>(to + operand_at(row, 2 * ch)) = x;
+      *reinterpret_cast<uint4*>(to + operand_at(row, 2 * ch + 1)) = y;
+    };
     for (; todo > 0; --todo) {
       const int key0 = now.tile * kTileKeys, total = now.len + now.fresh;
       wait_stage(raw_full + raw, raw_phase, &given_up, a.p.status);
@@ -237,42 +283,51 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
         const bool any = __any_sync(0xffffffffu, zero);
         if (lane == 0) zero_rows[buf][cw] = any;
       }
-#pragma unroll 2
-      for (int i = 0; i < kItems; ++i) {
-        int row, ch;
-        place(i, row, ch);
-        const uint4 v = *reinterpret_cast<const uint4*>(kt + S::at(row, ch * 16));
-        uint4 x, y;
-        int8_to_f16(v.x, x.x, x.y), int8_to_f16(v.y, x.z, x.w), int8_to_f16(v.z, y.x, y.y), int8_to_f16(v.w, y.z, y.w);
-        *reinterpret_cast<uint4*>(to + operand_at(row, 2 * ch)) = x;
-        *reinterpret_cast<uint4*>(to + operand_at(row, 2 * ch + 1)) = y;
+#pragma unroll
+      for (int i0 = 0; i0 < kItems; i0 += kTogether) {
+        uint4 v[kTogether];
+        fetch(kt, i0, v);
+#pragma unroll
+        for (int i = 0; i < kTogether; ++i) {
+          uint4 x, y;
+          int8_to_f16(v[i].x, x.x, x.y), int8_to_f16(v[i].y, x.z, x.w);
+          int8_to_f16(v[i].z, y.x, y.y), int8_to_f16(v[i].w, y.z, y.w);
+          put(to, i0 + i, x, y);
+        }
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) arrive(k_full + buf);
       const bool drafts = key0 + kTileKeys > now.len;
-#pragma unroll 2
-      for (int i = 0; i < kItems; ++i) {
-        int row, ch;
-        place(i, row, ch);
-        uint4 v = *reinterpret_cast<const uint4*>(kt + S::kBytes + S::at(row, ch * 16));
+#pragma unroll
+      for (int i0 = 0; i0 < kItems; i0 += kTogether) {
+        uint4 v[kTogether];
+        fetch(kt + S::kBytes, i0, v);
         if (drafts) {
           // codes behind the last key are anything, and a NaN code of a draft that its reader does not see must not
           // reach it through 0 * NaN: both are cleared
-          if (key0 + row >= total) v = make_uint4(0, 0, 0, 0);
-          if (key0 + row >= now.len) {
-            v.x &= ~__vcmpeq4(v.x & 0x7f7f7f7fu, 0x7f7f7f7fu);
-            v.y &= ~__vcmpeq4(v.y & 0x7f7f7f7fu, 0x7f7f7f7fu);
-            v.z &= ~__vcmpeq4(v.z & 0x7f7f7f7fu, 0x7f7f7f7fu);
-            v.w &= ~__vcmpeq4(v.w & 0x7f7f7f7fu, 0x7f7f7f7fu);
+#pragma unroll
+          for (int i = 0; i < kTogether; ++i) {
+            int row, ch;
+            place(i0 + i, row, ch);
+            if (key0 + row >= total) v[i] = make_uint4(0, 0, 0, 0);
+            if (key0 + row >= now.len) {
+              v[i].x &= ~__vcmpeq4(v[i].x & 0x7f7f7f7fu, 0x7f7f7f7fu);
+              v[i].y &= ~__vcmpeq4(v[i].y & 0x7f7f7f7fu, 0x7f7f7f7fu);
+              v[i].z &= ~__vcmpeq4(v[i].z & 0x7f7f7f7fu, 0x7f7f7f7fu);
+              v[i].w &= ~__vcmpeq4(v[i].w & 0x7f7f7f7fu, 0x7f7f7f7fu);
+            }
           }
         }
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-        uint32_t x[8];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) x[2 * k] = e4m3_to_f16((uint16_t)w[k]), x[2 * k + 1] = e4m3_to_f16((uint16_t)(w[k] >> 16));
-        *reinterpret_cast<uint4*>(to + W::kOperand + operand_at(row, 2 * ch)) = make_uint4(x[0], x[1], x[2], x[3]);
-        *reinterpret_cast<uint4*>(to + W::kOperand + operand_at(row, 2 * ch + 1)) = make_uint4(x[4], x[5], x[6], x[7]);
+        for (int i = 0; i < kTogether; ++i) {
+          const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+          uint32_t x[8];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            x[2 * k] = e4m3_to_f16((uint16_t)w[k]), x[2 * k + 1] = e4m3_to_f16((uint16_t)(w[k] >> 16));
+          put(to + W::kOperand, i0 + i, make_uint4(x[0], x[1], x[2], x[3]), make_uint4(x[4], x[5], x[6], x[7]));
+        }
       }
       fence_proxy_async_smem();
       __syncwarp();
@@ -286,9 +341,10 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
     if constexpr (QT == 2) regs_increase<W::kSoftmaxRegs>();
     const int t = warp / 4;
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;   // of TMEM
-    const uint32_t s_at = tmem + lanes + W::kS + t * kTileKeys, o_at = tmem + lanes + W::kO + t * D;
+    const uint32_t s_tiles = tmem + lanes + W::kS + t * 2 * kTileKeys, o_at = tmem + lanes + W::kO + t * D;
     int buf = 0, segment = 0;
-    uint32_t phase = 0, s_phase = 0, o_phase = 0;
+    uint32_t phase = 0, s_phase = 0, o_phase = 0;   // s_phase: a bit per score tile
+    uint32_t pv_phase = 1;                          // of the row tile's last product
     // The two row tiles take turns in their exponentials, so that one is in its products while the other has the
     // special-function unit (left alone they fall into step: both wait, then both want it).
     if (QT == 2 && t == 1) asm volatile("bar.arrive 2, 256;" ::: "memory");
@@ -347,16 +403,31 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
                   for (int z = 0; z < 4; ++z) w[4 * k + z] = pack2(x[2 * z] * inverse, x[2 * z + 1] * inverse, __half());
                 }
               }
-              asm volatile(
-                  "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
-                  "%14, %15, %16};" ::"r"(tmem + lanes + W::kQ + t * (D / 2) + c0 / 2 + i * 16),
-                  "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "r"(w[8]),
-                  "r"(w[9]), "r"(w[10]), "r"(w[11]), "r"(w[12]), "r"(w[13]), "r"(w[14]), "r"(w[15])
-                  : "memory");
+              if constexpr (W::kQShared) {
+                const int r128 = warp % 4 * 32 + lane;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                  const int ch = (c0 + 32 * i) / 8 + k;
+                  *reinterpret_cast<uint4*>(queries + t * W::kQTile + ch / 8 * W::kQPanel + r128 * 128 +
+                                            (((ch % 8) ^ (r128 & 7)) << 4)) =
+                      make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+                }
+              } else {
+                asm volatile(
+                    "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
+                    "%14, %15, %16};" ::"r"(tmem + lanes + W::kQ + t * (D / 2) + c0 / 2 + i * 16),
+                    "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "r"(w[8]),
+                    "r"(w[9]), "r"(w[10]), "r"(w[11]), "r"(w[12]), "r"(w[13]), "r"(w[14]), "r"(w[15])
+                    : "memory");
+              }
             }
           }
-          tmem_wait_st();
-          tc_fence_before();
+          if constexpr (W::kQShared) {
+            fence_proxy_async_smem();
+          } else {
+            tmem_wait_st();
+            tc_fence_before();
+          }
         }
         __syncwarp();
         if (lane == 0) arrive(q_full + t);
@@ -364,8 +435,10 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
 #pragma unroll 1
       for (int tile = first_tile; tile < last; ++tile) {
         if (act) {
-          wait_stage(s_full + t, s_phase, &given_up, a.p.status);
-          s_phase ^= 1;
+          const int si = (tile - first_tile) & 1;
+          const uint32_t s_at = s_tiles + si * kTileKeys;
+          wait_stage(s_full[t] + si, s_phase >> si & 1, &given_up, a.p.status);
+          s_phase ^= 1u << si;
           if (warp_live) {
             wait_stage(k_full + buf, phase, &given_up, a.p.status);   // long there: orders the reads of params, zero_rows
             tc_fence_after();
@@ -432,6 +505,9 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
               m = next;
               l *= keep;
               if (tile != first_tile) {   // the first product of a row tile overwrites O
+                // the products of the tile before must be done (those of older tiles are: this tile's scores came after)
+                wait_stage(pv_done + t, pv_phase, &given_up, a.p.status);
+                tc_fence_after();
                 const uint64_t keep2 = f2_pack(keep, keep);
 #pragma unroll 1
                 for (int i = 0; i < D / 32; ++i) {
@@ -484,7 +560,8 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
             pass_turn(t);
           }
           __syncwarp();
-          if (lane == 0) arrive(p_full + t);
+          if (lane == 0) arrive(p_full[t] + si);
+          pv_phase ^= 1;
         }
         if (++buf == W::kBufs) buf = 0, phase ^= 1;
       }
