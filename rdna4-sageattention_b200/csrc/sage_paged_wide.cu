@@ -36,7 +36,7 @@ struct Wide {
   static constexpr int kO = 0, kS = QT * D, kQ = kS + QT * 2 * kTileKeys;
   static_assert(kQ + (kQShared ? 0 : QT * D / 2) <= 512, "TMEM columns");
   static constexpr int kQPanel = 128 * 128, kQTile = kPanels * kQPanel;   // bytes in shared memory: 64 channels, a row tile
-  static constexpr int kParams = 4 * kTileKeys;            // floats of a tile: factor, log2 V scale, inverse, gain
+  static constexpr int kParams = 5 * kTileKeys;            // floats of a tile: factor, log2 V scale, inverse, gain, V scale
   static constexpr int kSmem = 1024 + kBufs * 2 * kOperand + kRaw * (Tile<D>::kStage + 2 * kTileKeys * 4) +
                                kBufs * kParams * 4 + (kQShared ? QT * kQTile : 0);
   static_assert(kSmem <= 227 * 1024, "shared memory");
@@ -68,6 +68,33 @@ __device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uin
       : "memory");
 }
 
+// 32 lanes x 16 (8) consecutive 32-bit columns.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
+// Bit i: byte i of the word is not zero.
+__device__ __forceinline__ uint32_t nonzero_bytes(uint32_t w) {
+  return ((__vcmpne4(w, 0) & 0x01010101u) * 0x10204080u) >> 28;
+}
+
 // Instruction descriptor, kind::f16: fp16 A and B, fp32 D; b_mn: B is stored with N contiguous.
 __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool b_mn) {
   return (1u << 4) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
@@ -85,10 +112,6 @@ __device__ __forceinline__ int operand_at(int row, int ch) {
   return ch / 8 * (kTileKeys * 128) + row * 128 + (((ch % 8) ^ (row & 7)) << 4);
 }
 
-// Turns of the two softmax warpgroups: each waits for its own named barrier, which the other arrives at.
-__device__ __forceinline__ void take_turn(int t) { asm volatile("bar.sync %0, 256;" ::"r"(2 + t) : "memory"); }
-__device__ __forceinline__ void pass_turn(int t) { asm volatile("bar.arrive %0, 256;" ::"r"(3 - t) : "memory"); }
-
 template <typename T, int D>
 __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
     paged_wide_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap k_map,
@@ -101,7 +124,8 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
   __shared__ uint64_t raw_full[W::kRaw], raw_empty[W::kRaw], k_full[W::kBufs], v_full[W::kBufs], buf_empty[W::kBufs];
   __shared__ uint64_t s_full[QT][2], p_full[QT][2], q_full[QT], o_full[QT], pv_done[QT], all_done[QT];
   __shared__ uint32_t tmem_base;
-  __shared__ int given_up, zero_rows[W::kBufs][2];
+  __shared__ int given_up;
+  __shared__ float q_scale[QT][128];
   unsigned char* operands = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   unsigned char* queries = operands + W::kBufs * 2 * W::kOperand;   // kQShared
   unsigned char* stages = queries + (W::kQShared ? QT * W::kQTile : 0);
@@ -230,7 +254,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
   } else if (warp > W::kSoftmaxWarps) {
     // ------------------------------------------------------------------------------------------------ converters
     if constexpr (QT == 2) regs_decrease<W::kOtherRegs>();
-    const int ct = tid - 32 * (W::kSoftmaxWarps + 1 + QT), cw = ct / 32;
+    const int ct = tid - 32 * (W::kSoftmaxWarps + 1 + QT);
     int raw = 0, buf = 0;
     uint32_t raw_phase = 0, phase = 0;
     // The eight lanes of a phase of a 16-byte access take four neighbouring chunks of a raw row and of the row that
@@ -280,8 +304,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
         // not see the key must not meet 0 * NaN or 0 * infinity here
         out[2 * kTileKeys + ct] = !there ? 0.0f : zero ? 1.0f : vs > 0x1p-120f ? __fdividef(1.0f, vs) : 0x1p120f;
         out[3 * kTileKeys + ct] = zero ? -kZeroLog : 0.0f;
-        const bool any = __any_sync(0xffffffffu, zero);
-        if (lane == 0) zero_rows[buf][cw] = any;
+        out[4 * kTileKeys + ct] = vs;
       }
 #pragma unroll
       for (int i0 = 0; i0 < kItems; i0 += kTogether) {
@@ -342,83 +365,117 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
     const int t = warp / 4;
     const uint32_t lanes = (uint32_t)(warp % 4 * 32) << 16;   // of TMEM
     const uint32_t s_tiles = tmem + lanes + W::kS + t * 2 * kTileKeys, o_at = tmem + lanes + W::kO + t * D;
+    const bool mask_vectors = a.T % 16 == 0 && (reinterpret_cast<uintptr_t>(a.mask) & 15) == 0 && a.mask_i % 16 == 0 &&
+                              a.mask_b % 16 == 0;
     int buf = 0, segment = 0;
     uint32_t phase = 0, s_phase = 0, o_phase = 0;   // s_phase: a bit per score tile
     uint32_t pv_phase = 1;                          // of the row tile's last product
-    // The two row tiles take turns in their exponentials, so that one is in its products while the other has the
-    // special-function unit (left alone they fall into step: both wait, then both want it).
-    if (QT == 2 && t == 1) asm volatile("bar.arrive 2, 256;" ::: "memory");
     while (todo > 0) {
       // ---- a row tile, or this CTA's part of it: key tiles first_tile ... last - 1
       const int first_tile = now.tile, last = (int)min((int64_t)now.tiles, now.tile + todo);
-      const bool act = active(now, t), paired = QT == 2 && active(now, QT - 1);   // tile 0 is active where tile 1 is
+      const bool act = active(now, t);
       const int row = now.unit % a.row_tiles * W::kRows + t * 128 + warp % 4 * 32 + lane, token = row / a.group;
       const int head = now.unit / a.row_tiles * a.group + row % a.group;
       const bool warp_live = act && row - lane < now.fresh * a.group, live = token < now.fresh;
       float m = -3.402823466e38f, l = 0.0f, row_scale = 1.0f;
       if (act) {
         if (warp_live) {
-          // the row in fp16, scaled by a power of two of its largest value, as D / 2 TMEM columns
-          const T* src = static_cast<const T*>(a.q) + now.b * a.q_st.b + token * a.q_st.s + head * a.q_st.h;
-          constexpr int kPart = D == 256 ? 128 : D;   // channels held in registers at once
-          uint4 v[kPart / 8];
-          auto fetch = [&](int c0) {
+          if constexpr (D == 128) {
+            // 16 lanes a row, two rows at a time: whole lines (a row a lane would touch each line eight times over)
+            const int tile_row = now.unit % a.row_tiles * W::kRows + t * 128, base = warp % 4 * 32 + lane / 16, ch = lane % 16;
+            uint4 v[16];
+            int tok = (tile_row + base) / a.group, in_group = (tile_row + base) - tok * a.group;
+            const T* heads = static_cast<const T*>(a.q) + now.b * a.q_st.b + (int64_t)(now.unit / a.row_tiles) * a.group * a.q_st.h;
 #pragma unroll
-            for (int i = 0; i < kPart / 8; ++i)
-              v[i] = live ? *reinterpret_cast<const uint4*>(src + c0 + 8 * i) : make_uint4(0, 0, 0, 0);
-          };
-          fetch(0);
-          float inverse = 1.0f;
-          if constexpr (!std::is_same<T, __half>::value) {
-            uint32_t top = 0;
+            for (int i = 0; i < 16; ++i) {
+              const T* src = heads + tok * a.q_st.s + in_group * a.q_st.h;
+              v[i] = tok < now.fresh ? *reinterpret_cast<const uint4*>(src + ch * 8) : make_uint4(0, 0, 0, 0);
+              in_group += 2;
+              if (in_group >= a.group) in_group -= a.group, ++tok;
+              if (in_group >= a.group) in_group -= a.group, ++tok;
+            }
 #pragma unroll
-            for (int c0 = D - kPart; c0 >= 0; c0 -= kPart) {
-              if (D > kPart) fetch(c0);
+            for (int i = 0; i < 16; ++i) {
+              const int r128 = base + 2 * i;
+              uint4 w = v[i];
+              if constexpr (!std::is_same<T, __half>::value) {
+                uint32_t top = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu),
+                                        __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
+#pragma unroll
+                for (int o = 1; o < 16; o *= 2) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
+                top = max(top & 0xffffu, top >> 16);
+                // 2^e with e the exponent of the row's largest value (zero, infinite and NaN rows: 1; tiny ones: 2^-100)
+                const int e = top == 0 || top >= 0x7f80u ? 127 : max((int)(top >> 7), 27);
+                const float inverse = __int_as_float((254 - e) << 23);
+                if (ch == 0) q_scale[t][r128] = __int_as_float(e << 23);
+                float x[8];
+                unpack8(v[i], x, T());
+                w = make_uint4(pack2(x[0] * inverse, x[1] * inverse, __half()), pack2(x[2] * inverse, x[3] * inverse, __half()),
+                               pack2(x[4] * inverse, x[5] * inverse, __half()), pack2(x[6] * inverse, x[7] * inverse, __half()));
+              }
+              *reinterpret_cast<uint4*>(queries + t * W::kQTile + ch / 8 * W::kQPanel + r128 * 128 +
+                                        (((ch % 8) ^ (r128 & 7)) << 4)) = w;
+            }
+            __syncwarp();
+            if constexpr (!std::is_same<T, __half>::value) row_scale = q_scale[t][warp % 4 * 32 + lane];
+          } else {
+            // the row in fp16, scaled by a power of two of its largest value, as D / 2 TMEM columns
+            const T* src = static_cast<const T*>(a.q) + now.b * a.q_st.b + token * a.q_st.s + head * a.q_st.h;
+            constexpr int kPart = D == 256 ? 128 : D;   // channels held in registers at once
+            uint4 v[kPart / 8];
+            auto fetch = [&](int c0) {
 #pragma unroll
               for (int i = 0; i < kPart / 8; ++i)
-                top = __vmaxu2(top, __vmaxu2(__vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu),
-                                             __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu)));
-            }
-            top = max(top & 0xffffu, top >> 16);
-            // 2^e with e the exponent of that value (zero, infinite and NaN rows: 1; tiny ones: 2^-100)
-            const int e = top == 0 || top >= 0x7f80u ? 127 : max((int)(top >> 7), 27);
-            row_scale = __int_as_float(e << 23);
-            inverse = __int_as_float((254 - e) << 23);
-          }
+                v[i] = live ? *reinterpret_cast<const uint4*>(src + c0 + 8 * i) : make_uint4(0, 0, 0, 0);
+            };
+            fetch(0);
+            float inverse = 1.0f;
+            if constexpr (!std::is_same<T, __half>::value) {
+              uint32_t top = 0;
 #pragma unroll
-          for (int c0 = 0; c0 < D; c0 += kPart) {
-            if (c0 > 0) fetch(c0);
+              for (int c0 = D - kPart; c0 >= 0; c0 -= kPart) {
+                if (D > kPart) fetch(c0);
 #pragma unroll
-            for (int i = 0; i < kPart / 32; ++i) {   // 32 channels: 16 columns
-              uint32_t w[16];
-#pragma unroll
-              for (int k = 0; k < 4; ++k) {
-                const uint4 y = v[4 * i + k];
-                if constexpr (std::is_same<T, __half>::value) {
-                  w[4 * k] = y.x, w[4 * k + 1] = y.y, w[4 * k + 2] = y.z, w[4 * k + 3] = y.w;
-                } else {
-                  float x[8];
-                  unpack8(y, x, T());
-#pragma unroll
-                  for (int z = 0; z < 4; ++z) w[4 * k + z] = pack2(x[2 * z] * inverse, x[2 * z + 1] * inverse, __half());
-                }
+                for (int i = 0; i < kPart / 8; ++i)
+                  top = __vmaxu2(top, __vmaxu2(__vmaxu2(v[i].x & 0x7fff7fffu, v[i].y & 0x7fff7fffu),
+                                               __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu)));
               }
-              if constexpr (W::kQShared) {
-                const int r128 = warp % 4 * 32 + lane;
+              top = max(top & 0xffffu, top >> 16);
+              // 2^e with e the exponent of that value (zero, infinite and NaN rows: 1; tiny ones: 2^-100)
+              const int e = top == 0 || top >= 0x7f80u ? 127 : max((int)(top >> 7), 27);
+              row_scale = __int_as_float(e << 23);
+              inverse = __int_as_float((254 - e) << 23);
+            }
+#pragma unroll
+            for (int c0 = 0; c0 < D; c0 += kPart) {
+              if (c0 > 0) fetch(c0);
+#pragma unroll
+              for (int i = 0; i < kPart / 32; ++i) {   // 32 channels: 16 columns
+                uint32_t w[16];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                  const int ch = (c0 + 32 * i) / 8 + k;
-                  *reinterpret_cast<uint4*>(queries + t * W::kQTile + ch / 8 * W::kQPanel + r128 * 128 +
-                                            (((ch % 8) ^ (r128 & 7)) << 4)) =
-                      make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+                  const uint4 y = v[4 * i + k];
+                  if constexpr (std::is_same<T, __half>::value) {
+                    w[4 * k] = y.x, w[4 * k + 1] = y.y, w[4 * k + 2] = y.z, w[4 * k + 3] = y.w;
+                  } else {
+                    float x[8];
+                    unpack8(y, x, T());
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) w[4 * k + z] = pack2(x[2 * z] * inverse, x[2 * z + 1] * inverse, __half());
+                  }
                 }
-              } else {
-                asm volatile(
-                    "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, "
-                    "%14, %15, %16};" ::"r"(tmem + lanes + W::kQ + t * (D / 2) + c0 / 2 + i * 16),
-                    "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]), "r"(w[8]),
-                    "r"(w[9]), "r"(w[10]), "r"(w[11]), "r"(w[12]), "r"(w[13]), "r"(w[14]), "r"(w[15])
-                    : "memory");
+                if constexpr (W::kQShared) {
+                  const int r128 = warp % 4 * 32 + lane;
+#pragma unroll
+                  for (int k = 0; k < 4; ++k) {
+                    const int ch = (c0 + 32 * i) / 8 + k;
+                    *reinterpret_cast<uint4*>(queries + t * W::kQTile + ch / 8 * W::kQPanel + r128 * 128 +
+                                              (((ch % 8) ^ (r128 & 7)) << 4)) =
+                        make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+                  }
+                } else {
+                  tmem_st16(tmem + lanes + W::kQ + t * (D / 2) + c0 / 2 + i * 16, w);
+                }
               }
             }
           }
@@ -440,124 +497,149 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
           wait_stage(s_full[t] + si, s_phase >> si & 1, &given_up, a.p.status);
           s_phase ^= 1u << si;
           if (warp_live) {
-            wait_stage(k_full + buf, phase, &given_up, a.p.status);   // long there: orders the reads of params, zero_rows
+            wait_stage(k_full + buf, phase, &given_up, a.p.status);   // long there: orders the reads of params
             tc_fence_after();
             const float* factor = params + buf * W::kParams;
             const int key0 = tile * kTileKeys;
             const bool drafts = key0 + kTileKeys > now.len;
-            uint64_t seen = ~uint64_t(0);
-            if (drafts) {
-              // bit j: the row sees key key0 + j (what is behind the last key has a factor of its own that hides it)
-              const int t0 = key0 - now.len;   // number of the first key as a draft
-              seen = t0 >= 0 ? 0 : (uint64_t(1) << -t0) - 1;
-              if (live) {
-                const int from = max(t0, 0);
-                if (a.mask != nullptr) {
-                  const uint8_t* mask = a.mask + now.b * a.mask_b + token * a.mask_i;
-                  const int to = min(t0 + kTileKeys, now.fresh);
-#pragma unroll 8
-                  for (int d = from; d < to; ++d) seen |= (uint64_t)(mask[d] != 0) << (d - t0);
-                } else if (token >= from) {
-                  const int count = min(token - t0 + 1, kTileKeys);
-                  seen |= count == kTileKeys ? ~uint64_t(0) : (uint64_t(1) << count) - 1;
-                }
-              }
-            }
-            uint64_t x[kTileKeys / 2];   // two scores each
-#pragma unroll
-            for (int part = 0; part < 2; ++part) {
-              uint32_t r[32];
-              tmem_ld32(s_at + 32 * part, r);
-              tmem_wait_ld();
-              const uint64_t scale2 = f2_pack(row_scale, row_scale);
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float4 f = *reinterpret_cast<const float4*>(factor + 32 * part + 4 * i);
-                const float4 g = *reinterpret_cast<const float4*>(factor + kTileKeys + 32 * part + 4 * i);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                  const int c = 4 * i + 2 * h;
-                  uint64_t v = f2_pack(__uint_as_float(r[c]), __uint_as_float(r[c + 1]));
-                  if constexpr (!std::is_same<T, __half>::value) v = f2_mul(v, scale2);
-                  x[16 * part + c / 2] = f2_fma(v, h ? f2_pack(f.z, f.w) : f2_pack(f.x, f.y), h ? f2_pack(g.z, g.w) : f2_pack(g.x, g.y));
-                }
-              }
-            }
-            if (drafts) {
-#pragma unroll
-              for (int i = 0; i < kTileKeys / 2; ++i) {
-                float u, v;
-                f2_unpack(x[i], u, v);
-                x[i] = f2_pack(seen >> (2 * i) & 1 ? u : -INFINITY, seen >> (2 * i + 1) & 1 ? v : -INFINITY);
-              }
-            }
-            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int i = 0; i < kTileKeys / 2; ++i) {
-              float u, v;
-              f2_unpack(x[i], u, v);
-              top[i % 4] = fmaxf(fmaxf(top[i % 4], u), v);
-            }
-            const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-            if (__any_sync(0xffffffffu, most > m + 8.0f)) {
-              const float next = most > m + 8.0f ? most : m;
-              const float keep = next == m ? 1.0f : fast_exp2(m - next);
-              m = next;
-              l *= keep;
-              if (tile != first_tile) {   // the first product of a row tile overwrites O
-                // the products of the tile before must be done (those of older tiles are: this tile's scores came after)
-                wait_stage(pv_done + t, pv_phase, &given_up, a.p.status);
-                tc_fence_after();
-                const uint64_t keep2 = f2_pack(keep, keep);
-#pragma unroll 1
-                for (int i = 0; i < D / 32; ++i) {
-                  uint32_t r[32];
-                  tmem_ld32(o_at + 32 * i, r);
-                  tmem_wait_ld();
-#pragma unroll
-                  for (int k = 0; k < 32; k += 2) {
-                    float u, v;
-                    f2_unpack(f2_mul(f2_pack(__uint_as_float(r[k]), __uint_as_float(r[k + 1])), keep2), u, v);
-                    r[k] = __float_as_uint(u), r[k + 1] = __float_as_uint(v);
-                  }
-                  tmem_st32(o_at + 32 * i, r);
-                }
-              }
-            }
-            if ((zero_rows[buf][0] | zero_rows[buf][1]) != 0) {
-#pragma unroll
-              for (int i = 0; i < kTileKeys / 4; ++i) {
-                const float4 g = *reinterpret_cast<const float4*>(factor + 3 * kTileKeys + 4 * i);
-                x[2 * i] = f2_add(x[2 * i], f2_pack(g.x, g.y)), x[2 * i + 1] = f2_add(x[2 * i + 1], f2_pack(g.z, g.w));
-              }
-            }
-            const uint64_t minus_m = f2_pack(-m, -m);
-            if (paired) take_turn(t);
-            uint64_t sum[2] = {f2_pack(l, 0.0f), f2_pack(0.0f, 0.0f)};
             uint32_t packed[32];
+            bool again = true;
+            // Most tiles: every row sees every key and no maximum moves.  The weights are computed on that assumption in
+            // one straight run, p vs = 2^(s - m') vs and l from 2^(s - m') itself, and looked over afterwards; where it did
+            // not hold the scores are still in TMEM, and the tile is done over.  (What a key needs is read by every lane
+            // of eight warps, and the words returned are what shared memory is busy with: two a key here, not three.)
+            if (tile != first_tile && !drafts) {
+              const uint64_t scale2 = f2_pack(row_scale, row_scale), minus_m = f2_pack(-m, -m);
+              uint64_t sum[2] = {f2_pack(l, 0.0f), f2_pack(0.0f, 0.0f)};
+              float top[2] = {0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < kTileKeys / 4; ++i) {
-              const float4 inv = *reinterpret_cast<const float4*>(factor + 2 * kTileKeys + 4 * i);
+              for (int part = 0; part < 2; ++part) {
+                uint32_t r[32];
+                tmem_ld32(s_at + 32 * part, r);
+                tmem_wait_ld();
 #pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const int c = 2 * i + h;
-                float u, v;
-                f2_unpack(f2_add(x[c], minus_m), u, v);
-                u = fast_exp2(u), v = fast_exp2(v);
-                sum[h] = f2_fma(f2_pack(u, v), h ? f2_pack(inv.z, inv.w) : f2_pack(inv.x, inv.y), sum[h]);
-                packed[c] = pack_weights(u, v);
+                for (int i = 0; i < 8; ++i) {
+                  const int k = 32 * part + 4 * i;
+                  const float4 f = *reinterpret_cast<const float4*>(factor + k);
+                  const float4 w = *reinterpret_cast<const float4*>(factor + 4 * kTileKeys + k);
+#pragma unroll
+                  for (int h = 0; h < 2; ++h) {
+                    const int c = 4 * i + 2 * h;
+                    uint64_t v = f2_pack(__uint_as_float(r[c]), __uint_as_float(r[c + 1]));
+                    if constexpr (!std::is_same<T, __half>::value) v = f2_mul(v, scale2);
+                    float p, q;
+                    f2_unpack(f2_fma(v, h ? f2_pack(f.z, f.w) : f2_pack(f.x, f.y), minus_m), p, q);
+                    const uint64_t e = f2_pack(fast_exp2(p), fast_exp2(q));
+                    sum[h] = f2_add(e, sum[h]);
+                    f2_unpack(f2_mul(e, h ? f2_pack(w.z, w.w) : f2_pack(w.x, w.y)), p, q);
+                    top[h] = fmaxf(fmaxf(top[h], p), q);
+                    packed[16 * part + c / 2] = pack_weights(p, q);
+                  }
+                }
+              }
+              float p, q;
+              f2_unpack(f2_add(sum[0], sum[1]), p, q);
+              p += q;
+              // a weight above 2^8, or one whose V row is zero above all bounds
+              again = __any_sync(0xffffffffu, !(fmaxf(top[0], top[1]) <= 256.0f && p < 0x1p120f));
+              if (!again) l = p;
+            }
+            if (!again) {
+              tmem_st32(s_at, packed);
+            } else {
+              // which keys the row sees: bit j is key key0 + j (what is behind the last key has a factor that hides it)
+              uint64_t seen = ~uint64_t(0);
+              if (drafts) {
+                const int t0 = key0 - now.len;   // number of the first key as a draft
+                seen = t0 >= 0 ? 0 : (uint64_t(1) << -t0) - 1;
+                if (live) {
+                  const int from = max(t0, 0);
+                  if (a.mask != nullptr) {
+                    const uint8_t* mask = a.mask + now.b * a.mask_b + token * a.mask_i;
+                    const int to = min(t0 + kTileKeys, now.fresh);
+                    if (mask_vectors) {   // rows of whole 16-byte vectors
+#pragma unroll 5
+                      for (int d = from & ~15; d < to; d += 16) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(mask + d);
+                        const uint64_t bits = nonzero_bytes(v.x) | nonzero_bytes(v.y) << 4 | nonzero_bytes(v.z) << 8 |
+                                              nonzero_bytes(v.w) << 12;
+                        seen |= d >= t0 ? bits << (d - t0) : bits >> (t0 - d);
+                      }
+                    } else {
+#pragma unroll 8
+                      for (int d = from; d < to; ++d) seen |= (uint64_t)(mask[d] != 0) << (d - t0);
+                    }
+                    if (now.fresh - t0 < kTileKeys) seen &= (uint64_t(1) << (now.fresh - t0)) - 1;
+                  } else if (token >= from) {
+                    const int count = min(token - t0 + 1, kTileKeys);
+                    seen |= count == kTileKeys ? ~uint64_t(0) : (uint64_t(1) << count) - 1;
+                  }
+                }
+              }
+              // the exponents of 16 keys; small loops on purpose: this code runs once or twice a row tile, and what it
+              // costs is fetching it
+              auto exponents = [&](int k, float (&x)[16]) {
+                uint32_t r[16];
+                tmem_ld16(s_at + 16 * k, r);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                  const float4 f = *reinterpret_cast<const float4*>(factor + 16 * k + i);
+                  const float4 g = *reinterpret_cast<const float4*>(factor + kTileKeys + 16 * k + i);
+                  const float fs[4] = {f.x, f.y, f.z, f.w}, gs[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+                  for (int h = 0; h < 4; ++h) {
+                    x[i + h] = fmaf(__uint_as_float(r[i + h]) * row_scale, fs[h], gs[h]);
+                    if (!(seen >> (16 * k + i + h) & 1)) x[i + h] = -INFINITY;
+                  }
+                }
+              };
+              float most = -INFINITY;
+#pragma unroll 1
+              for (int k = 0; k < kTileKeys / 16; ++k) {
+                float x[16];
+                exponents(k, x);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) most = fmaxf(most, x[i]);
+              }
+              if (__any_sync(0xffffffffu, most > m + 8.0f)) {
+                const float next = most > m + 8.0f ? most : m;
+                const float keep = next == m ? 1.0f : fast_exp2(m - next);
+                m = next;
+                l *= keep;
+                if (tile != first_tile) {   // the first product of a row tile overwrites O
+                  // the products of the tile before must be done (older ones are: this tile's scores came after them)
+                  wait_stage(pv_done + t, pv_phase, &given_up, a.p.status);
+                  tc_fence_after();
+#pragma unroll 1
+                  for (int i = 0; i < D / 16; ++i) {
+                    uint32_t r[16];
+                    tmem_ld16(o_at + 16 * i, r);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * keep);
+                    tmem_st16(o_at + 16 * i, r);
+                  }
+                }
+              }
+#pragma unroll 1
+              for (int k = 0; k < kTileKeys / 16; ++k) {   // the weights of 16 keys take 8 columns, all read by then
+                float x[16];
+                exponents(k, x);
+                uint32_t w[8];
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                  const float2 inv = *reinterpret_cast<const float2*>(factor + 2 * kTileKeys + 16 * k + i);
+                  const float2 gain = *reinterpret_cast<const float2*>(factor + 3 * kTileKeys + 16 * k + i);
+                  const float p = fast_exp2(x[i] - m + gain.x), q = fast_exp2(x[i + 1] - m + gain.y);
+                  l = fmaf(q, inv.y, fmaf(p, inv.x, l));
+                  w[i / 2] = pack_weights(p, q);
+                }
+                tmem_st8(s_at + 8 * k, w);
               }
             }
-            float u, v;
-            f2_unpack(f2_add(sum[0], sum[1]), u, v);
-            l = u + v;
-            tmem_st32(s_at, packed);
-            if (paired) pass_turn(t);
             tmem_wait_st();
             tc_fence_before();
-          } else if (paired) {
-            take_turn(t);
-            pass_turn(t);
           }
           __syncwarp();
           if (lane == 0) arrive(p_full[t] + si);
