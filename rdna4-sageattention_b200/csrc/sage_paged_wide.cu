@@ -383,38 +383,48 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
           if constexpr (D == 128) {
             // 16 lanes a row, two rows at a time: whole lines (a row a lane would touch each line eight times over)
             const int tile_row = now.unit % a.row_tiles * W::kRows + t * 128, base = warp % 4 * 32 + lane / 16, ch = lane % 16;
-            uint4 v[16];
             int tok = (tile_row + base) / a.group, in_group = (tile_row + base) - tok * a.group;
             const T* heads = static_cast<const T*>(a.q) + now.b * a.q_st.b + (int64_t)(now.unit / a.row_tiles) * a.group * a.q_st.h;
+            // a small loop with the next rows under way: unrolled, fetching the code would take longer than the rows
+            uint4 v[4];
+            auto fetch = [&] {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const T* src = heads + tok * a.q_st.s + in_group * a.q_st.h;
-              v[i] = tok < now.fresh ? *reinterpret_cast<const uint4*>(src + ch * 8) : make_uint4(0, 0, 0, 0);
-              in_group += 2;
-              if (in_group >= a.group) in_group -= a.group, ++tok;
-              if (in_group >= a.group) in_group -= a.group, ++tok;
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int r128 = base + 2 * i;
-              uint4 w = v[i];
-              if constexpr (!std::is_same<T, __half>::value) {
-                uint32_t top = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu),
-                                        __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
-#pragma unroll
-                for (int o = 1; o < 16; o *= 2) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
-                top = max(top & 0xffffu, top >> 16);
-                // 2^e with e the exponent of the row's largest value (zero, infinite and NaN rows: 1; tiny ones: 2^-100)
-                const int e = top == 0 || top >= 0x7f80u ? 127 : max((int)(top >> 7), 27);
-                const float inverse = __int_as_float((254 - e) << 23);
-                if (ch == 0) q_scale[t][r128] = __int_as_float(e << 23);
-                float x[8];
-                unpack8(v[i], x, T());
-                w = make_uint4(pack2(x[0] * inverse, x[1] * inverse, __half()), pack2(x[2] * inverse, x[3] * inverse, __half()),
-                               pack2(x[4] * inverse, x[5] * inverse, __half()), pack2(x[6] * inverse, x[7] * inverse, __half()));
+              for (int i = 0; i < 4; ++i) {
+                v[i] = tok < now.fresh ? *reinterpret_cast<const uint4*>(heads + tok * a.q_st.s + in_group * a.q_st.h + ch * 8)
+                                       : make_uint4(0, 0, 0, 0);
+                in_group += 2;
+                if (in_group >= a.group) in_group -= a.group, ++tok;
+                if (in_group >= a.group) in_group -= a.group, ++tok;
               }
-              *reinterpret_cast<uint4*>(queries + t * W::kQTile + ch / 8 * W::kQPanel + r128 * 128 +
-                                        (((ch % 8) ^ (r128 & 7)) << 4)) = w;
+            };
+            fetch();
+#pragma unroll 1
+            for (int i0 = 0; i0 < 16; i0 += 4) {
+              uint4 w[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) w[i] = v[i];
+              if (i0 < 12) fetch();
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int r128 = base + 2 * (i0 + i);
+                if constexpr (!std::is_same<T, __half>::value) {
+                  uint32_t top = __vmaxu2(__vmaxu2(w[i].x & 0x7fff7fffu, w[i].y & 0x7fff7fffu),
+                                          __vmaxu2(w[i].z & 0x7fff7fffu, w[i].w & 0x7fff7fffu));
+#pragma unroll
+                  for (int o = 1; o < 16; o *= 2) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
+                  top = max(top & 0xffffu, top >> 16);
+                  // 2^e with e the exponent of the row's largest value (zero, infinite and NaN rows: 1; tiny ones: 2^-100)
+                  const int e = top == 0 || top >= 0x7f80u ? 127 : max((int)(top >> 7), 27);
+                  const float inverse = __int_as_float((254 - e) << 23);
+                  if (ch == 0) q_scale[t][r128] = __int_as_float(e << 23);
+                  float x[8];
+                  unpack8(w[i], x, T());
+                  w[i] = make_uint4(pack2(x[0] * inverse, x[1] * inverse, __half()), pack2(x[2] * inverse, x[3] * inverse, __half()),
+                                    pack2(x[4] * inverse, x[5] * inverse, __half()), pack2(x[6] * inverse, x[7] * inverse, __half()));
+                }
+                *reinterpret_cast<uint4*>(queries + t * W::kQTile + ch / 8 * W::kQPanel + r128 * 128 +
+                                          (((ch % 8) ^ (r128 & 7)) << 4)) = w[i];
+              }
             }
             __syncwarp();
             if constexpr (!std::is_same<T, __half>::value) row_scale = q_scale[t][warp % 4 * 32 + lane];
