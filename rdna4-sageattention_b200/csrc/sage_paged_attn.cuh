@@ -249,10 +249,14 @@ __device__ __forceinline__ void load_tiles(const PagedAttnArgs& a, const CUtenso
     for (int s = 0; s < count; ++s) mbar_drain(full + s, s < slot ? phase : phase ^ 1);
 }
 
+// SMs of the current device (148 without one), asked for once per device.
 inline int sm_count() {
+  static std::atomic<int> known[64];
   int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 148;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+  if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
   return n;
 }
 

@@ -145,47 +145,52 @@ def _raise_host_word(device: torch.device) -> None:
 
 
 _ready: dict[int, torch.device] = {}   # GPUs that step() has checked
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
-def step(tensors) -> torch.device:
+def step(*tensors) -> torch.device:
     """The prelude of a step call (paged cache, rotary positions), whose host time counts: all tensors on one supported
     GPU, and nothing reported there by earlier calls.  Returns the device."""
     index = tensors[0].get_device()
     for t in tensors:
-        if t.get_device() != index or index < 0:
+        if t.get_device() != index:
             raise Unsupported("tensors must be on one CUDA GPU")
     dev = _ready.get(index)
     if dev is None:
+        if index < 0:
+            raise Unsupported("tensors must be on one CUDA GPU")
         dev = torch.device("cuda", index)
         _check_arch(dev)
         host_word(dev)
         _ready[index] = dev
-    _raise_pending(dev)
+    if _host_words[index][1].value or index in _watch:
+        _raise_pending(dev)
     return dev
 
 
-def launch(dev: torch.device, what: str, entry, *args) -> None:
-    """entry(*args, status word, stream) on dev's current stream, with dev as the current device."""
-    index = dev.index
-    if torch._C._cuda_getDevice() == index:
-        rc = entry(*args, _host_words[index][2], torch._C._cuda_getCurrentRawStream(index))
+def launch(index: int, what: str, entry, *args) -> None:
+    """entry(*args, stream) on the current stream of GPU `index`, with that GPU as the current device."""
+    if _current_device() == index:
+        rc = entry(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(dev):
-            rc = entry(*args, _host_words[index][2], torch._C._cuda_getCurrentRawStream(index))
+        with torch.cuda.device(index):
+            rc = entry(*args, _raw_stream(index))
     if rc != 0:
         _lib.check(rc, what)
     if _CHECK and not torch.cuda.is_current_stream_capturing():
-        check_status(dev)
+        check_status(torch.device("cuda", index))
 
 
 def step_rows(t: torch.Tensor, layout: str):
     """(tensor, address, (batch, seq, head) strides) of 4-D rows the kernels take: _bsh without its cost where it has
     nothing to do."""
-    st, at = t.stride(), t.data_ptr()
-    if st[3] == 1 and not (st[0] | st[1] | st[2]) & 7 and not at & 15:
-        return t, at, ((st[0], st[2], st[1]) if layout == "HND" else st[:3])
-    t, st = _bsh(t, layout)
-    return t, t.data_ptr(), st
+    b, x, y, d = t.stride()
+    at = t.data_ptr()
+    if d != 1 or (b | x | y) & 7 or at & 15:
+        t, (b, x, y) = _bsh(t, layout)
+        return t, t.data_ptr(), (b, x, y)
+    return t, at, ((b, y, x) if layout == "HND" else (b, x, y))
 
 
 def _watch_status(device: torch.device) -> None:

@@ -18,7 +18,10 @@ from __future__ import annotations
 import torch
 
 from . import _attention, _lib
-from ._attention import DTYPES, HEAD_DIMS, Unsupported, launch, step, step_rows
+from ._attention import DTYPES, HEAD_DIMS, Unsupported, _current_device, _raw_stream, launch, step, step_rows
+
+_alloc = torch._C._cuda_cudaCachingAllocator_raw_alloc
+_free = torch._C._cuda_cudaCachingAllocator_raw_delete
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 
@@ -43,8 +46,8 @@ class PagedKV:
             raise Unsupported("k8 and v8 must be 16-byte aligned")
         self.k8, self.ks, self.v8, self.vs = k8, ks, v8, vs
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k8.shape
-        if k8.is_cuda:
-            _attention.host_word(k8.device)   # allocated here rather than by a first call under graph capture
+        # error word of the device: allocated here rather than by a first call under graph capture
+        self._word = _attention.host_word(k8.device) if k8.is_cuda else None
 
     @classmethod
     def empty(cls, num_pages, page_size, kv_heads, head_dim, device="cuda"):
@@ -63,17 +66,18 @@ class PagedKV:
                 self.page_size)
 
 
-def _table(page_table):
-    return page_table.data_ptr(), page_table.stride(0), page_table.shape[1]
-
-
-def _check_table(kv, page_table, lens, counts, B):
-    if page_table.dim() != 2 or page_table.dtype != torch.int32 or page_table.shape[0] != B or page_table.shape[1] == 0 \
-            or page_table.stride(1) != 1:
+def _check_table(page_table, lens, counts, B):
+    """(address, row stride, pages) of the table, and the addresses of lens and counts."""
+    shape, stride = page_table.shape, page_table.stride()
+    if len(shape) != 2 or page_table.dtype != torch.int32 or shape[0] != B or shape[1] == 0 or stride[1] != 1:
         raise Unsupported(f"page_table must be int32 [{B}, pages] with contiguous rows")
-    for name, t in (("lens", lens), ("counts", counts)):
-        if t is not None and (t.shape != (B,) or t.dtype != torch.int32 or not t.is_contiguous()):
-            raise Unsupported(f"{name} must be contiguous int32 [{B}]")
+    if lens.dtype != torch.int32 or lens.shape != (B,) or not lens.is_contiguous():
+        raise Unsupported(f"lens must be contiguous int32 [{B}]")
+    if counts is None:
+        return page_table.data_ptr(), stride[0], shape[1], lens.data_ptr(), None
+    if counts.dtype != torch.int32 or counts.shape != (B,) or not counts.is_contiguous():
+        raise Unsupported(f"counts must be contiguous int32 [{B}]")
+    return page_table.data_ptr(), stride[0], shape[1], lens.data_ptr(), counts.data_ptr()
 
 
 def _check_rows(kv, x, layout, heads=None):
@@ -82,14 +86,20 @@ def _check_rows(kv, x, layout, heads=None):
         raise Unsupported(f"layout {layout!r}")
     if x.dtype not in DTYPES:
         raise Unsupported(f"dtype {x.dtype} (fp16 or bf16 required)")
-    if x.dim() != 4 or x.shape[-1] != kv.head_dim:
+    shape = x.shape
+    if len(shape) != 4 or shape[3] != kv.head_dim:
         raise Unsupported(f"4D tensors with head_dim {kv.head_dim} required")
-    B, H, S = (x.shape[0], x.shape[1], x.shape[2]) if layout == "HND" else (x.shape[0], x.shape[2], x.shape[1])
+    B, H, S = shape[:3] if layout == "HND" else (shape[0], shape[2], shape[1])
     if H % kv.kv_heads or H == 0 or (heads is not None and H != heads):
         raise Unsupported(f"heads {H} do not fit the cache's {kv.kv_heads} kv heads")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise Unsupported("the paged cache has no backward pass: call it under torch.no_grad()")
+    if x.requires_grad:
+        _no_grad()
     return B, S, H
+
+
+def _no_grad():
+    if torch.is_grad_enabled():
+        raise Unsupported("the paged cache has no backward pass: call it under torch.no_grad()")
 
 
 def paged_kv_append(kv, k, v, page_table, lens, counts=None, tensor_layout="HND"):
@@ -99,15 +109,19 @@ def paged_kv_append(kv, k, v, page_table, lens, counts=None, tensor_layout="HND"
     B, S, Hkv = _check_rows(kv, k, tensor_layout, kv.kv_heads)
     if v.shape != k.shape or v.dtype != k.dtype:
         raise Unsupported("k and v must match in shape and dtype")
-    _check_rows(kv, v, tensor_layout)
-    _check_table(kv, page_table, lens, counts, B)
-    dev = step((kv.k8, k, v, page_table, lens) if counts is None else (kv.k8, k, v, page_table, lens, counts))
+    if v.requires_grad:
+        _no_grad()
+    table = _check_table(page_table, lens, counts, B)
+    if counts is None:
+        dev = step(kv.k8, k, v, page_table, lens)
+    else:
+        dev = step(kv.k8, k, v, page_table, lens, counts)
     if B == 0 or S == 0:
         return
     k, kp, ks = step_rows(k, tensor_layout)
     v, vp, vs = step_rows(v, tensor_layout)
-    launch(dev, "sage_paged_append", _lib.lib().sage_paged_append, kp, vp, DTYPES[k.dtype], B, S, Hkv, kv.head_dim, *ks,
-           *vs, *kv._pool(), *_table(page_table), lens.data_ptr(), None if counts is None else counts.data_ptr())
+    launch(dev.index, "sage_paged_append", _lib.lib().sage_paged_append, kp, vp, DTYPES[k.dtype], B, S, Hkv, kv.head_dim,
+           *ks, *vs, *kv._pool(), *table, kv._word)
 
 
 def paged_kv_read(kv, page_table, lens, max_len, dtype=torch.bfloat16, tensor_layout="HND"):
@@ -120,16 +134,17 @@ def paged_kv_read(kv, page_table, lens, max_len, dtype=torch.bfloat16, tensor_la
     if max_len < 0:
         raise ValueError(f"max_len {max_len}")
     B = lens.shape[0] if lens.dim() == 1 else -1
-    _check_table(kv, page_table, lens, None, B)
-    dev = step((kv.k8, page_table, lens))
+    table = _check_table(page_table, lens, None, B)
+    dev = step(kv.k8, page_table, lens)
     Hkv, D = kv.kv_heads, kv.head_dim
     shape = (B, Hkv, max_len, D) if tensor_layout == "HND" else (B, max_len, Hkv, D)
-    k, v = torch.empty(shape, device=dev, dtype=dtype), torch.empty(shape, device=dev, dtype=dtype)
+    k = torch.empty(shape, device=dev, dtype=dtype)
+    v = torch.empty_like(k)
     if 0 in shape:
         return k, v
     _, kp, st = step_rows(k, tensor_layout)
-    launch(dev, "sage_paged_read", _lib.lib().sage_paged_read, *kv._pool(), Hkv, D, *_table(page_table), lens.data_ptr(), B,
-           max_len, kp, v.data_ptr(), DTYPES[dtype], *st, *st)
+    launch(dev.index, "sage_paged_read", _lib.lib().sage_paged_read, *kv._pool(), Hkv, D, *table[:4], B, max_len, kp,
+           v.data_ptr(), DTYPES[dtype], *st, *st, kv._word)
     return k, v
 
 
@@ -138,15 +153,17 @@ def paged_kv_keep(kv, page_table, lens, keep, counts=None):
     without counts).  keep: int32 [B, N], strictly increasing in each row (the accepted path of a tree whose parents
     come before their children); entries from counts[b] on are not read."""
     B = lens.shape[0] if lens.dim() == 1 else -1
-    _check_table(kv, page_table, lens, counts, B)
+    table = _check_table(page_table, lens, counts, B)
     if keep.dim() != 2 or keep.shape[0] != B or keep.dtype != torch.int32 or (keep.shape[1] > 1 and keep.stride(1) != 1):
         raise Unsupported(f"keep must be int32 [{B}, N] with contiguous rows")
-    dev = step((kv.k8, page_table, lens, keep) if counts is None else (kv.k8, page_table, lens, keep, counts))
+    if counts is None:
+        dev = step(kv.k8, page_table, lens, keep)
+    else:
+        dev = step(kv.k8, page_table, lens, keep, counts)
     if keep.numel() == 0:
         return
-    launch(dev, "sage_paged_keep", _lib.lib().sage_paged_keep, *kv._pool(), kv.kv_heads, kv.head_dim, *_table(page_table),
-           lens.data_ptr(), keep.data_ptr(), keep.stride(0), keep.shape[1],
-           None if counts is None else counts.data_ptr(), B)
+    launch(dev.index, "sage_paged_keep", _lib.lib().sage_paged_keep, *kv._pool(), kv.kv_heads, kv.head_dim, *table[:4],
+           keep.data_ptr(), keep.stride(0), keep.shape[1], table[4], B, kv._word)
 
 
 def attention_paged_kv(q, kv, page_table, lens, tree_mask=None, counts=None, tensor_layout="HND", sm_scale=None,
@@ -158,31 +175,39 @@ def attention_paged_kv(q, kv, page_table, lens, tree_mask=None, counts=None, ten
     return_lse also the (B, H, T) fp32 log-sum-exp; tokens from counts[b] on, and rows that see nothing, are zero with
     log-sum-exp -inf."""
     B, T, H = _check_rows(kv, q, tensor_layout)
-    _check_table(kv, page_table, lens, counts, B)
+    table = _check_table(page_table, lens, counts, B)
     tensors = [kv.k8, q, page_table, lens]
     if counts is not None:
         tensors.append(counts)
+    mask, mask_b, mask_i = None, 0, 0
     if tree_mask is not None:
-        if tree_mask.dtype != torch.bool or tree_mask.shape not in ((T, T), (1, T, T), (B, T, T)):
+        shape = tree_mask.shape
+        if tree_mask.dtype != torch.bool or shape != (B, T, T) and shape != (T, T) and shape != (1, T, T):
             raise Unsupported(f"tree_mask must be bool [{T}, {T}] or [{B}, {T}, {T}]")
         tensors.append(tree_mask)
-    dev = step(tensors)
-    D = kv.head_dim
-    out = torch.empty((B, T, H, D), device=dev, dtype=q.dtype)
-    lse = torch.empty((B, H, T), device=dev, dtype=torch.float32) if return_lse else None
+        st = tree_mask.stride()
+        if st[-1] != 1:
+            tree_mask = tree_mask.contiguous()
+            st = tree_mask.stride()
+        mask, mask_i = tree_mask.data_ptr(), st[-2]
+        mask_b = st[0] if len(st) == 3 and shape[0] == B else 0
+    dev = step(*tensors)
+    q, qp, qs = step_rows(q, tensor_layout)
+    out = torch.empty_like(q)   # of a tensor that the kernels take, so it is one too
+    lse = q.new_empty((B, H, T), dtype=torch.float32) if return_lse else None
     if B and T:
-        mask, mask_b, mask_i = None, 0, 0
-        if tree_mask is not None:
-            tree_mask = tree_mask if tree_mask.stride(-1) == 1 else tree_mask.contiguous()
-            mask, mask_i = tree_mask.data_ptr(), tree_mask.stride(-2)
-            mask_b = tree_mask.stride(0) if tree_mask.dim() == 3 and tree_mask.shape[0] == B else 0
-        q, qp, qs = step_rows(q, tensor_layout)
-        L = _lib.lib()
-        ws_bytes = L.sage_paged_attention_workspace_bytes(B, T, H, kv.kv_heads, D)
-        ws = torch.empty(ws_bytes, device=dev, dtype=torch.uint8)
-        launch(dev, "sage_paged_attention", L.sage_paged_attention, qp, DTYPES[q.dtype], B, T, H, kv.kv_heads, D, *qs,
-               *kv._pool(), *_table(page_table), lens.data_ptr(), None if counts is None else counts.data_ptr(), mask,
-               mask_b, mask_i, float(sm_scale or 0.0), out.data_ptr(), T * H * D, H * D, D,
-               lse.data_ptr() if return_lse else None, ws.data_ptr(), ws_bytes)
-    out = out.transpose(1, 2) if tensor_layout == "HND" else out
+        _, op, os = step_rows(out, tensor_layout)
+        L, index = _lib.lib(), dev.index
+        ws_bytes = L.sage_paged_attention_workspace_bytes(B, T, H, kv.kv_heads, kv.head_dim)
+        # for the call alone: back with the stream's allocator as soon as the kernels are enqueued
+        stream = _raw_stream(index)
+        ws = _alloc(ws_bytes, stream) if _current_device() == index else None
+        hold = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws is None else None
+        try:
+            launch(index, "sage_paged_attention", L.sage_paged_attention, qp, DTYPES[q.dtype], B, T, H, kv.kv_heads,
+                   kv.head_dim, *qs, *kv._pool(), *table, mask, mask_b, mask_i, float(sm_scale or 0.0), op, *os,
+                   lse.data_ptr() if return_lse else None, ws if hold is None else hold.data_ptr(), ws_bytes, kv._word)
+        finally:
+            if hold is None:
+                _free(ws)
     return (out, lse) if return_lse else out

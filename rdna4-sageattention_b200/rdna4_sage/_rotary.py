@@ -79,22 +79,30 @@ def _check(q, k, positions, rope, layout):
     """Raise Unsupported with the reason if the kernel cannot run these inputs (devices aside)."""
     if layout not in ("HND", "NHD"):
         raise Unsupported(f"layout {layout!r}")
-    h_ax, s_ax = (1, 2) if layout == "HND" else (2, 1)
-    for x in (q,) if k is None else (q, k):
-        if x.dtype not in DTYPES or x.dtype != q.dtype:
-            raise Unsupported(f"dtype {x.dtype} (fp16 or bf16, one for q and k, required)")
-        if x.dim() != 4 or x.shape[-1] != rope.head_dim:
-            raise Unsupported(f"4D tensors with head_dim {rope.head_dim} required")
-        if x.shape[0] != q.shape[0] or x.shape[s_ax] != q.shape[s_ax]:
+    s_ax = 2 if layout == "HND" else 1
+    shape = q.shape
+    if q.dtype not in DTYPES or len(shape) != 4 or shape[3] != rope.head_dim:
+        _refuse(q, q, rope)
+    if k is not None:
+        other = k.shape
+        if k.dtype != q.dtype or len(other) != 4 or other[3] != rope.head_dim:
+            _refuse(q, k, rope)
+        if other[0] != shape[0] or other[s_ax] != shape[s_ax]:
             raise Unsupported("q and k must hold the same tokens")
     if positions.dtype not in (torch.int32, torch.int64):
         raise Unsupported(f"positions {positions.dtype} (int32 or int64 required)")
-    B, S = q.shape[0], q.shape[s_ax]
-    if positions.shape not in ((S,), (1, S), (B, S)):
-        raise Unsupported(f"positions {tuple(positions.shape)}: (S,) or (B, S) of ({B}, {S}) tokens required")
+    B, S, at = shape[0], shape[s_ax], positions.shape
+    if at != (B, S) and at != (S,) and at != (1, S):
+        raise Unsupported(f"positions {tuple(at)}: (S,) or (B, S) of ({B}, {S}) tokens required")
 
 
-def _launch(dev, q, k, positions, rope, layout, backward):
+def _refuse(q, x, rope):
+    if x.dtype not in DTYPES or x.dtype != q.dtype:
+        raise Unsupported(f"dtype {x.dtype} (fp16 or bf16, one for q and k, required)")
+    raise Unsupported(f"4D tensors with head_dim {rope.head_dim} required")
+
+
+def _launch(q, k, positions, rope, layout, backward):
     """(q, k) turned, new tensors in the inputs' layout (k may be None)."""
     if q.numel() == 0 or k is not None and k.numel() == 0:
         if q.numel() != 0 or k is not None and k.numel() != 0:
@@ -102,8 +110,11 @@ def _launch(dev, q, k, positions, rope, layout, backward):
         return torch.empty_like(q), None if k is None else torch.empty_like(k)
     q, qp, qs = step_rows(q, layout)
     q_out = torch.empty_like(q)   # of a tensor that the kernels take, so it is one too
-    B, S, H = (q.shape[0], q.shape[2], q.shape[1]) if layout == "HND" else q.shape[:3]
     _, qop, qos = step_rows(q_out, layout)
+    if layout == "HND":
+        B, H, S, D = q.shape
+    else:
+        B, S, H, D = q.shape
     if k is None:
         k_out, Hkv, kp, kop, ks, kos = None, 0, None, None, (0, 0, 0), (0, 0, 0)
     else:
@@ -111,19 +122,12 @@ def _launch(dev, q, k, positions, rope, layout, backward):
         k_out = torch.empty_like(k)
         _, kop, kos = step_rows(k_out, layout)
         Hkv = k.shape[1 if layout == "HND" else 2]
-    if positions.dim() == 1:
-        pb, ps = 0, positions.stride(0)
-    else:
-        pb, ps = positions.stride()
-        pb = 0 if positions.shape[0] == 1 else pb
-    launch(dev, "sage_rotary", _rotary_entry, qp, kp, DTYPES[q.dtype], B, S, H, Hkv, rope.head_dim, rope.rotary_dim,
+    ps = positions.stride()
+    pb = ps[0] if len(ps) == 2 and positions.shape[0] > 1 else 0
+    launch(q.get_device(), "sage_rotary", _lib.lib().sage_rotary, qp, kp, DTYPES[q.dtype], B, S, H, Hkv, D, rope.rotary_dim,
            rope.interleaved, *qs, *ks, qop, kop, *qos, *kos, positions.data_ptr(),
-           32 if positions.dtype == torch.int32 else 64, pb, ps, rope.turns.data_ptr(), rope.magnitude, backward)
+           32 if positions.dtype == torch.int32 else 64, pb, ps[-1], rope.turns.data_ptr(), rope.magnitude, backward)
     return q_out, k_out
-
-
-def _rotary_entry(*args):
-    return _lib.lib().sage_rotary(*args[:-2], args[-1])   # it reports nothing from the device
 
 
 class _RotaryFunction(torch.autograd.Function):
@@ -134,7 +138,7 @@ class _RotaryFunction(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(positions)
         ctx.rope, ctx.layout, ctx.turn_back = rope, layout, not backward
-        q_out, k_out = _launch(q.device, q, k, positions, rope, layout, backward)
+        q_out, k_out = _launch(q, k, positions, rope, layout, backward)
         return q_out if k is None else (q_out, k_out)
 
     @staticmethod
@@ -145,9 +149,9 @@ class _RotaryFunction(torch.autograd.Function):
         args = (positions, ctx.rope, ctx.layout, ctx.turn_back)
         if not torch.is_grad_enabled():
             if dq is not None:
-                dq, dk = _launch(dq.device, dq, dk, *args)
+                dq, dk = _launch(dq, dk, *args)
             elif dk is not None:
-                dk, _ = _launch(dk.device, dk, None, *args)
+                dk, _ = _launch(dk, None, *args)
         elif dq is not None and dk is not None:
             dq, dk = _RotaryFunction.apply(dq, dk, *args)
         elif dq is not None:
@@ -163,8 +167,11 @@ def rotary(q, k, positions, rope, tensor_layout="HND"):
     alone.  positions: int32 or int64 of any value, (S,) for all sequences or (B, S), on the GPU.  rope: a Rotary.
     Differentiable in q and k.  Raises Unsupported for inputs the kernel does not take."""
     _check(q, k, positions, rope, tensor_layout)
-    dev = step((q, positions, rope.turns) if k is None else (q, k, positions, rope.turns))
+    if k is None:
+        step(q, positions, rope.turns)
+    else:
+        step(q, k, positions, rope.turns)
     if (q.requires_grad or k is not None and k.requires_grad) and torch.is_grad_enabled():
         return _RotaryFunction.apply(q, k, positions, rope, tensor_layout, False)
-    q_out, k_out = _launch(dev, q, k, positions, rope, tensor_layout, False)
+    q_out, k_out = _launch(q, k, positions, rope, tensor_layout, False)
     return q_out if k is None else (q_out, k_out)
