@@ -212,20 +212,32 @@ int sage_attention_host_multi(const void* q, const void* k, const void* v, int d
                               int n_devices, const int* devices, void* const* workspaces, size_t workspace_bytes,
                               int* const* statuses, void* const* streams);
 
+/* Step calls: what a model does around attention for each step of a growing context.  Their arguments come in structs
+ * (same conventions as above: device pointers, element strides of the (batch, sequence, head) axes, nullable where
+ * said), which are read during the call only. */
+
 /* Rotary positions of q (B, S, H, D) and, with Hkv > 0, k (B, S, Hkv, D) into q_out / k_out (which may be the
  * inputs).  The first R channels (a multiple of 16) of a head are turned in pairs, channel i with i + R / 2, or 2 i
  * with 2 i + 1 when `interleaved`; the others are copied.  positions: device int32 or int64 (position_bits 32 or
- * 64), element strides psb, pss.  turns: device array of R / 2 frequencies in turns (radians per position / 2 pi)
- * as 64-bit fixed-point fractions.  magnitude multiplies the turned channels.  backward = 1 turns by the negative
- * angles: the gradient of the call with backward = 0.  The reference leaves positions to its callers. */
-int sage_rotary(const void* q, const void* k, int dtype, int B, int S, int H, int Hkv, int D, int R, int interleaved,
-                int64_t qsb, int64_t qss, int64_t qsh, int64_t ksb, int64_t kss, int64_t ksh, void* q_out, void* k_out,
-                int64_t qosb, int64_t qoss, int64_t qosh, int64_t kosb, int64_t koss, int64_t kosh,
-                const void* positions, int position_bits, int64_t psb, int64_t pss, const uint64_t* turns,
-                float magnitude, int backward, void* stream);
+ * 64), element strides of batch and token.  turns: device array of R / 2 frequencies in turns (radians per position /
+ * 2 pi) as 64-bit fixed-point fractions.  magnitude multiplies the turned channels.  backward = 1 turns by the
+ * negative angles: the gradient of the call with backward = 0.  The reference leaves positions to its callers. */
+typedef struct {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  const void* positions;
+  const uint64_t* turns;
+  int64_t q_st[3], k_st[3], q_out_st[3], k_out_st[3], position_st[2];
+  int32_t dtype, B, S, H, Hkv, D, R, interleaved, position_bits;
+  float magnitude;
+  int32_t backward;
+} sage_rotary_args;
+int sage_rotary(const sage_rotary_args* args, void* stream);
 
 /* The paged K/V cache (no counterpart in the reference, which quantises K and V anew in every call).  Buffers, all
- * contiguous:
+ * contiguous and 16-byte aligned:
  *   k8 [num_pages, Hkv, page_size, D] int8    ks [num_pages, Hkv, page_size] float
  *   v8 [num_pages, Hkv, page_size, D] e4m3    vs [num_pages, Hkv, page_size] float
  * page_size is a power of two from 16 to 256.  Each row (one token of one kv head) has its own scale, so a row is
@@ -235,44 +247,67 @@ int sage_rotary(const void* q, const void* k, int dtype, int B, int S, int H, in
  * page_table: device int32 [B, max_pages], rows table_stride apart: position p of sequence b is row
  * p % page_size of page page_table[b][p / page_size].  Entries that no position reaches are not read.
  * lens: device int32 [B].  For append, keep and attention it is the context length BEFORE this step's tokens, which
- * hold positions lens[b], lens[b] + 1, ...; counts (nullable, device int32 [B], 0..S) gives their number where a
+ * hold positions lens[b], lens[b] + 1, ...; counts (nullable, device int32 [B], 0 .. S) gives their number where a
  * padded batch holds fewer than S of them.
  * Lengths, counts and page numbers are checked on the device: what lies outside is neither read nor written, and
  * *status (nullable = the library's own word; pinned host memory will do) receives SAGE_ERR_INVALID. */
+typedef struct {
+  int8_t* k8;
+  float* ks;
+  uint8_t* v8;
+  float* vs;
+  const int32_t* page_table;
+  const int32_t* lens;
+  const int32_t* counts;
+  int* status;
+  int64_t table_stride;
+  int32_t num_pages, page_size, Hkv, D, max_pages, B;
+} sage_paged_kv;
 
-/* Quantise and write S tokens of k, v (B, S, Hkv, D).  Rows behind counts[b] leave the cache as it was. */
-int sage_paged_append(const void* k, const void* v, int dtype, int B, int S, int Hkv, int D, int64_t ksb, int64_t kss,
-                      int64_t ksh, int64_t vsb, int64_t vss, int64_t vsh, int8_t* k8, float* ks, uint8_t* v8, float* vs,
-                      int num_pages, int page_size, const int32_t* page_table, int64_t table_stride, int max_pages,
-                      const int32_t* lens, const int32_t* counts, int* status, void* stream);
-
-/* Read positions 0 .. S - 1 back into 16-bit k, v (B, S, Hkv, D): code * scale, rounded once; positions from lens[b]
- * on are zero. */
-int sage_paged_read(const int8_t* k8, const float* ks, const uint8_t* v8, const float* vs, int num_pages, int page_size,
-                    int Hkv, int D, const int32_t* page_table, int64_t table_stride, int max_pages, const int32_t* lens,
-                    int B, int S, void* k, void* v, int dtype, int64_t ksb, int64_t kss, int64_t ksh, int64_t vsb,
-                    int64_t vss, int64_t vsh, int* status, void* stream);
+/* sage_paged_append quantises and writes S tokens of k, v (B, S, Hkv, D); rows behind counts[b] leave the cache as it
+ * was.  sage_paged_read reads positions 0 .. S - 1 back into k, v: code * scale, rounded once; positions from lens[b]
+ * on are zero (counts is not used). */
+typedef struct {
+  sage_paged_kv kv;
+  void* k;
+  void* v;
+  int64_t k_st[3], v_st[3];
+  int32_t dtype, S;
+} sage_paged_rows_args;
+int sage_paged_append(const sage_paged_rows_args* args, void* stream);
+int sage_paged_read(const sage_paged_rows_args* args, void* stream);
 
 /* Drop rejected drafts: position lens[b] + keep[b][i] moves to lens[b] + i for i < counts[b] (N without counts).
  * keep: device int32 [B, N], rows keep_stride apart, strictly increasing (else the sequence stays as it was and the
  * status word is set). */
-int sage_paged_keep(int8_t* k8, float* ks, uint8_t* v8, float* vs, int num_pages, int page_size, int Hkv, int D,
-                    const int32_t* page_table, int64_t table_stride, int max_pages, const int32_t* lens,
-                    const int32_t* keep, int64_t keep_stride, int N, const int32_t* counts, int B, int* status,
-                    void* stream);
+typedef struct {
+  sage_paged_kv kv;
+  const int32_t* keep;
+  int64_t keep_stride;
+  int32_t N;
+} sage_paged_keep_args;
+int sage_paged_keep(const sage_paged_keep_args* args, void* stream);
 
 /* Attention of this step's T tokens q (B, T, H, D), whose K and V the cache already holds: token i of sequence b sees
  * the positions before lens[b] and, of the step's own tokens t, those with t <= i, or with mask[b][i][t] != 0
- * where a mask is given (bytes, element strides mask_b, mask_i, 1; mask_b = 0 shares one mask).  Tokens from
- * counts[b] on, and rows that see nothing, give zeros and lse = -infinity.  lse (nullable): [B, H, T] fp32.
- * workspace: device memory of sage_paged_attention_workspace_bytes(...) bytes, 16-byte aligned. */
+ * where a mask is given (bytes, element strides mask_st of batch and row; a batch stride of 0 shares one mask).
+ * Tokens from counts[b] on, and rows that see nothing, give zeros and lse = -infinity.  lse (nullable): [B, H, T] fp32.
+ * sm_scale <= 0 selects 1 / sqrt(D).  workspace: device memory of sage_paged_attention_workspace_bytes(...) bytes,
+ * 16-byte aligned, used by this call alone while it runs. */
+typedef struct {
+  sage_paged_kv kv;
+  const void* q;
+  void* out;
+  float* lse;
+  const uint8_t* mask;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t q_st[3], out_st[3], mask_st[2];
+  double sm_scale;
+  int32_t dtype, T, H;
+} sage_paged_attention_args;
 size_t sage_paged_attention_workspace_bytes(int B, int T, int H, int Hkv, int D);
-int sage_paged_attention(const void* q, int dtype, int B, int T, int H, int Hkv, int D, int64_t qsb, int64_t qss,
-                         int64_t qsh, const int8_t* k8, const float* ks, const uint8_t* v8, const float* vs,
-                         int num_pages, int page_size, const int32_t* page_table, int64_t table_stride, int max_pages,
-                         const int32_t* lens, const int32_t* counts, const uint8_t* mask, int64_t mask_b,
-                         int64_t mask_i, double sm_scale, void* out, int64_t osb, int64_t oss, int64_t osh, float* lse,
-                         void* workspace, size_t workspace_bytes, int* status, void* stream);
+int sage_paged_attention(const sage_paged_attention_args* args, void* stream);
 
 /* Failure-path self test (no counterpart in the reference): enqueues a kernel whose single wait is on a
  * barrier that nothing completes, bounded by limit_ms (1..2000) instead of the pipeline's 2 s.  When the

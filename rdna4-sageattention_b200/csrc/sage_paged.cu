@@ -14,34 +14,33 @@
 
 namespace sage {
 
-int paged_args(PagedArgs* out, void* k8, float* ks, void* v8, float* vs, int num_pages, int page_size, int Hkv, int D,
-               const int32_t* page_table, int64_t table_stride, int max_pages, const int32_t* lens, int* status) {
+int paged_args(PagedArgs* out, const sage_paged_kv& kv) {
   int shift = 4;
-  while (shift < 8 && (1 << shift) < page_size) ++shift;
-  if ((1 << shift) != page_size) {
-    set_error("page_size %d (a power of two from 16 to 256 required)", page_size);
+  while (shift < 8 && (1 << shift) < kv.page_size) ++shift;
+  if ((1 << shift) != kv.page_size) {
+    set_error("page_size %d (a power of two from 16 to 256 required)", kv.page_size);
     return SAGE_ERR_UNSUPPORTED;
   }
-  if (num_pages <= 0 || Hkv <= 0 || max_pages <= 0) {
-    set_error("empty cache (num_pages=%d Hkv=%d max_pages=%d)", num_pages, Hkv, max_pages);
+  if (kv.num_pages <= 0 || kv.Hkv <= 0 || kv.max_pages <= 0) {
+    set_error("empty cache (num_pages=%d Hkv=%d max_pages=%d)", kv.num_pages, kv.Hkv, kv.max_pages);
     return SAGE_ERR_UNSUPPORTED;
   }
-  if ((reinterpret_cast<uintptr_t>(k8) & 15u) || (reinterpret_cast<uintptr_t>(v8) & 15u) || k8 == nullptr ||
-      v8 == nullptr || ks == nullptr || vs == nullptr) {
-    set_error("cache buffers: k8 / v8 must be 16-byte aligned, ks and vs non-null");
-    return SAGE_ERR_INVALID;
-  }
-  if (page_table == nullptr || lens == nullptr) {
+  for (const void* p : {(const void*)kv.k8, (const void*)kv.ks, (const void*)kv.v8, (const void*)kv.vs})
+    if (p == nullptr || (reinterpret_cast<uintptr_t>(p) & 15u)) {
+      set_error("cache buffers k8, ks, v8 and vs must be 16-byte aligned");
+      return SAGE_ERR_INVALID;
+    }
+  if (kv.page_table == nullptr || kv.lens == nullptr) {
     set_error("page_table and lens must be device arrays");
     return SAGE_ERR_INVALID;
   }
-  int* word = status != nullptr ? status : default_status_word();
+  int* word = kv.status != nullptr ? kv.status : default_status_word();
   if (word == nullptr) {
     set_error("no status word on this device");
     return SAGE_ERR_LAUNCH;
   }
-  *out = PagedArgs{static_cast<int8_t*>(k8), ks, static_cast<uint8_t*>(v8), vs, num_pages, shift, Hkv, D, page_table,
-                   table_stride, max_pages, lens, word};
+  *out = PagedArgs{kv.k8, kv.ks, kv.v8, kv.vs, kv.num_pages, shift, kv.Hkv, kv.D, kv.page_table, kv.table_stride,
+                   kv.max_pages, kv.lens, word};
   return SAGE_OK;
 }
 
@@ -249,23 +248,28 @@ using namespace sage;
 
 extern "C" {
 
-int sage_paged_append(const void* k, const void* v, int dtype, int B, int S, int Hkv, int D, int64_t ksb, int64_t kss,
-                      int64_t ksh, int64_t vsb, int64_t vss, int64_t vsh, int8_t* k8, float* ks, uint8_t* v8, float* vs,
-                      int num_pages, int page_size, const int32_t* page_table, int64_t table_stride, int max_pages,
-                      const int32_t* lens, const int32_t* counts, int* status, void* stream) {
-  NvtxRange nvtx("sage_paged_append");
+// The arguments that append and read share, checked.
+static int rows_args(PagedArgs* p, const sage_paged_rows_args* args, const char* what) {
   set_error("%s", "");
-  int rc = check_rows(dtype, B, S, Hkv, D);
-  if (rc == SAGE_OK) rc = check_rows_pointer(k, ksb, kss, ksh, "k");
-  if (rc == SAGE_OK) rc = check_rows_pointer(v, vsb, vss, vsh, "v");
+  if (args == nullptr) {
+    set_error("%s: no arguments", what);
+    return SAGE_ERR_INVALID;
+  }
+  int rc = check_rows(args->dtype, args->kv.B, args->S, args->kv.Hkv, args->kv.D);
+  if (rc == SAGE_OK) rc = check_rows_pointer(args->k, args->k_st, "k");
+  if (rc == SAGE_OK) rc = check_rows_pointer(args->v, args->v_st, "v");
+  return rc == SAGE_OK ? paged_args(p, args->kv) : rc;
+}
+
+int sage_paged_append(const sage_paged_rows_args* args, void* stream) {
+  NvtxRange nvtx("sage_paged_append");
   AppendArgs a{};
-  if (rc == SAGE_OK)
-    rc = paged_args(&a.p, k8, ks, v8, vs, num_pages, page_size, Hkv, D, page_table, table_stride, max_pages, lens,
-                    status);
+  const int rc = rows_args(&a.p, args, "append");
   if (rc != SAGE_OK) return rc;
-  a.x[0] = k, a.x[1] = v;
-  a.st[0] = {ksb, kss, ksh}, a.st[1] = {vsb, vss, vsh};
-  a.counts = counts;
+  const int B = args->kv.B, S = args->S, Hkv = args->kv.Hkv, D = args->kv.D, dtype = args->dtype;
+  a.x[0] = args->k, a.x[1] = args->v;
+  a.st[0] = strides3(args->k_st), a.st[1] = strides3(args->v_st);
+  a.counts = args->kv.counts;
   a.B = B, a.S = S;
   const int per_block = 256 / (D == 64 ? 8 : D == 256 ? 32 : 16);
   const int64_t blocks = ((int64_t)((S + kTokens - 1) / kTokens) * Hkv + per_block - 1) / per_block;
@@ -284,23 +288,14 @@ int sage_paged_append(const void* k, const void* v, int dtype, int B, int S, int
   });
 }
 
-int sage_paged_read(const int8_t* k8, const float* ks, const uint8_t* v8, const float* vs, int num_pages, int page_size,
-                    int Hkv, int D, const int32_t* page_table, int64_t table_stride, int max_pages, const int32_t* lens,
-                    int B, int S, void* k, void* v, int dtype, int64_t ksb, int64_t kss, int64_t ksh, int64_t vsb,
-                    int64_t vss, int64_t vsh, int* status, void* stream) {
+int sage_paged_read(const sage_paged_rows_args* args, void* stream) {
   NvtxRange nvtx("sage_paged_read");
-  set_error("%s", "");
-  int rc = check_rows(dtype, B, S, Hkv, D);
-  if (rc == SAGE_OK) rc = check_rows_pointer(k, ksb, kss, ksh, "k");
-  if (rc == SAGE_OK) rc = check_rows_pointer(v, vsb, vss, vsh, "v");
   ReadArgs a{};
-  if (rc == SAGE_OK)
-    rc = paged_args(&a.p, const_cast<int8_t*>(k8), const_cast<float*>(ks), const_cast<uint8_t*>(v8),
-                    const_cast<float*>(vs), num_pages, page_size, Hkv, D, page_table, table_stride, max_pages, lens,
-                    status);
+  const int rc = rows_args(&a.p, args, "read");
   if (rc != SAGE_OK) return rc;
-  a.out[0] = k, a.out[1] = v;
-  a.st[0] = {ksb, kss, ksh}, a.st[1] = {vsb, vss, vsh};
+  const int B = args->kv.B, S = args->S, Hkv = args->kv.Hkv, D = args->kv.D, dtype = args->dtype;
+  a.out[0] = args->k, a.out[1] = args->v;
+  a.st[0] = strides3(args->k_st), a.st[1] = strides3(args->v_st);
   a.B = B, a.S = S;
   const int64_t blocks = ((int64_t)((S + kRun - 1) / kRun) * Hkv * (D / 8) + 255) / 256;
   if (blocks > (1 << 23) || B > 65535) {   // 32-bit thread numbers, grid limit
@@ -318,27 +313,23 @@ int sage_paged_read(const int8_t* k8, const float* ks, const uint8_t* v8, const 
   });
 }
 
-int sage_paged_keep(int8_t* k8, float* ks, uint8_t* v8, float* vs, int num_pages, int page_size, int Hkv, int D,
-                    const int32_t* page_table, int64_t table_stride, int max_pages, const int32_t* lens,
-                    const int32_t* keep, int64_t keep_stride, int N, const int32_t* counts, int B, int* status,
-                    void* stream) {
+int sage_paged_keep(const sage_paged_keep_args* args, void* stream) {
   NvtxRange nvtx("sage_paged_keep");
   set_error("%s", "");
+  if (args == nullptr || args->keep == nullptr) {
+    set_error("keep must be a device array");
+    return SAGE_ERR_INVALID;
+  }
+  const int B = args->kv.B, N = args->N, Hkv = args->kv.Hkv, D = args->kv.D;
   int rc = check_rows(SAGE_BF16, B, N, Hkv, D);
   KeepArgs a{};
-  if (rc == SAGE_OK)
-    rc = paged_args(&a.p, k8, ks, v8, vs, num_pages, page_size, Hkv, D, page_table, table_stride, max_pages, lens,
-                    status);
-  if (rc == SAGE_OK && keep == nullptr) {
-    set_error("keep must be a device array");
-    rc = SAGE_ERR_INVALID;
-  }
+  if (rc == SAGE_OK) rc = paged_args(&a.p, args->kv);
   if (rc == SAGE_OK && (int64_t)B * Hkv > INT_MAX) {
     set_error("keep: %d sequences of %d heads are too many for one call", B, Hkv);
     rc = SAGE_ERR_UNSUPPORTED;
   }
   if (rc != SAGE_OK) return rc;
-  a.keep = keep, a.keep_stride = keep_stride, a.counts = counts, a.N = N;
+  a.keep = args->keep, a.keep_stride = args->keep_stride, a.counts = args->kv.counts, a.N = N;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return by_head_dim(D, [&](auto d) {
     keep_kernel<decltype(d)::value><<<B * Hkv, 256, 0, st>>>(a);

@@ -55,7 +55,6 @@ __device__ __forceinline__ uint32_t e4m3_to_f16(uint16_t v) {
 }
 
 // Host side: the cache arguments of an entry point, checked.
-int paged_args(PagedArgs* out, void* k8, float* ks, void* v8, float* vs, int num_pages, int page_size, int Hkv, int D,
-               const int32_t* page_table, int64_t table_stride, int max_pages, const int32_t* lens, int* status);
+int paged_args(PagedArgs* out, const sage_paged_kv& kv);
 
 }  // namespace sage

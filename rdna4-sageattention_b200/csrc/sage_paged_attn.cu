@@ -626,37 +626,30 @@ extern "C" size_t sage_paged_attention_workspace_bytes(int B, int T, int H, int 
   return slots * (D * sizeof(float) + sizeof(float2));
 }
 
-extern "C" int sage_paged_attention(const void* q, int dtype, int B, int T, int H, int Hkv, int D, int64_t qsb,
-                                    int64_t qss, int64_t qsh, const int8_t* k8, const float* ks, const uint8_t* v8,
-                                    const float* vs, int num_pages, int page_size, const int32_t* page_table,
-                                    int64_t table_stride, int max_pages, const int32_t* lens, const int32_t* counts,
-                                    const uint8_t* mask, int64_t mask_b, int64_t mask_i, double sm_scale, void* out,
-                                    int64_t osb, int64_t oss, int64_t osh, float* lse, void* workspace,
-                                    size_t workspace_bytes, int* status, void* stream) {
+extern "C" int sage_paged_attention(const sage_paged_attention_args* args, void* stream) {
   NvtxRange nvtx("sage_paged_attention");
   set_error("%s", "");
+  if (args == nullptr) {
+    set_error("paged attention: no arguments");
+    return SAGE_ERR_INVALID;
+  }
+  const sage_paged_kv& kv = args->kv;
+  const int dtype = args->dtype, B = kv.B, T = args->T, H = args->H, Hkv = kv.Hkv, D = kv.D;
   int rc = check_rows(dtype, B, T, H, D);
   if (rc == SAGE_OK && (Hkv <= 0 || H % Hkv != 0)) {
     set_error("heads %d must be a multiple of kv heads %d", H, Hkv);
     rc = SAGE_ERR_UNSUPPORTED;
   }
-  if (rc == SAGE_OK) rc = check_rows_pointer(q, qsb, qss, qsh, "q");
-  if (rc == SAGE_OK) rc = check_rows_pointer(out, osb, oss, osh, "out");
+  if (rc == SAGE_OK) rc = check_rows_pointer(args->q, args->q_st, "q");
+  if (rc == SAGE_OK) rc = check_rows_pointer(args->out, args->out_st, "out");
   PagedAttnArgs a{};
-  if (rc == SAGE_OK)
-    rc = paged_args(&a.p, const_cast<int8_t*>(k8), const_cast<float*>(ks), const_cast<uint8_t*>(v8),
-                    const_cast<float*>(vs), num_pages, page_size, Hkv, D, page_table, table_stride, max_pages, lens,
-                    status);
-  if (rc == SAGE_OK && (int64_t)max_pages * page_size > (int64_t)INT_MAX - T - kTileKeys) {
-    set_error("%d pages of %d keys: positions must fit 32 bits", max_pages, page_size);
+  if (rc == SAGE_OK) rc = paged_args(&a.p, kv);
+  if (rc == SAGE_OK && (int64_t)kv.max_pages * kv.page_size > (int64_t)INT_MAX - T - kTileKeys) {
+    set_error("%d pages of %d keys: positions must fit 32 bits", kv.max_pages, kv.page_size);
     rc = SAGE_ERR_UNSUPPORTED;
   }
-  if (rc == SAGE_OK && (((reinterpret_cast<uintptr_t>(ks) | reinterpret_cast<uintptr_t>(vs)) & 15u) != 0)) {
-    set_error("ks and vs must be 16-byte aligned");
-    rc = SAGE_ERR_INVALID;
-  }
-  if (rc == SAGE_OK && (int64_t)num_pages * page_size > (int64_t)INT_MAX / Hkv) {
-    set_error("%d pages of %d keys and %d heads: cache rows must fit 32 bits", num_pages, page_size, Hkv);
+  if (rc == SAGE_OK && (int64_t)kv.num_pages * kv.page_size > (int64_t)INT_MAX / Hkv) {
+    set_error("%d pages of %d keys and %d heads: cache rows must fit 32 bits", kv.num_pages, kv.page_size, Hkv);
     rc = SAGE_ERR_UNSUPPORTED;
   }
   if (rc == SAGE_OK && (int64_t)B * T * H > INT_MAX / 64) {
@@ -664,23 +657,24 @@ extern "C" int sage_paged_attention(const void* q, int dtype, int B, int T, int 
     rc = SAGE_ERR_UNSUPPORTED;
   }
   const size_t need = rc == SAGE_OK ? sage_paged_attention_workspace_bytes(B, T, H, Hkv, D) : 0;
-  if (rc == SAGE_OK && (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u))) {
-    set_error("workspace of %zu bytes (16-byte aligned) required, got %zu", need, workspace_bytes);
+  if (rc == SAGE_OK && (args->workspace == nullptr || args->workspace_bytes < (int64_t)need ||
+                        (reinterpret_cast<uintptr_t>(args->workspace) & 15u))) {
+    set_error("workspace of %zu bytes (16-byte aligned) required, got %lld", need, (long long)args->workspace_bytes);
     rc = SAGE_ERR_INVALID;
   }
   if (rc != SAGE_OK) return rc;
-  a.q = q, a.q_st = {qsb, qss, qsh};
-  a.out = out, a.out_st = {osb, oss, osh};
-  a.lse = lse, a.counts = counts;
-  a.mask = mask, a.mask_b = mask_b, a.mask_i = mask_i;
+  a.q = args->q, a.q_st = strides3(args->q_st);
+  a.out = args->out, a.out_st = strides3(args->out_st);
+  a.lse = args->lse, a.counts = kv.counts;
+  a.mask = args->mask, a.mask_b = args->mask_st[0], a.mask_i = args->mask_st[1];
   a.B = B, a.T = T, a.H = H, a.group = H / Hkv;
   const bool many = wide((int64_t)T * a.group, D);
   const Shape shape = row_tile((int64_t)T * a.group, D);
   const int tile_rows = many ? wide_rows(D) : 8 * shape.nr * shape.wm;
   a.row_tiles = (T * a.group + tile_rows - 1) / tile_rows;
   a.ctas = many ? wide_ctas() : shared_ctas(D, shape);
-  a.scale = (float)((sm_scale > 0.0 ? sm_scale : 1.0 / std::sqrt((double)D)) * 1.4426950408889634);
-  a.part_o = static_cast<float*>(workspace);
+  a.scale = (float)((args->sm_scale > 0.0 ? args->sm_scale : 1.0 / std::sqrt((double)D)) * 1.4426950408889634);
+  a.part_o = static_cast<float*>(args->workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)2 * a.ctas * tile_rows * D);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return by_head_dim(D, [&](auto d) {

@@ -126,41 +126,43 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryArgs a) {
 
 using namespace sage;
 
-extern "C" int sage_rotary(const void* q, const void* k, int dtype, int B, int S, int H, int Hkv, int D, int R,
-                           int interleaved, int64_t qsb, int64_t qss, int64_t qsh, int64_t ksb, int64_t kss,
-                           int64_t ksh, void* q_out, void* k_out, int64_t qosb, int64_t qoss, int64_t qosh,
-                           int64_t kosb, int64_t koss, int64_t kosh, const void* positions, int position_bits,
-                           int64_t psb, int64_t pss, const uint64_t* turns, float magnitude, int backward,
-                           void* stream) {
+extern "C" int sage_rotary(const sage_rotary_args* args, void* stream) {
   NvtxRange nvtx("sage_rotary");
   set_error("%s", "");
+  if (args == nullptr) {
+    set_error("rotary: no arguments");
+    return SAGE_ERR_INVALID;
+  }
+  const sage_rotary_args& x = *args;
+  const int dtype = x.dtype, B = x.B, S = x.S, H = x.H, Hkv = x.Hkv, D = x.D, R = x.R;
+  const bool interleaved = x.interleaved != 0;
   int rc = check_rows(dtype, B, S, H, D);
   if (rc != SAGE_OK) return rc;
-  if (R < 16 || R > D || R % 16 != 0 || Hkv < 0 || (position_bits != 32 && position_bits != 64)) {
+  if (R < 16 || R > D || R % 16 != 0 || Hkv < 0 || (x.position_bits != 32 && x.position_bits != 64)) {
     set_error("rotary: rotary_dim %d (a multiple of 16 up to head_dim %d), kv heads %d, %d-bit positions", R, D, Hkv,
-              position_bits);
+              x.position_bits);
     return SAGE_ERR_UNSUPPORTED;
   }
-  if (positions == nullptr || turns == nullptr) {
+  if (x.positions == nullptr || x.turns == nullptr) {
     set_error("rotary: positions and turns must be device arrays");
     return SAGE_ERR_INVALID;
   }
-  rc = check_rows_pointer(q, qsb, qss, qsh, "q");
-  if (rc == SAGE_OK) rc = check_rows_pointer(q_out, qosb, qoss, qosh, "q_out");
-  if (rc == SAGE_OK && Hkv > 0) rc = check_rows_pointer(k, ksb, kss, ksh, "k");
-  if (rc == SAGE_OK && Hkv > 0) rc = check_rows_pointer(k_out, kosb, koss, kosh, "k_out");
+  rc = check_rows_pointer(x.q, x.q_st, "q");
+  if (rc == SAGE_OK) rc = check_rows_pointer(x.q_out, x.q_out_st, "q_out");
+  if (rc == SAGE_OK && Hkv > 0) rc = check_rows_pointer(x.k, x.k_st, "k");
+  if (rc == SAGE_OK && Hkv > 0) rc = check_rows_pointer(x.k_out, x.k_out_st, "k_out");
   if (rc != SAGE_OK) return rc;
   RotaryArgs a{};
-  a.in[0] = q, a.in[1] = k, a.out[0] = q_out, a.out[1] = k_out;
-  a.in_st[0] = {qsb, qss, qsh}, a.in_st[1] = {ksb, kss, ksh};
-  a.out_st[0] = {qosb, qoss, qosh}, a.out_st[1] = {kosb, koss, kosh};
+  a.in[0] = x.q, a.in[1] = x.k, a.out[0] = x.q_out, a.out[1] = x.k_out;
+  a.in_st[0] = strides3(x.q_st), a.in_st[1] = strides3(x.k_st);
+  a.out_st[0] = strides3(x.q_out_st), a.out_st[1] = strides3(x.k_out_st);
   a.heads[0] = H, a.heads[1] = Hkv;
   a.S = S, a.D = D, a.R = R;
   a.tokens = (int64_t)B * S;
-  a.positions = positions, a.pos64 = position_bits == 64, a.pos_b = psb, a.pos_s = pss;
-  a.turns = turns;
-  a.magnitude = magnitude;
-  a.sine_sign = backward ? -1.0f : 1.0f;
+  a.positions = x.positions, a.pos64 = x.position_bits == 64, a.pos_b = x.position_st[0], a.pos_s = x.position_st[1];
+  a.turns = x.turns;
+  a.magnitude = x.magnitude;
+  a.sine_sign = x.backward ? -1.0f : 1.0f;
   const int64_t blocks = (a.tokens * (D / 16) + 255) / 256;
   if (blocks > (1 << 23)) {   // 32-bit thread numbers
     set_error("rotary: %lld tokens are too many for one call", (long long)a.tokens);

@@ -81,6 +81,12 @@ inline int check_rows_pointer(const void* p, int64_t sb, int64_t ss, int64_t sh,
   return SAGE_OK;
 }
 
+inline Strides3 strides3(const int64_t (&st)[3]) { return Strides3{st[0], st[1], st[2]}; }
+
+inline int check_rows_pointer(const void* p, const int64_t (&st)[3], const char* name) {
+  return check_rows_pointer(p, st[0], st[1], st[2], name);
+}
+
 inline int launch_result(const char* what) {
   const cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess) return SAGE_OK;

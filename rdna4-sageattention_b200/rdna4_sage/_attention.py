@@ -169,13 +169,13 @@ def step(*tensors) -> torch.device:
     return dev
 
 
-def launch(index: int, what: str, entry, *args) -> None:
-    """entry(*args, stream) on the current stream of GPU `index`, with that GPU as the current device."""
+def launch(index: int, what: str, entry, args: bytes) -> None:
+    """entry(args, stream) on the current stream of GPU `index`, with that GPU as the current device."""
     if _current_device() == index:
-        rc = entry(*args, _raw_stream(index))
+        rc = entry(args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            rc = entry(*args, _raw_stream(index))
+            rc = entry(args, _raw_stream(index))
     if rc != 0:
         _lib.check(rc, what)
     if _CHECK and not torch.cuda.is_current_stream_capturing():

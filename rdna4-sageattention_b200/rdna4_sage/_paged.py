@@ -42,12 +42,12 @@ class PagedKV:
         for t in (k8, ks, v8, vs):
             if not t.is_contiguous() or t.device != k8.device:
                 raise Unsupported("cache buffers must be contiguous tensors on one device")
-        if k8.data_ptr() % 16 or v8.data_ptr() % 16:
-            raise Unsupported("k8 and v8 must be 16-byte aligned")
+        if any(t.data_ptr() % 16 for t in (k8, ks, v8, vs)):
+            raise Unsupported("cache buffers must be 16-byte aligned")
         self.k8, self.ks, self.v8, self.vs = k8, ks, v8, vs
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k8.shape
         # error word of the device: allocated here rather than by a first call under graph capture
-        self._word = _attention.host_word(k8.device) if k8.is_cuda else None
+        self._word = _attention.host_word(k8.device) if k8.is_cuda else 0
 
     @classmethod
     def empty(cls, num_pages, page_size, kv_heads, head_dim, device="cuda"):
@@ -61,23 +61,21 @@ class PagedKV:
     def device(self):
         return self.k8.device
 
-    def _pool(self):
-        return (self.k8.data_ptr(), self.ks.data_ptr(), self.v8.data_ptr(), self.vs.data_ptr(), self.num_pages,
-                self.page_size)
+    def _args(self, table, lens, counts, B):
+        """The cache part of a call's arguments."""
+        return (self.k8.data_ptr(), self.ks.data_ptr(), self.v8.data_ptr(), self.vs.data_ptr(), table.data_ptr(),
+                lens.data_ptr(), 0 if counts is None else counts.data_ptr(), self._word, table.stride(0), self.num_pages,
+                self.page_size, self.kv_heads, self.head_dim, table.shape[1], B)
 
 
 def _check_table(page_table, lens, counts, B):
-    """(address, row stride, pages) of the table, and the addresses of lens and counts."""
-    shape, stride = page_table.shape, page_table.stride()
-    if len(shape) != 2 or page_table.dtype != torch.int32 or shape[0] != B or shape[1] == 0 or stride[1] != 1:
+    shape = page_table.shape
+    if len(shape) != 2 or page_table.dtype != torch.int32 or shape[0] != B or shape[1] == 0 or page_table.stride(1) != 1:
         raise Unsupported(f"page_table must be int32 [{B}, pages] with contiguous rows")
     if lens.dtype != torch.int32 or lens.shape != (B,) or not lens.is_contiguous():
         raise Unsupported(f"lens must be contiguous int32 [{B}]")
-    if counts is None:
-        return page_table.data_ptr(), stride[0], shape[1], lens.data_ptr(), None
-    if counts.dtype != torch.int32 or counts.shape != (B,) or not counts.is_contiguous():
+    if counts is not None and (counts.dtype != torch.int32 or counts.shape != (B,) or not counts.is_contiguous()):
         raise Unsupported(f"counts must be contiguous int32 [{B}]")
-    return page_table.data_ptr(), stride[0], shape[1], lens.data_ptr(), counts.data_ptr()
 
 
 def _check_rows(kv, x, layout, heads=None):
@@ -111,7 +109,7 @@ def paged_kv_append(kv, k, v, page_table, lens, counts=None, tensor_layout="HND"
         raise Unsupported("k and v must match in shape and dtype")
     if v.requires_grad:
         _no_grad()
-    table = _check_table(page_table, lens, counts, B)
+    _check_table(page_table, lens, counts, B)
     if counts is None:
         dev = step(kv.k8, k, v, page_table, lens)
     else:
@@ -120,8 +118,8 @@ def paged_kv_append(kv, k, v, page_table, lens, counts=None, tensor_layout="HND"
         return
     k, kp, ks = step_rows(k, tensor_layout)
     v, vp, vs = step_rows(v, tensor_layout)
-    launch(dev.index, "sage_paged_append", _lib.lib().sage_paged_append, kp, vp, DTYPES[k.dtype], B, S, Hkv, kv.head_dim,
-           *ks, *vs, *kv._pool(), *table, kv._word)
+    launch(dev.index, "sage_paged_append", _lib.lib().sage_paged_append,
+           _lib.PACK_ROWS(*kv._args(page_table, lens, counts, B), kp, vp, *ks, *vs, DTYPES[k.dtype], S))
 
 
 def paged_kv_read(kv, page_table, lens, max_len, dtype=torch.bfloat16, tensor_layout="HND"):
@@ -134,7 +132,7 @@ def paged_kv_read(kv, page_table, lens, max_len, dtype=torch.bfloat16, tensor_la
     if max_len < 0:
         raise ValueError(f"max_len {max_len}")
     B = lens.shape[0] if lens.dim() == 1 else -1
-    table = _check_table(page_table, lens, None, B)
+    _check_table(page_table, lens, None, B)
     dev = step(kv.k8, page_table, lens)
     Hkv, D = kv.kv_heads, kv.head_dim
     shape = (B, Hkv, max_len, D) if tensor_layout == "HND" else (B, max_len, Hkv, D)
@@ -143,8 +141,8 @@ def paged_kv_read(kv, page_table, lens, max_len, dtype=torch.bfloat16, tensor_la
     if 0 in shape:
         return k, v
     _, kp, st = step_rows(k, tensor_layout)
-    launch(dev.index, "sage_paged_read", _lib.lib().sage_paged_read, *kv._pool(), Hkv, D, *table[:4], B, max_len, kp,
-           v.data_ptr(), DTYPES[dtype], *st, *st, kv._word)
+    launch(dev.index, "sage_paged_read", _lib.lib().sage_paged_read,
+           _lib.PACK_ROWS(*kv._args(page_table, lens, None, B), kp, v.data_ptr(), *st, *st, DTYPES[dtype], max_len))
     return k, v
 
 
@@ -153,7 +151,7 @@ def paged_kv_keep(kv, page_table, lens, keep, counts=None):
     without counts).  keep: int32 [B, N], strictly increasing in each row (the accepted path of a tree whose parents
     come before their children); entries from counts[b] on are not read."""
     B = lens.shape[0] if lens.dim() == 1 else -1
-    table = _check_table(page_table, lens, counts, B)
+    _check_table(page_table, lens, counts, B)
     if keep.dim() != 2 or keep.shape[0] != B or keep.dtype != torch.int32 or (keep.shape[1] > 1 and keep.stride(1) != 1):
         raise Unsupported(f"keep must be int32 [{B}, N] with contiguous rows")
     if counts is None:
@@ -162,8 +160,8 @@ def paged_kv_keep(kv, page_table, lens, keep, counts=None):
         dev = step(kv.k8, page_table, lens, keep, counts)
     if keep.numel() == 0:
         return
-    launch(dev.index, "sage_paged_keep", _lib.lib().sage_paged_keep, *kv._pool(), kv.kv_heads, kv.head_dim, *table[:4],
-           keep.data_ptr(), keep.stride(0), keep.shape[1], table[4], B, kv._word)
+    launch(dev.index, "sage_paged_keep", _lib.lib().sage_paged_keep,
+           _lib.PACK_KEEP(*kv._args(page_table, lens, counts, B), keep.data_ptr(), keep.stride(0), keep.shape[1]))
 
 
 def attention_paged_kv(q, kv, page_table, lens, tree_mask=None, counts=None, tensor_layout="HND", sm_scale=None,
@@ -175,11 +173,11 @@ def attention_paged_kv(q, kv, page_table, lens, tree_mask=None, counts=None, ten
     return_lse also the (B, H, T) fp32 log-sum-exp; tokens from counts[b] on, and rows that see nothing, are zero with
     log-sum-exp -inf."""
     B, T, H = _check_rows(kv, q, tensor_layout)
-    table = _check_table(page_table, lens, counts, B)
+    _check_table(page_table, lens, counts, B)
     tensors = [kv.k8, q, page_table, lens]
     if counts is not None:
         tensors.append(counts)
-    mask, mask_b, mask_i = None, 0, 0
+    mask, mask_b, mask_i = 0, 0, 0
     if tree_mask is not None:
         shape = tree_mask.shape
         if tree_mask.dtype != torch.bool or shape != (B, T, T) and shape != (T, T) and shape != (1, T, T):
@@ -204,9 +202,10 @@ def attention_paged_kv(q, kv, page_table, lens, tree_mask=None, counts=None, ten
         ws = _alloc(ws_bytes, stream) if _current_device() == index else None
         hold = torch.empty(ws_bytes, device=dev, dtype=torch.uint8) if ws is None else None
         try:
-            launch(index, "sage_paged_attention", L.sage_paged_attention, qp, DTYPES[q.dtype], B, T, H, kv.kv_heads,
-                   kv.head_dim, *qs, *kv._pool(), *table, mask, mask_b, mask_i, float(sm_scale or 0.0), op, *os,
-                   lse.data_ptr() if return_lse else None, ws if hold is None else hold.data_ptr(), ws_bytes, kv._word)
+            launch(index, "sage_paged_attention", L.sage_paged_attention,
+                   _lib.PACK_ATTENTION(*kv._args(page_table, lens, counts, B), qp, op, lse.data_ptr() if return_lse else 0,
+                                       mask, ws if hold is None else hold.data_ptr(), ws_bytes, *qs, *os, mask_b, mask_i,
+                                       float(sm_scale or 0.0), DTYPES[q.dtype], T, H))
         finally:
             if hold is None:
                 _free(ws)

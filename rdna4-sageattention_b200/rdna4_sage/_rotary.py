@@ -116,7 +116,7 @@ def _launch(q, k, positions, rope, layout, backward):
     else:
         B, S, H, D = q.shape
     if k is None:
-        k_out, Hkv, kp, kop, ks, kos = None, 0, None, None, (0, 0, 0), (0, 0, 0)
+        k_out, Hkv, kp, kop, ks, kos = None, 0, 0, 0, (0, 0, 0), (0, 0, 0)
     else:
         k, kp, ks = step_rows(k, layout)
         k_out = torch.empty_like(k)
@@ -124,9 +124,10 @@ def _launch(q, k, positions, rope, layout, backward):
         Hkv = k.shape[1 if layout == "HND" else 2]
     ps = positions.stride()
     pb = ps[0] if len(ps) == 2 and positions.shape[0] > 1 else 0
-    launch(q.get_device(), "sage_rotary", _lib.lib().sage_rotary, qp, kp, DTYPES[q.dtype], B, S, H, Hkv, D, rope.rotary_dim,
-           rope.interleaved, *qs, *ks, qop, kop, *qos, *kos, positions.data_ptr(),
-           32 if positions.dtype == torch.int32 else 64, pb, ps[-1], rope.turns.data_ptr(), rope.magnitude, backward)
+    args = _lib.PACK_ROTARY(qp, kp, qop, kop, positions.data_ptr(), rope.turns.data_ptr(), *qs, *ks, *qos, *kos, pb, ps[-1],
+                            DTYPES[q.dtype], B, S, H, Hkv, D, rope.rotary_dim, rope.interleaved,
+                            32 if positions.dtype == torch.int32 else 64, rope.magnitude, backward)
+    launch(q.get_device(), "sage_rotary", _lib.lib().sage_rotary, args)
     return q_out, k_out
 
 

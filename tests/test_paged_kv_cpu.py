@@ -1,6 +1,9 @@
 """Refusals and host arithmetic of rotary positions and the paged K/V cache, without a GPU."""
 import ctypes
 import math
+import os
+import struct
+import subprocess
 
 import pytest
 import torch
@@ -142,33 +145,61 @@ def test_rotary_frequencies():
 
 def test_c_entries_check_their_arguments_without_gpu():
     L = _lib.lib()
-    p, OK = 256, [8] * 3
-    pool = [p, p, p, p, 4, 16]
-    table = [p, 2, 2, p]
+    p, st = 256, [8, 8, 8]
     bad, unsupported = _lib.SAGE_ERR_INVALID, _lib.SAGE_ERR_UNSUPPORTED
-    rot = lambda D=64, R=64, q=p, k=p, bits=32, turns=p: L.sage_rotary(  # noqa: E731
-        q, k, 0, 1, 3, 2, 1, D, R, 0, *OK, *OK, p, p, *OK, *OK, p, bits, 3, 1, turns, 1.0, 0, None)
+
+    def rot(q=p, k=p, turns=p, D=64, R=64, bits=32):
+        return L.sage_rotary(_lib.PACK_ROTARY(q, k, p, p, p, turns, *st * 4, 3, 1, 0, 1, 3, 2, 1, D, R, 0, bits, 1.0, 0), None)
     assert rot(D=80) == unsupported and rot(R=24) == unsupported and rot(bits=16) == unsupported
-    assert rot(q=8) == bad and rot(k=None) == bad and rot(turns=None) == bad
+    assert rot(q=8) == bad and rot(k=0) == bad and rot(turns=0) == bad and L.sage_rotary(None, None) == bad
 
-    def app(D=64, k=p, pool=pool, table=table, S=3):
-        return L.sage_paged_append(k, p, 0, 2, S, 2, D, *OK, *OK, *pool, *table, None, p, None)
-    assert app(D=80) == unsupported and b"head_dim 80" in L.sage_last_error()
-    assert app(k=8) == bad and app(S=0) == unsupported
-    assert app(pool=[p, p, p, p, 4, 24]) == unsupported and b"page_size 24" in L.sage_last_error()
-    assert app(pool=[p, p, p, p, 0, 16]) == unsupported
-    assert app(pool=[8, p, p, p, 4, 16]) == bad and app(pool=[p, None, p, p, 4, 16]) == bad
-    assert app(table=[None, 2, 2, p]) == bad and app(table=[p, 2, 2, None]) == bad
-    rd = lambda S=5, k=p, dt=0: L.sage_paged_read(*pool, 2, 64, *table, 2, S, k, p, dt, *OK, *OK, p, None)  # noqa: E731
-    assert rd(S=0) == unsupported and rd(k=4) == bad and rd(dt=2) == unsupported
-    kp = lambda keep=p, N=3: L.sage_paged_keep(*pool, 2, 64, *table, keep, 3, N, None, 2, p, None)  # noqa: E731
-    assert kp(keep=None) == bad and kp(N=0) == unsupported
+    def kv(k8=p, ks=p, table=p, lens=p, pages=4, page=16, Hkv=2, D=64, most=2):
+        return k8, ks, p, p, table, lens, 0, p, 2, pages, page, Hkv, D, most, 2
 
-    def att(H=4, q=p, table=table, ws=0, T=3):
-        return L.sage_paged_attention(q, 0, 2, T, H, 2, 64, *OK, *pool, *table, None, None, 0, 0, 0.0, p, *OK, None,
-                                      None, ws, p, None)
-    assert att(H=3) == unsupported and att(q=8) == bad and att(T=0) == unsupported
-    assert att(table=[p, 2, 2 ** 27, p]) == unsupported and b"32 bits" in L.sage_last_error()
+    def rows(entry, k=p, S=3, dtype=0, **kw):
+        return getattr(L, entry)(_lib.PACK_ROWS(*kv(**kw), k, p, *st * 2, dtype, S), None)
+    for entry in ("sage_paged_append", "sage_paged_read"):
+        assert rows(entry, D=80) == unsupported and b"head_dim 80" in L.sage_last_error()
+        assert rows(entry, k=8) == bad and rows(entry, S=0) == unsupported and rows(entry, dtype=2) == unsupported
+        assert rows(entry, page=24) == unsupported and b"page_size 24" in L.sage_last_error()
+        assert rows(entry, pages=0) == unsupported and rows(entry, k8=8) == bad and rows(entry, ks=0) == bad
+        assert rows(entry, table=0) == bad and rows(entry, lens=0) == bad and rows(entry, ks=260) == bad
+        assert getattr(L, entry)(None, None) == bad
+
+    def keep(keep=p, N=3, **kw):
+        return L.sage_paged_keep(_lib.PACK_KEEP(*kv(**kw), keep, 3, N), None)
+    assert keep(keep=0) == bad and keep(N=0) == unsupported and keep(page=8) == unsupported
+
+    def att(q=p, H=4, T=3, ws=p, ws_bytes=0, **kw):
+        return L.sage_paged_attention(_lib.PACK_ATTENTION(*kv(**kw), q, p, 0, 0, ws, ws_bytes, *st * 2, 0, 0, 0.0, 0, T, H), None)
+    assert att(H=3) == unsupported and att(q=8) == bad and att(T=0) == unsupported and L.sage_paged_attention(None, None) == bad
+    assert att(most=2 ** 27) == unsupported and b"positions must fit 32 bits" in L.sage_last_error()
+    assert att(pages=2 ** 27) == unsupported and b"cache rows must fit 32 bits" in L.sage_last_error()
+    need = L.sage_paged_attention_workspace_bytes(2, 3, 4, 2, 64)
+    assert need > 0 and att(ws_bytes=need - 1) == bad and b"workspace" in L.sage_last_error()
+    assert att(ws=0, ws_bytes=need) == bad and att(ws=264, ws_bytes=need) == bad
+    for shape in ((0, 3, 4, 2, 64), (2, 3, 3, 2, 64), (2, 3, 4, 2, 80)):
+        assert L.sage_paged_attention_workspace_bytes(*shape) == 0
+
+
+def test_argument_structs_match_the_header(tmp_path):
+    # the formats that Python packs, against the compiler's layout of the structs
+    src, exe = tmp_path / "layout.c", tmp_path / "layout"
+    fields = {"sage_rotary_args": ("positions", "q_st", "position_st", "dtype", "magnitude", "backward"),
+              "sage_paged_rows_args": ("k", "k_st", "v_st", "dtype", "S"), "sage_paged_keep_args": ("keep", "keep_stride", "N"),
+              "sage_paged_attention_args": ("q", "workspace_bytes", "mask_st", "sm_scale", "dtype", "H")}
+    src.write_text('#include <stdio.h>\n#include <stddef.h>\n#include "sage_b200.h"\nint main(void) {\n' + "".join(
+        f'printf("%zu ", offsetof({s}, {f}));\n' for s, fs in fields.items() for f in fs) + "return 0; }\n")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    subprocess.run(["gcc", "-I", os.path.join(root, "include"), str(src), "-o", str(exe)], check=True)
+    got = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
+    size = struct.calcsize
+    kv = _lib.PAGED_KV
+    want = [size("4P"), size("6P"), size("6P12q"), size("6P14q"), size("6P14q9i"), size("6P14q9if"),
+            size(kv), size(kv + "2P"), size(kv + "2P3q"), size(kv + "2P6q"), size(kv + "2P6qi"),
+            size(kv), size(kv + "P"), size(kv + "Pq"),
+            size(kv), size(kv + "5P"), size(kv + "5P7q"), size(kv + "5P9q"), size(kv + "5P9qd"), size(kv + "5P9qd2i")]
+    assert got == want
 
 
 def test_reference_codes_by_hand():
