@@ -61,7 +61,6 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
   uint64_t* empty = full + kStages;
   float* join_o = reinterpret_cast<float*>(empty + kStages);                            // [rows][D + 4]
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {
     given_up = 0;
     for (int s = 0; s < kStages; ++s) {
@@ -70,6 +69,10 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
     }
     fence_barrier_init();
   }
+  // Nothing of the stream's earlier work is read before it is done; only then may the join start, which reads the lengths
+  // before it waits for this kernel.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   const int64_t list = list_length<kThreads>(a, warp_sums);
   const int share = sharers(a, list);
@@ -202,78 +205,114 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
           step(2 * i, u.x, v.x), step(2 * i + 1, u.y, v.y);
         }
       }
-      // of the lane's two keys: factor of the score, log2 of the V scale, its inverse, and what the exponent of a zero row
-      // gains over its part in the maximum
-      float factor[2], log_v[2], inverse_v[2], gain[2];
-      bool zero = false;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float vs = ks[kTileKeys + keys[h]];
-        factor[h] = ks[keys[h]] * a.scale;
-        log_v[h] = __log2f(vs);
-        // finite whatever the scale is (unwritten memory): rows that see a NaN scale are NaN by its logarithm, and rows that do
-        // not see the key must not meet 0 * NaN or 0 * infinity here
-        inverse_v[h] = vs > 0x1p-120f ? __fdividef(1.0f, vs) : 0x1p120f;
-        gain[h] = 0.0f;
-        if (vs == 0.0f) zero = true, log_v[h] = kZeroLog, inverse_v[h] = 1.0f, gain[h] = -kZeroLog;
-      }
-      bool more = false;
-#pragma unroll
-      for (int r = 0; r < NR; ++r)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float& x = s[r][2 * h + e];
-            if constexpr (!std::is_same<T, __half>::value) x *= row_scale[r][e];
-            x = fmaf(x, factor[h], log_v[h]);
-            if (drafts) {
-              const int t = key0 + keys[h] - now.len, token = (row0 + 8 * r + 2 * c + e) / a.group;
-              const bool seen = t < 0 || (t < now.fresh && token < now.fresh &&
-                                          (a.mask != nullptr ? a.mask[now.b * a.mask_b + token * a.mask_i + t] != 0
-                                                             : t <= token));
-              if (!seen) x = -INFINITY;
-            }
-            more |= x > m[r][e] + 8.0f;
-          }
-      if (__any_sync(0xffffffffu, more)) {
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          float keep[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float top = fmaxf(s[r][e], s[r][2 + e]);
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-            const float next = top > m[r][e] + 8.0f ? top : m[r][e];
-            keep[e] = next == m[r][e] ? 1.0f : fast_exp2(m[r][e] - next);
-            m[r][e] = next;
-            l[r][e] *= keep[e];
-          }
-#pragma unroll
-          for (int t = 0; t < NT; ++t) o[r][t][0] *= keep[0], o[r][t][1] *= keep[1], o[r][t][2] *= keep[0], o[r][t][3] *= keep[1];
-        }
-      }
-      if (__any_sync(0xffffffffu, zero)) {
+      // Most groups: every row sees every key and no maximum moves.  The weights are computed on that assumption, p vs =
+      // 2^(s - m') vs and l from 2^(s - m') itself, and looked over afterwards; where it did not hold (a weight above 2^8, a
+      // key whose V row is zero far above the others) the group is done over from its scores.
+      const float factor[2] = {ks[keys[0]] * a.scale, ks[keys[1]] * a.scale};
+      const float v_scale[2] = {ks[kTileKeys + keys[0]], ks[kTileKeys + keys[1]]};
+      uint32_t pf[NR][2];
+      bool again = true;
+      if constexpr (!std::is_same<T, __half>::value) {
 #pragma unroll
         for (int r = 0; r < NR; ++r)
 #pragma unroll
-          for (int x = 0; x < 4; ++x) s[r][x] += gain[x / 2];
+          for (int x = 0; x < 4; ++x) s[r][x] *= row_scale[r][x & 1];
       }
-      uint32_t pf[NR][2];
+      if (!drafts) {
+        float sum[NR][2], top = 0.0f, most = 0.0f;
 #pragma unroll
-      for (int r = 0; r < NR; ++r)
+        for (int r = 0; r < NR; ++r) {
+          sum[r][0] = l[r][0], sum[r][1] = l[r][1];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float u = fast_exp2(fmaf(s[r][2 * h], factor[h], -m[r][0]));
+            const float v = fast_exp2(fmaf(s[r][2 * h + 1], factor[h], -m[r][1]));
+            sum[r][0] += u, sum[r][1] += v;
+            top = fmaxf(fmaxf(top, u * v_scale[h]), v * v_scale[h]);
+            pf[r][h] = pack_weights(u * v_scale[h], v * v_scale[h]);
+          }
+          most = r == 0 ? sum[0][0] + sum[0][1] : most + (sum[r][0] + sum[r][1]);
+        }
+        again = __any_sync(0xffffffffu, !(top <= 256.0f && most < 0x1p120f));
+        if (!again) {
+#pragma unroll
+          for (int r = 0; r < NR; ++r) {
+            l[r][0] = sum[r][0], l[r][1] = sum[r][1];
+            pf[r][0] = transposed(pf[r][0]), pf[r][1] = transposed(pf[r][1]);
+          }
+        }
+      }
+      if (again) {
+        // of the lane's two keys: log2 of the V scale, its inverse, and what the exponent of a zero row gains over its part in
+        // the maximum
+        float log_v[2], inverse_v[2], gain[2];
+        bool zero = false;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float p[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            p[e] = fast_exp2(s[r][2 * h + e] - m[r][e]);
-            l[r][e] = fmaf(p[e], inverse_v[h], l[r][e]);
-          }
-          pf[r][h] = transposed(pack_weights(p[0], p[1]));
+          const float vs = v_scale[h];
+          log_v[h] = __log2f(vs);
+          // finite whatever the scale is (unwritten memory): rows that see a NaN scale are NaN by its logarithm, and rows that do
+          // not see the key must not meet 0 * NaN or 0 * infinity here
+          inverse_v[h] = vs > 0x1p-120f ? __fdividef(1.0f, vs) : 0x1p120f;
+          gain[h] = 0.0f;
+          if (vs == 0.0f) zero = true, log_v[h] = kZeroLog, inverse_v[h] = 1.0f, gain[h] = -kZeroLog;
         }
+        bool more = false;
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float& x = s[r][2 * h + e];
+              x = fmaf(x, factor[h], log_v[h]);   // scaled by its row already
+              if (drafts) {
+                const int t = key0 + keys[h] - now.len, token = (row0 + 8 * r + 2 * c + e) / a.group;
+                const bool seen = t < 0 || (t < now.fresh && token < now.fresh &&
+                                            (a.mask != nullptr ? a.mask[now.b * a.mask_b + token * a.mask_i + t] != 0
+                                                               : t <= token));
+                if (!seen) x = -INFINITY;
+              }
+              more |= x > m[r][e] + 8.0f;
+            }
+        if (__any_sync(0xffffffffu, more)) {
+#pragma unroll
+          for (int r = 0; r < NR; ++r) {
+            float keep[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float top = fmaxf(s[r][e], s[r][2 + e]);
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+              const float next = top > m[r][e] + 8.0f ? top : m[r][e];
+              keep[e] = next == m[r][e] ? 1.0f : fast_exp2(m[r][e] - next);
+              m[r][e] = next;
+              l[r][e] *= keep[e];
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) o[r][t][0] *= keep[0], o[r][t][1] *= keep[1], o[r][t][2] *= keep[0], o[r][t][3] *= keep[1];
+          }
+        }
+        if (__any_sync(0xffffffffu, zero)) {
+#pragma unroll
+          for (int r = 0; r < NR; ++r)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) s[r][x] += gain[x / 2];
+        }
+#pragma unroll
+        for (int r = 0; r < NR; ++r)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float p[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              p[e] = fast_exp2(s[r][2 * h + e] - m[r][e]);
+              l[r][e] = fmaf(p[e], inverse_v[h], l[r][e]);
+            }
+            pf[r][h] = transposed(pack_weights(p[0], p[1]));
+          }
+      }
       // four keys a lane; a word of four channels of each is two output tiles
       auto product = [&](int i, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
 #pragma unroll
@@ -574,8 +613,7 @@ static int launch_paged_attn(const PagedAttnArgs& a, cudaStream_t st) {
     if (e == cudaSuccess && dev < 64) prepared.fetch_or(uint64_t(1) << dev);
   }
   if (e == cudaSuccess) {
-    paged_attn_kernel<T, D, NR, WM><<<a.ctas, kThreads, C::kSmem, st>>>(a, k_map, v_map);
-    e = cudaGetLastError();
+    e = launch_early(paged_attn_kernel<T, D, NR, WM>, dim3(a.ctas), kThreads, C::kSmem, st, a, k_map, v_map);
   }
   if (e == cudaSuccess) return SAGE_OK;
   set_error("paged attention: %s", cudaGetErrorString(e));
@@ -586,16 +624,9 @@ template <typename T, int D>
 static int launch_join(const PagedAttnArgs& a, int tile_rows, bool many, cudaStream_t st) {
   const int used = std::min(tile_rows, a.T * a.group), per_block = many ? 32 : kJoinThreads / 32;
   const int blocks = (used + per_block - 1) / per_block;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(a.B * a.p.Hkv * a.row_tiles * blocks));
-  cfg.blockDim = dim3(kJoinThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, many ? wide_join_kernel<T, D> : paged_join_kernel<T, D>, a, tile_rows, blocks);
+  const dim3 grid((unsigned)(a.B * a.p.Hkv * a.row_tiles * blocks));
+  const cudaError_t e = launch_early(many ? wide_join_kernel<T, D> : paged_join_kernel<T, D>, grid, kJoinThreads, 0, st, a,
+                                     tile_rows, blocks);
   if (e == cudaSuccess) return SAGE_OK;
   set_error("paged attention: %s", cudaGetErrorString(e));
   return SAGE_ERR_LAUNCH;

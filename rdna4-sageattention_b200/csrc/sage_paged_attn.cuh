@@ -260,6 +260,23 @@ inline int sm_count() {
   return n;
 }
 
+// Launch that may begin while the stream's kernel before it ends (its blocks are placed and set themselves up); the kernel
+// waits with griddepcontrol.wait before it touches global memory.
+template <typename... P, typename... A>
+inline cudaError_t launch_early(void (*kernel)(P...), dim3 grid, int threads, int smem, cudaStream_t st, const A&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // The codes as [rows, D] bytes; a box is the rows of a page that a tile of keys takes, 128 bytes of each (or all of them).
 template <int D>
 inline bool code_map(CUtensorMap* map, const void* base, uint64_t rows, int page_size) {

@@ -132,7 +132,6 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
   float* scales = reinterpret_cast<float*>(stages + W::kRaw * S::kStage);
   float* params = scales + W::kRaw * 2 * kTileKeys;
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (tid == 0) {
     given_up = 0;
     for (int i = 0; i < W::kRaw; ++i) mbar_init(raw_full + i, 1), mbar_init(raw_empty + i, W::kConverters);
@@ -150,6 +149,10 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
     }
     fence_barrier_init();
   }
+  // Nothing of the stream's earlier work is read before it is done; only then may the join start, which reads the lengths
+  // before it waits for this kernel.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   const int64_t list = list_length<W::kThreads>(a, warp_sums);
   const int share = sharers(a, list);
@@ -740,8 +743,7 @@ static int launch_wide(const PagedAttnArgs& a, cudaStream_t st) {
     if (e == cudaSuccess && dev < 64) prepared.fetch_or(uint64_t(1) << dev);
   }
   if (e == cudaSuccess) {
-    paged_wide_kernel<T, D><<<a.ctas, W::kThreads, W::kSmem, st>>>(a, k_map, v_map);
-    e = cudaGetLastError();
+    e = launch_early(paged_wide_kernel<T, D>, dim3(a.ctas), W::kThreads, W::kSmem, st, a, k_map, v_map);
   }
   if (e == cudaSuccess) return SAGE_OK;
   set_error("paged attention: %s", cudaGetErrorString(e));
