@@ -35,11 +35,10 @@ struct Config {
   // CTAs of an SM: as the registers of a thread allow (96 for four CTAs, 128 for three, 168 for two)
   static constexpr int kCtas = NR == 1 && D <= 128 ? 4 : D == 64 ? 3 : 2;
   static constexpr int kRows = 8 * NR * WM;               // of a row tile
-  static constexpr int kJoin = WM < kWarps ? kRows * (D + 4) * 4 : 0;
   static constexpr int kPerStage = Tile<D>::kStage + 2 * kTileKeys * 4 + 16;
-  static constexpr int kFit = (232448 / kCtas - 2048 - 1024 - kJoin) / kPerStage;
+  static constexpr int kFit = (232448 / kCtas - 2048 - 1024) / kPerStage;
   static constexpr int kStages = kFit < 8 ? kFit : 8;
-  static constexpr int kSmem = 1024 + kStages * kPerStage + kJoin;
+  static constexpr int kSmem = 1024 + kStages * kPerStage;
   static_assert(kStages >= 2, "two stages at the least");
 };
 
@@ -59,7 +58,6 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
   float* scales = reinterpret_cast<float*>(stages + kStages * S::kStage);               // [stage][ks, vs][64]
   uint64_t* full = reinterpret_cast<uint64_t*>(scales + kStages * 2 * kTileKeys);
   uint64_t* empty = full + kStages;
-  float* join_o = reinterpret_cast<float*>(empty + kStages);                            // [rows][D + 4]
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   if (tid == 0) {
     given_up = 0;
@@ -348,12 +346,12 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
         }
       }
     }
-    __syncwarp();
-    if (lane == 0) arrive(empty + slot);
-    if (++slot == kStages) slot = 0, phase ^= 1;
-
-    const bool last_tile = now.tile + 1 == now.tiles;
-    if (last_tile || todo == 1) {
+    const bool last_tile = now.tile + 1 == now.tiles, ends = last_tile || todo == 1;
+    if (WK == 1 || !ends) {
+      __syncwarp();
+      if (lane == 0) arrive(empty + slot);
+    }
+    if (ends) {
       // the row tile ends here, or this CTA's part of it does
       const bool whole = last_tile && first_tile == 0;
       const int64_t part = (2 * (int64_t)blockIdx.x + (segment > 0)) * C::kRows;
@@ -366,8 +364,14 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
           l[r][e] += __shfl_xor_sync(0xffffffffu, l[r][e], 16);
         }
       if constexpr (WK > 1) {
-        // the warps of a row tile join through shared memory, in their order
+        // The warps of a row tile join through the stage that all of them have read by then, eight rows of each at a time:
+        // every warp leaves its part, every thread adds up eight channels of a row in the order of the warps.
         auto consumers_sync = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
+        float* area = reinterpret_cast<float*>(stages + slot * S::kStage);   // [warp][8 rows][D]
+        static_assert(kWarps * 8 * D * 4 <= S::kStage, "the parts must fit a stage");
+        auto place = [](int row, int quad) {   // four channels; permuted against bank conflicts
+          return (row * (D / 4) + (quad ^ (row >> 1 & 3) ^ (S::kWide ? (quad >> 4 & 1) << 2 : 0))) * 4;
+        };
         if (n == 0) {
 #pragma unroll
           for (int r = 0; r < NR; ++r)
@@ -375,44 +379,57 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
             for (int e = 0; e < 2; ++e) join_ml[warp][8 * r + 2 * c + e] = make_float2(m[r][e], l[r][e]);
         }
         consumers_sync();
-        float factor[NR][2];
 #pragma unroll
-        for (int r = 0; r < NR; ++r)
+        for (int r = 0; r < NR; ++r) {
+          if (r > 0) consumers_sync();
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float top = -3.402823466e38f, sum = 0.0f;
+          for (int t = 0; t < NT; t += 2)
 #pragma unroll
-            for (int w = 0; w < WK; ++w) top = fmaxf(top, join_ml[w * WM + wm][8 * r + 2 * c + e].x);
+            for (int e = 0; e < 2; ++e)
+              *reinterpret_cast<float4*>(area + warp * (8 * D) + place(2 * c + e, S::channel(n, t, 0) / 4)) =
+                  make_float4(o[r][t][e], o[r][t][2 + e], o[r][t + 1][e], o[r][t + 1][2 + e]);
+          consumers_sync();
+#pragma unroll 1
+          for (int item = tid; item < WM * D; item += 32 * kWarps) {
+            const int of = item / (D / 8), g = of / 8, rr = of % 8, d = item % (D / 8) * 8;
+            float top = -3.402823466e38f, sum = 0.0f, x[8] = {};
+#pragma unroll
+            for (int w = 0; w < WK; ++w) top = fmaxf(top, join_ml[w * WM + g][8 * r + rr].x);
 #pragma unroll
             for (int w = 0; w < WK; ++w) {
-              const float2 x = join_ml[w * WM + wm][8 * r + 2 * c + e];
-              sum += fast_exp2(x.x - top) * x.y;
+              const float2 ml = join_ml[w * WM + g][8 * r + rr];
+              const float f = fast_exp2(ml.x - top);
+              sum = fmaf(f, ml.y, sum);
+              const float* from = area + (w * WM + g) * (8 * D);
+              const float4 u = *reinterpret_cast<const float4*>(from + place(rr, d / 4));
+              const float4 v = *reinterpret_cast<const float4*>(from + place(rr, d / 4 + 1));
+              x[0] = fmaf(f, u.x, x[0]), x[1] = fmaf(f, u.y, x[1]), x[2] = fmaf(f, u.z, x[2]), x[3] = fmaf(f, u.w, x[3]);
+              x[4] = fmaf(f, v.x, x[4]), x[5] = fmaf(f, v.y, x[5]), x[6] = fmaf(f, v.z, x[6]), x[7] = fmaf(f, v.w, x[7]);
             }
-            factor[r][e] = fast_exp2(m[r][e] - top);
-            m[r][e] = top, l[r][e] = sum;
+            const int in_tile = g * 8 * NR + 8 * r + rr, row = now.unit % a.row_tiles * C::kRows + in_tile;
+            const int token = row / a.group, head = head0 + row % a.group;
+            if (row >= a.T * a.group) continue;
+            if (whole) {
+              const bool seen = token < now.fresh && sum != 0.0f;
+              const float inverse = 1.0f / sum;
+#pragma unroll
+              for (int z = 0; z < 8; ++z) x[z] = seen ? x[z] * inverse : 0.0f;
+              store8(static_cast<T*>(a.out) + now.b * a.out_st.b + token * a.out_st.s + head * a.out_st.h + d, x);
+              if (a.lse != nullptr && d == 0)
+                a.lse[((int64_t)now.b * a.H + head) * a.T + token] =
+                    seen ? (top + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+            } else {
+              float* to = a.part_o + (part + in_tile) * D + d;
+              *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
+              *reinterpret_cast<float4*>(to + 4) = make_float4(x[4], x[5], x[6], x[7]);
+              if (d == 0) a.part_ml[part + in_tile] = make_float2(top, sum);
+            }
           }
-#pragma unroll 1
-        for (int w = 0; w < WK; ++w) {
-          if (w == wk) {
-#pragma unroll
-            for (int r = 0; r < NR; ++r)
-#pragma unroll
-              for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  // channels 2t and 2t + 1 of the lane lie next to each other
-                  float2* at = reinterpret_cast<float2*>(join_o + (wm * 8 * NR + 8 * r + 2 * c + e) * (D + 4) +
-                                                         S::channel(n, t, 0));
-                  float2 x = make_float2(o[r][t][e] * factor[r][e], o[r][t][2 + e] * factor[r][e]);
-                  if (w > 0) x.x += at->x, x.y += at->y;
-                  if (w < WK - 1) *at = x;
-                  o[r][t][e] = x.x, o[r][t][2 + e] = x.y;
-                }
-          }
-          consumers_sync();
         }
-      }
-      if (wk == WK - 1) {
+        fence_proxy_async_smem();   // before the stage's next load
+        __syncwarp();
+        if (lane == 0) arrive(empty + slot);
+      } else {
 #pragma unroll
         for (int r = 0; r < NR; ++r)
 #pragma unroll
@@ -445,6 +462,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
       ++segment;
       fresh_unit = true;
     }
+    if (++slot == kStages) slot = 0, phase ^= 1;
     if (todo > 1) advance(a, now);
   }
 }
