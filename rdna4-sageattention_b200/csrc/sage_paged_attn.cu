@@ -72,19 +72,9 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  const int64_t list = list_length<kThreads>(a, warp_sums);
-  const int share = sharers(a, list);
-  if ((int)blockIdx.x >= share) return;
-  const int64_t first = (int64_t)blockIdx.x * list / share, end = (int64_t)(blockIdx.x + 1) * list / share;
   Cursor now;
-  {
-    int64_t within;
-    find<kThreads>(a, first, warp_sums, found, now.b, within);   // ends with a barrier of the CTA
-    now.tiles = sequence(a, now.b, now.len, now.fresh);
-    now.unit = (int)(within / now.tiles);
-    now.tile = (int)(within - (int64_t)now.unit * now.tiles);
-  }
-  int64_t todo = end - first;
+  int64_t todo = locate<kThreads>(a, warp_sums, found, now);
+  if (todo == 0) return;
   int slot = 0;
   uint32_t phase = 0;
 
@@ -479,8 +469,18 @@ __device__ __forceinline__ int sharing(const PagedAttnArgs& a, int b, int unit, 
     mine += t;
     if (s < b) before += t;
   }
-  scan_before<kJoinThreads>(mine, warp_sums, list);
-  scan_before<kJoinThreads>(before, warp_sums, start);
+  {   // both sums over the block with one pair of barriers
+#pragma unroll
+    for (int o = 16; o > 0; o /= 2) {
+      mine += __shfl_xor_sync(0xffffffffu, mine, o);
+      before += __shfl_xor_sync(0xffffffffu, before, o);
+    }
+    if (threadIdx.x % 32 == 0) warp_sums[threadIdx.x / 32] = mine, warp_sums[kJoinThreads / 32 + threadIdx.x / 32] = before;
+    __syncthreads();
+    list = start = 0;
+#pragma unroll
+    for (int w = 0; w < kJoinThreads / 32; ++w) list += warp_sums[w], start += warp_sums[kJoinThreads / 32 + w];
+  }
   const int tiles = sequence(a, b, len, fresh);
   list *= per;
   start = start * per + (int64_t)unit * tiles;
@@ -498,7 +498,7 @@ __device__ __forceinline__ int sharing(const PagedAttnArgs& a, int b, int unit, 
 // of a row tile are joined in the order of its keys.  A warp takes a row.
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAttnArgs a, int tile_rows, int blocks_per_unit) {
-  __shared__ int64_t warp_sums[kJoinThreads / 32];
+  __shared__ int64_t warp_sums[2 * kJoinThreads / 32];
   const int64_t id = blockIdx.x / blocks_per_unit;
   const int per = a.p.Hkv * a.row_tiles, b = (int)(id / per), unit = (int)(id - (int64_t)b * per);
   int fresh, c0, c1, slot;
@@ -556,7 +556,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAtt
 // 32 rows, a lane a row, a warp a quarter of its channels.
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) wide_join_kernel(const PagedAttnArgs a, int tile_rows, int blocks_per_unit) {
-  __shared__ int64_t warp_sums[kJoinThreads / 32];
+  __shared__ int64_t warp_sums[2 * kJoinThreads / 32];
   const int64_t id = blockIdx.x / blocks_per_unit;
   const int per = a.p.Hkv * a.row_tiles, b = (int)(id / per), unit = (int)(id - (int64_t)b * per);
   int fresh, c0, c1, slot;
@@ -721,6 +721,10 @@ extern "C" int sage_paged_attention(const sage_paged_attention_args* args, void*
   const Shape shape = row_tile((int64_t)T * a.group, D);
   const int tile_rows = many ? wide_rows(D) : 8 * shape.nr * shape.wm;
   a.row_tiles = (T * a.group + tile_rows - 1) / tile_rows;
+  if (((int64_t)kv.max_pages * kv.page_size / kTileKeys + 1) * a.row_tiles * Hkv > (int64_t)UINT_MAX) {
+    set_error("%d tokens of %d heads over %d pages of %d keys are too many for one call", T, H, kv.max_pages, kv.page_size);
+    return SAGE_ERR_UNSUPPORTED;
+  }
   a.ctas = many ? wide_ctas() : shared_ctas(D, shape);
   a.scale = (float)((args->sm_scale > 0.0 ? args->sm_scale : 1.0 / std::sqrt((double)D)) * 1.4426950408889634);
   a.part_o = static_cast<float*>(args->workspace);

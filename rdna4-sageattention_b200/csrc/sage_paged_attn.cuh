@@ -69,40 +69,8 @@ __device__ __forceinline__ int64_t scan_before(int64_t v, int64_t* warp_sums, in
   return before + x - v;
 }
 
-// The list's length: key tiles over all sequences, kv heads and row tiles.
-template <int THREADS>
-__device__ __forceinline__ int64_t list_length(const PagedAttnArgs& a, int64_t* warp_sums) {
-  int64_t mine = 0;
-  int len, fresh;
-  for (int b = threadIdx.x; b < a.B; b += THREADS) mine += sequence(a, b, len, fresh);
-  int64_t total;
-  scan_before<THREADS>(mine, warp_sums, total);
-  return total * (a.p.Hkv * a.row_tiles);
-}
-
 __device__ __forceinline__ int sharers(const PagedAttnArgs& a, int64_t list) {
   return (int)min((int64_t)a.ctas, (list + kMinTiles - 1) / kMinTiles);
-}
-
-// Where the list's element x lies: sequence b and the element's number within the sequence.
-template <int THREADS>
-__device__ __forceinline__ void find(const PagedAttnArgs& a, int64_t x, int64_t* warp_sums, int64_t* found, int& b,
-                                     int64_t& within) {
-  int64_t carry = 0;
-  int len, fresh;
-  const int per = a.p.Hkv * a.row_tiles;
-  for (int base = 0; base < a.B; base += THREADS) {
-    const int mine = base + threadIdx.x;
-    const int64_t v = mine < a.B ? (int64_t)sequence(a, mine, len, fresh) * per : 0;
-    int64_t total;
-    const int64_t at = carry + scan_before<THREADS>(v, warp_sums, total);
-    if (x >= at && x < at + v) found[0] = mine, found[1] = x - at;
-    carry += total;
-    if (x < carry) break;
-  }
-  __syncthreads();
-  b = (int)found[0];
-  within = found[1];
 }
 
 // A place in the list.
@@ -110,6 +78,40 @@ struct Cursor {
   int b, unit, tile;        // sequence, kv head * row_tiles + row tile, key tile
   int tiles, len, fresh;    // of the sequence
 };
+
+// The CTA's stretch of the list: its first place, and its length (0: none; the call then returns at once, for all threads).
+// Ends with a barrier of the CTA.
+template <int THREADS>
+__device__ __forceinline__ int64_t locate(const PagedAttnArgs& a, int64_t* warp_sums, int64_t* found, Cursor& now) {
+  const int per = a.p.Hkv * a.row_tiles;
+  int len, fresh;
+  int64_t mine = 0, total;
+  for (int b = threadIdx.x; b < a.B; b += THREADS) mine += sequence(a, b, len, fresh);
+  int64_t at = scan_before<THREADS>(mine, warp_sums, total) * per;   // one sequence a thread: where it begins
+  const int64_t list = total * per;
+  const int share = sharers(a, list);
+  if ((int)blockIdx.x >= share) return 0;
+  const int64_t first = (int64_t)blockIdx.x * list / share, end = (int64_t)(blockIdx.x + 1) * list / share;
+  if (a.B <= THREADS) {
+    if (first >= at && first < at + mine * per) found[0] = threadIdx.x, found[1] = first - at;
+  } else {
+    int64_t carry = 0;
+    for (int base = 0; base < a.B; base += THREADS) {
+      const int b = base + threadIdx.x;
+      const int64_t v = b < a.B ? (int64_t)sequence(a, b, len, fresh) * per : 0;
+      at = carry + scan_before<THREADS>(v, warp_sums, total);
+      if (first >= at && first < at + v) found[0] = b, found[1] = first - at;
+      carry += total;
+      if (first < carry) break;
+    }
+  }
+  __syncthreads();
+  now.b = (int)found[0];
+  now.tiles = sequence(a, now.b, now.len, now.fresh);
+  now.unit = (int)((uint32_t)found[1] / (uint32_t)now.tiles);   // below tiles * per, checked to fit 32 bits
+  now.tile = (int)(found[1] - (int64_t)now.unit * now.tiles);
+  return end - first;
+}
 
 __device__ __forceinline__ void advance(const PagedAttnArgs& a, Cursor& c) {
   if (++c.tile < c.tiles) return;

@@ -154,25 +154,18 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  const int64_t list = list_length<W::kThreads>(a, warp_sums);
-  const int share = sharers(a, list);
-  if ((int)blockIdx.x >= share) return;
   if (warp == 0) {
     tmem_alloc(&tmem_base, 512);
     tmem_relinquish();
   }
-  const int64_t first = (int64_t)blockIdx.x * list / share, end = (int64_t)(blockIdx.x + 1) * list / share;
   Cursor now;
-  {
-    int64_t within;
-    tc_fence_before();
-    find<W::kThreads>(a, first, warp_sums, found, now.b, within);   // ends with a barrier of the CTA
-    tc_fence_after();
-    now.tiles = sequence(a, now.b, now.len, now.fresh);
-    now.unit = (int)(within / now.tiles);
-    now.tile = (int)(within - (int64_t)now.unit * now.tiles);
+  tc_fence_before();
+  int64_t todo = locate<W::kThreads>(a, warp_sums, found, now);
+  tc_fence_after();
+  if (todo == 0) {   // no barrier since the allocation: the scan's lie behind it
+    if (warp == 0) tmem_dealloc(tmem_base, 512);
+    return;
   }
-  int64_t todo = end - first;
   const uint32_t tmem = tmem_base;
   // whether row tile t of the unit holds a live row
   auto active = [&](const Cursor& c, int t) { return c.unit % a.row_tiles * W::kRows + t * 128 < c.fresh * a.group; };
