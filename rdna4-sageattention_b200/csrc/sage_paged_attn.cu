@@ -611,8 +611,10 @@ static Shape row_tile(int64_t rows, int D) {
   return rows <= 16 ? Shape{2, 1} : rows <= 32 ? Shape{2, 2} : Shape{2, 4};
 }
 
-// From this many rows of a kv head on, the kernel for many rows.
-static bool wide(int64_t rows, int D) { return rows > (D == 256 ? 16 : 32); }
+// From which rows of a kv head on the kernel for many rows is taken.  Measured on B200, 8 sequences of 8190 keys, 8 kv heads
+// (D 256: 16), us, few / many: D 128: 32 rows 74 / 87, 36 rows 108 / 86, 256 rows 373 / 111; D 64: 64 rows 70 / 78, 96 rows
+// 123 / 79; D 96: 64 rows 87 / 91, 96 rows 155 / 92; D 256: 32 rows 230 / 239, 48 rows 437 / 245.
+static bool wide(int64_t rows, int D) { return rows > (D == 64 || D == 96 ? 64 : 32); }
 
 static int shared_ctas(int D, Shape s) { return sm_count() * (s.nr == 1 && D <= 128 ? 4 : D == 64 ? 3 : 2); }
 

@@ -21,9 +21,9 @@ struct Wide {
   static constexpr int QT = D == 256 ? 1 : 2;
   static constexpr int kSoftmaxWarps = 4 * QT, kConverters = 4;
   // QT 2: 16 warps (one idle), so that the two warpgroups of the other roles hand registers to the two of softmax: 512
-  // threads of 128 at launch, then 256 of 152 and 256 of 104
+  // threads of 128 at launch, then 256 of 176 and 256 of 80
   static constexpr int kThreads = QT == 2 ? 512 : 32 * (kSoftmaxWarps + 1 + QT + kConverters);
-  static constexpr int kLaunchRegs = 128, kSoftmaxRegs = 152, kOtherRegs = 104;
+  static constexpr int kLaunchRegs = 128, kSoftmaxRegs = 176, kOtherRegs = 80;
   static_assert(QT != 2 || 256 * (kSoftmaxRegs + kOtherRegs) <= 512 * kLaunchRegs, "register split");
   static constexpr int kRows = 128 * QT;
   static constexpr int kPanels = (D + 63) / 64;            // of 64 channels: 128 bytes a key
@@ -42,14 +42,17 @@ struct Wide {
   static_assert(kSmem <= 227 * 1024, "shared memory");
 };
 
-// D(tmem) (+)= A(tmem) * B(smem), fp16 operands, fp32 accumulator.
+// D(tmem) (+)= A(tmem) * B(smem), fp16 operands, fp32 accumulator.  The whole warp calls; one lane, always the same, issues.
+// (With a branch to one lane around the loop the addresses are moved to uniform registers one by one: 87 us for 8 x 64 rows
+// over 8190 keys, D 128, 80 us this way.)
 __device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
                                            uint32_t accumulate) {
   asm volatile(
       "{\n"
-      ".reg .pred p;\n"
+      ".reg .pred p, e;\n"
+      "elect.sync _|e, 0xffffffff;\n"
       "setp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
       "}\n" ::"r"(d_tmem),
       "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
@@ -60,9 +63,10 @@ __device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uin
                                            uint32_t accumulate) {
   asm volatile(
       "{\n"
-      ".reg .pred p;\n"
+      ".reg .pred p, e;\n"
+      "elect.sync _|e, 0xffffffff;\n"
       "setp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
       "}\n" ::"r"(d_tmem),
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
@@ -93,6 +97,17 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
 // Bit i: byte i of the word is not zero.
 __device__ __forceinline__ uint32_t nonzero_bytes(uint32_t w) {
   return ((__vcmpne4(w, 0) & 0x01010101u) * 0x10204080u) >> 28;
+}
+
+// tc_commit of the lane that issues.
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  asm volatile(
+      "{\n"
+      ".reg .pred e;\n"
+      "elect.sync _|e, 0xffffffff;\n"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n"
+      "}\n" ::"r"(smem_u32(bar))
+      : "memory");
 }
 
 // Instruction descriptor, kind::f16: fp16 A and B, fp32 D; b_mn: B is stored with N contiguous.
@@ -176,74 +191,72 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
   } else if (warp > W::kSoftmaxWarps && warp <= W::kSoftmaxWarps + QT) {
     // ------------------------------------------------------------------------------------------------ products
     if constexpr (QT == 2) regs_decrease<W::kOtherRegs>();
-    if (lane == 0) {
-      constexpr uint32_t kScores = idesc_f16(128, kTileKeys, false), kValues = idesc_f16(128, D, true);
-      const int t = warp - W::kSoftmaxWarps - 1;
-      const uint64_t k_desc = smem_desc_kmajor(smem_u32(operands), 128);
-      const uint64_t v_desc = smem_desc_nmajor(smem_u32(operands) + W::kOperand, W::kPanel);
-      const uint64_t q_desc = smem_desc_kmajor(smem_u32(queries) + t * W::kQTile, 128);
-      const uint32_t s_at = tmem + W::kS + t * 2 * kTileKeys, q_at = tmem + W::kQ + t * (D / 2), o_at = tmem + W::kO + t * D;
-      int buf = 0;               // of the tile whose values are next, and of the one whose scores are next
-      int ahead = 0;
-      uint32_t phase = 0, ahead_phase = 0, p_phase = 0, q_phase = 0;   // p_phase: a bit per score tile
-      // scores of the next tile into score tile i
-      auto scores = [&](int i) {
-        wait_stage(k_full + ahead, ahead_phase, &given_up, a.p.status);
-        tc_fence_after();
-        const uint64_t k = k_desc + ahead * (2 * W::kOperand / 16);
+    constexpr uint32_t kScores = idesc_f16(128, kTileKeys, false), kValues = idesc_f16(128, D, true);
+    const int t = __shfl_sync(0xffffffffu, warp - W::kSoftmaxWarps - 1, 0);
+    const uint64_t k_desc = smem_desc_kmajor(smem_u32(operands), 128);
+    const uint64_t v_desc = smem_desc_nmajor(smem_u32(operands) + W::kOperand, W::kPanel);
+    const uint64_t q_desc = smem_desc_kmajor(smem_u32(queries) + t * W::kQTile, 128);
+    const uint32_t s_at = tmem + W::kS + t * 2 * kTileKeys, q_at = tmem + W::kQ + t * (D / 2), o_at = tmem + W::kO + t * D;
+    int buf = 0;               // of the tile whose values are next, and of the one whose scores are next
+    int ahead = 0;
+    uint32_t phase = 0, ahead_phase = 0, p_phase = 0, q_phase = 0;   // p_phase: a bit per score tile
+    // scores of the next tile into score tile i
+    auto scores = [&](int i) {
+      wait_stage(k_full + ahead, ahead_phase, &given_up, a.p.status);
+      tc_fence_after();
+      const uint64_t k = k_desc + ahead * (2 * W::kOperand / 16);
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s) {
-          const uint64_t ks = k + (s / 4 * W::kPanel + s % 4 * 32) / 16;
-          if constexpr (W::kQShared)
-            mma_f16_ss(s_at + i * kTileKeys, q_desc + (s / 4 * W::kQPanel + s % 4 * 32) / 16, ks, kScores, s > 0);
-          else
-            mma_f16_ts(s_at + i * kTileKeys, q_at + s * 8, ks, kScores, s > 0);
-        }
-        tc_commit(s_full[t] + i);
-      };
-      auto next = [](int& b, uint32_t& p) {
-        if (++b == W::kBufs) b = 0, p ^= 1;
-      };
-      while (todo > 0) {
-        const int tiles = (int)min((int64_t)(now.tiles - now.tile), todo);
-        if (active(now, t)) {
-          wait_stage(q_full + t, q_phase, &given_up, a.p.status);
-          q_phase ^= 1;
-          scores(0), next(ahead, ahead_phase);
-          if (tiles > 1) scores(1), next(ahead, ahead_phase);
-#pragma unroll 1
-          for (int j = 0; j < tiles; ++j) {
-            const int i = j & 1;
-            wait_stage(v_full + buf, phase, &given_up, a.p.status);
-            wait_stage(p_full[t] + i, p_phase >> i & 1, &given_up, a.p.status);
-            p_phase ^= 1u << i;
-            tc_fence_after();
-            const uint64_t v = v_desc + buf * (2 * W::kOperand / 16);
-#pragma unroll
-            for (int s = 0; s < kTileKeys / 16; ++s)
-              mma_f16_ts(o_at, s_at + i * kTileKeys + s * 8, v + s * (2048 / 16), kValues, j > 0 || s > 0);
-            tc_commit(pv_done + t);
-            tc_commit(buf_empty + buf);
-            next(buf, phase);
-            if (j + 2 < tiles) scores(i), next(ahead, ahead_phase);
-          }
-          tc_commit(o_full + t);
-        } else {   // no row of this row tile is live
-#pragma unroll 1
-          for (int j = 0; j < tiles; ++j) {
-            wait_stage(v_full + buf, phase, &given_up, a.p.status);
-            arrive(buf_empty + buf);
-            next(buf, phase);
-          }
-          ahead = buf, ahead_phase = phase;
-        }
-        todo -= tiles;
-        now.tile += tiles - 1;
-        if (todo > 0) advance(a, now);
+      for (int s = 0; s < D / 16; ++s) {
+        const uint64_t ks = k + (s / 4 * W::kPanel + s % 4 * 32) / 16;
+        if constexpr (W::kQShared)
+          mma_f16_ss(s_at + i * kTileKeys, q_desc + (s / 4 * W::kQPanel + s % 4 * 32) / 16, ks, kScores, s > 0);
+        else
+          mma_f16_ts(s_at + i * kTileKeys, q_at + s * 8, ks, kScores, s > 0);
       }
-      tc_commit(all_done + t);   // nothing is in flight when the CTA ends
-      wait_stage(all_done + t, 0, &given_up, a.p.status);
+      commit(s_full[t] + i);
+    };
+    auto next = [](int& b, uint32_t& p) {
+      if (++b == W::kBufs) b = 0, p ^= 1;
+    };
+    while (todo > 0) {
+      const int tiles = __shfl_sync(0xffffffffu, (int)min((int64_t)(now.tiles - now.tile), todo), 0);   // known to be uniform
+      if (active(now, t)) {
+        wait_stage(q_full + t, q_phase, &given_up, a.p.status);
+        q_phase ^= 1;
+        scores(0), next(ahead, ahead_phase);
+        if (tiles > 1) scores(1), next(ahead, ahead_phase);
+#pragma unroll 1
+        for (int j = 0; j < tiles; ++j) {
+          const int i = j & 1;
+          wait_stage(v_full + buf, phase, &given_up, a.p.status);
+          wait_stage(p_full[t] + i, p_phase >> i & 1, &given_up, a.p.status);
+          p_phase ^= 1u << i;
+          tc_fence_after();
+          const uint64_t v = v_desc + buf * (2 * W::kOperand / 16);
+#pragma unroll
+          for (int s = 0; s < kTileKeys / 16; ++s)
+            mma_f16_ts(o_at, s_at + i * kTileKeys + s * 8, v + s * (2048 / 16), kValues, j > 0 || s > 0);
+          commit(pv_done + t);
+          commit(buf_empty + buf);
+          next(buf, phase);
+          if (j + 2 < tiles) scores(i), next(ahead, ahead_phase);
+        }
+        commit(o_full + t);
+      } else {   // no row of this row tile is live
+#pragma unroll 1
+        for (int j = 0; j < tiles; ++j) {
+          wait_stage(v_full + buf, phase, &given_up, a.p.status);
+          if (lane == 0) arrive(buf_empty + buf);
+          next(buf, phase);
+        }
+        ahead = buf, ahead_phase = phase;
+      }
+      todo -= tiles;
+      now.tile += tiles - 1;
+      if (todo > 0) advance(a, now);
     }
+    commit(all_done + t);   // nothing is in flight when the CTA ends
+    wait_stage(all_done + t, 0, &given_up, a.p.status);
     __syncwarp();
   } else if (warp > W::kSoftmaxWarps + QT + W::kConverters) {
     if constexpr (QT == 2) regs_decrease<W::kOtherRegs>();   // idle
@@ -256,9 +269,9 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
     // The eight lanes of a phase of a 16-byte access take four neighbouring chunks of a raw row and of the row that
     // differs in bits 0 and 2: different banks in the raw tile (bit 2) and in the operand tile (bit 0), whose rows are
     // twice as long.
-    constexpr int kItems = kTileKeys * (D / 16) / 128;
+    constexpr int kItems = kTileKeys * (D / 16) / (32 * W::kConverters);
     auto place = [&](int i, int& row, int& ch) {
-      const int item = ct + i * 128;
+      const int item = ct + i * 32 * W::kConverters;
       if constexpr (D == 96) {
         row = item / 6, ch = item % 6;
       } else {
