@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
       }
     }
     const bool last_tile = now.tile + 1 == now.tiles, ends = last_tile || todo == 1;
-    if (WK == 1 || !ends) {
+    if (!ends) {
       __syncwarp();
       if (lane == 0) arrive(empty + slot);
     }
@@ -353,102 +353,71 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
           l[r][e] += __shfl_xor_sync(0xffffffffu, l[r][e], 8);
           l[r][e] += __shfl_xor_sync(0xffffffffu, l[r][e], 16);
         }
-      if constexpr (WK > 1) {
-        // The warps of a row tile join through the stage that all of them have read by then, eight rows of each at a time:
-        // every warp leaves its part, every thread adds up eight channels of a row in the order of the warps.
-        auto consumers_sync = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
-        float* area = reinterpret_cast<float*>(stages + slot * S::kStage);   // [warp][8 rows][D]
-        static_assert(kWarps * 8 * D * 4 <= S::kStage, "the parts must fit a stage");
-        auto place = [](int row, int quad) {   // four channels; permuted against bank conflicts
-          return (row * (D / 4) + (quad ^ (row >> 1 & 3) ^ (S::kWide ? (quad >> 4 & 1) << 2 : 0))) * 4;
-        };
-        if (n == 0) {
-#pragma unroll
-          for (int r = 0; r < NR; ++r)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) join_ml[warp][8 * r + 2 * c + e] = make_float2(m[r][e], l[r][e]);
-        }
-        consumers_sync();
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-          if (r > 0) consumers_sync();
-#pragma unroll
-          for (int t = 0; t < NT; t += 2)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              *reinterpret_cast<float4*>(area + warp * (8 * D) + place(2 * c + e, S::channel(n, t, 0) / 4)) =
-                  make_float4(o[r][t][e], o[r][t][2 + e], o[r][t + 1][e], o[r][t + 1][2 + e]);
-          consumers_sync();
-#pragma unroll 1
-          for (int item = tid; item < WM * D; item += 32 * kWarps) {
-            const int of = item / (D / 8), g = of / 8, rr = of % 8, d = item % (D / 8) * 8;
-            float top = -3.402823466e38f, sum = 0.0f, x[8] = {};
-#pragma unroll
-            for (int w = 0; w < WK; ++w) top = fmaxf(top, join_ml[w * WM + g][8 * r + rr].x);
-#pragma unroll
-            for (int w = 0; w < WK; ++w) {
-              const float2 ml = join_ml[w * WM + g][8 * r + rr];
-              const float f = fast_exp2(ml.x - top);
-              sum = fmaf(f, ml.y, sum);
-              const float* from = area + (w * WM + g) * (8 * D);
-              const float4 u = *reinterpret_cast<const float4*>(from + place(rr, d / 4));
-              const float4 v = *reinterpret_cast<const float4*>(from + place(rr, d / 4 + 1));
-              x[0] = fmaf(f, u.x, x[0]), x[1] = fmaf(f, u.y, x[1]), x[2] = fmaf(f, u.z, x[2]), x[3] = fmaf(f, u.w, x[3]);
-              x[4] = fmaf(f, v.x, x[4]), x[5] = fmaf(f, v.y, x[5]), x[6] = fmaf(f, v.z, x[6]), x[7] = fmaf(f, v.w, x[7]);
-            }
-            const int in_tile = g * 8 * NR + 8 * r + rr, row = now.unit % a.row_tiles * C::kRows + in_tile;
-            const int token = row / a.group, head = head0 + row % a.group;
-            if (row >= a.T * a.group) continue;
-            if (whole) {
-              const bool seen = token < now.fresh && sum != 0.0f;
-              const float inverse = 1.0f / sum;
-#pragma unroll
-              for (int z = 0; z < 8; ++z) x[z] = seen ? x[z] * inverse : 0.0f;
-              store8(static_cast<T*>(a.out) + now.b * a.out_st.b + token * a.out_st.s + head * a.out_st.h + d, x);
-              if (a.lse != nullptr && d == 0)
-                a.lse[((int64_t)now.b * a.H + head) * a.T + token] =
-                    seen ? (top + log2f(sum)) * 0.69314718055994531f : -INFINITY;
-            } else {
-              float* to = a.part_o + (part + in_tile) * D + d;
-              *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
-              *reinterpret_cast<float4*>(to + 4) = make_float4(x[4], x[5], x[6], x[7]);
-              if (d == 0) a.part_ml[part + in_tile] = make_float2(top, sum);
-            }
-          }
-        }
-        fence_proxy_async_smem();   // before the stage's next load
-        __syncwarp();
-        if (lane == 0) arrive(empty + slot);
-      } else {
+      // The warps of a row tile join through the stage that all of them have read by then, eight rows of each at a time:
+      // every warp leaves its part, every thread adds up eight channels of a row in the order of the warps.
+      auto consumers_sync = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
+      float* area = reinterpret_cast<float*>(stages + slot * S::kStage);   // [warp][8 rows][D]
+      static_assert(kWarps * 8 * D * 4 <= S::kStage, "the parts must fit a stage");
+      auto place = [](int row, int quad) {   // four channels; permuted against bank conflicts
+        return (row * (D / 4) + (quad ^ (row >> 1 & 3) ^ (S::kWide ? (quad >> 4 & 1) << 2 : 0))) * 4;
+      };
+      if (n == 0) {
 #pragma unroll
         for (int r = 0; r < NR; ++r)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int row = row0 + 8 * r + 2 * c + e, token = row / a.group, head = head0 + row % a.group;
-            if (row >= a.T * a.group) continue;
-            const bool live = token < now.fresh;
-            if (whole) {
-              T* dst = static_cast<T*>(a.out) + now.b * a.out_st.b + token * a.out_st.s + head * a.out_st.h;
-              const float inverse = !live || l[r][e] == 0.0f ? 0.0f : 1.0f / l[r][e];
-#pragma unroll
-              for (int t = 0; t < NT; t += 2)
-                *reinterpret_cast<uint2*>(dst + S::channel(n, t, 0)) =
-                    live ? make_uint2(pack2(o[r][t][e] * inverse, o[r][t][2 + e] * inverse, T()),
-                                      pack2(o[r][t + 1][e] * inverse, o[r][t + 1][2 + e] * inverse, T()))
-                         : make_uint2(0, 0);
-              if (a.lse != nullptr && n == 0)
-                a.lse[((int64_t)now.b * a.H + head) * a.T + token] =
-                    !live || l[r][e] == 0.0f ? -INFINITY : (m[r][e] + log2f(l[r][e])) * 0.69314718055994531f;
-            } else {
-              const int64_t at = part + wm * 8 * NR + 8 * r + 2 * c + e;
-#pragma unroll
-              for (int t = 0; t < NT; t += 2)
-                *reinterpret_cast<float4*>(a.part_o + at * D + S::channel(n, t, 0)) =
-                    make_float4(o[r][t][e], o[r][t][2 + e], o[r][t + 1][e], o[r][t + 1][2 + e]);
-              if (n == 0) a.part_ml[at] = make_float2(m[r][e], l[r][e]);
-            }
-          }
+          for (int e = 0; e < 2; ++e) join_ml[warp][8 * r + 2 * c + e] = make_float2(m[r][e], l[r][e]);
       }
+      consumers_sync();
+#pragma unroll
+      for (int r = 0; r < NR; ++r) {
+        if (r > 0) consumers_sync();
+#pragma unroll
+        for (int t = 0; t < NT; t += 2)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            *reinterpret_cast<float4*>(area + warp * (8 * D) + place(2 * c + e, S::channel(n, t, 0) / 4)) =
+                make_float4(o[r][t][e], o[r][t][2 + e], o[r][t + 1][e], o[r][t + 1][2 + e]);
+        consumers_sync();
+#pragma unroll 1
+        for (int item = tid; item < WM * D; item += 32 * kWarps) {
+          const int of = item / (D / 8), g = of / 8, rr = of % 8, d = item % (D / 8) * 8;
+          float top = -3.402823466e38f, sum = 0.0f, x[8] = {};
+#pragma unroll
+          for (int w = 0; w < WK; ++w) top = fmaxf(top, join_ml[w * WM + g][8 * r + rr].x);
+#pragma unroll
+          for (int w = 0; w < WK; ++w) {
+            const float2 ml = join_ml[w * WM + g][8 * r + rr];
+            const float f = fast_exp2(ml.x - top);
+            sum = fmaf(f, ml.y, sum);
+            const float* from = area + (w * WM + g) * (8 * D);
+            const float4 u = *reinterpret_cast<const float4*>(from + place(rr, d / 4));
+            const float4 v = *reinterpret_cast<const float4*>(from + place(rr, d / 4 + 1));
+            x[0] = fmaf(f, u.x, x[0]), x[1] = fmaf(f, u.y, x[1]), x[2] = fmaf(f, u.z, x[2]), x[3] = fmaf(f, u.w, x[3]);
+            x[4] = fmaf(f, v.x, x[4]), x[5] = fmaf(f, v.y, x[5]), x[6] = fmaf(f, v.z, x[6]), x[7] = fmaf(f, v.w, x[7]);
+          }
+          const int in_tile = g * 8 * NR + 8 * r + rr, row = now.unit % a.row_tiles * C::kRows + in_tile;
+          const int token = row / a.group, head = head0 + row % a.group;
+          if (row >= a.T * a.group) continue;
+          if (whole) {
+            const bool seen = token < now.fresh && sum != 0.0f;
+            const float inverse = 1.0f / sum;
+#pragma unroll
+            for (int z = 0; z < 8; ++z) x[z] = seen ? x[z] * inverse : 0.0f;
+            store8(static_cast<T*>(a.out) + now.b * a.out_st.b + token * a.out_st.s + head * a.out_st.h + d, x);
+            if (a.lse != nullptr && d == 0)
+              a.lse[((int64_t)now.b * a.H + head) * a.T + token] =
+                  seen ? (top + log2f(sum)) * 0.69314718055994531f : -INFINITY;
+          } else {
+            float* to = a.part_o + (part + in_tile) * D + d;
+            *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<float4*>(to + 4) = make_float4(x[4], x[5], x[6], x[7]);
+            if (d == 0) a.part_ml[part + in_tile] = make_float2(top, sum);
+          }
+        }
+      }
+      fence_proxy_async_smem();   // before the stage's next load
+      __syncwarp();
+      if (lane == 0) arrive(empty + slot);
       ++segment;
       fresh_unit = true;
     }
@@ -599,22 +568,22 @@ __global__ void __launch_bounds__(kJoinThreads) wide_join_kernel(const PagedAttn
     a.lse[((int64_t)b * a.H + head) * a.T + token] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
 }
 
-// Row tiles: the smallest that hold the rows of a kv head, 64 rows (D 256: 32) at the most.  Columns come in eights, so a
-// single token of up to eight heads a group takes one column tile; two a warp share the converted codes, four do not fit
-// the registers, and D 256 has room for one.
+// The row tile that holds the rows of a kv head (32 at the most, D 256: 16; more go to the kernel for many rows).  Columns
+// come in eights, so a single token of up to eight heads a group takes one column tile; two a warp share the converted
+// codes, D 256 has registers for one.
 struct Shape {
   int nr, wm;
 };
 static Shape row_tile(int64_t rows, int D) {
   if (rows <= 8) return {1, 1};
-  if (D == 256) return rows <= 16 ? Shape{1, 2} : Shape{1, 4};
-  return rows <= 16 ? Shape{2, 1} : rows <= 32 ? Shape{2, 2} : Shape{2, 4};
+  if (D == 256) return {1, 2};
+  return {2, rows <= 16 ? 1 : 2};
 }
 
 // From which rows of a kv head on the kernel for many rows is taken.  Measured on B200, 8 sequences of 8190 keys, 8 kv heads
-// (D 256: 16), us, few / many: D 128: 32 rows 74 / 87, 36 rows 108 / 86, 256 rows 373 / 111; D 64: 64 rows 70 / 78, 96 rows
-// 123 / 79; D 96: 64 rows 87 / 91, 96 rows 155 / 92; D 256: 32 rows 230 / 239, 48 rows 437 / 245.
-static bool wide(int64_t rows, int D) { return rows > (D == 64 || D == 96 ? 64 : 32); }
+// (D 256: 16), us, few / many: D 128: 32 rows 74 / 79, 36 rows 108 / 78; D 64: 32 rows 46 / 66, 36 rows 70 / 67; D 96: 32 rows
+// 55 / 75, 36 rows 86 / 75; D 256: 16 rows 133 / 202, 17 rows 227 / 204.
+static bool wide(int64_t rows, int D) { return rows > (D == 256 ? 16 : 32); }
 
 static int shared_ctas(int D, Shape s) { return sm_count() * (s.nr == 1 && D <= 128 ? 4 : D == 64 ? 3 : 2); }
 
@@ -655,14 +624,11 @@ static int launch_join(const PagedAttnArgs& a, int tile_rows, bool many, cudaStr
 template <typename T, int D>
 static int launch_paged_attn(const PagedAttnArgs& a, Shape s, cudaStream_t st) {
   if constexpr (D == 256)
-    return s.wm == 1   ? launch_paged_attn<T, D, 1, 1>(a, st)
-           : s.wm == 2 ? launch_paged_attn<T, D, 1, 2>(a, st)
-                       : launch_paged_attn<T, D, 1, 4>(a, st);
+    return s.wm == 1 ? launch_paged_attn<T, D, 1, 1>(a, st) : launch_paged_attn<T, D, 1, 2>(a, st);
   else
     return s.nr == 1   ? launch_paged_attn<T, D, 1, 1>(a, st)
            : s.wm == 1 ? launch_paged_attn<T, D, 2, 1>(a, st)
-           : s.wm == 2 ? launch_paged_attn<T, D, 2, 2>(a, st)
-                       : launch_paged_attn<T, D, 2, 4>(a, st);
+                       : launch_paged_attn<T, D, 2, 2>(a, st);
 }
 
 }  // namespace sage
