@@ -325,7 +325,8 @@ int sage_selftest_counter_timeout(int* status, int* words, int limit_ms, void* s
  * device); returns the code it held (SAGE_OK when no kernel reported an error). */
 int sage_status_sync(int* status, void* stream);
 
-/* Debug builds (compiled with SAGE_DEBUG; libsage_b200_debug.so) check their own accesses on the device:
+/* Debug builds (compiled with SAGE_DEBUG; libsage_b200_debug.so) check their own accesses on the device (the dense
+ * attention kernels and the quantisers; the step calls check lengths, counts and pages in every build):
  * every global store of a kernel must land inside the buffers its launch was given, TMA copies must start on
  * a 16-byte column inside their tensor, and varlen offsets must stay inside the packed tensors.  A failed
  * check skips the access and records it; no check traps.  This reads and clears the first record of `unit`

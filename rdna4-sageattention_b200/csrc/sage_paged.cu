@@ -7,6 +7,10 @@
 // from one.  The product with 127 / a resp. 448 / a is off by less than 2^-21 (the reciprocal by 2^-23, three roundings by
 // 2^-24), so pushed outwards by 2^-21 it falls on the right side of every border, and no division per element is needed.
 // Rows with an infinity or NaN store scale NaN and codes 0; rows with a < 2^-100 store zeros.
+//
+// Measured on B200, 8 kv heads, D 128: append of 4 x 8190 tokens (ragged, 25 us at the measured copy rate) 41 us, bound by its
+// instructions; read of 8 x 32760 positions 240 us, 98 % of that rate (with 16 channels a thread, two stores half a line
+// apart, 304); keep of 12 rows of 256 sequences 6 us, a chain of dependent loads.
 #include "../../include/sage_b200.h"
 #include "sage_internal.h"
 #include "sage_paged.cuh"

@@ -22,6 +22,13 @@
 //
 // Both products are taken transposed, S^T = K Q^T and O^T = V^T P^T: keys and channels fill the 16 rows of an mma tile
 // and the query rows its 8 columns, so that the 1 to 8 rows of a single token's group cost one column tile.
+//
+// Bound by memory: one token (4 query rows a kv head) over 16 sequences of 16 to 32 thousand keys, 8 kv heads, D 128, takes
+// 145 to 156 us on B200, 85 to 92 % of the measured copy rate; issue slots are 57 % taken.  Steps on the way, us: one CTA a row
+// 11122; shared list, rows times keys, cp.async 257; transposed products, TMA 175; no logarithm and no comparison a key where
+// no maximum moves 156; warps joining all at once 145.  One token over 1024 keys takes 10.9 us with the join, most of it
+// start-up and dependent loads.  D 256 reaches 87 % of the rate for 8 rows and 63 % for 16, for which each key is converted
+// twice: two column tiles a warp do not fit the registers.
 #include "sage_paged_attn.cuh"
 
 namespace sage {

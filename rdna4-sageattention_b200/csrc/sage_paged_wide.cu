@@ -12,6 +12,11 @@
 // Codes convert exactly, so there is nothing to choose there.
 // TMEM (512 columns): O_t at t D, the score tiles of t at QT D + 128 t, P over the first half of its scores; Q_t behind
 // them where it fits (D 64 and 256), else in shared memory (D 96 and 128).
+//
+// 8 trees of 64 drafts (256 rows a kv head) over up to 8190 keys, 8 kv heads, D 128: 88 us on B200, 583 TFLOP/s, where the
+// few-rows kernel takes 373 (8190 keys each) against 107 here.  No unit is full: tensor pipe 27 %, issue 42 %.  A key tile
+// passes through conversion, scores, softmax and values in about 2000 cycles, and leaving out the exponentials, the loads of
+// what a key needs, or most of either product changes the time by less than 10 % each.
 #include "sage_paged_attn.cuh"
 
 namespace sage {

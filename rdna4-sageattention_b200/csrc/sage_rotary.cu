@@ -7,6 +7,9 @@
 // The angle is reduced in integers: a frequency is held in turns (w / 2 pi) as a 64-bit fixed-point fraction, so the
 // fraction of a turn at position p is the low 64 bits of p * turns, exact for any position (a product in 32-bit
 // floats is off by 0.06 radians at p = 10^6).  Its upper 32 bits go to sincospi.
+//
+// Bound by memory: 4 x 8192 tokens of 40 heads, D 128, take 114 us on B200, 5.9 TB/s or 90 % of the measured copy rate (with
+// one head under way at a time 245 us).
 #include <algorithm>
 
 #include "../../include/sage_b200.h"

@@ -319,6 +319,25 @@ def test_many_sequences():
     check_attention(queries(300, 2, 4, 64), cache, table, lens)
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_row_tiles_without_live_rows(D):
+    # 800 query rows of a kv head in several row tiles, some of which hold no token of a padded batch's short sequences
+    T, lens, counts = 200, [70, 1, 500, 0], [200, 3, 0, 64]
+    cache, table = filled(lens, T, 32, 2, D, seed=4)
+    q = queries(4, T, 8, D)
+    a, lse = check_attention(q, cache, table, lens, None, counts)
+    for b, n in enumerate(counts):
+        assert not bool(a[b, n:].any()) and bool((lse[b, :, n:] == -math.inf).all())
+    check_attention(q, cache, table, lens, trees(4, T), counts, layout="HND")
+
+
+@pytest.mark.parametrize("T", [1, 12])
+def test_more_sequences_than_threads(T):
+    lens = [(53 * i) % 97 for i in range(700)]
+    cache, table = filled(lens, T, 16, 1, 64)
+    check_attention(queries(700, T, 4, 64), cache, table, lens, trees(1, T)[0] if T > 1 else None)
+
+
 def test_offsets_past_32_bits():
     # a pool of 2^31 + codes a tensor: the sequences sit in its last and its first pages
     page, Hkv, D = 256, 8, 256
