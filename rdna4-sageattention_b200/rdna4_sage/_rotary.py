@@ -162,17 +162,45 @@ class _RotaryFunction(torch.autograd.Function):
         return dq, dk, None, None, None, None
 
 
+_MARK = "rdna4_sage capture"
+
+
+def _accumulator(x, stream):
+    """The node that adds up the gradient of leaf `x`, for a graph recorded while `stream` is captured.  A leaf has one
+    node, tied to the stream where the oldest graph alive made it; from another stream's, a captured backward pass would
+    wait for work outside the capture, which breaks the capture off.  Autograd does not tell a node's stream, but a mark
+    outlives the last reference held here only if another graph holds the node."""
+    edge = torch.autograd.graph.get_gradient_edge
+    node = edge(x).node
+    if node.metadata.get(_MARK) == stream:   # an earlier call of this capture
+        return node
+    node.metadata[_MARK] = stream
+    del node
+    node = edge(x).node
+    if _MARK in node.metadata:
+        del node.metadata[_MARK]
+        raise Unsupported("a graph of this leaf from outside the capture is alive, so its gradient cannot be captured: "
+                          "release that graph first (or pass a view of the leaf if it was recorded on this stream)")
+    node.metadata[_MARK] = stream
+    return node
+
+
 def rotary(q, k, positions, rope, tensor_layout="HND"):
     """q and k turned to their positions: (B, H, S, D) and (B, Hkv, S, D) for "HND", (B, S, H, D) and (B, S, Hkv, D) for
     "NHD", fp16 or bf16; new tensors of the same shapes and types (rounded once).  k may be None: the result is q
     alone.  positions: int32 or int64 of any value, (S,) for all sequences or (B, S), on the GPU.  rope: a Rotary.
-    Differentiable in q and k.  Raises Unsupported for inputs the kernel does not take."""
+    Differentiable in q and k.  A backward pass can be captured into a CUDA graph if no other graph of the same leaves is
+    alive then; a leaf q or k that breaks this is refused, leaves further back are the caller's.  Raises Unsupported for
+    inputs the kernel does not take."""
     _check(q, k, positions, rope, tensor_layout)
     if k is None:
         step(q, positions, rope.turns)
     else:
         step(q, k, positions, rope.turns)
     if (q.requires_grad or k is not None and k.requires_grad) and torch.is_grad_enabled():
+        if torch.cuda.is_current_stream_capturing():   # the nodes are held until the graph below holds them
+            at = torch.cuda.current_stream(q.device).cuda_stream
+            held = [_accumulator(x, at) for x in (q, k) if x is not None and x.requires_grad and x.is_leaf]  # noqa: F841
         return _RotaryFunction.apply(q, k, positions, rope, tensor_layout, False)
     q_out, k_out = _launch(q, k, positions, rope, tensor_layout, False)
     return q_out if k is None else (q_out, k_out)

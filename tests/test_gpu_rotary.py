@@ -156,3 +156,52 @@ def test_streams_graph_and_compile_free_use():
     hit = torch.zeros_like(q, dtype=torch.bool)
     hit[0, 0, 3, 5] = hit[0, 0, 3, 5 + 48] = True
     assert torch.equal(y[~hit], want[0][~hit]) and not bool(torch.isfinite(y[hit]).any())
+
+
+def leaves(seed=3):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q, k = (torch.randn(2, 5, h, 128, device="cuda", generator=g).bfloat16() for h in (8, 2))
+    dq, dk = (torch.randn(2, 5, h, 128, device="cuda", generator=g).bfloat16() for h in (8, 2))
+    return q.requires_grad_(), k.requires_grad_(), dq, dk, torch.arange(5, device="cuda"), rdna4_sage.Rotary(128)
+
+
+def test_captured_gradient():
+    """Two calls on the same leaves in one capture, replayed with other gradients and positions."""
+    q, k, dq, dk, pos, rope = leaves()
+
+    def run():
+        a, b = rdna4_sage.rotary(q, k, pos, rope, "NHD")
+        c = rdna4_sage.rotary(q, None, pos, rope, "NHD")
+        return torch.autograd.grad((a, b, c), (q, k), (dq, dk, dq))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for turn in range(3):
+        dq.mul_(-0.5)
+        pos.add_(100 * turn)
+        graph.replay()
+        want = run()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_captured_gradient_of_a_leaf_in_another_graph_is_refused():
+    q, k, dq, dk, pos, rope = leaves()
+    alive = rdna4_sage.rotary(q, k, pos, rope, "NHD")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x = torch.zeros_like(dq)
+        with pytest.raises(rdna4_sage.Unsupported, match="outside the capture"):
+            rdna4_sage.rotary(q, k, pos, rope, "NHD")
+        with torch.no_grad():
+            y = rdna4_sage.rotary(q, k, pos, rope, "NHD")   # without a gradient there is nothing to refuse
+    graph.replay()
+    assert torch.equal(y[0], alive[0]) and torch.equal(y[1], alive[1]) and not bool(x.any())
+    got = torch.autograd.grad(alive, (q, k), (dq, dk))        # the graph that was alive still answers
+    want = torch.autograd.grad(rdna4_sage.rotary(q, k, pos, rope, "NHD"), (q, k), (dq, dk))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])

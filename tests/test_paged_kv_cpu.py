@@ -210,3 +210,23 @@ def test_reference_codes_by_hand():
     c, _ = P.codes(torch.tensor([[448.0, 17.0, -17.0, 0.0009765625]]), 448)
     assert c[0].tolist() == [448, 18, -18, 0.001953125]     # 17 lies between 16 and 18; 2^-10 between 0 and 2^-9
     assert ctypes.sizeof(ctypes.c_int) == 4
+
+
+def test_a_leaf_of_an_older_graph_is_told_from_a_free_one():
+    """The check of a captured gradient, which needs no GPU: `stream` is only compared."""
+    from rdna4_sage import _rotary
+    x = torch.randn(3, requires_grad=True)
+    node = _rotary._accumulator(x, 7)                  # free
+    assert _rotary._accumulator(x, 7) is node          # again in the same capture
+    with pytest.raises(rdna4_sage.Unsupported, match="outside the capture"):
+        _rotary._accumulator(x, 8)
+    del node
+    _rotary._accumulator(x, 8)
+    y = x * 2
+    for _ in range(2):                                 # a refusal leaves no mark that would let the next call through
+        with pytest.raises(rdna4_sage.Unsupported, match="outside the capture"):
+            _rotary._accumulator(x, 7)
+    y.sum().backward()
+    assert torch.equal(x.grad, torch.full_like(x, 2.0))
+    del y
+    _rotary._accumulator(x, 7)
