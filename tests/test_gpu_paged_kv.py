@@ -533,3 +533,36 @@ def test_empty_batches():
     rdna4_sage.paged_kv_append(kv, q[:, :, :2], q[:, :, :2], table, ints([10]), tensor_layout="NHD")
     assert rdna4_sage.paged_kv_read(kv, table, ints([10]), 0)[0].shape == (1, 2, 0, 64)
     rdna4_sage.paged_kv_keep(kv, table, ints([10]), torch.zeros((1, 0), dtype=torch.int32, device=DEV))
+
+
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+@pytest.mark.parametrize("T", [2, 17])                                  # 8 and 68 rows of a kv head
+def test_every_page_size(D, page, T):
+    lens = [page - 1, 2 * page, 5]
+    cache, table = filled(lens, T, page, 2, D, seed=page + T)
+    check_attention(queries(3, T, 8, D, seed=T), cache, table, lens, trees(3, T), [T, T - 1, 1])
+
+
+@pytest.mark.parametrize("T", [3, 40])
+@pytest.mark.parametrize("layout", ["NHD", "HND"])
+def test_views_of_a_projection_bytes_of_v_and_shared_pages(T, layout):
+    """q, k and v as views of one tensor, both aligned and not, and one that all heads share; V's codes as bytes; two
+    sequences whose context lies in the same pages."""
+    H, Hkv, D, page, lens = 8, 2, 128, 16, [32, 32]
+    cache, table = filled(lens, T, page, Hkv, D, seed=T)
+    table[1, :2] = table[0, :2]
+    g = torch.Generator(device=DEV).manual_seed(T)
+    for pad in (0, 8, 3):                                               # channels in front of q
+        x = torch.randn((2, T, pad + (H + 2 * Hkv) * D), device=DEV, generator=g).bfloat16()
+        q, k, v = (t.unflatten(-1, (-1, D)) for t in x[..., pad:].split([H * D, Hkv * D, Hkv * D], -1))
+        k = k[:, :, :1].expand(-1, -1, Hkv, -1)
+        want = {n: t.clone() for n, t in cache.items()}
+        P.append(want, k, v, table, lens)
+        turn = (lambda t: t.transpose(1, 2)) if layout == "HND" else (lambda t: t)
+        kv = rdna4_sage.PagedKV(cache["k8"], cache["ks"], cache["v8"].view(torch.uint8), cache["vs"])
+        rdna4_sage.paged_kv_append(kv, turn(k), turn(v), table, ints(lens), tensor_layout=layout)
+        same_cache(cache, want)
+        plain, _ = check_attention(q.contiguous(), cache, table, lens)
+        got = rdna4_sage.attention_paged_kv(turn(q), kv, table, ints(lens), tensor_layout=layout)
+        assert torch.equal(turn(got).double(), plain)
