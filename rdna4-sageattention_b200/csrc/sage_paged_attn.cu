@@ -59,7 +59,9 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
   constexpr int WK = kWarps / WM, NS = D / 16, NT = D / 16, kStages = C::kStages;
   extern __shared__ unsigned char smem_raw[];
   __shared__ int64_t warp_sums[kThreads / 32], found[2];
-  __shared__ float2 join_ml[kWarps][8 * NR];
+  // of two row tiles, in turns: a warp may write its part of the next row tile while a slower one still reads this one's; it
+  // comes to the one after only through that row tile's barriers, which the slower one has to reach as well
+  __shared__ float2 join_ml[2][kWarps][8 * NR];
   __shared__ int given_up;
   unsigned char* stages = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   float* scales = reinterpret_cast<float*>(stages + kStages * S::kStage);               // [stage][ks, vs][64]
@@ -95,7 +97,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
   uint32_t qf[NR][NS][2];
   float o[NR][NT][4], m[NR][2], l[NR][2], row_scale[NR][2];
   bool fresh_unit = true;
-  int segment = 0;                    // 0 for the first row tile that this CTA works on
+  int segment = 0;                    // row tiles that this CTA has finished
   int first_tile = now.tile;          // of the row tile, by this CTA
   int row0 = 0, head0 = 0;            // first query row of this warp, first query head of the kv head
   for (; todo > 0; --todo) {
@@ -368,11 +370,12 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
       auto place = [](int row, int quad) {   // four channels; permuted against bank conflicts
         return (row * (D / 4) + (quad ^ (row >> 1 & 3) ^ (S::kWide ? (quad >> 4 & 1) << 2 : 0))) * 4;
       };
+      float2 (*parts)[8 * NR] = join_ml[segment & 1];
       if (n == 0) {
 #pragma unroll
         for (int r = 0; r < NR; ++r)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) join_ml[warp][8 * r + 2 * c + e] = make_float2(m[r][e], l[r][e]);
+          for (int e = 0; e < 2; ++e) parts[warp][8 * r + 2 * c + e] = make_float2(m[r][e], l[r][e]);
       }
       consumers_sync();
 #pragma unroll
@@ -390,10 +393,10 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
           const int of = item / (D / 8), g = of / 8, rr = of % 8, d = item % (D / 8) * 8;
           float top = -3.402823466e38f, sum = 0.0f, x[8] = {};
 #pragma unroll
-          for (int w = 0; w < WK; ++w) top = fmaxf(top, join_ml[w * WM + g][8 * r + rr].x);
+          for (int w = 0; w < WK; ++w) top = fmaxf(top, parts[w * WM + g][8 * r + rr].x);
 #pragma unroll
           for (int w = 0; w < WK; ++w) {
-            const float2 ml = join_ml[w * WM + g][8 * r + rr];
+            const float2 ml = parts[w * WM + g][8 * r + rr];
             const float f = fast_exp2(ml.x - top);
             sum = fmaf(f, ml.y, sum);
             const float* from = area + (w * WM + g) * (8 * D);

@@ -566,3 +566,18 @@ def test_views_of_a_projection_bytes_of_v_and_shared_pages(T, layout):
         plain, _ = check_attention(q.contiguous(), cache, table, lens)
         got = rdna4_sage.attention_paged_kv(turn(q), kv, table, ints(lens), tensor_layout=layout)
         assert torch.equal(turn(got).double(), plain)
+
+
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+@pytest.mark.parametrize("T,H", [(1, 4), (2, 8), (4, 8), (8, 16)])      # 2, 8, 16 and 64 rows of a kv head
+def test_row_tiles_of_one_key_tile(D, T, H):
+    """A CTA walks many row tiles that end with the key tile they begin with: the parts of one must not be overtaken by
+    the next one's.  Every run gives the same bits."""
+    lens = [(29 * i) % (63 - T) for i in range(400)]
+    cache, table = filled(lens, T, 16, 2, D, seed=D)
+    q = queries(400, T, H, D, seed=T)
+    want, lse = check_attention(q, cache, table, lens)
+    kv, at = handle(cache), ints(lens)
+    for _ in range(30):
+        o, l2 = rdna4_sage.attention_paged_kv(q, kv, table, at, tensor_layout="NHD", return_lse=True)
+        assert torch.equal(o.double(), want) and torch.equal(l2, lse)
