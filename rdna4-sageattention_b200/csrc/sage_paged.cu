@@ -62,7 +62,7 @@ struct AppendArgs {
   const void* x[2];   // K, V
   Strides3 st[2];
   const int* counts;
-  int B, S;
+  int S;
 };
 
 // A group of LPR lanes (a power of two, D / 8 of them with data) holds kTokens consecutive tokens of one head of K and of V,
@@ -142,7 +142,7 @@ struct ReadArgs {
   PagedArgs p;
   void* out[2];
   Strides3 st[2];
-  int B, S;
+  int S;
 };
 
 // A thread reads 8 codes of kRun consecutive tokens (a run never leaves its page) of K and of V, all of them under way at
@@ -274,7 +274,7 @@ int sage_paged_append(const sage_paged_rows_args* args, void* stream) {
   a.x[0] = args->k, a.x[1] = args->v;
   a.st[0] = strides3(args->k_st), a.st[1] = strides3(args->v_st);
   a.counts = args->kv.counts;
-  a.B = B, a.S = S;
+  a.S = S;
   const int per_block = 256 / (D == 64 ? 8 : D == 256 ? 32 : 16);
   const int64_t blocks = ((int64_t)((S + kTokens - 1) / kTokens) * Hkv + per_block - 1) / per_block;
   if (blocks > (1 << 23) || B > 65535) {   // 32-bit thread numbers, grid limit
@@ -300,7 +300,7 @@ int sage_paged_read(const sage_paged_rows_args* args, void* stream) {
   const int B = args->kv.B, S = args->S, Hkv = args->kv.Hkv, D = args->kv.D, dtype = args->dtype;
   a.out[0] = args->k, a.out[1] = args->v;
   a.st[0] = strides3(args->k_st), a.st[1] = strides3(args->v_st);
-  a.B = B, a.S = S;
+  a.S = S;
   const int64_t blocks = ((int64_t)((S + kRun - 1) / kRun) * Hkv * (D / 8) + 255) / 256;
   if (blocks > (1 << 23) || B > 65535) {   // 32-bit thread numbers, grid limit
     set_error("read: %d sequences of %d tokens and %d heads are too many for one call", B, S, Hkv);

@@ -49,7 +49,8 @@ struct Config {
   static_assert(kStages >= 2, "two stages at the least");
 };
 
-// A row tile has 8 NR WM rows: WM groups of 4 / WM warps that share its keys, NR column tiles of 8 rows a warp.
+// The rows of a kv head are one row tile of 8 NR WM rows: WM groups of 4 / WM warps that share its keys, NR column tiles of 8
+// rows a warp.
 template <typename T, int D, int NR, int WM>
 __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
     paged_attn_kernel(const PagedAttnArgs a, const __grid_constant__ CUtensorMap k_map,
@@ -99,11 +100,11 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
   bool fresh_unit = true;
   int segment = 0;                    // row tiles that this CTA has finished
   int first_tile = now.tile;          // of the row tile, by this CTA
-  int row0 = 0, head0 = 0;            // first query row of this warp, first query head of the kv head
+  const int row0 = wm * 8 * NR;       // first query row of this warp
+  int head0 = 0;                      // first query head of the kv head
   for (; todo > 0; --todo) {
     if (fresh_unit) {
-      row0 = now.unit % a.row_tiles * C::kRows + wm * 8 * NR;
-      head0 = now.unit / a.row_tiles * a.group;
+      head0 = now.unit * a.group;
       fresh_unit = false;
       first_tile = now.tile;
 #pragma unroll
@@ -405,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
             x[0] = fmaf(f, u.x, x[0]), x[1] = fmaf(f, u.y, x[1]), x[2] = fmaf(f, u.z, x[2]), x[3] = fmaf(f, u.w, x[3]);
             x[4] = fmaf(f, v.x, x[4]), x[5] = fmaf(f, v.y, x[5]), x[6] = fmaf(f, v.z, x[6]), x[7] = fmaf(f, v.w, x[7]);
           }
-          const int in_tile = g * 8 * NR + 8 * r + rr, row = now.unit % a.row_tiles * C::kRows + in_tile;
+          const int row = g * 8 * NR + 8 * r + rr;
           const int token = row / a.group, head = head0 + row % a.group;
           if (row >= a.T * a.group) continue;
           if (whole) {
@@ -418,10 +419,10 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
               a.lse[((int64_t)now.b * a.H + head) * a.T + token] =
                   seen ? (top + log2f(sum)) * 0.69314718055994531f : -INFINITY;
           } else {
-            float* to = a.part_o + (part + in_tile) * D + d;
+            float* to = a.part_o + (part + row) * D + d;
             *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
             *reinterpret_cast<float4*>(to + 4) = make_float4(x[4], x[5], x[6], x[7]);
-            if (d == 0) a.part_ml[part + in_tile] = make_float2(top, sum);
+            if (d == 0) a.part_ml[part + row] = make_float2(top, sum);
           }
         }
       }
@@ -476,59 +477,69 @@ __device__ __forceinline__ int sharing(const PagedAttnArgs& a, int b, int unit, 
 // Joins the partial rows of the row tiles that fell to several CTAs, and writes the rows that see nothing at all; the CTAs
 // of a row tile are joined in the order of its keys.  A warp takes a row.
 template <typename T, int D>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedAttnArgs a, int tile_rows, int blocks_per_unit) {
+__global__ void __launch_bounds__(kJoinThreads, 8) paged_join_kernel(const PagedAttnArgs a, int tile_rows, int blocks_per_unit) {
   __shared__ int64_t warp_sums[2 * kJoinThreads / 32];
   const int64_t id = blockIdx.x / blocks_per_unit;
-  const int per = a.p.Hkv * a.row_tiles, b = (int)(id / per), unit = (int)(id - (int64_t)b * per);
+  const int b = (int)(id / a.p.Hkv), unit = (int)(id - (int64_t)b * a.p.Hkv);   // a row tile holds all rows of a kv head
   int fresh, c0, c1, slot;
   const int tiles = sharing(a, b, unit, warp_sums, fresh, c0, c1, slot);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (tiles > 0 && c0 == c1) return;   // the CTA wrote the rows itself
   const int lane = threadIdx.x % 32;
-  for (int row = blockIdx.x % blocks_per_unit * (kJoinThreads / 32) + threadIdx.x / 32; row < tile_rows;
-       row += blocks_per_unit * (kJoinThreads / 32)) {
-    const int r = unit % a.row_tiles * tile_rows + row;
-    if (r >= a.T * a.group) break;
-    const int token = r / a.group, head = unit / a.row_tiles * a.group + r % a.group;
-    const bool live = tiles > 0 && token < fresh;
-    float top = -3.402823466e38f, sum = 0.0f, o[D / 32];
+  const int row = blockIdx.x % blocks_per_unit * (kJoinThreads / 32) + threadIdx.x / 32;
+  if (row >= a.T * a.group) return;
+  const int token = row / a.group, head = unit * a.group + row % a.group;
+  const bool live = tiles > 0 && token < fresh;
+  float top = -3.402823466e38f, sum = 0.0f, o[D / 32];
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) o[i] = 0.0f;
-    if (live) {
-      for (int x = c0 + lane; x <= c1; x += 32)
-        top = fmaxf(top, a.part_ml[(2 * (int64_t)x + (x == c0 ? slot : 0)) * tile_rows + row].x);
+  for (int i = 0; i < D / 32; ++i) o[i] = 0.0f;
+  if (live) {
+    for (int x = c0 + lane; x <= c1; x += 32)
+      top = fmaxf(top, a.part_ml[(2 * (int64_t)x + (x == c0 ? slot : 0)) * tile_rows + row].x);
 #pragma unroll
-      for (int x = 16; x > 0; x /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-#pragma unroll 4
-      for (int x = c0; x <= c1; ++x) {
+    for (int x = 16; x > 0; x /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    constexpr int kAtOnce = 4;   // parts under way at once: the loads are what this kernel waits for
+#pragma unroll 1
+    for (int x0 = c0; x0 <= c1; x0 += kAtOnce) {
+      float2 ml[kAtOnce];
+      float v[kAtOnce][D / 32];
+#pragma unroll
+      for (int z = 0; z < kAtOnce; ++z) {
+        const int x = min(x0 + z, c1);   // the last one again, left out below
         const int64_t at = (2 * (int64_t)x + (x == c0 ? slot : 0)) * tile_rows + row;
-        const float2 ml = a.part_ml[at];
-        const float f = fast_exp2(ml.x - top);
-        sum = fmaf(f, ml.y, sum);
+        ml[z] = a.part_ml[at];
 #pragma unroll
         for (int i = 0; i < D / 32; i += D % 64 ? 1 : 2) {
           if constexpr (D % 64 == 0) {
-            const float2 v = *reinterpret_cast<const float2*>(a.part_o + at * D + i * 32 + lane * 2);
-            o[i] = fmaf(f, v.x, o[i]), o[i + 1] = fmaf(f, v.y, o[i + 1]);
+            const float2 w = *reinterpret_cast<const float2*>(a.part_o + at * D + i * 32 + lane * 2);
+            v[z][i] = w.x, v[z][i + 1] = w.y;
           } else {
-            o[i] = fmaf(f, a.part_o[at * D + i * 32 + lane], o[i]);
+            v[z][i] = a.part_o[at * D + i * 32 + lane];
           }
         }
       }
-    }
-    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-    T* dst = static_cast<T*>(a.out) + b * a.out_st.b + token * a.out_st.s + head * a.out_st.h;
 #pragma unroll
-    for (int i = 0; i < D / 32; i += D % 64 ? 1 : 2) {
-      if constexpr (D % 64 == 0)
-        *reinterpret_cast<uint32_t*>(dst + i * 32 + lane * 2) = pack2(o[i] * inverse, o[i + 1] * inverse, T());
-      else
-        dst[i * 32 + lane] = T(o[i] * inverse);
+      for (int z = 0; z < kAtOnce; ++z) {
+        if (x0 + z > c1) break;
+        const float f = fast_exp2(ml[z].x - top);
+        sum = fmaf(f, ml[z].y, sum);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) o[i] = fmaf(f, v[z][i], o[i]);
+      }
     }
-    if (a.lse != nullptr && lane == 0)
-      a.lse[((int64_t)b * a.H + head) * a.T + token] =
-          sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
   }
+  const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+  T* dst = static_cast<T*>(a.out) + b * a.out_st.b + token * a.out_st.s + head * a.out_st.h;
+#pragma unroll
+  for (int i = 0; i < D / 32; i += D % 64 ? 1 : 2) {
+    if constexpr (D % 64 == 0)
+      *reinterpret_cast<uint32_t*>(dst + i * 32 + lane * 2) = pack2(o[i] * inverse, o[i + 1] * inverse, T());
+    else
+      dst[i * 32 + lane] = T(o[i] * inverse);
+  }
+  if (a.lse != nullptr && lane == 0)
+    a.lse[((int64_t)b * a.H + head) * a.T + token] =
+        sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
 }
 
 // The same for the partial rows of the kernel for many rows (four channels of all rows, then the next four): a block takes
@@ -699,6 +710,10 @@ extern "C" int sage_paged_attention(const sage_paged_attention_args* args, void*
   const Shape shape = row_tile((int64_t)T * a.group, D);
   const int tile_rows = many ? wide_rows(D) : 8 * shape.nr * shape.wm;
   a.row_tiles = (T * a.group + tile_rows - 1) / tile_rows;
+  if (!many && a.row_tiles != 1) {   // its kernel holds all rows of a kv head
+    set_error("paged attention: %d rows in tiles of %d", T * a.group, tile_rows);
+    return SAGE_ERR_UNSUPPORTED;
+  }
   if (((int64_t)kv.max_pages * kv.page_size / kTileKeys + 1) * a.row_tiles * Hkv > (int64_t)UINT_MAX) {
     set_error("%d tokens of %d heads over %d pages of %d keys are too many for one call", T, H, kv.max_pages, kv.page_size);
     return SAGE_ERR_UNSUPPORTED;
