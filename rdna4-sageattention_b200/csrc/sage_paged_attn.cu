@@ -3,16 +3,19 @@
 // Row (b, i, h) sees the keys j < lens[b] and the drafted keys lens[b] + t with t <= i (no mask) or mask[b, i, t]:
 //   s_j = sm_scale * ks_j * (q . k8_j),   p_j = exp(s_j - m),   o = sum_j p_j vs_j v8_j / sum_j p_j
 //
-// One pass over the keys with a running maximum.  The row scale of V goes into the exponent, so that the products with
-// V take weights of at most 1 (2^8 with the lazy maximum below) that fp16 holds to 2^-11 whatever the scales are:
-//   t_j = log2(e) s_j + log2(vs_j),   m' = max t_j,   p'_j = 2^(t_j - m'),   O = sum p'_j v8_j,   l = sum p'_j / vs_j
-//   o = O / l,   lse = ln 2 (m' + log2 l)
-// A row of V that is all zeros has no such logarithm: it counts in m' with -100 and in l with its plain weight, and its
-// p', whatever it is, meets zero codes.  (Scales of V rows may lie up to 2^100 apart; the weight of a row further below
-// the others is lost from l.)
-// m' moves only when it is exceeded by more than 8, as in the dense kernel, and O is rescaled only then.
+// One pass over the keys with two running references, of the scores and of the scores with the V scale in them:
+//   x_j = log2(e) s_j,               m ~ max x_j,    l = sum 2^(x_j - m)
+//   t_j = x_j + log2(vs_j),          m' ~ max t_j,   p'_j = 2^(t_j - m'),   O = sum p'_j v8_j
+//   o = 2^(m' - m) O / l,   lse = ln 2 (m + log2 l)
+// The products with V take weights p' that fp16 holds whatever the scales are, and l knows nothing of V: a scale of 2^-109 or
+// 2^119, the ends of what append writes, takes nothing from it, and a NaN row of V leaves the log-sum-exp as it is.
+// One exponential serves both: p'_j = 2^(x_j - m') vs_j and l in units of 2^m' with one factor 2^(m' - m) a group; where that
+// may leave the range of fp32 (V scales beyond 2^+-40) p'_j = 2^(x_j - m) vs_j 2^(m - m'), in this order, in the code for rare groups.
+// m and m' are whole numbers, so the factors and all rescaling are exact powers of two; log2 vs serves only to place m'.  They
+// move, both, when one is exceeded by more than 8, as in the dense kernel, and O is rescaled then.
 // Both products run on fp16 operands with fp32 accumulators: int8 and e4m3 codes are exact in fp16, bf16 queries are
-// scaled by a power of two of their row (what is below 2^-24 of the row's largest value is rounded).  l and m' are fp32.
+// scaled by a power of two of their row (what is below 2^-24 of the row's largest value is rounded).  The references
+// and l are fp32.
 //
 // The query rows of a kv head (T tokens of H / Hkv heads) are cut into row tiles, the keys into tiles of 64.  All
 // (sequence, kv head, row tile, key tile) of a call form one list that the CTAs share evenly, whatever the lengths are: a
@@ -24,9 +27,9 @@
 // and the query rows its 8 columns, so that the 1 to 8 rows of a single token's group cost one column tile.
 //
 // Bound by memory: one token (4 query rows a kv head) over 16 sequences of 16 to 32 thousand keys, 8 kv heads, D 128, takes
-// 145 to 156 us on B200, 85 to 92 % of the measured copy rate; issue slots are 57 % taken.  Steps on the way, us: one CTA a row
+// 147 to 157 us on B200, 85 to 91 % of the measured copy rate; issue slots are 57 % taken.  Steps on the way, us: one CTA a row
 // 11122; shared list, rows times keys, cp.async 257; transposed products, TMA 175; no logarithm and no comparison a key where
-// no maximum moves 156; warps joining all at once 145.  One token over 1024 keys takes 10.9 us with the join, most of it
+// no maximum moves 156; warps joining all at once 145; two references 148.  One token over 1024 keys takes 11.7 us with the join, most of it
 // start-up and dependent loads.  D 256 reaches 87 % of the rate for 8 rows and 63 % for 16, for which each key is converted
 // twice: two column tiles a warp do not fit the registers.
 #include "sage_paged_attn.cuh"
@@ -36,6 +39,12 @@ namespace sage {
 constexpr int kWarps = 4;                              // consumer warps
 constexpr int kThreads = 32 * (kWarps + 1);
 constexpr int kJoinThreads = 128;
+
+// What the join of a CTA's warps needs of a query row: the factor of each warp's O, 1 / l and 2^(m' - m).
+struct alignas(16) JoinRow {
+  float factor[4];
+  float inverse, unit;
+};
 
 template <int D, int NR, int WM>
 struct Config {
@@ -60,9 +69,8 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
   constexpr int WK = kWarps / WM, NS = D / 16, NT = D / 16, kStages = C::kStages;
   extern __shared__ unsigned char smem_raw[];
   __shared__ int64_t warp_sums[kThreads / 32], found[2];
-  // of two row tiles, in turns: a warp may write its part of the next row tile while a slower one still reads this one's; it
-  // comes to the one after only through that row tile's barriers, which the slower one has to reach as well
-  __shared__ float2 join_ml[2][kWarps][8 * NR];
+  __shared__ RowState join_state[kWarps][8 * NR];
+  __shared__ JoinRow join_row[C::kRows];
   __shared__ int given_up;
   unsigned char* stages = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   float* scales = reinterpret_cast<float*>(stages + kStages * S::kStage);               // [stage][ks, vs][64]
@@ -96,7 +104,8 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
   // -------------------------------------------------------------------- consumers
   const int n = lane / 4, c = lane % 4, wm = warp % WM, wk = warp / WM;
   uint32_t qf[NR][NS][2];
-  float o[NR][NT][4], m[NR][2], l[NR][2], row_scale[NR][2];
+  float o[NR][NT][4], row_scale[NR][2];
+  Softmax sm[NR][2];
   bool fresh_unit = true;
   int segment = 0;                    // row tiles that this CTA has finished
   int first_tile = now.tile;          // of the row tile, by this CTA
@@ -111,8 +120,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
       for (int r = 0; r < NR; ++r) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) o[r][t][0] = o[r][t][1] = o[r][t][2] = o[r][t][3] = 0.0f;
-        m[r][0] = m[r][1] = -3.402823466e38f;
-        l[r][0] = l[r][1] = 0.0f;
+        sm[r][0].clear(), sm[r][1].clear();
         const int row = row0 + 8 * r + n, token = row / a.group;
         const bool live = token < now.fresh;
         const T* src = static_cast<const T*>(a.q) + now.b * a.q_st.b + token * a.q_st.s + (head0 + row % a.group) * a.q_st.h;
@@ -203,9 +211,8 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
           step(2 * i, u.x, v.x), step(2 * i + 1, u.y, v.y);
         }
       }
-      // Most groups: every row sees every key and no maximum moves.  The weights are computed on that assumption, p vs =
-      // 2^(s - m') vs and l from 2^(s - m') itself, and looked over afterwards; where it did not hold (a weight above 2^8, a
-      // key whose V row is zero far above the others) the group is done over from its scores.
+      // Most groups: every row sees every key and no reference moves.  The weights are computed on that assumption and
+      // looked over afterwards; where it did not hold the group is done over from its scores.
       const float factor[2] = {ks[keys[0]] * a.scale, ks[keys[1]] * a.scale};
       const float v_scale[2] = {ks[kTileKeys + keys[0]], ks[kTileKeys + keys[1]]};
       uint32_t pf[NR][2];
@@ -217,53 +224,46 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
           for (int x = 0; x < 4; ++x) s[r][x] *= row_scale[r][x & 1];
       }
       if (!drafts) {
-        float sum[NR][2], top = 0.0f, most = 0.0f;
+        uint64_t l[NR];   // the lane's two rows as a pair
+        float top = 0.0f;
+        uint32_t most = 0;
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
-          sum[r][0] = l[r][0], sum[r][1] = l[r][1];
+          const uint64_t minus_t = f2_pack(-sm[r][0].t, -sm[r][1].t);
+          float x, y;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float u = fast_exp2(fmaf(s[r][2 * h], factor[h], -m[r][0]));
-            const float v = fast_exp2(fmaf(s[r][2 * h + 1], factor[h], -m[r][1]));
-            sum[r][0] += u, sum[r][1] += v;
-            top = fmaxf(fmaxf(top, u * v_scale[h]), v * v_scale[h]);
-            pf[r][h] = pack_weights(u * v_scale[h], v * v_scale[h]);
+            f2_unpack(f2_fma(f2_pack(s[r][2 * h], s[r][2 * h + 1]), f2_pack(factor[h], factor[h]), minus_t), x, y);
+            const uint64_t u = f2_pack(fast_exp2(x), fast_exp2(y));
+            l[r] = h == 0 ? u : f2_add(l[r], u);
+            f2_unpack(f2_mul(u, f2_pack(v_scale[h], v_scale[h])), x, y);
+            top = fmaxf(fmaxf(top, x), y);
+            pf[r][h] = pack_weights(x, y);
           }
-          most = r == 0 ? sum[0][0] + sum[0][1] : most + (sum[r][0] + sum[r][1]);
+          l[r] = f2_mul(l[r], f2_pack(sm[r][0].ratio, sm[r][1].ratio));
+          f2_unpack(l[r], x, y);
+          most = max(max(most, bits(x)), bits(y));
         }
-        again = __any_sync(0xffffffffu, !(top <= 256.0f && most < 0x1p120f));
+        again = __any_sync(0xffffffffu, !(top <= kMostWeight) || most > bits(2 * kMostSum));
         if (!again) {
 #pragma unroll
           for (int r = 0; r < NR; ++r) {
-            l[r][0] = sum[r][0], l[r][1] = sum[r][1];
+            f2_unpack(f2_add(f2_pack(sm[r][0].l, sm[r][1].l), l[r]), sm[r][0].l, sm[r][1].l);
             pf[r][0] = transposed(pf[r][0]), pf[r][1] = transposed(pf[r][1]);
           }
         }
       }
       if (again) {
-        // of the lane's two keys: log2 of the V scale, its inverse, and what the exponent of a zero row gains over its part in
-        // the maximum
-        float log_v[2], inverse_v[2], gain[2];
-        bool zero = false;
+        const float log_v[2] = {__log2f(v_scale[0]), __log2f(v_scale[1])};   // of a zero row -infinity
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float vs = v_scale[h];
-          log_v[h] = __log2f(vs);
-          // finite whatever the scale is (unwritten memory): rows that see a NaN scale are NaN by its logarithm, and rows that do
-          // not see the key must not meet 0 * NaN or 0 * infinity here
-          inverse_v[h] = vs > 0x1p-120f ? __fdividef(1.0f, vs) : 0x1p120f;
-          gain[h] = 0.0f;
-          if (vs == 0.0f) zero = true, log_v[h] = kZeroLog, inverse_v[h] = 1.0f, gain[h] = -kZeroLog;
-        }
-        bool more = false;
+        for (int r = 0; r < NR; ++r) {
+          float keep[2];
 #pragma unroll
-        for (int r = 0; r < NR; ++r)
+          for (int e = 0; e < 2; ++e) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
+            for (int h = 0; h < 2; ++h) {
               float& x = s[r][2 * h + e];
-              x = fmaf(x, factor[h], log_v[h]);   // scaled by its row already
+              x *= factor[h];                     // scaled by its row already
               if (drafts) {
                 const int t = key0 + keys[h] - now.len, token = (row0 + 8 * r + 2 * c + e) / a.group;
                 const bool seen = t < 0 || (t < now.fresh && token < now.fresh &&
@@ -271,45 +271,29 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
                                                                : t <= token));
                 if (!seen) x = -INFINITY;
               }
-              more |= x > m[r][e] + 8.0f;
             }
-        if (__any_sync(0xffffffffu, more)) {
+            float top = fmaxf(s[r][e], s[r][2 + e]), top_v = fmaxf(s[r][e] + log_v[0], s[r][2 + e] + log_v[1]);
 #pragma unroll
-          for (int r = 0; r < NR; ++r) {
-            float keep[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float top = fmaxf(s[r][e], s[r][2 + e]);
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-              const float next = top > m[r][e] + 8.0f ? top : m[r][e];
-              keep[e] = next == m[r][e] ? 1.0f : fast_exp2(m[r][e] - next);
-              m[r][e] = next;
-              l[r][e] *= keep[e];
+            for (int z = 4; z < 32; z *= 2) {
+              top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, z));
+              top_v = fmaxf(top_v, __shfl_xor_sync(0xffffffffu, top_v, z));
             }
-#pragma unroll
-            for (int t = 0; t < NT; ++t) o[r][t][0] *= keep[0], o[r][t][1] *= keep[1], o[r][t][2] *= keep[0], o[r][t][3] *= keep[1];
+            keep[e] = sm[r][e].move(top, top_v);   // by less than they wait for too: here it costs nothing
           }
-        }
-        if (__any_sync(0xffffffffu, zero)) {
 #pragma unroll
-          for (int r = 0; r < NR; ++r)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) s[r][x] += gain[x / 2];
-        }
-#pragma unroll
-        for (int r = 0; r < NR; ++r)
+          for (int t = 0; t < NT; ++t) o[r][t][0] *= keep[0], o[r][t][1] *= keep[1], o[r][t][2] *= keep[0], o[r][t][3] *= keep[1];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             float p[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              p[e] = fast_exp2(s[r][2 * h + e] - m[r][e]);
-              l[r][e] = fmaf(p[e], inverse_v[h], l[r][e]);
+              const float x = s[r][2 * h + e], u = fast_exp2(x - sm[r][e].m());
+              sm[r][e].l += u;
+              p[e] = x == -INFINITY ? 0.0f : u * v_scale[h] * sm[r][e].score_unit();   // an unseen key's scale may be anything
             }
             pf[r][h] = transposed(pack_weights(p[0], p[1]));
           }
+        }
       }
       // four keys a lane; a word of four channels of each is two output tiles
       auto product = [&](int i, uint32_t w0, uint32_t w1, uint32_t w2, uint32_t w3) {
@@ -359,9 +343,9 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
       for (int r = 0; r < NR; ++r)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          l[r][e] += __shfl_xor_sync(0xffffffffu, l[r][e], 4);
-          l[r][e] += __shfl_xor_sync(0xffffffffu, l[r][e], 8);
-          l[r][e] += __shfl_xor_sync(0xffffffffu, l[r][e], 16);
+          sm[r][e].l += __shfl_xor_sync(0xffffffffu, sm[r][e].l, 4);
+          sm[r][e].l += __shfl_xor_sync(0xffffffffu, sm[r][e].l, 8);
+          sm[r][e].l += __shfl_xor_sync(0xffffffffu, sm[r][e].l, 16);
         }
       // The warps of a row tile join through the stage that all of them have read by then, eight rows of each at a time:
       // every warp leaves its part, every thread adds up eight channels of a row in the order of the warps.
@@ -371,14 +355,42 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
       auto place = [](int row, int quad) {   // four channels; permuted against bank conflicts
         return (row * (D / 4) + (quad ^ (row >> 1 & 3) ^ (S::kWide ? (quad >> 4 & 1) << 2 : 0))) * 4;
       };
-      float2 (*parts)[8 * NR] = join_ml[segment & 1];
+      // A barrier stands between each thing written here and its readers, and between those and the next row tile's writers,
+      // whichever warp is ahead: states are read before the second barrier, the rows' factors are written after the first.
       if (n == 0) {
 #pragma unroll
         for (int r = 0; r < NR; ++r)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) parts[warp][8 * r + 2 * c + e] = make_float2(m[r][e], l[r][e]);
+          for (int e = 0; e < 2; ++e) join_state[warp][8 * r + 2 * c + e] = sm[r][e].state();
       }
       consumers_sync();
+      if (tid < C::kRows) {   // a thread a row: the warps' factors, the sum of the weights
+        const int g = tid / (8 * NR);
+        RowState all{kLowest, 0.0f, kLowest};
+#pragma unroll
+        for (int w = 0; w < WK; ++w) {
+          const RowState& state = join_state[w * WM + g][tid % (8 * NR)];
+          all.m = fmaxf(all.m, state.m), all.t = fmaxf(all.t, state.t);
+        }
+        JoinRow& to = join_row[tid];
+#pragma unroll
+        for (int w = 0; w < WK; ++w) {
+          const RowState& state = join_state[w * WM + g][tid % (8 * NR)];
+          all.l = fmaf(fast_exp2(state.m - all.m), state.l, all.l);
+          to.factor[w] = fast_exp2(state.t - all.t);
+        }
+        if (tid < a.T * a.group) {
+          const int token = tid / a.group, head = head0 + tid % a.group;
+          const bool seen = token < now.fresh && all.l != 0.0f;
+          to.inverse = seen ? 1.0f / all.l : 0.0f;
+          to.unit = fast_exp2(all.t - all.m);
+          if (!whole)
+            a.part_state[part + tid] = all;
+          else if (a.lse != nullptr)
+            a.lse[((int64_t)now.b * a.H + head) * a.T + token] =
+                seen ? (all.m + log2f(all.l)) * 0.69314718055994531f : -INFINITY;
+        }
+      }
 #pragma unroll
       for (int r = 0; r < NR; ++r) {
         if (r > 0) consumers_sync();
@@ -392,37 +404,29 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
 #pragma unroll 1
         for (int item = tid; item < WM * D; item += 32 * kWarps) {
           const int of = item / (D / 8), g = of / 8, rr = of % 8, d = item % (D / 8) * 8;
-          float top = -3.402823466e38f, sum = 0.0f, x[8] = {};
-#pragma unroll
-          for (int w = 0; w < WK; ++w) top = fmaxf(top, parts[w * WM + g][8 * r + rr].x);
+          const int row = g * 8 * NR + 8 * r + rr;
+          if (row >= a.T * a.group) continue;
+          const JoinRow& by = join_row[row];
+          float x[8] = {};
 #pragma unroll
           for (int w = 0; w < WK; ++w) {
-            const float2 ml = parts[w * WM + g][8 * r + rr];
-            const float f = fast_exp2(ml.x - top);
-            sum = fmaf(f, ml.y, sum);
+            const float f = by.factor[w];
             const float* from = area + (w * WM + g) * (8 * D);
             const float4 u = *reinterpret_cast<const float4*>(from + place(rr, d / 4));
             const float4 v = *reinterpret_cast<const float4*>(from + place(rr, d / 4 + 1));
             x[0] = fmaf(f, u.x, x[0]), x[1] = fmaf(f, u.y, x[1]), x[2] = fmaf(f, u.z, x[2]), x[3] = fmaf(f, u.w, x[3]);
             x[4] = fmaf(f, v.x, x[4]), x[5] = fmaf(f, v.y, x[5]), x[6] = fmaf(f, v.z, x[6]), x[7] = fmaf(f, v.w, x[7]);
           }
-          const int row = g * 8 * NR + 8 * r + rr;
-          const int token = row / a.group, head = head0 + row % a.group;
-          if (row >= a.T * a.group) continue;
           if (whole) {
-            const bool seen = token < now.fresh && sum != 0.0f;
-            const float inverse = 1.0f / sum;
+            const float inverse = by.inverse, unit = by.unit;
 #pragma unroll
-            for (int z = 0; z < 8; ++z) x[z] = seen ? x[z] * inverse : 0.0f;
+            for (int z = 0; z < 8; ++z) x[z] = inverse != 0.0f ? x[z] * inverse * unit : 0.0f;   // 0: sees nothing
+            const int token = row / a.group, head = head0 + row % a.group;
             store8(static_cast<T*>(a.out) + now.b * a.out_st.b + token * a.out_st.s + head * a.out_st.h + d, x);
-            if (a.lse != nullptr && d == 0)
-              a.lse[((int64_t)now.b * a.H + head) * a.T + token] =
-                  seen ? (top + log2f(sum)) * 0.69314718055994531f : -INFINITY;
           } else {
             float* to = a.part_o + (part + row) * D + d;
             *reinterpret_cast<float4*>(to) = make_float4(x[0], x[1], x[2], x[3]);
             *reinterpret_cast<float4*>(to + 4) = make_float4(x[4], x[5], x[6], x[7]);
-            if (d == 0) a.part_ml[part + row] = make_float2(top, sum);
           }
         }
       }
@@ -490,24 +494,29 @@ __global__ void __launch_bounds__(kJoinThreads, 8) paged_join_kernel(const Paged
   if (row >= a.T * a.group) return;
   const int token = row / a.group, head = unit * a.group + row % a.group;
   const bool live = tiles > 0 && token < fresh;
-  float top = -3.402823466e38f, sum = 0.0f, o[D / 32];
+  float top = kLowest, top_t = kLowest, sum = 0.0f, o[D / 32];
 #pragma unroll
   for (int i = 0; i < D / 32; ++i) o[i] = 0.0f;
   if (live) {
-    for (int x = c0 + lane; x <= c1; x += 32)
-      top = fmaxf(top, a.part_ml[(2 * (int64_t)x + (x == c0 ? slot : 0)) * tile_rows + row].x);
+    for (int x = c0 + lane; x <= c1; x += 32) {
+      const RowState state = a.part_state[(2 * (int64_t)x + (x == c0 ? slot : 0)) * tile_rows + row];
+      top = fmaxf(top, state.m), top_t = fmaxf(top_t, state.t);
+    }
 #pragma unroll
-    for (int x = 16; x > 0; x /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+    for (int x = 16; x > 0; x /= 2) {
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+      top_t = fmaxf(top_t, __shfl_xor_sync(0xffffffffu, top_t, x));
+    }
     constexpr int kAtOnce = 4;   // parts under way at once: the loads are what this kernel waits for
 #pragma unroll 1
     for (int x0 = c0; x0 <= c1; x0 += kAtOnce) {
-      float2 ml[kAtOnce];
+      RowState state[kAtOnce];
       float v[kAtOnce][D / 32];
 #pragma unroll
       for (int z = 0; z < kAtOnce; ++z) {
         const int x = min(x0 + z, c1);   // the last one again, left out below
         const int64_t at = (2 * (int64_t)x + (x == c0 ? slot : 0)) * tile_rows + row;
-        ml[z] = a.part_ml[at];
+        state[z] = a.part_state[at];
 #pragma unroll
         for (int i = 0; i < D / 32; i += D % 64 ? 1 : 2) {
           if constexpr (D % 64 == 0) {
@@ -521,21 +530,21 @@ __global__ void __launch_bounds__(kJoinThreads, 8) paged_join_kernel(const Paged
 #pragma unroll
       for (int z = 0; z < kAtOnce; ++z) {
         if (x0 + z > c1) break;
-        const float f = fast_exp2(ml[z].x - top);
-        sum = fmaf(f, ml[z].y, sum);
+        const float f = fast_exp2(state[z].t - top_t);
+        sum = fmaf(fast_exp2(state[z].m - top), state[z].l, sum);
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) o[i] = fmaf(f, v[z][i], o[i]);
       }
     }
   }
-  const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum, unit_v = fast_exp2(top_t - top);
   T* dst = static_cast<T*>(a.out) + b * a.out_st.b + token * a.out_st.s + head * a.out_st.h;
 #pragma unroll
   for (int i = 0; i < D / 32; i += D % 64 ? 1 : 2) {
     if constexpr (D % 64 == 0)
-      *reinterpret_cast<uint32_t*>(dst + i * 32 + lane * 2) = pack2(o[i] * inverse, o[i + 1] * inverse, T());
+      *reinterpret_cast<uint32_t*>(dst + i * 32 + lane * 2) = pack2(o[i] * inverse * unit_v, o[i + 1] * inverse * unit_v, T());
     else
-      dst[i * 32 + lane] = T(o[i] * inverse);
+      dst[i * 32 + lane] = T(o[i] * inverse * unit_v);
   }
   if (a.lse != nullptr && lane == 0)
     a.lse[((int64_t)b * a.H + head) * a.T + token] =
@@ -559,17 +568,19 @@ __global__ void __launch_bounds__(kJoinThreads) wide_join_kernel(const PagedAttn
   if (r >= a.T * a.group) return;
   const int token = r / a.group, head = unit / a.row_tiles * a.group + r % a.group;
   const bool live = tiles > 0 && token < fresh;
-  float top = -3.402823466e38f, sum = 0.0f, o[kChannels];
+  float top = kLowest, top_t = kLowest, sum = 0.0f, o[kChannels];
 #pragma unroll
   for (int i = 0; i < kChannels; ++i) o[i] = 0.0f;
   if (live) {
-    for (int x = c0; x <= c1; ++x)
-      top = fmaxf(top, a.part_ml[(2 * (int64_t)x + (x == c0 ? slot : 0)) * tile_rows + row].x);
+    for (int x = c0; x <= c1; ++x) {
+      const RowState state = a.part_state[(2 * (int64_t)x + (x == c0 ? slot : 0)) * tile_rows + row];
+      top = fmaxf(top, state.m), top_t = fmaxf(top_t, state.t);
+    }
     for (int x = c0; x <= c1; ++x) {
       const int64_t first = (2 * (int64_t)x + (x == c0 ? slot : 0)) * tile_rows;
-      const float2 ml = a.part_ml[first + row];
-      const float f = fast_exp2(ml.x - top);
-      sum = fmaf(f, ml.y, sum);
+      const RowState state = a.part_state[first + row];
+      const float f = fast_exp2(state.t - top_t);
+      sum = fmaf(fast_exp2(state.m - top), state.l, sum);
       const float* part = a.part_o + first * D + (int64_t)d0 * tile_rows + row * 4;
 #pragma unroll
       for (int i = 0; i < kChannels; i += 4) {
@@ -579,9 +590,9 @@ __global__ void __launch_bounds__(kJoinThreads) wide_join_kernel(const PagedAttn
       }
     }
   }
-  const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum, unit_v = fast_exp2(top_t - top);
 #pragma unroll
-  for (int i = 0; i < kChannels; ++i) o[i] *= inverse;
+  for (int i = 0; i < kChannels; ++i) o[i] *= inverse, o[i] *= unit_v;
   T* dst = static_cast<T*>(a.out) + b * a.out_st.b + token * a.out_st.s + head * a.out_st.h + d0;
 #pragma unroll
   for (int i = 0; i < kChannels; i += 8) store8(dst + i, o + i);
@@ -661,7 +672,7 @@ extern "C" size_t sage_paged_attention_workspace_bytes(int B, int T, int H, int 
   const int64_t rows = (int64_t)T * (H / Hkv);
   const Shape s = row_tile(rows, D);
   const size_t slots = wide(rows, D) ? (size_t)2 * wide_ctas() * wide_rows(D) : (size_t)2 * shared_ctas(D, s) * 8 * s.nr * s.wm;
-  return slots * (D * sizeof(float) + sizeof(float2));
+  return slots * (D * sizeof(float) + sizeof(RowState));
 }
 
 extern "C" int sage_paged_attention(const sage_paged_attention_args* args, void* stream) {
@@ -721,7 +732,7 @@ extern "C" int sage_paged_attention(const sage_paged_attention_args* args, void*
   a.ctas = many ? wide_ctas() : shared_ctas(D, shape);
   a.scale = (float)((args->sm_scale > 0.0 ? args->sm_scale : 1.0 / std::sqrt((double)D)) * 1.4426950408889634);
   a.part_o = static_cast<float*>(args->workspace);
-  a.part_ml = reinterpret_cast<float2*>(a.part_o + (size_t)2 * a.ctas * tile_rows * D);
+  a.part_state = reinterpret_cast<RowState*>(a.part_o + (size_t)2 * a.ctas * tile_rows * D);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return by_head_dim(D, [&](auto d) {
     constexpr int kD = decltype(d)::value;

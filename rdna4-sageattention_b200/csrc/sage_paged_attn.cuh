@@ -15,7 +15,18 @@ namespace sage {
 
 constexpr int kTileKeys = 64;
 constexpr int kMinTiles = 2;               // tiles a CTA takes at the least
-constexpr float kZeroLog = -100.0f;        // log2 of a zero V scale in the running maximum
+constexpr float kLowest = -3.402823466e38f;   // of a reference: nothing seen yet
+constexpr float kLazy = 8.0f;              // log2 of what may exceed a reference before it moves
+constexpr float kMostWeight = 256.0f;      // 2^kLazy
+constexpr float kMostSum = 256.0f;         // a mean of plain weights above it moves a reference
+constexpr float kTame = 40.0f;             // of the references' ratio, log2: what 2^(x - t) can carry
+constexpr float kMostRatio = 120.0f;       // of the references, log2: binds where every V row so far is zero (weights 0)
+
+// What is known of a query row beside its O: the reference of its scores, the sum of its weights, the reference of its
+// scores with the V scale in them (all three in the units of 2^x).
+struct alignas(16) RowState {
+  float m, l, t;
+};
 
 struct PagedAttnArgs {
   PagedArgs p;
@@ -32,7 +43,7 @@ struct PagedAttnArgs {
   int ctas;            // CTAs that share the list
   float scale;         // sm_scale * log2(e)
   float* part_o;       // [2 * ctas][rows of a tile][D]
-  float2* part_ml;     // [2 * ctas][rows of a tile]
+  RowState* part_state;   // [2 * ctas][rows of a tile]
 };
 
 // Context length and fresh tokens of sequence b; returns its key tiles (0 where no row has anything to see).
@@ -167,7 +178,36 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Two weights -> an fp16 pair, the largest finite number for what is above it (only weights of zero rows are).
+// What the online softmax knows of a query row: t, the reference of its scores with the V scale in them (m'); ratio =
+// 2^(t - m), where m is the reference of the scores themselves; l, the sum of 2^(x - m).  A ratio at which 2^(x - t) may leave
+// the range of fp32 is negative: what is multiplied by it fails a comparison of bits().
+struct Softmax {
+  float t, ratio, l;
+
+  __device__ __forceinline__ void clear() { t = kLowest, ratio = 1.0f, l = 0.0f; }
+  __device__ __forceinline__ float exponent() const { return (float)((__float_as_int(ratio) >> 23 & 255) - 127); }
+  __device__ __forceinline__ float m() const { return t - exponent(); }
+  __device__ __forceinline__ float v_unit() const { return fabsf(ratio); }                                        // 2^(t - m)
+  __device__ __forceinline__ float score_unit() const { return __int_as_float((254 << 23) - __float_as_int(v_unit())); }   // 2^(m - t)
+  // Whether a score x, or the same with the V scale in it, exceeds its reference by more than they wait for.
+  __device__ __forceinline__ bool exceeded(float x, float with_v) const { return x > m() + kLazy || with_v > t + kLazy; }
+  // Moves the references to the largest of either, rescales l, and returns the factor of O.
+  __device__ __forceinline__ float move(float top, float top_v) {
+    const float before = m(), old = exponent();
+    const float next = fmaxf(before, ceilf(top)), step = before - next;
+    const float now = fminf(fmaxf(fmaxf(old + step, ceilf(top_v) - next), -kMostRatio), kMostRatio);
+    t = next + now;
+    ratio = copysignf(__int_as_float(((int)now + 127) << 23), kTame - fabsf(now));
+    l *= fast_exp2(step);
+    return fast_exp2(step + (old - now));
+  }
+  __device__ __forceinline__ RowState state() const { return RowState{m(), l, t}; }
+};
+
+// As a bit pattern a positive float orders as it does as a number, with NaN and every negative one above.
+__device__ __forceinline__ uint32_t bits(float x) { return __float_as_uint(x); }
+
+// Two weights -> an fp16 pair, the largest finite number for what is above it.
 __device__ __forceinline__ uint32_t pack_weights(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));

@@ -3,12 +3,12 @@
 //
 // A CTA (one per SM) owns QT row tiles of 128 query rows of one kv head and walks its stretch of the list:
 //   softmax warps   one warpgroup per row tile, one thread per row: q to TMEM (fp16), then per key tile S from TMEM,
-//                   weights (fp16) back over S, O rescaled in TMEM when the maximum moves, epilogue
+//                   weights (fp16) back over S, O rescaled in TMEM when the references move, epilogue
 //   producer warp   TMA of the raw codes and scales into a ring
 //   MMA warps       one per row tile: S_t = Q_t K^T, O_t += P_t V (A from TMEM); two score tiles a row tile, so that the
 //                   scores of the next key tile are there when the softmax of this one ends
 //   4 converter warps   int8 and e4m3 codes to fp16 operand tiles in shared memory, once for all QT * 128 rows, and what
-//                   the rows need of each key (factor of its score, log2 of its V scale, the inverse of that)
+//                   the rows need of each key (factor of its score, its V scale, the log2 of that)
 // Codes convert exactly, so there is nothing to choose there.
 // TMEM (512 columns): O_t at t D, the score tiles of t at QT D + 128 t, P over the first half of its scores; Q_t behind
 // them where it fits (D 64 and 256), else in shared memory (D 96 and 128).
@@ -41,7 +41,7 @@ struct Wide {
   static constexpr int kO = 0, kS = QT * D, kQ = kS + QT * 2 * kTileKeys;
   static_assert(kQ + (kQShared ? 0 : QT * D / 2) <= 512, "TMEM columns");
   static constexpr int kQPanel = 128 * 128, kQTile = kPanels * kQPanel;   // bytes in shared memory: 64 channels, a row tile
-  static constexpr int kParams = 5 * kTileKeys;            // floats of a tile: factor, log2 V scale, inverse, gain, V scale
+  static constexpr int kParams = 3 * kTileKeys;            // floats of a tile: factor, V scale, its log2
   static constexpr int kSmem = 1024 + kBufs * 2 * kOperand + kRaw * (Tile<D>::kStage + 2 * kTileKeys * 4) +
                                kBufs * kParams * 4 + (kQShared ? QT * kQTile : 0);
   static_assert(kSmem <= 227 * 1024, "shared memory");
@@ -311,14 +311,10 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
         const float* sc = scales + raw * 2 * kTileKeys;
         float* out = params + buf * W::kParams;
         const float vs = sc[kTileKeys + ct];
-        const bool there = key0 + ct < total, zero = there && vs == 0.0f;
+        const bool there = key0 + ct < total;   // no row sees the others
         out[ct] = there ? sc[ct] * a.scale : 0.0f;
-        out[kTileKeys + ct] = !there ? -INFINITY : zero ? kZeroLog : __log2f(vs);
-        // finite whatever the scale is (unwritten memory): rows that see a NaN scale are NaN by its logarithm, and rows that do
-        // not see the key must not meet 0 * NaN or 0 * infinity here
-        out[2 * kTileKeys + ct] = !there ? 0.0f : zero ? 1.0f : vs > 0x1p-120f ? __fdividef(1.0f, vs) : 0x1p120f;
-        out[3 * kTileKeys + ct] = zero ? -kZeroLog : 0.0f;
-        out[4 * kTileKeys + ct] = vs;
+        out[kTileKeys + ct] = there ? vs : 0.0f;
+        out[2 * kTileKeys + ct] = __log2f(there ? vs : 0.0f);   // of a zero row -infinity
       }
 #pragma unroll
       for (int i0 = 0; i0 < kItems; i0 += kTogether) {
@@ -391,7 +387,9 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
       const int row = now.unit % a.row_tiles * W::kRows + t * 128 + warp % 4 * 32 + lane, token = row / a.group;
       const int head = now.unit / a.row_tiles * a.group + row % a.group;
       const bool warp_live = act && row - lane < now.fresh * a.group, live = token < now.fresh;
-      float m = -3.402823466e38f, l = 0.0f, row_scale = 1.0f;
+      Softmax sm;
+      sm.clear();
+      float row_scale = 1.0f;
       if (act) {
         if (warp_live) {
           if constexpr (D == 128) {
@@ -528,13 +526,13 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
             const bool drafts = key0 + kTileKeys > now.len;
             uint32_t packed[32];
             bool again = true;
-            // Most tiles: every row sees every key and no maximum moves.  The weights are computed on that assumption in
-            // one straight run, p vs = 2^(s - m') vs and l from 2^(s - m') itself, and looked over afterwards; where it did
-            // not hold the scores are still in TMEM, and the tile is done over.  (What a key needs is read by every lane
-            // of eight warps, and the words returned are what shared memory is busy with: two a key here, not three.)
+            // Most tiles: every row sees every key and no reference moves.  The weights are computed on that assumption in
+            // one straight run and looked over afterwards; where it did not hold the scores are still in TMEM, and the tile
+            // is done over.  (What a key needs is read by every lane of eight warps, and the words returned are what shared
+            // memory is busy with: two a key here, not three.)
             if (tile != first_tile && !drafts) {
-              const uint64_t scale2 = f2_pack(row_scale, row_scale), minus_m = f2_pack(-m, -m);
-              uint64_t sum[2] = {f2_pack(l, 0.0f), f2_pack(0.0f, 0.0f)};
+              const uint64_t scale2 = f2_pack(row_scale, row_scale), minus_t = f2_pack(-sm.t, -sm.t);
+              uint64_t sum[2] = {f2_pack(0.0f, 0.0f), f2_pack(0.0f, 0.0f)};
               float top[2] = {0.0f, 0.0f};
 #pragma unroll
               for (int part = 0; part < 2; ++part) {
@@ -545,17 +543,17 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
                 for (int i = 0; i < 8; ++i) {
                   const int k = 32 * part + 4 * i;
                   const float4 f = *reinterpret_cast<const float4*>(factor + k);
-                  const float4 w = *reinterpret_cast<const float4*>(factor + 4 * kTileKeys + k);
+                  const float4 w = *reinterpret_cast<const float4*>(factor + kTileKeys + k);
 #pragma unroll
                   for (int h = 0; h < 2; ++h) {
                     const int c = 4 * i + 2 * h;
                     uint64_t v = f2_pack(__uint_as_float(r[c]), __uint_as_float(r[c + 1]));
                     if constexpr (!std::is_same<T, __half>::value) v = f2_mul(v, scale2);
                     float p, q;
-                    f2_unpack(f2_fma(v, h ? f2_pack(f.z, f.w) : f2_pack(f.x, f.y), minus_m), p, q);
-                    const uint64_t e = f2_pack(fast_exp2(p), fast_exp2(q));
-                    sum[h] = f2_add(e, sum[h]);
-                    f2_unpack(f2_mul(e, h ? f2_pack(w.z, w.w) : f2_pack(w.x, w.y)), p, q);
+                    f2_unpack(f2_fma(v, h ? f2_pack(f.z, f.w) : f2_pack(f.x, f.y), minus_t), p, q);
+                    const uint64_t u = f2_pack(fast_exp2(p), fast_exp2(q));
+                    sum[h] = f2_add(u, sum[h]);
+                    f2_unpack(f2_mul(u, h ? f2_pack(w.z, w.w) : f2_pack(w.x, w.y)), p, q);
                     top[h] = fmaxf(fmaxf(top[h], p), q);
                     packed[16 * part + c / 2] = pack_weights(p, q);
                   }
@@ -563,10 +561,9 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
               }
               float p, q;
               f2_unpack(f2_add(sum[0], sum[1]), p, q);
-              p += q;
-              // a weight above 2^8, or one whose V row is zero above all bounds
-              again = __any_sync(0xffffffffu, !(fmaxf(top[0], top[1]) <= 256.0f && p < 0x1p120f));
-              if (!again) l = p;
+              p = (p + q) * sm.ratio;
+              again = __any_sync(0xffffffffu, !(fmaxf(top[0], top[1]) <= kMostWeight) || bits(p) > bits(kTileKeys * kMostSum));
+              if (!again) sm.l += p;
             }
             if (!again) {
               tmem_st32(s_at, packed);
@@ -600,37 +597,46 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
                   }
                 }
               }
-              // the exponents of 16 keys; small loops on purpose: this code runs once or twice a row tile, and what it
-              // costs is fetching it
-              auto exponents = [&](int k, float (&x)[16]) {
+              // the scores of 16 keys; small loops on purpose: this code runs once or twice a row tile, and what it costs
+              // is fetching it
+              auto scaled = [&](int k, float (&x)[16]) {
                 uint32_t r[16];
                 tmem_ld16(s_at + 16 * k, r);
                 tmem_wait_ld();
 #pragma unroll
                 for (int i = 0; i < 16; i += 4) {
                   const float4 f = *reinterpret_cast<const float4*>(factor + 16 * k + i);
-                  const float4 g = *reinterpret_cast<const float4*>(factor + kTileKeys + 16 * k + i);
-                  const float fs[4] = {f.x, f.y, f.z, f.w}, gs[4] = {g.x, g.y, g.z, g.w};
 #pragma unroll
-                  for (int h = 0; h < 4; ++h) {
-                    x[i + h] = fmaf(__uint_as_float(r[i + h]) * row_scale, fs[h], gs[h]);
+                  for (int h = 0; h < 4; h += 2) {
+                    uint64_t v = f2_pack(__uint_as_float(r[i + h]), __uint_as_float(r[i + h + 1]));
+                    if constexpr (!std::is_same<T, __half>::value) v = f2_mul(v, f2_pack(row_scale, row_scale));
+                    f2_unpack(f2_mul(v, h ? f2_pack(f.z, f.w) : f2_pack(f.x, f.y)), x[i + h], x[i + h + 1]);
                     if (!(seen >> (16 * k + i + h) & 1)) x[i + h] = -INFINITY;
+                    if (!(seen >> (16 * k + i + h + 1) & 1)) x[i + h + 1] = -INFINITY;
                   }
                 }
               };
-              float most = -INFINITY;
+              float most = -INFINITY, most_t = -INFINITY;
 #pragma unroll 1
               for (int k = 0; k < kTileKeys / 16; ++k) {
                 float x[16];
-                exponents(k, x);
+                scaled(k, x);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) most = fmaxf(most, x[i]);
+                for (int i = 0; i < 16; i += 4) {
+                  const float4 log_v = *reinterpret_cast<const float4*>(factor + 2 * kTileKeys + 16 * k + i);
+#pragma unroll
+                  for (int h = 0; h < 4; h += 2) {
+                    float p, q;
+                    f2_unpack(f2_add(f2_pack(x[i + h], x[i + h + 1]), h ? f2_pack(log_v.z, log_v.w) : f2_pack(log_v.x, log_v.y)), p, q);
+                    most = fmaxf(fmaxf(most, x[i + h]), x[i + h + 1]);
+                    most_t = fmaxf(fmaxf(most_t, p), q);
+                  }
+                }
               }
-              if (__any_sync(0xffffffffu, most > m + 8.0f)) {
-                const float next = most > m + 8.0f ? most : m;
-                const float keep = next == m ? 1.0f : fast_exp2(m - next);
-                m = next;
-                l *= keep;
+              const bool moves = sm.exceeded(most, most_t);
+              if (__any_sync(0xffffffffu, moves)) {
+                float keep = 1.0f;
+                if (moves) keep = sm.move(most, most_t);
                 if (tile != first_tile) {   // the first product of a row tile overwrites O
                   // the products of the tile before must be done (older ones are: this tile's scores came after them)
                   wait_stage(pv_done + t, pv_phase, &given_up, a.p.status);
@@ -646,21 +652,28 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
                   }
                 }
               }
+              const float m = sm.m(), unit = sm.score_unit();
+              uint64_t sum = f2_pack(0.0f, 0.0f);
 #pragma unroll 1
               for (int k = 0; k < kTileKeys / 16; ++k) {   // the weights of 16 keys take 8 columns, all read by then
                 float x[16];
-                exponents(k, x);
+                scaled(k, x);
                 uint32_t w[8];
 #pragma unroll
                 for (int i = 0; i < 16; i += 2) {
-                  const float2 inv = *reinterpret_cast<const float2*>(factor + 2 * kTileKeys + 16 * k + i);
-                  const float2 gain = *reinterpret_cast<const float2*>(factor + 3 * kTileKeys + 16 * k + i);
-                  const float p = fast_exp2(x[i] - m + gain.x), q = fast_exp2(x[i + 1] - m + gain.y);
-                  l = fmaf(q, inv.y, fmaf(p, inv.x, l));
-                  w[i / 2] = pack_weights(p, q);
+                  const float2 vs = *reinterpret_cast<const float2*>(factor + kTileKeys + 16 * k + i);
+                  const uint64_t u = f2_pack(fast_exp2(x[i] - m), fast_exp2(x[i + 1] - m));
+                  sum = f2_add(sum, u);
+                  float p, q;
+                  f2_unpack(f2_mul(f2_mul(u, f2_pack(vs.x, vs.y)), f2_pack(unit, unit)), p, q);
+                  // the scale of a key not seen may be anything
+                  w[i / 2] = pack_weights(x[i] == -INFINITY ? 0.0f : p, x[i + 1] == -INFINITY ? 0.0f : q);
                 }
                 tmem_st8(s_at + 8 * k, w);
               }
+              float p, q;
+              f2_unpack(sum, p, q);
+              sm.l += p + q;
             }
             tmem_wait_st();
             tc_fence_before();
@@ -683,7 +696,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
       const int64_t first_row = (2 * (int64_t)blockIdx.x + (segment > 0)) * W::kRows;
       const int in_tile = t * 128 + warp % 4 * 32 + lane;
       float* part = a.part_o + first_row * D + in_tile * 4;
-      const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+      const float inverse = sm.l == 0.0f ? 0.0f : 1.0f / sm.l;
       if (warp_live) {
 #pragma unroll 1
         for (int i = 0; i < D / 32; ++i) {
@@ -695,7 +708,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
             for (int k = 0; k < 32; k += 8) {
               float x[8];
 #pragma unroll
-              for (int z = 0; z < 8; ++z) x[z] = live && l != 0.0f ? __uint_as_float(r[k + z]) * inverse : 0.0f;
+              for (int z = 0; z < 8; ++z) x[z] = live && sm.l != 0.0f ? __uint_as_float(r[k + z]) * inverse * sm.v_unit() : 0.0f;
               store8(dst + 32 * i + k, x);
             }
           } else if (mine && live) {
@@ -711,9 +724,9 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
       if (mine && whole) {
         if (a.lse != nullptr)
           a.lse[((int64_t)now.b * a.H + head) * a.T + token] =
-              !live || l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+              !live || sm.l == 0.0f ? -INFINITY : (sm.m() + log2f(sm.l)) * 0.69314718055994531f;
       } else if (mine && live) {
-        a.part_ml[first_row + in_tile] = make_float2(m, l);
+        a.part_state[first_row + in_tile] = sm.state();
       }
       ++segment;
       todo -= last - first_tile;

@@ -1,0 +1,98 @@
+"""Attention over the paged cache at the ends of its ranges, against the definitions in 64 bits (paged_reference.py).
+
+Tolerances, per output row, with A = sum p |v| / sum p, as in test_gpu_paged_kv.py: half a step of the result's type; for
+each score (D + 8) 2^-24 of sum |q k| <= S, once in the sum over V and once in the sum of the weights; 2^-20 for
+exponentials and their arguments; (n / 16 + 16) 2^-24 for the sums over n keys; 2^-11 for a weight rounded to fp16, and
+2^-25 of the row's largest weight times scale, times 448, for what fp16 cannot hold of each.  The floor is half of
+the type's smallest step, so results of any size are compared."""
+import math
+
+import pytest
+import torch
+
+import paged_reference as P
+import rdna4_sage
+from rdna4_sage import _attention
+from test_gpu_paged_kv import DEV, filled, handle, ints, queries, trees
+
+pytestmark = pytest.mark.gpu
+
+
+def compare(q, cache, table, lens, mask=None, sm_scale=None, lost=2.0 ** -25):
+    """Result and log-sum-exp within the bounds above; returns the results of both sides."""
+    o, lse = rdna4_sage.attention_paged_kv(q, handle(cache), table, ints(lens), mask, None, "NHD", sm_scale, True)
+    _attention.check_status(torch.device("cuda", 0))
+    want, want_lse, mean, S, top = P.attention(q, cache, table, lens, mask, None, sm_scale)
+    n, D, info = max(lens) + q.shape[1], q.shape[-1], torch.finfo(q.dtype)
+    weight = 2 * ((D + 8) * 2.0 ** -24 * S + 2.0 ** -22 * want_lse.transpose(1, 2).abs().nan_to_num(0, 0, 0) +
+                  2.0 ** -20 + (n / 16 + 16) * 2.0 ** -24)
+    tol = info.eps / 2 * want.abs() + mean * (2.0 ** -11 + weight[..., None]) + (n * lost * 448 * top)[..., None] + \
+        info.smallest_normal * info.eps / 2
+    off = (o.double() - want).abs()
+    assert torch.equal(o.isnan(), want.isnan())
+    assert bool((off <= tol)[~want.isnan()].all()), float((off / tol).nan_to_num(0).max())
+    seen = want_lse > -math.inf
+    assert torch.equal(lse > -math.inf, seen)
+    ltol = (weight.transpose(1, 2) + 2.0 ** -23 * want_lse.abs())[seen]
+    lo = (lse.double() - want_lse).abs()[seen]
+    assert bool((lo <= ltol).all()), float((lo / ltol).max())
+    return o, lse
+
+
+SHAPES = [(64, 1, 2), (96, 2, 8), (128, 1, 8), (128, 4, 16), (256, 1, 8), (256, 3, 8),     # D, T, H over 2 kv heads: few rows
+          (64, 24, 8), (128, 40, 4), (96, 33, 4), (256, 17, 4)]                            # many
+
+
+@pytest.mark.parametrize("D,T,H", SHAPES)
+@pytest.mark.parametrize("power", [-101, 124])
+def test_v_rows_of_the_smallest_and_largest_size(D, T, H, power):
+    # scales near 2^-108 and 2^117, the ends of what append writes: neither the weights' sum nor a result is lost
+    lens = [5000, 70]
+    cache, table = filled(lens, T, 32, 2, D, seed=D + T)
+    cache["vs"].mul_(2.0 ** power)
+    for size in (0.3, 3.0):
+        compare(queries(2, T, H, D, size=size), cache, table, lens, trees(2, T) if T > 2 else None)
+
+
+@pytest.mark.parametrize("D,T,H", SHAPES)
+def test_v_rows_of_both_ends_in_one_context(D, T, H):
+    lens = [1500, 200]
+    cache, table = filled(lens, T, 64, 2, D, seed=D)
+    plain, lse = compare(queries(2, T, H, D), cache, table, lens)
+    for b in range(2):
+        p, r = P.place(cache, table, b, range(0, lens[b], 2))
+        cache["vs"][p, :, r] *= 2.0 ** 110
+        p, r = P.place(cache, table, b, range(1, lens[b], 2))
+        cache["vs"][p, :, r] *= 2.0 ** -95
+        p, r = P.place(cache, table, b, range(0, lens[b], 50))
+        cache["vs"][p, :, r] = 0.0
+        cache["v8"].view(torch.uint8)[p, :, r] = 0
+    compare(queries(2, T, H, D), cache, table, lens)
+
+
+@pytest.mark.parametrize("D,T,H", SHAPES)
+def test_v_rows_that_are_zero_up_to_the_last(D, T, H):
+    # zero rows count in the weights' sum only, whatever came before and comes after them
+    lens = [900, 130]
+    cache, table = filled(lens, T, 16, 2, D, seed=T)
+    for b in range(2):
+        p, r = P.place(cache, table, b, range(0, lens[b] - 3))
+        cache["vs"][p, :, r] = 0.0
+        cache["v8"].view(torch.uint8)[p, :, r] = 0
+    cache["vs"].mul_(2.0 ** -60)
+    compare(queries(2, T, H, D), cache, table, lens)
+
+
+@pytest.mark.parametrize("D,T,H", SHAPES)
+@pytest.mark.parametrize("at", [0, 100, 803])
+def test_a_v_row_with_nan_leaves_the_log_sum_exp(D, T, H, at):
+    # as append writes it: scale NaN, codes 0.  The result of a row that sees it is NaN, its log-sum-exp is that of its scores
+    lens = [804, 77]
+    cache, table = filled(lens, T, 32, 2, D, seed=at)
+    q = queries(2, T, H, D)
+    a, la = compare(q, cache, table, lens)
+    p, r = P.place(cache, table, 0, [at])
+    cache["vs"][p, :, r] = math.nan
+    cache["v8"].view(torch.uint8)[p, :, r] = 0
+    b, lb = compare(q, cache, table, lens)
+    assert bool(b[0].isnan().all()) and torch.equal(b[1], a[1]) and torch.equal(lb[1], la[1])
