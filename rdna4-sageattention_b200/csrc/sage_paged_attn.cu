@@ -5,17 +5,19 @@
 //
 // One pass over the keys with two running references, of the scores and of the scores with the V scale in them:
 //   x_j = log2(e) s_j,               m ~ max x_j,    l = sum 2^(x_j - m)
-//   t_j = x_j + log2(vs_j),          m' ~ max t_j,   p'_j = 2^(t_j - m'),   O = sum p'_j v8_j
+//   t_j = x_j + log2(vs_j),      m' ~ max t_j - 8,   p'_j = 2^(t_j - m'),   O = sum p'_j v8_j
 //   o = 2^(m' - m) O / l,   lse = ln 2 (m + log2 l)
-// The products with V take weights p' that fp16 holds whatever the scales are, and l knows nothing of V: a scale of 2^-109 or
-// 2^119, the ends of what append writes, takes nothing from it, and a NaN row of V leaves the log-sum-exp as it is.
+// The products with V take weights p' in fp16, which are placed high in its range, the row's largest (with its scale) at 2^7
+// to 2^15: p' keeps 11 bits down to 2^-21 of that one, and below it is off by 2^-32 of it (with the largest at 1, 2^-14 and
+// 2^-25: hundreds of thousands of keys at 2^-24 of a dominating one came out 1 % off).  l knows nothing of V: a scale of
+// 2^-109 or 2^119, the ends of what append writes, takes nothing from it, and a NaN row of V leaves the log-sum-exp as it is.
 // One exponential serves both: p'_j = 2^(x_j - m') vs_j and l in units of 2^m' with one factor 2^(m' - m) a group; where that
 // may leave the range of fp32 (V scales beyond 2^+-40) p'_j = 2^(x_j - m) vs_j 2^(m - m'), in this order, in the code for rare groups.
 // m and m' are whole numbers, so the factors and all rescaling are exact powers of two; log2 vs serves only to place m'.  They
-// move, both, when one is exceeded by more than 8, as in the dense kernel, and O is rescaled then.
+// move, both, when a score exceeds m by more than 8, as in the dense kernel, or a weight 2^15, and O is rescaled then.
 // Both products run on fp16 operands with fp32 accumulators: int8 and e4m3 codes are exact in fp16, bf16 queries are
 // scaled by a power of two of their row (what is below 2^-24 of the row's largest value is rounded).  The references
-// and l are fp32.
+// and l are fp32.  The tensor cores cut O towards zero at its last place every four keys: up to 2^-25 of it a key of the warp.
 //
 // The query rows of a kv head (T tokens of H / Hkv heads) are cut into row tiles, the keys into tiles of 64.  All
 // (sequence, kv head, row tile, key tile) of a call form one list that the CTAs share evenly, whatever the lengths are: a

@@ -17,7 +17,9 @@ constexpr int kTileKeys = 64;
 constexpr int kMinTiles = 2;               // tiles a CTA takes at the least
 constexpr float kLowest = -3.402823466e38f;   // of a reference: nothing seen yet
 constexpr float kLazy = 8.0f;              // log2 of what may exceed a reference before it moves
-constexpr float kMostWeight = 256.0f;      // 2^kLazy
+constexpr float kHigh = 8.0f;              // log2 of a row's largest weight when its reference is placed
+constexpr float kMostWeight = 32768.0f;    // a weight above it moves a reference
+constexpr float kMostLog = 15.0f;          // its log2
 constexpr float kMostSum = 256.0f;         // a mean of plain weights above it moves a reference
 constexpr float kTame = 40.0f;             // of the references' ratio, log2: what 2^(x - t) can carry
 constexpr float kMostRatio = 120.0f;       // of the references, log2: binds where every V row so far is zero (weights 0)
@@ -190,12 +192,12 @@ struct Softmax {
   __device__ __forceinline__ float v_unit() const { return fabsf(ratio); }                                        // 2^(t - m)
   __device__ __forceinline__ float score_unit() const { return __int_as_float((254 << 23) - __float_as_int(v_unit())); }   // 2^(m - t)
   // Whether a score x, or the same with the V scale in it, exceeds its reference by more than they wait for.
-  __device__ __forceinline__ bool exceeded(float x, float with_v) const { return x > m() + kLazy || with_v > t + kLazy; }
+  __device__ __forceinline__ bool exceeded(float x, float with_v) const { return x > m() + kLazy || with_v > t + kMostLog; }
   // Moves the references to the largest of either, rescales l, and returns the factor of O.
   __device__ __forceinline__ float move(float top, float top_v) {
     const float before = m(), old = exponent();
     const float next = fmaxf(before, ceilf(top)), step = before - next;
-    const float now = fminf(fmaxf(fmaxf(old + step, ceilf(top_v) - next), -kMostRatio), kMostRatio);
+    const float now = fminf(fmaxf(fmaxf(old + step, ceilf(top_v) - kHigh - next), -kMostRatio), kMostRatio);
     t = next + now;
     ratio = copysignf(__int_as_float(((int)now + 127) << 23), kTame - fabsf(now));
     l *= fast_exp2(step);

@@ -96,3 +96,33 @@ def test_a_v_row_with_nan_leaves_the_log_sum_exp(D, T, H, at):
     cache["v8"].view(torch.uint8)[p, :, r] = 0
     b, lb = compare(q, cache, table, lens)
     assert bool(b[0].isnan().all()) and torch.equal(b[1], a[1]) and torch.equal(lb[1], la[1])
+
+
+@pytest.mark.parametrize("D,T,H,B", [(64, 1, 8, 600), (128, 2, 8, 320), (256, 1, 4, 320), (64, 24, 4, 150), (128, 17, 4, 150)])
+@pytest.mark.parametrize("x", [3.78125, 2.953125, 2.53125])
+def test_one_dominating_key_over_a_long_context(D, T, H, B, x):
+    """A key at the front with score 20, hundreds of thousands of others at x: 2^-23.4 to 2^-25.2 of its weight each, 1 to 4
+    percent of the result together, and all of them rounded alike.  A row's largest weight is held at 2^7 or more, so what
+    fp16 cannot hold of a weight (half of its smallest step, 2^-25) is 2^-32 of that.  As many sequences over the same pages
+    as there are CTAs, so that a CTA works through all of the keys."""
+    n = 400000
+    cache, table = filled([n], T, 256, 1, D, seed=1)
+    g = torch.Generator(device=DEV).manual_seed(D)
+    k = torch.zeros((1, n + T, 1, D), device=DEV)
+    k[..., 0] = x
+    k[:, 0, :, 0] = 20.0
+    P.append(cache, k.bfloat16(), (1 + 0.5 * torch.rand(k.shape, device=DEV, generator=g)).bfloat16(), table, [0])
+    q = torch.zeros((1, T, H, D), device=DEV, dtype=torch.float16)
+    q[..., 0] = 1
+    o, lse = compare(q, cache, table, [n], sm_scale=1.0, lost=2.0 ** -32)
+    want, want_lse, mean, S, top = P.attention(q, cache, table, [n], sm_scale=1.0)
+    got, got_lse = rdna4_sage.attention_paged_kv(q.expand(B, -1, -1, -1), handle(cache), table.expand(B, -1), ints([n] * B),
+                                                 None, None, "NHD", 1.0, True)
+    # The tensor cores take four keys at a time and cut the sum towards zero at the accumulator's last place (seen with +1,
+    # small terms, -1: four terms of 0.9985 last places leave 3, those of 0.5 leave 1): less than 2^-23 of it each time, so
+    # 2^-25 for a key.  With few rows four warps share the keys.  The sum of the weights is rounded, by 2^-24 for 16 keys.
+    keys = n / 4 if T * H <= (16 if D == 256 else 32) else n
+    weight = 2 * ((D + 8) * 2.0 ** -24 * S.max() + 2.0 ** -22 * want_lse.max() + 2.0 ** -20) + (keys / 16 + 16) * 2.0 ** -24
+    tol = 2.0 ** -11 * want + mean * (2.0 ** -11 + weight + keys * 2.0 ** -25) + (n * 2.0 ** -32 * 448 * top)[..., None]
+    assert bool(((got.double() - want).abs() <= tol).all()), float(((got.double() - want).abs() / tol).max())
+    assert bool(((got_lse.double() - want_lse).abs() <= weight + 2.0 ** -23 * want_lse).all())
