@@ -144,8 +144,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
             for (int e = 0; e < 4; ++e) top = max(top, (e < 2 ? w[s].x : w[s].y) >> (16 * (e & 1)) & 0x7fffu);
           top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          // 2^e with e the exponent of the row's largest value (zero, infinite and NaN rows: 1; tiny ones: 2^-100)
-          const int e = top == 0 || top >= 0x7f80u ? 127 : max((int)(top >> 7), 27);
+          const int e = row_exponent(top);
           const float inverse = __int_as_float((254 - e) << 23);
 #pragma unroll
           for (int s = 0; s < NS; ++s) {
@@ -219,12 +218,13 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
       const float v_scale[2] = {ks[kTileKeys + keys[0]], ks[kTileKeys + keys[1]]};
       uint32_t pf[NR][2];
       bool again = true;
-      if constexpr (!std::is_same<T, __half>::value) {
-#pragma unroll
-        for (int r = 0; r < NR; ++r)
-#pragma unroll
-          for (int x = 0; x < 4; ++x) s[r][x] *= row_scale[r][x & 1];
-      }
+      // x - t of the lane's two rows.  The factor of the key comes first: a row's scale may be as large as 2^126.
+      auto less = [&](int r, uint64_t score, uint64_t by, uint64_t minus_t) {
+        if constexpr (std::is_same<T, __half>::value)
+          return f2_fma(score, by, minus_t);
+        else
+          return f2_fma(f2_mul(score, by), f2_pack(row_scale[r][0], row_scale[r][1]), minus_t);
+      };
       if (!drafts) {
         uint64_t l[NR];   // the lane's two rows as a pair
         float top = 0.0f;
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
           float x, y;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            f2_unpack(f2_fma(f2_pack(s[r][2 * h], s[r][2 * h + 1]), f2_pack(factor[h], factor[h]), minus_t), x, y);
+            f2_unpack(less(r, f2_pack(s[r][2 * h], s[r][2 * h + 1]), f2_pack(factor[h], factor[h]), minus_t), x, y);
             const uint64_t u = f2_pack(fast_exp2(x), fast_exp2(y));
             l[r] = h == 0 ? u : f2_add(l[r], u);
             f2_unpack(f2_mul(u, f2_pack(v_scale[h], v_scale[h])), x, y);
@@ -265,7 +265,8 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               float& x = s[r][2 * h + e];
-              x *= factor[h];                     // scaled by its row already
+              x *= factor[h];
+              if constexpr (!std::is_same<T, __half>::value) x *= row_scale[r][e];
               if (drafts) {
                 const int t = key0 + keys[h] - now.len, token = (row0 + 8 * r + 2 * c + e) / a.group;
                 const bool seen = t < 0 || (t < now.fresh && token < now.fresh &&

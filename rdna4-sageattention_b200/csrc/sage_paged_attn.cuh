@@ -206,6 +206,13 @@ struct Softmax {
   __device__ __forceinline__ RowState state() const { return RowState{m(), l, t}; }
 };
 
+// The exponent (biased) of a power of two near the largest value of a bf16 row, whose bits without the sign are `top`: with it
+// the row is divided before it becomes fp16.  Zero, infinite and NaN rows: 1; tiny ones: 2^-100; the largest: 2^126, the last
+// one whose inverse is normal (the row is then below 4).
+__device__ __forceinline__ int row_exponent(uint32_t top) {
+  return top == 0 || top >= 0x7f80u ? 127 : min(max((int)(top >> 7), 27), 253);
+}
+
 // As a bit pattern a positive float orders as it does as a number, with NaN and every negative one above.
 __device__ __forceinline__ uint32_t bits(float x) { return __float_as_uint(x); }
 

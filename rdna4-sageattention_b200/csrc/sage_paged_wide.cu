@@ -425,8 +425,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
 #pragma unroll
                   for (int o = 1; o < 16; o *= 2) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
                   top = max(top & 0xffffu, top >> 16);
-                  // 2^e with e the exponent of the row's largest value (zero, infinite and NaN rows: 1; tiny ones: 2^-100)
-                  const int e = top == 0 || top >= 0x7f80u ? 127 : max((int)(top >> 7), 27);
+                  const int e = row_exponent(top);
                   const float inverse = __int_as_float((254 - e) << 23);
                   if (ch == 0) q_scale[t][r128] = __int_as_float(e << 23);
                   float x[8];
@@ -463,8 +462,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
                                                __vmaxu2(v[i].z & 0x7fff7fffu, v[i].w & 0x7fff7fffu)));
               }
               top = max(top & 0xffffu, top >> 16);
-              // 2^e with e the exponent of that value (zero, infinite and NaN rows: 1; tiny ones: 2^-100)
-              const int e = top == 0 || top >= 0x7f80u ? 127 : max((int)(top >> 7), 27);
+              const int e = row_exponent(top);
               row_scale = __int_as_float(e << 23);
               inverse = __int_as_float((254 - e) << 23);
             }
@@ -547,10 +545,14 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
 #pragma unroll
                   for (int h = 0; h < 2; ++h) {
                     const int c = 4 * i + 2 * h;
-                    uint64_t v = f2_pack(__uint_as_float(r[c]), __uint_as_float(r[c + 1]));
-                    if constexpr (!std::is_same<T, __half>::value) v = f2_mul(v, scale2);
+                    const uint64_t score = f2_pack(__uint_as_float(r[c]), __uint_as_float(r[c + 1]));
+                    const uint64_t by = h ? f2_pack(f.z, f.w) : f2_pack(f.x, f.y);
                     float p, q;
-                    f2_unpack(f2_fma(v, h ? f2_pack(f.z, f.w) : f2_pack(f.x, f.y), minus_t), p, q);
+                    // the factor of the key first: a row's scale may be as large as 2^126
+                    if constexpr (std::is_same<T, __half>::value)
+                      f2_unpack(f2_fma(score, by, minus_t), p, q);
+                    else
+                      f2_unpack(f2_fma(f2_mul(score, by), scale2, minus_t), p, q);
                     const uint64_t u = f2_pack(fast_exp2(p), fast_exp2(q));
                     sum[h] = f2_add(u, sum[h]);
                     f2_unpack(f2_mul(u, h ? f2_pack(w.z, w.w) : f2_pack(w.x, w.y)), p, q);
@@ -608,9 +610,10 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
                   const float4 f = *reinterpret_cast<const float4*>(factor + 16 * k + i);
 #pragma unroll
                   for (int h = 0; h < 4; h += 2) {
-                    uint64_t v = f2_pack(__uint_as_float(r[i + h]), __uint_as_float(r[i + h + 1]));
+                    uint64_t v = f2_mul(f2_pack(__uint_as_float(r[i + h]), __uint_as_float(r[i + h + 1])),
+                                        h ? f2_pack(f.z, f.w) : f2_pack(f.x, f.y));
                     if constexpr (!std::is_same<T, __half>::value) v = f2_mul(v, f2_pack(row_scale, row_scale));
-                    f2_unpack(f2_mul(v, h ? f2_pack(f.z, f.w) : f2_pack(f.x, f.y)), x[i + h], x[i + h + 1]);
+                    f2_unpack(v, x[i + h], x[i + h + 1]);
                     if (!(seen >> (16 * k + i + h) & 1)) x[i + h] = -INFINITY;
                     if (!(seen >> (16 * k + i + h + 1) & 1)) x[i + h + 1] = -INFINITY;
                   }

@@ -126,3 +126,19 @@ def test_one_dominating_key_over_a_long_context(D, T, H, B, x):
     tol = 2.0 ** -11 * want + mean * (2.0 ** -11 + weight + keys * 2.0 ** -25) + (n * 2.0 ** -32 * 448 * top)[..., None]
     assert bool(((got.double() - want).abs() <= tol).all()), float(((got.double() - want).abs() / tol).max())
     assert bool(((got_lse.double() - want_lse).abs() <= weight + 2.0 ** -23 * want_lse).all())
+
+
+@pytest.mark.parametrize("D,T,H", SHAPES)
+@pytest.mark.parametrize("big", [3e38, 2.0 ** 127, 1.2e38])
+def test_queries_of_the_largest_size(D, T, H, big):
+    # One channel of each query near the end of bf16's range and small codes of K under it, the others a thousandth of that:
+    # scores of a few units with the smallest sm_scale that fp32 holds well.
+    lens = [300, 41]
+    cache, table = filled(lens, T, 32, 2, D, seed=D)
+    g = torch.Generator(device=DEV).manual_seed(T)
+    cache["k8"][..., 0] = torch.randint(-2, 3, cache["k8"].shape[:3], device=DEV, generator=g).to(torch.int8)
+    cache["ks"].copy_(torch.rand(cache["ks"].shape, device=DEV, generator=g) + 0.5)
+    q = queries(2, T, H, D, size=1e35)
+    q[..., 0] = torch.where(q[..., 0] > 0, big, -big)
+    o, lse = compare(q, cache, table, lens, sm_scale=2.0 ** -125)
+    assert float(lse.std()) > 0.5                        # the scores are no zeros
