@@ -249,7 +249,8 @@ int sage_rotary(const sage_rotary_args* args, void* stream);
  * lens: device int32 [B].  For append, keep and attention it is the context length BEFORE this step's tokens, which
  * hold positions lens[b], lens[b] + 1, ...; counts (nullable, device int32 [B], 0 .. S) gives their number where a
  * padded batch holds fewer than S of them.
- * Lengths, counts and page numbers are checked on the device: what lies outside is neither read nor written, and
+ * Lengths, counts and page numbers are checked on the device: a sequence with a negative length, or a count outside its
+ * range, is left as it was; what lies outside the table or the cache is neither read nor written; and
  * *status (nullable = the library's own word; pinned host memory will do) receives SAGE_ERR_INVALID. */
 typedef struct {
   int8_t* k8;

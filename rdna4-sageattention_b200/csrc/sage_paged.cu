@@ -86,11 +86,15 @@ __global__ void __launch_bounds__(256) append_kernel(const AppendArgs a) {
       x[w][r] = s0 + r < a.S && lane * 8 < D ? *reinterpret_cast<const uint4*>(src + r * a.st[w].s)
                                              : make_uint4(0, 0, 0, 0);
   }
-  const int n = a.counts != nullptr ? a.counts[b] : a.S, len = a.p.lens[b];
-  if (n < 0 || n > a.S) raise_invalid(a.p);
+  const int len = a.p.lens[b];
+  int n = a.counts != nullptr ? a.counts[b] : a.S;
+  if (n < 0 || n > a.S || len < 0) {   // none of the sequence's tokens: some would land in its context
+    raise_invalid(a.p);
+    n = 0;
+  }
 #pragma unroll
   for (int r = 0; r < kTokens; ++r) {
-    const bool live = s0 + r < min(n, a.S);
+    const bool live = s0 + r < n;
     const int64_t dst = live ? paged_row(a.p, b, h, (int64_t)len + s0 + r) : -1;
     // The largest magnitudes of the K row (low half) and of the V row, as 16-bit patterns: without the sign they order as
     // the numbers do, with infinity and NaN above every finite one.
@@ -213,7 +217,8 @@ __global__ void __launch_bounds__(256) keep_kernel(const KeepArgs a) {
   const int b = blockIdx.x / a.p.Hkv, h = blockIdx.x % a.p.Hkv;
   const int n = a.counts != nullptr ? a.counts[b] : a.N;
   const int* keep = a.keep + b * a.keep_stride;
-  bool bad = n < 0 || n > a.N;
+  const int64_t base = a.p.lens[b];
+  bool bad = n < 0 || n > a.N || base < 0;
   if (!bad)
     for (int i = threadIdx.x; i < n; i += 256) bad |= keep[i] < 0 || (i > 0 && keep[i] <= keep[i - 1]);
   if (__syncthreads_or(bad)) {
@@ -223,7 +228,6 @@ __global__ void __launch_bounds__(256) keep_kernel(const KeepArgs a) {
   const int r = threadIdx.x / (2 * LPR), w = threadIdx.x / LPR % 2, lane = threadIdx.x % LPR;
   uint8_t* codes = w == 0 ? reinterpret_cast<uint8_t*>(a.p.k8) : a.p.v8;
   float* scales = w == 0 ? a.p.ks : a.p.vs;
-  const int64_t base = a.p.lens[b];
   for (int i0 = 0; i0 < n; i0 += ROWS) {
     const int i = i0 + r;
     int64_t src = -1, dst = -1;
