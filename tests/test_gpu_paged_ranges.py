@@ -142,3 +142,22 @@ def test_queries_of_the_largest_size(D, T, H, big):
     q[..., 0] = torch.where(q[..., 0] > 0, big, -big)
     o, lse = compare(q, cache, table, lens, sm_scale=2.0 ** -125)
     assert float(lse.std()) > 0.5                        # the scores are no zeros
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_scales_are_the_quotients_rounded_once(dtype):
+    """Every finite largest value of a row that the type has.  a / 127 and a / 448, rounded to fp32: the reference divides in
+    64 bits and rounds again, which is the same, since a quotient with a 11-bit numerator and a 7-bit odd divisor lies on a
+    border between two floats or at least 2^-32 of itself away from it."""
+    x = torch.arange(2 ** 15 - 1, dtype=torch.int16, device=DEV).view(dtype)
+    x = x[torch.isfinite(x)]
+    k = torch.zeros((1, x.numel(), 1, 64), device=DEV, dtype=dtype)
+    k[0, :, 0, 3] = x
+    page = 256
+    table = torch.arange((x.numel() + page - 1) // page, dtype=torch.int32, device=DEV)[None]
+    got, want = (P.new_cache(table.numel(), page, 1, 64, DEV) for _ in range(2))
+    P.append(want, k, -k, table, [0])
+    rdna4_sage.paged_kv_append(handle(got), k, -k, table, ints([0]), tensor_layout="NHD")
+    for name in ("ks", "vs", "k8"):
+        assert torch.equal(got[name], want[name]), name
+    assert torch.equal(got["v8"].view(torch.uint8), want["v8"].view(torch.uint8))
