@@ -12,6 +12,7 @@ import math
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -167,6 +168,11 @@ def step(*tensors) -> torch.device:
     if _host_words[index][1].value or index in _watch:
         _raise_pending(dev)
     return dev
+
+
+def forward_mode() -> bool:
+    """Whether tensors may carry tangents: a level of forward-mode differentiation is open."""
+    return forward_ad._current_level >= 0
 
 
 def launch(index: int, what: str, entry, args: bytes) -> None:

@@ -16,9 +16,11 @@ the device (or check_status) raises RuntimeError.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _attention, _lib
-from ._attention import DTYPES, HEAD_DIMS, Unsupported, _current_device, _raw_stream, launch, step, step_rows
+from ._attention import (DTYPES, HEAD_DIMS, Unsupported, _current_device, _raw_stream, forward_mode, launch, step,
+                         step_rows)
 
 _alloc = torch._C._cuda_cudaCachingAllocator_raw_alloc
 _free = torch._C._cuda_cudaCachingAllocator_raw_delete
@@ -90,14 +92,15 @@ def _check_rows(kv, x, layout, heads=None):
     B, H, S = shape[:3] if layout == "HND" else (shape[0], shape[2], shape[1])
     if H % kv.kv_heads or H == 0 or (heads is not None and H != heads):
         raise Unsupported(f"heads {H} do not fit the cache's {kv.kv_heads} kv heads")
-    if x.requires_grad:
-        _no_grad()
+    _no_grad(x)
     return B, S, H
 
 
-def _no_grad():
-    if torch.is_grad_enabled():
+def _no_grad(x):
+    if x.requires_grad and torch.is_grad_enabled():
         raise Unsupported("the paged cache has no backward pass: call it under torch.no_grad()")
+    if forward_mode() and forward_ad.unpack_dual(x).tangent is not None:
+        raise Unsupported("the paged cache has no derivatives: pass the primal of a dual tensor")
 
 
 def paged_kv_append(kv, k, v, page_table, lens, counts=None, tensor_layout="HND"):
@@ -107,8 +110,7 @@ def paged_kv_append(kv, k, v, page_table, lens, counts=None, tensor_layout="HND"
     B, S, Hkv = _check_rows(kv, k, tensor_layout, kv.kv_heads)
     if v.shape != k.shape or v.dtype != k.dtype:
         raise Unsupported("k and v must match in shape and dtype")
-    if v.requires_grad:
-        _no_grad()
+    _no_grad(v)
     _check_table(page_table, lens, counts, B)
     if counts is None:
         dev = step(kv.k8, k, v, page_table, lens)

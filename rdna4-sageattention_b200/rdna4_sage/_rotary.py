@@ -8,9 +8,10 @@ from __future__ import annotations
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
-from ._attention import DTYPES, HEAD_DIMS, Unsupported, launch, step, step_rows
+from ._attention import DTYPES, HEAD_DIMS, Unsupported, forward_mode, launch, step, step_rows
 
 SCALINGS = (None, "linear", "ntk", "ramp")
 
@@ -148,18 +149,29 @@ class _RotaryFunction(torch.autograd.Function):
         dq = dq if ctx.needs_input_grad[0] else None
         dk = dk if ctx.needs_input_grad[1] else None
         args = (positions, ctx.rope, ctx.layout, ctx.turn_back)
-        if not torch.is_grad_enabled():
-            if dq is not None:
-                dq, dk = _launch(dq, dk, *args)
-            elif dk is not None:
-                dk, _ = _launch(dk, None, *args)
-        elif dq is not None and dk is not None:
-            dq, dk = _RotaryFunction.apply(dq, dk, *args)
-        elif dq is not None:
-            dq = _RotaryFunction.apply(dq, None, *args)
+        if dq is not None:
+            dq, dk = _turn(dq, dk, *args)
         elif dk is not None:
-            dk = _RotaryFunction.apply(dk, None, *args)
+            dk, _ = _turn(dk, None, *args)
         return dq, dk, None, None, None, None
+
+
+def _turn(q, k, positions, rope, layout, backward):
+    """(q, k) turned (k may be None), with the derivatives that the inputs ask for."""
+    if forward_mode():
+        # the op is linear: the tangent of a result is the op on the tangent
+        (q, tq), (k, tk) = forward_ad.unpack_dual(q), (None, None) if k is None else forward_ad.unpack_dual(k)
+        if tq is not None or tk is not None:
+            out = _turn(q, k, positions, rope, layout, backward)
+            if tq is not None and tk is not None:
+                tangents = _turn(tq, tk, positions, rope, layout, backward)
+            else:
+                tangents = [None if t is None else _turn(t, None, positions, rope, layout, backward)[0] for t in (tq, tk)]
+            return tuple(y if t is None else forward_ad.make_dual(y, t) for y, t in zip(out, tangents))
+    if (q.requires_grad or k is not None and k.requires_grad) and torch.is_grad_enabled():
+        out = _RotaryFunction.apply(q, k, positions, rope, layout, backward)
+        return (out, None) if k is None else out
+    return _launch(q, k, positions, rope, layout, backward)
 
 
 _MARK = "rdna4_sage capture"
@@ -189,7 +201,7 @@ def rotary(q, k, positions, rope, tensor_layout="HND"):
     """q and k turned to their positions: (B, H, S, D) and (B, Hkv, S, D) for "HND", (B, S, H, D) and (B, S, Hkv, D) for
     "NHD", fp16 or bf16; new tensors of the same shapes and types (rounded once).  k may be None: the result is q
     alone.  positions: int32 or int64 of any value, (S,) for all sequences or (B, S), on the GPU.  rope: a Rotary.
-    Differentiable in q and k.  A backward pass can be captured into a CUDA graph if no other graph of the same leaves is
+    Differentiable in q and k, in reverse and in forward mode (dual tensors).  A backward pass can be captured into a CUDA graph if no other graph of the same leaves is
     alive then; a leaf q or k that breaks this is refused, leaves further back are the caller's.  Raises Unsupported for
     inputs the kernel does not take."""
     _check(q, k, positions, rope, tensor_layout)
@@ -201,6 +213,5 @@ def rotary(q, k, positions, rope, tensor_layout="HND"):
         if torch.cuda.is_current_stream_capturing():   # the nodes are held until the graph below holds them
             at = torch.cuda.current_stream(q.device).cuda_stream
             held = [_accumulator(x, at) for x in (q, k) if x is not None and x.requires_grad and x.is_leaf]  # noqa: F841
-        return _RotaryFunction.apply(q, k, positions, rope, tensor_layout, False)
-    q_out, k_out = _launch(q, k, positions, rope, tensor_layout, False)
+    q_out, k_out = _turn(q, k, positions, rope, tensor_layout, False)
     return q_out if k is None else (q_out, k_out)
