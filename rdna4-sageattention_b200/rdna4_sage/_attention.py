@@ -146,8 +146,9 @@ def _raise_host_word(device: torch.device) -> None:
 
 
 _ready: dict[int, torch.device] = {}   # GPUs that step() has checked
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
+# absent from a torch built without CUDA, where step() refuses every call before they are used
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
 def step(*tensors) -> torch.device:

@@ -22,8 +22,8 @@ from . import _attention, _lib
 from ._attention import (DTYPES, HEAD_DIMS, Unsupported, _current_device, _raw_stream, forward_mode, launch, step,
                          step_rows)
 
-_alloc = torch._C._cuda_cudaCachingAllocator_raw_alloc
-_free = torch._C._cuda_cudaCachingAllocator_raw_delete
+_alloc = getattr(torch._C, "_cuda_cudaCachingAllocator_raw_alloc", None)   # absent from a torch built without CUDA
+_free = getattr(torch._C, "_cuda_cudaCachingAllocator_raw_delete", None)
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 
