@@ -184,13 +184,17 @@ def _accumulator(x, stream):
     outlives the last reference held here only if another graph holds the node."""
     edge = torch.autograd.graph.get_gradient_edge
     node = edge(x).node
-    if node.metadata.get(_MARK) == stream:   # an earlier call of this capture
+    before = node.metadata.get(_MARK)
+    if before == stream:   # an earlier call of this capture
         return node
     node.metadata[_MARK] = stream
     del node
     node = edge(x).node
     if _MARK in node.metadata:
-        del node.metadata[_MARK]
+        if before is None:
+            del node.metadata[_MARK]
+        else:
+            node.metadata[_MARK] = before
         raise Unsupported("a graph of this leaf from outside the capture is alive, so its gradient cannot be captured: "
                           "release that graph first (or pass a view of the leaf if it was recorded on this stream)")
     node.metadata[_MARK] = stream

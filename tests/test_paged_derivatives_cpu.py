@@ -88,3 +88,18 @@ def test_the_cache_refuses_dual_tensors():
                     rdna4_sage.attention_paged_kv(dual(q), kv, table, lens, tensor_layout="NHD")
         with pytest.raises(Unsupported, match="CUDA GPU"):           # a plain tensor at a dual level goes on
             rdna4_sage.attention_paged_kv(q, kv, table, lens, tensor_layout="NHD")
+
+
+def test_a_refused_capture_leaves_the_mark_of_an_earlier_one():
+    """A graph captured on stream 7 is alive: a capture on 8 is refused, another one on 7 still is not."""
+    x = torch.randn(3, requires_grad=True)
+    node = _rotary._accumulator(x, 7)
+    y = x * 2
+    del node
+    with pytest.raises(Unsupported, match="outside the capture"):
+        _rotary._accumulator(x, 8)
+    _rotary._accumulator(x, 7)
+    with pytest.raises(Unsupported, match="outside the capture"):
+        _rotary._accumulator(x, 8)
+    y.sum().backward()
+    assert torch.equal(x.grad, torch.full_like(x, 2.0))
