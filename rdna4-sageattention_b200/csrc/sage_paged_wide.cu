@@ -599,80 +599,74 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
                   }
                 }
               }
-              // the scores of 16 keys; small loops on purpose: this code runs once or twice a row tile, and what it costs
-              // is fetching it
-              auto scaled = [&](int k, float (&x)[16]) {
-                uint32_t r[16];
-                tmem_ld16(s_at + 16 * k, r);
-                tmem_wait_ld();
-#pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                  const float4 f = *reinterpret_cast<const float4*>(factor + 16 * k + i);
-#pragma unroll
-                  for (int h = 0; h < 4; h += 2) {
-                    uint64_t v = f2_mul(f2_pack(__uint_as_float(r[i + h]), __uint_as_float(r[i + h + 1])),
-                                        h ? f2_pack(f.z, f.w) : f2_pack(f.x, f.y));
-                    if constexpr (!std::is_same<T, __half>::value) v = f2_mul(v, f2_pack(row_scale, row_scale));
-                    f2_unpack(v, x[i + h], x[i + h + 1]);
-                    if (!(seen >> (16 * k + i + h) & 1)) x[i + h] = -INFINITY;
-                    if (!(seen >> (16 * k + i + h + 1) & 1)) x[i + h + 1] = -INFINITY;
-                  }
-                }
-              };
-              float most = -INFINITY, most_t = -INFINITY;
-#pragma unroll 1
-              for (int k = 0; k < kTileKeys / 16; ++k) {
-                float x[16];
-                scaled(k, x);
-#pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                  const float4 log_v = *reinterpret_cast<const float4*>(factor + 2 * kTileKeys + 16 * k + i);
-#pragma unroll
-                  for (int h = 0; h < 4; h += 2) {
-                    float p, q;
-                    f2_unpack(f2_add(f2_pack(x[i + h], x[i + h + 1]), h ? f2_pack(log_v.z, log_v.w) : f2_pack(log_v.x, log_v.y)), p, q);
-                    most = fmaxf(fmaxf(most, x[i + h]), x[i + h + 1]);
-                    most_t = fmaxf(fmaxf(most_t, p), q);
-                  }
-                }
-              }
-              const bool moves = sm.exceeded(most, most_t);
-              if (__any_sync(0xffffffffu, moves)) {
-                float keep = 1.0f;
-                if (moves) keep = sm.move(most, most_t);
-                if (tile != first_tile) {   // the first product of a row tile overwrites O
-                  // the products of the tile before must be done (older ones are: this tile's scores came after them)
-                  wait_stage(pv_done + t, pv_phase, &given_up, a.p.status);
-                  tc_fence_after();
-#pragma unroll 1
-                  for (int i = 0; i < D / 16; ++i) {
-                    uint32_t r[16];
-                    tmem_ld16(o_at + 16 * i, r);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * keep);
-                    tmem_st16(o_at + 16 * i, r);
-                  }
-                }
-              }
-              const float m = sm.m(), unit = sm.score_unit();
+              // 16 keys at a time, once for the references and once for the weights; one small loop on purpose: this code runs
+              // once or twice a row tile, and what it costs is fetching it
+              float most = -INFINITY, most_t = -INFINITY, m = 0.0f, unit = 0.0f;
               uint64_t sum = f2_pack(0.0f, 0.0f);
 #pragma unroll 1
-              for (int k = 0; k < kTileKeys / 16; ++k) {   // the weights of 16 keys take 8 columns, all read by then
-                float x[16];
-                scaled(k, x);
-                uint32_t w[8];
+              for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll 1
+                for (int k = 0; k < kTileKeys / 16; ++k) {
+                  const float* by = factor + 16 * k;
+                  float x[16];
+                  uint32_t r[16];
+                  tmem_ld16(s_at + 16 * k, r);
+                  tmem_wait_ld();
+                  const uint32_t see = (uint32_t)(seen >> (16 * k));
 #pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                  const float2 vs = *reinterpret_cast<const float2*>(factor + kTileKeys + 16 * k + i);
-                  const uint64_t u = f2_pack(fast_exp2(x[i] - m), fast_exp2(x[i + 1] - m));
-                  sum = f2_add(sum, u);
-                  float p, q;
-                  f2_unpack(f2_mul(f2_mul(u, f2_pack(vs.x, vs.y)), f2_pack(unit, unit)), p, q);
-                  // the scale of a key not seen may be anything
-                  w[i / 2] = pack_weights(x[i] == -INFINITY ? 0.0f : p, x[i + 1] == -INFINITY ? 0.0f : q);
+                  for (int i = 0; i < 16; i += 2) {
+                    const float2 f = *reinterpret_cast<const float2*>(by + i);
+                    uint64_t v = f2_mul(f2_pack(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), f2_pack(f.x, f.y));
+                    if constexpr (!std::is_same<T, __half>::value) v = f2_mul(v, f2_pack(row_scale, row_scale));
+                    f2_unpack(v, x[i], x[i + 1]);
+                    if (!(see >> i & 1)) x[i] = -INFINITY;
+                    if (!(see >> (i + 1) & 1)) x[i + 1] = -INFINITY;
+                  }
+                  if (pass == 0) {
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) {
+                      const float2 log_v = *reinterpret_cast<const float2*>(by + 2 * kTileKeys + i);
+                      float p, q;
+                      f2_unpack(f2_add(f2_pack(x[i], x[i + 1]), f2_pack(log_v.x, log_v.y)), p, q);
+                      most = fmaxf(fmaxf(most, x[i]), x[i + 1]);
+                      most_t = fmaxf(fmaxf(most_t, p), q);
+                    }
+                  } else {
+                    uint32_t w[8];
+#pragma unroll
+                    for (int i = 0; i < 16; i += 2) {
+                      const float2 vs = *reinterpret_cast<const float2*>(by + kTileKeys + i);
+                      const uint64_t u = f2_pack(fast_exp2(x[i] - m), fast_exp2(x[i + 1] - m));
+                      sum = f2_add(sum, u);
+                      float p, q;
+                      f2_unpack(f2_mul(f2_mul(u, f2_pack(vs.x, vs.y)), f2_pack(unit, unit)), p, q);
+                      // the scale of a key not seen may be anything
+                      w[i / 2] = pack_weights(x[i] == -INFINITY ? 0.0f : p, x[i + 1] == -INFINITY ? 0.0f : q);
+                    }
+                    tmem_st8(s_at + 8 * k, w);   // over 8 columns of scores, all read by then
+                  }
                 }
-                tmem_st8(s_at + 8 * k, w);
+                if (pass > 0) break;
+                const bool moves = sm.exceeded(most, most_t);
+                if (__any_sync(0xffffffffu, moves)) {
+                  float keep = 1.0f;
+                  if (moves) keep = sm.move(most, most_t);
+                  if (tile != first_tile) {   // the first product of a row tile overwrites O
+                    // the products of the tile before must be done (older ones are: this tile's scores came after them)
+                    wait_stage(pv_done + t, pv_phase, &given_up, a.p.status);
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int i = 0; i < D / 16; ++i) {
+                      uint32_t r[16];
+                      tmem_ld16(o_at + 16 * i, r);
+                      tmem_wait_ld();
+#pragma unroll
+                      for (int k = 0; k < 16; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * keep);
+                      tmem_st16(o_at + 16 * i, r);
+                    }
+                  }
+                }
+                m = sm.m(), unit = sm.score_unit();
               }
               float p, q;
               f2_unpack(sum, p, q);
