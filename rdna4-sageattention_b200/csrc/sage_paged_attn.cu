@@ -257,6 +257,19 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
       }
       if (again) {
         const float log_v[2] = {__log2f(v_scale[0]), __log2f(v_scale[1])};   // of a zero row -infinity
+        // what the lane's rows do not see, bit 4 r + 2 e + h; a loop, since fetching this code is what it costs
+        uint32_t hidden = 0;
+        if (drafts) {
+#pragma unroll 1
+          for (int i = 0; i < 4 * NR; ++i) {
+            const int row = row0 + 8 * (i / 4) + 2 * c + i / 2 % 2, key = g + S::slot_key(n + i % 2 * 8);
+            const int t = key0 + key - now.len;   // number of the key as a draft
+            const bool seen = t < 0 || (t < now.fresh && row < now.fresh * a.group &&
+                                        (a.mask != nullptr ? a.mask[now.b * a.mask_b + row / a.group * a.mask_i + t] != 0
+                                                           : t * a.group <= row));
+            hidden |= (uint32_t)!seen << i;
+          }
+        }
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
           float keep[2];
@@ -267,13 +280,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
               float& x = s[r][2 * h + e];
               x *= factor[h];
               if constexpr (!std::is_same<T, __half>::value) x *= row_scale[r][e];
-              if (drafts) {
-                const int t = key0 + keys[h] - now.len, token = (row0 + 8 * r + 2 * c + e) / a.group;
-                const bool seen = t < 0 || (t < now.fresh && token < now.fresh &&
-                                            (a.mask != nullptr ? a.mask[now.b * a.mask_b + token * a.mask_i + t] != 0
-                                                               : t <= token));
-                if (!seen) x = -INFINITY;
-              }
+              if (hidden >> (4 * r + 2 * e + h) & 1) x = -INFINITY;
             }
             float top = fmaxf(s[r][e], s[r][2 + e]), top_v = fmaxf(s[r][e] + log_v[0], s[r][2 + e] + log_v[1]);
 #pragma unroll
