@@ -29,11 +29,12 @@
 // and the query rows its 8 columns, so that the 1 to 8 rows of a single token's group cost one column tile.
 //
 // Bound by memory: one token (4 query rows a kv head) over 16 sequences of 16 to 32 thousand keys, 8 kv heads, D 128, takes
-// 147 to 157 us on B200, 85 to 91 % of the measured copy rate; issue slots are 57 % taken.  Steps on the way, us: one CTA a row
-// 11122; shared list, rows times keys, cp.async 257; transposed products, TMA 175; no logarithm and no comparison a key where
-// no maximum moves 156; warps joining all at once 145; two references 148.  One token over 1024 keys takes 11.7 us with the join, most of it
-// start-up and dependent loads.  D 256 reaches 87 % of the rate for 8 rows and 63 % for 16, for which each key is converted
-// twice: two column tiles a warp do not fit the registers.
+// 149 to 163 us on B200 (one box and another), 82 to 89 % of the measured copy rate; issue slots are 58 % taken.  D 64, 96 and
+// 256 reach 72, 84 and 91 %.  Steps on the way, us: one CTA a row 11122; shared list, rows times keys, cp.async 257; transposed
+// products, TMA 175; no logarithm and no comparison a key where no maximum moves 156; warps joining all at once 146; two
+// references 149.  One token over 1024 keys takes 11.3 us with the join, most of it start-up and dependent loads.  With more than
+// 16 rows (D 256: 8) each key is converted twice, since more column tiles a warp do not fit the registers: 8 drafts of 8
+// sequences over 8190 keys, D 128, take 56 us, 28 % of the rate.
 #include "sage_paged_attn.cuh"
 
 namespace sage {
@@ -622,9 +623,15 @@ static Shape row_tile(int64_t rows, int D) {
   return {2, rows <= 16 ? 1 : 2};
 }
 
-// From which rows of a kv head on the kernel for many rows is taken.  Measured on B200, 8 sequences of 8190 keys, 8 kv heads
-// (D 256: 16), us, few / many: D 128: 32 rows 74 / 79, 36 rows 108 / 78; D 64: 32 rows 46 / 66, 36 rows 70 / 67; D 96: 32 rows
-// 55 / 75, 36 rows 86 / 75; D 256: 16 rows 133 / 202, 17 rows 227 / 204.
+// From which rows of a kv head on the kernel for many rows is taken: when they do not fit this kernel's row tile.  Up to there it
+// is the faster one whatever the batch and the context are.  Measured on B200 on the device, 32 rows (D 256: 16) of 8 kv heads, us,
+// few / many:
+//   sequences x keys   1 x 500    1 x 4000   8 x 250    8 x 1000   64 x 250   8 x 8190   64 x 2000
+//   D 64               12 / 15    22 / 31    15 / 18    18 / 24    32 / 44    39 / 55    78 / 112
+//   D 96               12 / 17    25 / 40    16 / 20    20 / 27    38 / 48    47 / 61    97 / 126
+//   D 128              14 / 19    26 / 47    19 / 24    24 / 32    44 / 58    57 / 67    118 / 140
+//   D 256              14 / 24    26 / 63    17 / 25    24 / 39    41 / 69    65 / 95    125 / 197
+// Two row tiles here took 108 us for 36 rows of 8 x 8190 keys, D 128, where the other kernel took 78 (D 64: 70 / 67, D 96: 86 / 75).
 static bool wide(int64_t rows, int D) { return rows > (D == 256 ? 16 : 32); }
 
 static int shared_ctas(int D, Shape s) { return sm_count() * (s.nr == 1 && D <= 128 ? 4 : D == 64 ? 3 : 2); }

@@ -13,10 +13,11 @@
 // TMEM (512 columns): O_t at t D, the score tiles of t at QT D + 128 t, P over the first half of its scores; Q_t behind
 // them where it fits (D 64 and 256), else in shared memory (D 96 and 128).
 //
-// 8 trees of 64 drafts (256 rows a kv head) over up to 8190 keys, 8 kv heads, D 128: 88 us on B200, 583 TFLOP/s, where the
-// few-rows kernel takes 373 (8190 keys each) against 107 here.  No unit is full: tensor pipe 27 %, issue 42 %.  A key tile
-// passes through conversion, scores, softmax and values in about 2000 cycles, and leaving out the exponentials, the loads of
-// what a key needs, or most of either product changes the time by less than 10 % each.
+// 8 trees of 64 drafts (256 rows a kv head) over up to 8190 keys, 8 kv heads, D 128: 89 us on B200, 578 TFLOP/s (8190 keys
+// each: 107, where the few-rows kernel took 373).  48 us with up to 2048 keys, so a good 30 us do not grow with the keys: the start
+// of each CTA's stretch, partial rows and their join.  No unit is full: tensor pipe 34 %, issue 47 %.  A key tile passes through
+// conversion, scores, softmax and values in about 2000 cycles, and leaving out the exponentials, the loads of what a key needs, or
+// most of either product changes the time by less than 10 % each.
 #include "sage_paged_attn.cuh"
 
 namespace sage {
@@ -393,7 +394,9 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
       if (act) {
         if (warp_live) {
           if constexpr (D == 128) {
-            // 16 lanes a row, two rows at a time: whole lines (a row a lane would touch each line eight times over)
+            // 16 lanes a row, two rows at a time: whole lines (a row a lane touches each line eight times over).  Not taken
+            // for D 64 and 256, whose rows go to TMEM, where a lane holds its own row, nor for D 96, whose 12 chunks do not
+            // divide a warp: they load a row a lane.
             const int tile_row = now.unit % a.row_tiles * W::kRows + t * 128, base = warp % 4 * 32 + lane / 16, ch = lane % 16;
             int tok = (tile_row + base) / a.group, in_group = (tile_row + base) - tok * a.group;
             const T* heads = static_cast<const T*>(a.q) + now.b * a.q_st.b + (int64_t)(now.unit / a.row_tiles) * a.group * a.q_st.h;
