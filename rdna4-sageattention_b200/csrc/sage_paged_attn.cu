@@ -12,7 +12,7 @@
 // 2^-25: hundreds of thousands of keys at 2^-24 of a dominating one came out 1 % off).  l knows nothing of V: a scale of
 // 2^-109 or 2^119, the ends of what append writes, takes nothing from it, and a NaN row of V leaves the log-sum-exp as it is.
 // One exponential serves both: p'_j = 2^(x_j - m') vs_j and l in units of 2^m' with one factor 2^(m' - m) a group; where that
-// may leave the range of fp32 (V scales beyond 2^+-40) p'_j = 2^(x_j - m) vs_j 2^(m - m'), in this order, in the code for rare groups.
+// may leave the range of fp32 (V scales above 2^72) p'_j = 2^(x_j - m) vs_j 2^(m - m'), in this order, in the code for rare groups.
 // m and m' are whole numbers, so the factors and all rescaling are exact powers of two; log2 vs serves only to place m'.  They
 // move, both, when a score exceeds m by more than 8, as in the dense kernel, or a weight 2^15, and O is rescaled then.
 // Both products run on fp16 operands with fp32 accumulators: int8 and e4m3 codes are exact in fp16, bf16 queries are

@@ -21,8 +21,10 @@ constexpr float kHigh = 8.0f;              // log2 of a row's largest weight whe
 constexpr float kMostWeight = 32768.0f;    // a weight above it moves a reference
 constexpr float kMostLog = 15.0f;          // its log2
 constexpr float kMostSum = 256.0f;         // a mean of plain weights above it moves a reference
-constexpr float kTame = 40.0f;             // of the references' ratio, log2: what 2^(x - t) can carry
-constexpr float kMostRatio = 120.0f;       // of the references, log2: binds where every V row so far is zero (weights 0)
+// Bounds of the references' ratio, log2.  From -110 up the sum of 64 numbers 2^(x - t) stays below 2^125; the lower bound binds
+// where every V row so far is zero (their weights are 0) and for V scales below 2^-102, whose weights then lie up to 2^7 lower in
+// fp16.  Up to 64 the weights down to 2^-62 of the largest are normal numbers.  120 is beyond all that append writes.
+constexpr float kLeastRatio = -110.0f, kTameRatio = 64.0f, kMostRatio = 120.0f;
 
 // What is known of a query row beside its O: the reference of its scores, the sum of its weights, the reference of its
 // scores with the V scale in them (all three in the units of 2^x).
@@ -197,9 +199,9 @@ struct Softmax {
   __device__ __forceinline__ float move(float top, float top_v) {
     const float before = m(), old = exponent();
     const float next = fmaxf(before, ceilf(top)), step = before - next;
-    const float now = fminf(fmaxf(fmaxf(old + step, ceilf(top_v) - kHigh - next), -kMostRatio), kMostRatio);
+    const float now = fminf(fmaxf(fmaxf(old + step, ceilf(top_v) - kHigh - next), kLeastRatio), kMostRatio);
     t = next + now;
-    ratio = copysignf(__int_as_float(((int)now + 127) << 23), kTame - fabsf(now));
+    ratio = copysignf(__int_as_float(((int)now + 127) << 23), kTameRatio - now);
     l *= fast_exp2(step);
     return fast_exp2(step + (old - now));
   }

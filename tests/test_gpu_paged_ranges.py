@@ -44,9 +44,10 @@ SHAPES = [(64, 1, 2), (96, 2, 8), (128, 1, 8), (128, 4, 16), (256, 1, 8), (256, 
 
 
 @pytest.mark.parametrize("D,T,H", SHAPES)
-@pytest.mark.parametrize("power", [-101, 124])
+@pytest.mark.parametrize("power", [-101, -97, -80, -40, 60, 75, 84, 124])
 def test_v_rows_of_the_smallest_and_largest_size(D, T, H, power):
-    # scales near 2^-108 and 2^117, the ends of what append writes: neither the weights' sum nor a result is lost
+    # scales near 2^-108 and 2^117, the ends of what append writes, and between them, on either side of where one exponential
+    # no longer serves both sums: neither the weights' sum nor a result is lost
     lens = [5000, 70]
     cache, table = filled(lens, T, 32, 2, D, seed=D + T)
     cache["vs"].mul_(2.0 ** power)
