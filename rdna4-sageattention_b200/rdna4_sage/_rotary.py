@@ -26,6 +26,7 @@ class Rotary:
       scaling="ntk"     base * factor^(rotary_dim / (rotary_dim - 2)) in place of base
       scaling="ramp"    w_i (g / 1 + (1 - g) / factor), where g rises from 0 to 1 as the number of turns within
                         original_len positions, r_i = original_len w_i / (2 pi), rises from ramp[0] to ramp[1]
+                        (programs that let g rise with i between the two have other frequencies: give those themselves)
     `magnitude` multiplies the turned channels (default 1; for "ramp" 0.1 ln(factor) + 1).  `frequencies`: a tensor or
     list of rotary_dim / 2 radians per position in place of all this.
     """

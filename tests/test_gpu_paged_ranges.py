@@ -162,3 +162,33 @@ def test_scales_are_the_quotients_rounded_once(dtype):
     for name in ("ks", "vs", "k8"):
         assert torch.equal(got[name], want[name]), name
     assert torch.equal(got["v8"].view(torch.uint8), want["v8"].view(torch.uint8))
+
+
+@pytest.mark.parametrize("D,T,H", SHAPES)
+@pytest.mark.parametrize("power", [8, 17, 18, 19, 21, 26, 40, 80])
+def test_scores_far_beyond_the_fraction_of_fp32(D, T, H, power):
+    """Scores 2^power times a whole number up to 100, exact in fp32, in one channel: each row's largest belongs to one key, by
+    2^power or more, and the result is that key's V row.  One row of V is 2^40 times smaller than the others, so that the
+    references of scores and of weights lie apart."""
+    lens = [700, 45]
+    cache, table = filled(lens, T, 32, 2, D, seed=T)
+    cache["ks"].fill_(1.0)
+    cache["k8"].zero_()
+    g = torch.Generator(device=DEV).manual_seed(power)
+    for b in range(2):
+        at = torch.arange(lens[b] + T, device=DEV)
+        p, r = P.place(cache, table, b, at)
+        for head in range(2):
+            code = torch.randint(-90, 91, (lens[b] + T,), device=DEV, generator=g)
+            order = torch.randperm(lens[b], device=DEV, generator=g)
+            code[order[0]], code[order[1]] = 100, -100
+            cache["k8"][p, head, r, 0] = code.to(torch.int8)
+        p, r = P.place(cache, table, b, order[2:3])
+        cache["vs"][p, :, r] *= 2.0 ** -40
+    q = torch.zeros((2, T, H, D), device=DEV, dtype=torch.bfloat16)
+    q[..., 0] = 2.0 ** power * torch.where(torch.rand((2, T, H), device=DEV, generator=g) < 0.5, -1.0, 1.0)
+    o, lse = rdna4_sage.attention_paged_kv(q, handle(cache), table, ints(lens), None, None, "NHD", 1.0, True)
+    want, want_lse, *_ = P.attention(q, cache, table, lens, sm_scale=1.0)
+    # the other keys' weights are below exp(-2^8) each: nothing.  e4m3 times a scale, weight times scale in fp16, one rounding
+    assert bool(((o.double() - want).abs() <= (2.0 ** -8 + 2.0 ** -11 + 2.0 ** -20) * want.abs()).all())
+    assert bool(((lse.double() - want_lse).abs() <= 2.0 ** -22 * want_lse.abs()).all())
