@@ -172,8 +172,8 @@ def attention_paged_kv(q, kv, page_table, lens, tree_mask=None, counts=None, ten
     (B, T, H, D) for "NHD".  Token i of sequence b sees the context (positions before lens[b]) and of the step's own
     tokens those t <= i, or with tree_mask (bool [T, T] or [B, T, T]) those with tree_mask[b, i, t].  counts (int32 [B],
     0..T): the tokens of each sequence in a padded batch.  sm_scale: factor of the scores (default, and for values up to
-    0: 1 / sqrt(D)).  Returns the result in q's layout and dtype, and with return_lse also the (B, H, T) fp32 log-sum-exp; tokens from counts[b] on, and rows that see nothing, are zero with
-    log-sum-exp -inf."""
+    0: 1 / sqrt(D)).  Returns the result in q's layout and dtype, and with return_lse also the (B, H, T) fp32 log-sum-exp;
+    tokens from counts[b] on, and rows that see nothing, are zero with log-sum-exp -inf."""
     B, T, H = _check_rows(kv, q, tensor_layout)
     _check_table(page_table, lens, counts, B)
     tensors = [kv.k8, q, page_table, lens]
