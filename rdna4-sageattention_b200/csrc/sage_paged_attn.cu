@@ -29,12 +29,12 @@
 // and the query rows its 8 columns, so that the 1 to 8 rows of a single token's group cost one column tile.
 //
 // Bound by memory: one token (4 query rows a kv head) over 16 sequences of 16 to 32 thousand keys, 8 kv heads, D 128, takes
-// 149 to 163 us on B200 (one box and another), 82 to 89 % of the measured copy rate; issue slots are 58 % taken.  D 64, 96 and
-// 256 reach 72, 84 and 91 %.  Steps on the way, us: one CTA a row 11122; shared list, rows times keys, cp.async 257; transposed
-// products, TMA 175; no logarithm and no comparison a key where no maximum moves 156; warps joining all at once 146; two
-// references 149.  One token over 1024 keys takes 11.3 us with the join, most of it start-up and dependent loads.  With more than
-// 16 rows (D 256: 8) each key is converted twice, since more column tiles a warp do not fit the registers: 8 drafts of 8
-// sequences over 8190 keys, D 128, take 56 us, 28 % of the rate.
+// 149 to 157 us on B200 (by the box), 85 to 89 % of the measured copy rate; issue slots are 58 % taken.  D 64, 96 and 256
+// reach 72, 84 and 91 %.  Steps on the way, us: one CTA a row 11122; shared list, rows times keys, cp.async 257; transposed
+// products, TMA 175; no logarithm and no comparison a key where no maximum moves 156; warps joining all at once 147; two
+// references 149.  One token over 1024 keys takes 11.3 us with the join, most of it start-up and dependent loads.  With more
+// than 16 rows (D 256: 8) each key is converted twice, since more column tiles a warp do not fit the registers: 8 drafts of 8
+// sequences over 8190 keys, D 128, take 55 us, 29 % of the rate.
 #include "sage_paged_attn.cuh"
 
 namespace sage {
@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
   // -------------------------------------------------------------------- consumers
   const int n = lane / 4, c = lane % 4, wm = warp % WM, wk = warp / WM;
   uint32_t qf[NR][NS][2];
-  float o[NR][NT][4], row_scale[NR][2];
+  float o[NR][NT][4];
   Softmax sm[NR][2];
   bool fresh_unit = true;
   int segment = 0;                    // row tiles that this CTA has finished
@@ -154,8 +154,8 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
             qf[r][s][1] = pack2(__uint_as_float(w[s].y << 16) * inverse, __uint_as_float(w[s].y & 0xffff0000u) * inverse,
                                 __half());
           }
-          row_scale[r][0] = __int_as_float(__shfl_sync(0xffffffffu, e, 8 * c) << 23);
-          row_scale[r][1] = __int_as_float(__shfl_sync(0xffffffffu, e, 8 * c + 4) << 23);
+          sm[r][0].set_row_exponent(__shfl_sync(0xffffffffu, e, 8 * c));
+          sm[r][1].set_row_exponent(__shfl_sync(0xffffffffu, e, 8 * c + 4));
         }
       }
     }
@@ -224,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
         if constexpr (std::is_same<T, __half>::value)
           return f2_fma(score, by, minus_t);
         else
-          return f2_fma(f2_mul(score, by), f2_pack(row_scale[r][0], row_scale[r][1]), minus_t);
+          return f2_fma(f2_mul(score, by), f2_pack(sm[r][0].row_scale(), sm[r][1].row_scale()), minus_t);
       };
       if (!drafts) {
         uint64_t l[NR];   // the lane's two rows as a pair
@@ -243,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
             top = fmaxf(fmaxf(top, x), y);
             pf[r][h] = pack_weights(x, y);
           }
-          l[r] = f2_mul(l[r], f2_pack(sm[r][0].ratio, sm[r][1].ratio));
+          l[r] = f2_mul(l[r], f2_pack(sm[r][0].ratio(), sm[r][1].ratio()));
           f2_unpack(l[r], x, y);
           most = max(max(most, bits(x)), bits(y));
         }
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, Config<D, NR, WM>::kCtas)
             for (int h = 0; h < 2; ++h) {
               float& x = s[r][2 * h + e];
               x *= factor[h];
-              if constexpr (!std::is_same<T, __half>::value) x *= row_scale[r][e];
+              if constexpr (!std::is_same<T, __half>::value) x *= sm[r][e].row_scale();
               if (hidden >> (4 * r + 2 * e + h) & 1) x = -INFINITY;
             }
             float top = fmaxf(s[r][e], s[r][2 + e]), top_v = fmaxf(s[r][e] + log_v[0], s[r][2 + e] + log_v[1]);

@@ -566,7 +566,7 @@ __global__ void __launch_bounds__(Wide<D>::kThreads, 1)
               }
               float p, q;
               f2_unpack(f2_add(sum[0], sum[1]), p, q);
-              p = (p + q) * sm.ratio;
+              p = (p + q) * sm.ratio();
               again = __any_sync(0xffffffffu, !(fmaxf(top[0], top[1]) <= kMostWeight) || bits(p) > bits(kTileKeys * kMostSum));
               if (!again) sm.l += p;
             }
