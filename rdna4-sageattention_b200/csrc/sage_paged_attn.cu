@@ -29,7 +29,7 @@
 // and the query rows its 8 columns, so that the 1 to 8 rows of a single token's group cost one column tile.
 //
 // Bound by memory: one token (4 query rows a kv head) over 16 sequences of 16 to 32 thousand keys, 8 kv heads, D 128, takes
-// 149 to 157 us on B200 (by the box), 85 to 89 % of the measured copy rate; issue slots are 58 % taken.  D 64, 96 and 256
+// 149 to 157 us on B200 (by the GPU), 85 to 89 % of the measured copy rate; issue slots are 58 % taken.  D 64, 96 and 256
 // reach 72, 84 and 91 %.  Steps on the way, us: one CTA a row 11122; shared list, rows times keys, cp.async 257; transposed
 // products, TMA 175; no logarithm and no comparison a key where no maximum moves 156; warps joining all at once 147; two
 // references 149.  One token over 1024 keys takes 11.3 us with the join, most of it start-up and dependent loads.  With more
